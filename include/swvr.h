@@ -44,6 +44,7 @@ extern "C" {
 #define SWVR_BF16 0
 #define SWVR_F16 1
 #define SWVR_F32 2
+#define SWVR_F64 4  /* swvr_embedding and swvr_embedding_bwd only */
 
 /* status codes */
 #define SWVR_OK 0
@@ -301,6 +302,77 @@ int swvr_mse_loss(int64_t N, int64_t D, const float* O, const float* lse, const 
 int swvr_mse_loss_noalloc(int64_t N, int64_t D, const float* O, const float* lse, const void* target,
                           int target_dtype, int64_t ldt, const float* weight, float z_loss_weight, int reduction,
                           float* out, float* scale, float* gO, float* glse, void* stream);
+
+/* Embedding lookup, the readout of single tokens (no reference counterpart):
+ *   out[n] = scale * E[ids[n]]        ids [N] (int64 with id64 = 1, else int32),
+ *                                     E [V,D] (row stride lde), out [N,D]
+ * in E's dtype (SWVR_BF16, SWVR_F16, SWVR_F32 or SWVR_F64): the product in fp32
+ * (fp64), rounded once.  A negative id gives a row of zeros, an id of V or more
+ * a row of NaN; neither is read through.
+ * The gradient gE [V,D] (dense, every row written):
+ *   gE[v] = scale * sum over n with ids[n] = v of g[n]    g [N,D], row stride ldg >= 0
+ * summed in fp32 (fp64) in an order that the ids alone fix, so it is the same on
+ * every run.  D and the strides are unrestricted; pointers are aligned to
+ * their elements.  N and V are below 2^31. */
+int swvr_embedding(int dtype, int id64, int64_t N, int64_t V, int64_t D, const void* ids,
+                   const void* E, int64_t lde, double scale, void* out, void* stream);
+size_t swvr_embedding_bwd_workspace_size(int dtype, int64_t N, int64_t V, int64_t D);
+int swvr_embedding_bwd(int dtype, int id64, int64_t N, int64_t V, int64_t D, const void* ids,
+                       const void* g, int64_t ldg, double scale, void* gE,
+                       void* workspace, size_t workspace_bytes, void* stream);
+
+/* Distillation of the head from a teacher's top logits (no reference
+ * counterpart): with z = (logit_scale h W^T + bias) / temperature, LSE = logsumexp(z)
+ * and p = softmax(teacher / temperature) over a token's T entries,
+ *   kl[n]   = sum_k p[n,k] (log p[n,k] - z[n,ids[n,k]] + LSE[n])
+ *   term[n] = weight[n] (kl[n] + z_loss_weight LSE[n]^2)
+ * out: the terms ([N], SWVR_REDUCE_NONE), or one value: their sum times c, c = 1 (SUM) or
+ * 1 / (sum of the weights of the tokens that have an entry) (MEAN; 1 where that sum is 0).
+ * ids [N,T] (row stride ldi; int64 with id64 = 1, else int32), teacher [N,T] (row
+ * stride ldt, t_dtype).  An entry with a negative id or a teacher logit of -inf is
+ * absent; a token without entries, or of weight 0, has term 0.  An id of V or
+ * more makes its token's term NaN.  Ids may repeat within a token.  weight: fp32
+ * [N] or NULL (1).  T is 1 to SWVR_MAX_TEACHER.  h, W, bias as in swvr_fwd_mixed.
+ * lse [N] is written, c [1] too (not for NONE).  For the gradient: p and q
+ * ([N,T], the teacher's and the student's probabilities at the ids) and coef [N]
+ * are written (all NULL: no gradient).
+ * swvr_distill_bwd takes them back with g, the gradient of out ([N] or one
+ * value), and writes gh [N,K], gW [V,K] (their dtype tags) and gb [V] (fp32);
+ * each may be NULL.  Only ids is read of the teacher's lists.  chunk as in swvr_bwd. */
+#define SWVR_MAX_TEACHER 1024
+size_t swvr_distill_workspace_size(int dtype, int64_t N, int64_t K, int64_t V, int64_t T, int weighted);
+int swvr_distill(int dtype, int h_dtype, int w_dtype, int64_t N, int64_t K, int64_t V, int64_t T,
+                 const void* h, int64_t ldh, const void* W, int64_t ldw, const float* bias, float logit_scale,
+                 const void* ids, int id64, int64_t ldi, const void* teacher, int t_dtype, int64_t ldt,
+                 float temperature, const float* weight, float z_loss_weight, int reduction,
+                 float* out, float* c, float* lse, float* p, float* q, float* coef,
+                 void* workspace, size_t workspace_bytes, void* stream);
+size_t swvr_distill_bwd_workspace_size(int dtype, int w_dtype, int64_t N, int64_t K, int64_t V, int64_t T,
+                                       int64_t chunk, int need_gh);
+int swvr_distill_bwd(int dtype, int h_dtype, int w_dtype, int64_t N, int64_t K, int64_t V, int64_t T,
+                     const void* h, int64_t ldh, const void* W, int64_t ldw, const float* bias, float logit_scale,
+                     const void* ids, int id64, int64_t ldi, float temperature, float z_loss_weight, int reduction,
+                     const float* g, const float* c, const float* lse, const float* p, const float* q,
+                     const float* coef, int64_t chunk, void* gh, int gh_dtype, void* gW, int gW_dtype, float* gb,
+                     void* workspace, size_t workspace_bytes, void* stream);
+
+/* One token per row of logits [R,V] (row stride ld >= 0) from a uniform number u[r] in [0, 1)
+ * (fp64 with u64 = 1, else fp32), no reference counterpart.  A row's tokens in the order of
+ * their logits (larger first, equal ones by index), with w = exp((logit - largest) / temperature):
+ *   top_k  keeps the first k (k <= 0 or above V: all);
+ *   top_p  of those keeps the tokens before which the sum of w is below top_p times their sum
+ *          (1 or more: all; at least one token);
+ *   min_p  keeps those with w >= min_p (0 or less: all; at least one token).
+ * token[r]: the first in index order whose running sum of kept w exceeds u times their whole
+ * sum; logprob[r]: the logarithm of its share of that sum.  temperature 0 takes the first
+ * token of the order (logprob 0).  NaN counts as -inf; a row of nothing else gives token -1
+ * and logprob -inf.  A setting is one value, or with its _rows pointer one per row.  w is held
+ * as a whole number of 2^-44 (V up to 2^18; a bit less per doubling of V), so sums are exact,
+ * and a token of smaller weight than half of that is never drawn. */
+int swvr_sample(int dtype, int64_t R, int64_t V, const void* logits, int64_t ld, const void* u, int u64,
+                double temperature, const float* temperature_rows, int64_t top_k, const int* top_k_rows,
+                double top_p, const float* top_p_rows, double min_p, const float* min_p_rows,
+                int64_t* token, float* logprob, void* stream);
 
 /* Matrix-core throughput probe (measurement only; no reference counterpart):
  * `workgroups` workgroups of 8 waves, each wave `iters` steps of a 4 x 2 grid

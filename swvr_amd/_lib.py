@@ -12,7 +12,7 @@ import torch
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libswvr_hip.so")
 ABI_VERSION = 1
 
-BF16, F16, F32 = 0, 1, 2
+BF16, F16, F32, F64 = 0, 1, 2, 4
 DTYPE_TAG = {torch.bfloat16: BF16, torch.float16: F16, torch.float32: F32}
 
 OK, EINVAL, EDTYPE, EHIP, EWORKSPACE = 0, -1, -2, -3, -4
@@ -59,6 +59,17 @@ SIGNATURES = {
     "swvr_mse_loss_workspace_size": (_sz, [_i64]),
     "swvr_mse_loss": (_i, [_i64, _i64, _p, _p, _p, _i, _i64, _p, _f, _i, _p, _p, _p, _p, _p, _sz, _p]),
     "swvr_mse_loss_noalloc": (_i, [_i64, _i64, _p, _p, _p, _i, _i64, _p, _f, _i, _p, _p, _p, _p, _p]),
+    "swvr_embedding": (_i, [_i, _i, _i64, _i64, _i64, _p, _p, _i64, ctypes.c_double, _p, _p]),
+    "swvr_embedding_bwd_workspace_size": (_sz, [_i, _i64, _i64, _i64]),
+    "swvr_embedding_bwd": (_i, [_i, _i, _i64, _i64, _i64, _p, _p, _i64, ctypes.c_double, _p, _p, _sz, _p]),
+    "swvr_distill_workspace_size": (_sz, [_i, _i64, _i64, _i64, _i64, _i]),
+    "swvr_distill": (_i, [_i, _i, _i, _i64, _i64, _i64, _i64, _p, _i64, _p, _i64, _p, _f, _p, _i, _i64, _p, _i, _i64,
+                          _f, _p, _f, _i, _p, _p, _p, _p, _p, _p, _p, _sz, _p]),
+    "swvr_distill_bwd_workspace_size": (_sz, [_i, _i, _i64, _i64, _i64, _i64, _i64, _i]),
+    "swvr_distill_bwd": (_i, [_i, _i, _i, _i64, _i64, _i64, _i64, _p, _i64, _p, _i64, _p, _f, _p, _i, _i64, _f, _f, _i,
+                              _p, _p, _p, _p, _p, _p, _i64, _p, _i, _p, _i, _p, _p, _sz, _p]),
+    "swvr_sample": (_i, [_i, _i64, _i64, _p, _i64, _p, _i, ctypes.c_double, _p, _i64, _p, ctypes.c_double, _p,
+                         ctypes.c_double, _p, _p, _p, _p]),
     "swvr_probe_mfma": (_i, [_i64, _i64, _i, _p, _p]),
     "swvr_timing_enable": (_i, [_i]),
     "swvr_timing_collect": (_i, [ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_int64), _i]),
@@ -108,6 +119,25 @@ def ptr(t):
 
 def stream_of(device):
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+def call(fn, device, *args):
+    """fn(*args, the device's current stream) with the device current, checked.  (Through torch's raw stream and
+    device calls: torch.cuda.device and torch.cuda.current_stream take 4 us of a call's 11, and twice
+    that in autograd's thread.)"""
+    index = device.index
+    if torch._C._cuda_getDevice() == index:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc != OK:
+        check(rc)
+
+
+def address(t):
+    """``t``'s device address for a pointer argument (None: NULL)."""
+    return None if t is None else t.data_ptr()
 
 
 def bwd_tiling(dtype, N, K, V, D, chunk):

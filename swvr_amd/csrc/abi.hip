@@ -62,7 +62,8 @@ const char* kKindNames[kNumKinds] = {"fwd_tile_kernel",   "fwd_combine_kernel", 
                                      "bwd_scores_kernel", "bwd_gemm_kernel",    "bwd_reduce_kernel",
                                      "fill_zero_kernel",  "operand_packing",    "bwd_expand_kernel",
                                      "mse_loss",          "quantize_e4m3",      "readout_f64",
-                                     "probe_mfma"};
+                                     "probe_mfma",        "embedding",          "sort_ids",
+                                     "distill",           "sample_tokens"};
 
 bool is_dtype(int d) { return d == SWVR_BF16 || d == SWVR_F16 || d == SWVR_F32; }
 
@@ -173,7 +174,8 @@ int bwd_common(int dtype, int h_dtype, int w_dtype, int64_t N, int64_t K, int64_
                    int64_t chunk, void* gh, int gh_dtype, void* gW, int gW_dtype, void* gE, int gE_dtype, float* gb,
                    void* workspace, size_t workspace_bytes, void* stream, const void* hq = nullptr,
                    int64_t K8 = 0, int64_t ldhq = 0, const float* h_scale = nullptr, const void* Wq = nullptr,
-                   int64_t ldwq = 0, const float* w_scale = nullptr) {
+                   int64_t ldwq = 0, const float* w_scale = nullptr, const int* pt_id = nullptr,
+                   const float* pt_val = nullptr, int64_t n_pt = 0, int pt_T = 1) {
   g_err[0] = 0;
   int rc = check_common(dtype, N, K, V, D, h, ldh, W, ldw, E, lde);
   if (rc != SWVR_OK) return rc;
@@ -223,6 +225,10 @@ int bwd_common(int dtype, int h_dtype, int w_dtype, int64_t N, int64_t K, int64_
   p.h_scale = h_scale;
   p.w_scale = w_scale;
   p.K8 = (int)K8;
+  p.pt_id = pt_id;
+  p.pt_val = pt_val;
+  p.n_pt = n_pt;
+  p.pt_T = pt_T;
   hipError_t e = bwd_launch(dtype, plan, p, static_cast<hipStream_t>(stream));
   if (e != hipSuccess) return hip_fail(e, "backward launch");
   return SWVR_OK;
@@ -385,6 +391,286 @@ int swvr_bwd(int dtype, int64_t N, int64_t K, int64_t V, int64_t D, const void* 
              void* stream) {
   return swvr_bwd_mixed(dtype, dtype, dtype, N, K, V, D, h, ldh, W, ldw, E, lde, bias, logit_scale, O, lse, gO, glse,
                         chunk, gh, gh_dtype, gW, gW_dtype, gE, gE_dtype, gb, workspace, workspace_bytes, stream);
+}
+
+// ---------------------------------------------------------------- embedding lookup
+static int check_embed(int dtype, int id64, int64_t N, int64_t V, int64_t D, const void* ids) {
+  g_err[0] = 0;
+  if (!is_dtype(dtype) && dtype != SWVR_F64) return fail(SWVR_EDTYPE, "unsupported dtype tag %d", dtype);
+  if (id64 != 0 && id64 != 1) return fail(SWVR_EINVAL, "ids are int32 (0) or int64 (1), got %d", id64);
+  if (N < 0 || V < 0 || D < 0 || N > INT32_MAX || V > INT32_MAX - 1 || D > INT32_MAX)
+    return fail(SWVR_EINVAL, "bad sizes N=%lld V=%lld D=%lld", (long long)N, (long long)V, (long long)D);
+  if (N > 0 && !ids) return fail(SWVR_EINVAL, "ids must be non-null");
+  return SWVR_OK;
+}
+
+int swvr_embedding(int dtype, int id64, int64_t N, int64_t V, int64_t D, const void* ids, const void* E, int64_t lde,
+                   double scale, void* out, void* stream) {
+  const int rc = check_embed(dtype, id64, N, V, D, ids);
+  if (rc != SWVR_OK) return rc;
+  if (lde < D) return fail(SWVR_EINVAL, "lde=%lld must be >= D", (long long)lde);
+  if (N > 0 && D > 0 && ((V > 0 && !E) || !out)) return fail(SWVR_EINVAL, "E and out must be non-null");
+  swvr::EmbedParams p{};
+  p.dtype = dtype;
+  p.ids = ids;
+  p.id64 = id64;
+  p.N = N;
+  p.V = (int)V;
+  p.D = (int)D;
+  p.E = E;
+  p.lde = lde;
+  p.scale = scale;
+  p.out = out;
+  hipError_t e = swvr::embed_lookup_launch(p, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "embedding launch");
+  return SWVR_OK;
+}
+
+size_t swvr_embedding_bwd_workspace_size(int dtype, int64_t N, int64_t V, int64_t D) {
+  if ((!is_dtype(dtype) && dtype != SWVR_F64) || N < 0 || V < 0 || D < 0 || N > INT32_MAX || V > INT32_MAX - 1) return 0;
+  return swvr::embed_grad_workspace_bytes(dtype, N, V, D);
+}
+
+int swvr_embedding_bwd(int dtype, int id64, int64_t N, int64_t V, int64_t D, const void* ids, const void* g,
+                       int64_t ldg, double scale, void* gE, void* workspace, size_t workspace_bytes, void* stream) {
+  const int rc = check_embed(dtype, id64, N, V, D, ids);
+  if (rc != SWVR_OK) return rc;
+  if (ldg < 0) return fail(SWVR_EINVAL, "ldg=%lld must not be negative", (long long)ldg);
+  if (V > 0 && D > 0 && ((N > 0 && !g) || !gE)) return fail(SWVR_EINVAL, "g and gE must be non-null");
+  const size_t need = swvr::embed_grad_workspace_bytes(dtype, N, V, D);
+  if (!workspace || workspace_bytes < need)
+    return fail(SWVR_EWORKSPACE, "embedding workspace of %zu bytes needed, %zu given", need, workspace_bytes);
+  swvr::EmbedParams p{};
+  p.dtype = dtype;
+  p.ids = ids;
+  p.id64 = id64;
+  p.N = N;
+  p.V = (int)V;
+  p.D = (int)D;
+  p.scale = scale;
+  p.g = g;
+  p.ldg = ldg;
+  p.gE = gE;
+  hipError_t e = swvr::embed_grad_launch(p, static_cast<char*>(workspace), static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "embedding gradient launch");
+  return SWVR_OK;
+}
+
+// ---------------------------------------------------------------- distillation
+static size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
+
+static int check_distill(int dtype, int64_t N, int64_t V, int64_t T, int id64, const void* ids, int64_t ldi,
+                         float temperature, int reduction) {
+  g_err[0] = 0;
+  if (!is_dtype(dtype)) return fail(SWVR_EDTYPE, "unsupported operand dtype tag %d", dtype);
+  if (N < 0 || V < 0 || T < 1 || T > SWVR_MAX_TEACHER || N > INT32_MAX || V > INT32_MAX - 1 || N * T > INT32_MAX)
+    return fail(SWVR_EINVAL, "bad sizes N=%lld V=%lld T=%lld (T 1 to %d, N T below 2^31)", (long long)N, (long long)V,
+                (long long)T, SWVR_MAX_TEACHER);
+  if (id64 != 0 && id64 != 1) return fail(SWVR_EINVAL, "teacher ids are int32 (0) or int64 (1), got %d", id64);
+  if (ldi < 0) return fail(SWVR_EINVAL, "ldi=%lld must not be negative", (long long)ldi);
+  if (N > 0 && !ids) return fail(SWVR_EINVAL, "teacher ids must be non-null");
+  if (!(temperature > 0.f) || temperature > 3e38f)
+    return fail(SWVR_EINVAL, "temperature must be positive and finite, got %g", (double)temperature);
+  if (reduction < SWVR_REDUCE_NONE || reduction > SWVR_REDUCE_MEAN)
+    return fail(SWVR_EINVAL, "unknown reduction %d", reduction);
+  return SWVR_OK;
+}
+
+size_t swvr_distill_workspace_size(int dtype, int64_t N, int64_t K, int64_t V, int64_t T, int weighted) {
+  FwdPlan plan;
+  if (N < 0 || V < 0 || T < 0 || !fwd_plan(dtype, N, K, V, 0, &plan, weighted != 0)) return 0;
+  return up256(plan.ws_bytes) + up256((size_t)N * T * 4) + up256((size_t)V * 4) + up256(swvr::distill_part_bytes(N));
+}
+
+int swvr_distill(int dtype, int h_dtype, int w_dtype, int64_t N, int64_t K, int64_t V, int64_t T, const void* h,
+                 int64_t ldh, const void* W, int64_t ldw, const float* bias, float logit_scale, const void* ids,
+                 int id64, int64_t ldi, const void* teacher, int t_dtype, int64_t ldt, float temperature,
+                 const float* weight, float z_loss_weight, int reduction, float* out, float* c, float* lse, float* p,
+                 float* q, float* coef, void* workspace, size_t workspace_bytes, void* stream) {
+  int rc = check_distill(dtype, N, V, T, id64, ids, ldi, temperature, reduction);
+  if (rc != SWVR_OK) return rc;
+  if (!is_dtype(t_dtype)) return fail(SWVR_EDTYPE, "unsupported teacher dtype tag %d", t_dtype);
+  if (ldt < 0) return fail(SWVR_EINVAL, "ldt=%lld must not be negative", (long long)ldt);
+  if (N > 0 && (!teacher || !lse)) return fail(SWVR_EINVAL, "teacher logits and lse must be non-null");
+  if ((N > 0 || reduction) && !out) return fail(SWVR_EINVAL, "out must be non-null");
+  if (reduction && !c) return fail(SWVR_EINVAL, "c must be non-null");
+  if ((p == nullptr) != (q == nullptr) || (p == nullptr) != (coef == nullptr))
+    return fail(SWVR_EINVAL, "p, q and coef must all be given or all NULL");
+  const size_t need = swvr_distill_workspace_size(dtype, N, K, V, T, weight != nullptr);
+  if (!workspace || workspace_bytes < need)
+    return fail(SWVR_EWORKSPACE, "distillation workspace of %zu bytes needed, %zu given", need, workspace_bytes);
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  char* ws = static_cast<char*>(workspace);
+  FwdPlan plan;
+  fwd_plan(dtype, N, K, V, 0, &plan, weight != nullptr);
+  const size_t fwd_bytes = plan.ws_bytes;
+  float* z = reinterpret_cast<float*>(ws + up256(fwd_bytes));
+  float* sb = z + up256((size_t)N * T * 4) / 4;
+  float* part = sb + up256((size_t)V * 4) / 4;
+  const float inv_tau = 1.f / temperature, scale = logit_scale / temperature;
+  hipError_t e = hipSuccess;
+  if (bias && temperature != 1.f) {
+    if ((e = swvr::distill_scale(bias, V, inv_tau, sb, s)) != hipSuccess) return hip_fail(e, "bias launch");
+    bias = sb;
+  }
+  // the log-sum-exps: a readout without columns
+  rc = fwd_common(dtype, h_dtype, w_dtype, N, K, V, 0, h, ldh, W, ldw, W, 0, bias, scale, nullptr, lse, nullptr, nullptr,
+                  workspace, fwd_bytes, stream, weight != nullptr, weight);
+  if (rc != SWVR_OK) return rc;
+  swvr::DistillParams d{};
+  d.h = h;
+  d.ldh = ldh;
+  d.W = W;
+  d.ldw = ldw;
+  d.h_f32 = h_dtype != dtype;
+  d.w_f32 = w_dtype != dtype;
+  d.bias = bias;
+  d.scale = scale;
+  d.inv_tau = inv_tau;
+  d.N = (int)N;
+  d.K = (int)K;
+  d.V = (int)V;
+  d.T = (int)T;
+  d.ids = ids;
+  d.id64 = id64;
+  d.ldi = ldi;
+  d.teacher = teacher;
+  d.t_dtype = t_dtype;
+  d.ldt = ldt;
+  d.weight = weight;
+  d.lse = lse;
+  d.zw = z_loss_weight;
+  d.reduce = reduction;
+  d.z = z;
+  d.out = out;
+  d.p = p;
+  d.q = q;
+  d.coef = coef;
+  e = swvr::distill_loss(dtype, d, part, c, s);
+  if (e != hipSuccess) return hip_fail(e, "distillation launch");
+  return SWVR_OK;
+}
+
+size_t swvr_distill_bwd_workspace_size(int dtype, int w_dtype, int64_t N, int64_t K, int64_t V, int64_t T,
+                                       int64_t chunk, int need_gh) {
+  BwdPlan plan;
+  if (N < 0 || V < 0 || T < 0 || chunk <= 0 || !bwd_plan(dtype, N, K, V, 0, chunk, need_gh != 0, &plan, w_dtype != dtype))
+    return 0;
+  return up256(plan.ws_bytes) + up256((size_t)V * 4) + up256((size_t)N * 4) + 5 * up256((size_t)N * T * 4) +
+         up256((size_t)(V + 1) * 4);
+}
+
+int swvr_distill_bwd(int dtype, int h_dtype, int w_dtype, int64_t N, int64_t K, int64_t V, int64_t T, const void* h,
+                     int64_t ldh, const void* W, int64_t ldw, const float* bias, float logit_scale, const void* ids,
+                     int id64, int64_t ldi, float temperature, float z_loss_weight, int reduction, const float* g,
+                     const float* c, const float* lse, const float* p, const float* q, const float* coef,
+                     int64_t chunk, void* gh, int gh_dtype, void* gW, int gW_dtype, float* gb, void* workspace,
+                     size_t workspace_bytes, void* stream) {
+  int rc = check_distill(dtype, N, V, T, id64, ids, ldi, temperature, reduction);
+  if (rc != SWVR_OK) return rc;
+  if (chunk <= 0) return fail(SWVR_EINVAL, "chunk must be positive, got %lld", (long long)chunk);
+  if (N > 0 && (!g || !lse || !p || !q || !coef || (reduction && !c)))
+    return fail(SWVR_EINVAL, "g, c, lse, p, q and coef must be non-null");
+  if (gb && !bias) return fail(SWVR_EINVAL, "gb requested without a bias");
+  const size_t need = swvr_distill_bwd_workspace_size(dtype, w_dtype, N, K, V, T, chunk, gh != nullptr);
+  if (!workspace || workspace_bytes < need)
+    return fail(SWVR_EWORKSPACE, "distillation workspace of %zu bytes needed, %zu given", need, workspace_bytes);
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  BwdPlan plan;
+  bwd_plan(dtype, N, K, V, 0, chunk, gh != nullptr, &plan, w_dtype != dtype);
+  char* at = static_cast<char*>(workspace) + up256(plan.ws_bytes);
+  auto take = [&](size_t bytes) {
+    char* const x = at;
+    at += up256(bytes);
+    return x;
+  };
+  float* sb = reinterpret_cast<float*>(take((size_t)V * 4));
+  float* glse = reinterpret_cast<float*>(take((size_t)N * 4));
+  const size_t nt = (size_t)N * T * 4;
+  int* pt_id = reinterpret_cast<int*>(take(nt));
+  float* pt_val = reinterpret_cast<float*>(take(nt));
+  float* pt_t = reinterpret_cast<float*>(take(nt));
+  int* order = reinterpret_cast<int*>(take(nt));
+  int* sid = reinterpret_cast<int*>(take(nt));
+  int* seg = reinterpret_cast<int*>(take((size_t)(V + 1) * 4));
+  const float inv_tau = 1.f / temperature;
+  hipError_t e = hipSuccess;
+  if (bias && temperature != 1.f) {
+    if ((e = swvr::distill_scale(bias, V, inv_tau, sb, s)) != hipSuccess) return hip_fail(e, "bias launch");
+    bias = sb;
+  }
+  if (N > 0) {
+    swvr::DistillGradParams d{};
+    d.N = (int)N;
+    d.V = (int)V;
+    d.T = (int)T;
+    d.ids = ids;
+    d.id64 = id64;
+    d.ldi = ldi;
+    d.g = g;
+    d.reduce = reduction;
+    d.c = c;
+    d.lse = lse;
+    d.p = p;
+    d.q = q;
+    d.coef = coef;
+    d.zw = z_loss_weight;
+    d.glse = glse;
+    d.pt_id = pt_id;
+    d.pt_val = pt_val;
+    d.pt_t = gb ? pt_t : nullptr;
+    if ((e = swvr::distill_prep(d, s)) != hipSuccess) return hip_fail(e, "distillation launch");
+  }
+  rc = bwd_common(dtype, h_dtype, w_dtype, N, K, V, 0, h, ldh, W, ldw, W, 0, bias, logit_scale / temperature, nullptr,
+                  lse, nullptr, glse, chunk, gh, gh_dtype, gW, gW_dtype, nullptr, 0, gb, workspace,
+                  up256(plan.ws_bytes), stream, nullptr, 0, 0, nullptr, nullptr, 0, nullptr, pt_id, pt_val, N * T,
+                  (int)T);
+  if (rc != SWVR_OK) return rc;
+  if (gb && N > 0 && V > 0) {
+    if ((e = swvr::sort_ids(pt_id, 0, (int)(N * T), (int)V, order, sid, seg, s)) != hipSuccess ||
+        (e = swvr::distill_bias(order, seg, pt_t, (int)V, inv_tau, gb, s)) != hipSuccess)
+      return hip_fail(e, "bias gradient launch");
+  }
+  return SWVR_OK;
+}
+
+// ---------------------------------------------------------------- sampling
+int swvr_sample(int dtype, int64_t R, int64_t V, const void* logits, int64_t ld, const void* u, int u64,
+                double temperature, const float* temperature_rows, int64_t top_k, const int* top_k_rows, double top_p,
+                const float* top_p_rows, double min_p, const float* min_p_rows, int64_t* token, float* logprob,
+                void* stream) {
+  g_err[0] = 0;
+  if (!is_dtype(dtype)) return fail(SWVR_EDTYPE, "unsupported logits dtype tag %d", dtype);
+  if (R < 0 || V < 1 || R > INT32_MAX || V > INT32_MAX)
+    return fail(SWVR_EINVAL, "bad sizes R=%lld V=%lld", (long long)R, (long long)V);
+  if (ld < 0) return fail(SWVR_EINVAL, "ld=%lld must not be negative", (long long)ld);
+  if (u64 != 0 && u64 != 1) return fail(SWVR_EINVAL, "u is fp32 (0) or fp64 (1), got %d", u64);
+  if (!temperature_rows && !(temperature >= 0))
+    return fail(SWVR_EINVAL, "temperature must not be negative, got %g", temperature);
+  if (R == 0) return SWVR_OK;
+  if (!logits || !u || !token || !logprob) return fail(SWVR_EINVAL, "logits, u, token and logprob must be non-null");
+  const uintptr_t eb = dtype == SWVR_F32 ? 4 : 2;
+  if (reinterpret_cast<uintptr_t>(logits) % eb) return fail(SWVR_EINVAL, "logits must be aligned to their elements");
+  swvr::SampleParams p{};
+  p.R = R;
+  p.V = V;
+  p.logits = logits;
+  p.ld = ld;
+  p.u = u;
+  p.u64 = u64;
+  p.tau = temperature;
+  p.k = top_k;
+  p.p = top_p;
+  p.min_p = min_p;
+  p.tau_rows = temperature_rows;
+  p.k_rows = top_k_rows;
+  p.p_rows = top_p_rows;
+  p.min_p_rows = min_p_rows;
+  p.token = token;
+  p.logprob = logprob;
+  hipError_t e = swvr::sample_launch(dtype, p, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "sampling launch");
+  return SWVR_OK;
 }
 
 int swvr_timing_enable(int on) {

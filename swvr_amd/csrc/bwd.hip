@@ -293,6 +293,23 @@ __device__ __forceinline__ void store_ds_block(const f32x16_t& ds, void* stage, 
   }
 }
 
+// The caller's elements of dS over the staged ones of a chunk: one thread per entry, those of other chunks and of
+// inactive tokens left out.  Position of token tok of a 32-token block: stage_tok's inverse.
+template <class T>
+__global__ __launch_bounds__(256) void bwd_patch_kernel(const int* __restrict__ pt_id,
+                                                        const float* __restrict__ pt_val, int64_t n_pt, int pt_T,
+                                                        const int* __restrict__ inv, int v0, int cv, int n_tb32,
+                                                        T* __restrict__ stage) {
+  const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (e >= n_pt) return;
+  const int v = pt_id[e] - v0;
+  if (v < 0 || v >= cv) return;
+  const int q = inv[(uint32_t)e / (uint32_t)pt_T];
+  if (q < 0) return;
+  const int tok = q & 31, pos = ((tok >> 3) << 2) | (((tok >> 2) & 1) << 4) | (tok & 3);
+  stage[stage_off(v, (q & ~31) | pos, n_tb32)] = from_float<T>(pt_val[e]);
+}
+
 // Tile shape of the scores kernel per (dtype, padded D): BM tokens x BV
 // vocabulary rows per workgroup of WT x WV waves (two waves per SIMD for
 // bf16 / f16).  dE^T (DP x BV/WV per wave) and the score block share the
@@ -1795,6 +1812,13 @@ hipError_t bwd_run(const BwdPlan& plan, const BwdParams& p, hipStream_t stream) 
     sp.n_act = n_act;
     sp.DP = plan.DP;
     if ((e = dispatch_scores<T>(plan, sp, stream)) != hipSuccess) return e;
+    if (p.pt_id && need_stage && p.n_pt > 0) {
+      timing_begin(kKindDistill, stream);
+      bwd_patch_kernel<T><<<(unsigned)((p.n_pt + 255) / 256), 256, 0, stream>>>(
+          p.pt_id, p.pt_val, p.n_pt, p.pt_T, inv, v0, cv, (int)(plan.N_pad / 32), stage);
+      timing_end(kKindDistill, stream);
+      if ((e = hipGetLastError()) != hipSuccess) return e;
+    }
 
     bool fold_red = false;
     if (need_stage || gemm_de) {

@@ -30,7 +30,7 @@ typedef __attribute__((__vector_size__(8 * sizeof(_Float16)))) _Float16 f16x8_t;
 typedef __attribute__((__vector_size__(8 * sizeof(float)))) float f32x8_t;
 typedef __attribute__((__vector_size__(16 * sizeof(float)))) float f32x16_t;
 
-enum { kBF16 = 0, kF16 = 1, kF32 = 2, kFP8 = 3 };  // kFP8: h, W in OCP e4m3; E in bf16
+enum { kBF16 = 0, kF16 = 1, kF32 = 2, kFP8 = 3, kF64 = 4 };  // kFP8: h, W in OCP e4m3; E in bf16
 
 template <class T> struct Vec8;
 template <> struct Vec8<bf16_t> { typedef bf16x8_t type; };

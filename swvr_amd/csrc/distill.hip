@@ -1,0 +1,329 @@
+// Distillation of the head from a teacher's top logits (no counterpart in the reference).  With the scores
+// z = s / tau h W^T + b / tau and their log-sum-exp LSE over the vocabulary, and the teacher's distribution
+// p_n = softmax(t_n / tau) over the T entries (id, t) it gives for token n,
+//
+//   kl[n]   = sum_k p[n,k] (log p[n,k] - z[n, id[n,k]] + LSE[n])
+//   loss    = sum_n w[n] (kl[n] + zw LSE[n]^2) * c,     c = 1 / sum_n w[n] (mean), 1 (sum)
+//   dS[n,v] = c_n softmax(z)[n,v] - sum over k with id[n,k] = v of g_n p[n,k],
+//             g_n = g c w[n],  c_n = g_n (1 + 2 zw LSE[n]);
+//   gh = s / tau dS W,   gW = s / tau dS^T h,   gb = colsum(dS) / tau.
+//
+// LSE and the dense part of the gradients are the readout's forward and backward (with no embedding: D = 0,
+// gO = 0, gLSE = c_n), so the [N, V] scores are never in memory.  What is here is the sparse part:
+//   distill_dot_kernel    z at the teacher's ids: dot products of h's row with gathered rows of W in fp32
+//                         (2 N T K flops; bound by the gather, N T rows of W);
+//   distill_loss_kernel   p, the loss's terms and softmax(z) at the ids (one wave per token);
+//   distill_prep_kernel   c_n, and the values of dS at the ids, in fp32 and with p taken off there: after the
+//                         scores kernel has staged a chunk of dS, bwd_patch_kernel (bwd.hip) writes them over
+//                         its elements, so the difference is rounded once, not its two terms;
+//   distill_bias_kernel   takes the sums of g_n p off gb, over the entries sorted by id (sort_ids).
+// An entry with a negative id or a logit of -inf is absent; a token without entries, or of weight zero, has
+// loss 0, no share in c and no gradient.  An id of V or more makes its token's loss NaN.
+#include <cfloat>
+
+#include "common.hpp"
+#include "launch.hpp"
+
+namespace swvr {
+
+namespace {
+
+__device__ __forceinline__ float wave_sum(float x) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) x += __shfl_xor(x, off, 64);
+  return x;
+}
+__device__ __forceinline__ float wave_max(float x) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) x = fmaxf(x, __shfl_xor(x, off, 64));
+  return x;
+}
+
+__device__ __forceinline__ int64_t id_at(const DistillParams& p, int n, int k) {
+  const int64_t i = (int64_t)n * p.ldi + k;
+  return p.id64 ? static_cast<const int64_t*>(p.ids)[i] : (int64_t)static_cast<const int*>(p.ids)[i];
+}
+
+__device__ __forceinline__ float teacher_at(const DistillParams& p, int n, int k) {
+  const int64_t i = (int64_t)n * p.ldt + k;
+  return p.t_dtype == kBF16  ? (float)static_cast<const bf16_t*>(p.teacher)[i]
+         : p.t_dtype == kF16 ? (float)static_cast<const f16_t*>(p.teacher)[i]
+                             : static_cast<const float*>(p.teacher)[i];
+}
+
+__global__ __launch_bounds__(256) void distill_scale_kernel(const float* __restrict__ x, int64_t n, float s,
+                                                            float* __restrict__ y) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i < n) y[i] = x[i] * s;
+}
+
+// 8 consecutive values of a row stored as S, rounded to the compute dtype T.
+template <class T, class S>
+__device__ __forceinline__ void load8(const S* row, float (&v)[8]) {
+  typedef typename Vec8<S>::type V8;
+  const V8 x = *reinterpret_cast<const V8*>(row);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = (float)(T)x[i];
+}
+
+// z of kDotIds entries of a token per wave: h's 8 values of a lane serve them all.
+constexpr int kDotIds = 4;
+template <class T, class HS, class WS>
+__global__ __launch_bounds__(256) void distill_dot_kernel(DistillParams p) {
+  const int groups = (p.T + kDotIds - 1) / kDotIds;
+  const int64_t gw = (int64_t)blockIdx.x * 4 + wave_id();
+  if (gw >= (int64_t)p.N * groups) return;
+  const int n = (int)(gw / groups), k0 = (int)(gw % groups) * kDotIds;
+  if (p.weight && p.weight[n] == 0.f) return;
+  const int lane = lane_id();
+  const HS* const h = static_cast<const HS*>(p.h) + (int64_t)n * p.ldh;
+  const WS* w[kDotIds];
+  bool in[kDotIds];
+  int id[kDotIds];
+  bool any = false;
+#pragma unroll
+  for (int u = 0; u < kDotIds; ++u) {
+    const int64_t x = k0 + u < p.T ? id_at(p, n, k0 + u) : -1;
+    in[u] = x >= 0 && x < p.V;
+    id[u] = in[u] ? (int)x : 0;
+    w[u] = static_cast<const WS*>(p.W) + (int64_t)id[u] * p.ldw;
+    any |= in[u];
+  }
+  if (!any) return;
+  float acc[kDotIds];
+#pragma unroll
+  for (int u = 0; u < kDotIds; ++u) acc[u] = 0.f;
+  for (int k = lane * 8; k < p.K; k += 512) {
+    float a[8];
+    load8<T, HS>(h + k, a);
+#pragma unroll
+    for (int u = 0; u < kDotIds; ++u) {
+      if (!in[u]) continue;
+      float b[8];
+      load8<T, WS>(w[u] + k, b);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) acc[u] = fmaf(a[i], b[i], acc[u]);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kDotIds; ++u) {
+    const float s = wave_sum(acc[u]);
+    if (lane == u && in[u]) p.z[(int64_t)n * p.T + k0 + u] = s * p.scale + (p.bias ? p.bias[id[u]] : 0.f);
+  }
+}
+
+// One wave per token, 16 tokens per workgroup; the workgroup's sums of the terms and of the weights in token
+// order (mse_loss's reduction).
+constexpr int kTokensPerWave = 4, kTokensPerBlock = 4 * kTokensPerWave;
+__global__ __launch_bounds__(256) void distill_loss_kernel(DistillParams p, float* __restrict__ part, int n_blk) {
+  __shared__ float s_loss[4], s_w[4];
+  const int lane = lane_id(), wv = wave_id();
+  float wave_loss = 0.f, wave_w = 0.f;
+  for (int j = 0; j < kTokensPerWave; ++j) {
+    const int n = blockIdx.x * kTokensPerBlock + wv * kTokensPerWave + j;
+    if (n >= p.N) break;  // uniform across the wave
+    const float w = p.weight ? p.weight[n] : 1.f;
+    float m = kNegInf;
+    bool has = false;
+    for (int k = lane; k < p.T; k += 64) {
+      const float t = teacher_at(p, n, k) * p.inv_tau;
+      if (id_at(p, n, k) < 0 || t == kNegInf) continue;
+      has = true;
+      m = fmaxf(m, t);
+    }
+    m = wave_max(m);
+    const bool live = w != 0.f && __ballot(has) != 0;
+    if (!live) {
+      if (lane == 0) {
+        if (p.coef) p.coef[n] = 0.f;
+        if (p.reduce == 0) p.out[n] = 0.f;
+      }
+      if (p.p)
+        for (int k = lane; k < p.T; k += 64) p.p[(int64_t)n * p.T + k] = p.q[(int64_t)n * p.T + k] = 0.f;
+      continue;
+    }
+    float sum = 0.f;
+    for (int k = lane; k < p.T; k += 64) {
+      const float t = teacher_at(p, n, k) * p.inv_tau;
+      if (id_at(p, n, k) >= 0 && t != kNegInf) sum += expf(t - m);
+    }
+    const float lp = m + logf(wave_sum(sum)), lse = p.lse[n];
+    float kl = 0.f;
+    for (int k = lane; k < p.T; k += 64) {
+      const int64_t id = id_at(p, n, k);
+      const float t = teacher_at(p, n, k) * p.inv_tau;
+      const float logq = id >= p.V ? __builtin_nanf("") : id >= 0 ? p.z[(int64_t)n * p.T + k] - lse : kNegInf;
+      const float logp = t - lp, pk = id >= 0 && t != kNegInf ? expf(logp) : 0.f;
+      if (pk != 0.f) kl += pk * (logp - logq);  // NaN != 0
+      if (p.p) {
+        p.p[(int64_t)n * p.T + k] = pk;
+        p.q[(int64_t)n * p.T + k] = id >= p.V ? 0.f : expf(logq);
+      }
+    }
+    kl = wave_sum(kl);
+    float tok = kl;
+    if (p.zw != 0.f) tok += p.zw * (lse * lse);
+    tok *= w;
+    if (lane == 0) {
+      if (p.coef) p.coef[n] = w;
+      if (p.reduce == 0) p.out[n] = tok;
+    }
+    wave_loss += tok;
+    wave_w += w;
+  }
+  if (lane == 0) {
+    s_loss[wv] = wave_loss;
+    s_w[wv] = wave_w;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0 && part) {
+    part[blockIdx.x] = ((s_loss[0] + s_loss[1]) + s_loss[2]) + s_loss[3];
+    part[n_blk + blockIdx.x] = ((s_w[0] + s_w[1]) + s_w[2]) + s_w[3];
+  }
+}
+
+// The loss and c from the workgroups' sums; weights that sum to zero leave c = 1 (no token to learn from: 0).
+__global__ __launch_bounds__(256) void distill_reduce_kernel(const float* __restrict__ part, int n_blk, int mean,
+                                                             float* __restrict__ out, float* __restrict__ c) {
+  __shared__ float s_loss[256], s_w[256];
+  float a = 0.f, b = 0.f;
+  for (int i = threadIdx.x; i < n_blk; i += 256) {
+    a += part[i];
+    b += part[n_blk + i];
+  }
+  s_loss[threadIdx.x] = a;
+  s_w[threadIdx.x] = b;
+  __syncthreads();
+  for (int s = 128; s > 0; s >>= 1) {
+    if ((int)threadIdx.x < s) {
+      s_loss[threadIdx.x] += s_loss[threadIdx.x + s];
+      s_w[threadIdx.x] += s_w[threadIdx.x + s];
+    }
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) {
+    const float denom = mean && s_w[0] != 0.f ? s_w[0] : 1.f;
+    out[0] = s_loss[0] / denom;
+    c[0] = 1.f / denom;
+  }
+}
+
+// One wave per token: gLSE = c_n, and per entry the id (-1: no element of its own), dS there, and g_n p.
+// Entries of a token that repeat an id share one element of dS: the first of them holds their sum.
+__global__ __launch_bounds__(256) void distill_prep_kernel(DistillGradParams p) {
+  const int n = blockIdx.x * 4 + wave_id();
+  if (n >= p.N) return;
+  const int lane = lane_id();
+  const float w = p.coef[n];
+  const float gn = w == 0.f ? 0.f : p.g[p.reduce == 0 ? n : 0] * w * (p.reduce == 0 ? 1.f : p.c[0]);
+  float cn = p.zw != 0.f ? gn * (1.f + 2.f * p.zw * p.lse[n]) : gn;
+  // the backward leaves out tokens of gLSE = 0: one whose two terms cancel stays
+  if (cn == 0.f && gn != 0.f) cn = FLT_MIN;
+  if (w == 0.f) cn = 0.f;
+  if (lane == 0) p.glse[n] = cn;
+  for (int k = lane; k < p.T; k += 64) {
+    const int64_t e = (int64_t)n * p.T + k;
+    const int64_t at = (int64_t)n * p.ldi;
+    auto id_of = [&](int j) {
+      return p.id64 ? static_cast<const int64_t*>(p.ids)[at + j] : (int64_t)static_cast<const int*>(p.ids)[at + j];
+    };
+    const int64_t id = id_of(k);
+    bool own = w != 0.f && id >= 0 && id < p.V;
+    float sum = 0.f;
+    for (int j = 0; j < p.T; ++j) {
+      const bool same = id_of(j) == id;
+      if (same && j < k) own = false;
+      if (same) sum += p.p[(int64_t)n * p.T + j];
+    }
+    const float t = gn * sum;
+    p.pt_id[e] = own ? (int)id : -1;
+    p.pt_val[e] = cn * p.q[e] - t;
+    if (p.pt_t) p.pt_t[e] = t;
+  }
+}
+
+// gb[v] = (gb[v] - sum of t over the entries of v) / tau, a wave per id.
+__global__ __launch_bounds__(256) void distill_bias_kernel(const int* __restrict__ order, const int* __restrict__ seg,
+                                                           const float* __restrict__ t, int V, float inv_tau,
+                                                           float* __restrict__ gb) {
+  const int v = blockIdx.x * 4 + wave_id();
+  if (v >= V) return;
+  const int lane = lane_id(), i1 = seg[v + 1];
+  float s = 0.f;
+  for (int i = seg[v] + lane; i < i1; i += 256) {
+    float x[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) x[u] = i + 64 * u < i1 ? t[order[i + 64 * u]] : 0.f;
+    s += (x[0] + x[1]) + (x[2] + x[3]);
+  }
+  s = wave_sum(s);
+  if (lane == 0) gb[v] = (gb[v] - s) * inv_tau;
+}
+
+template <class T>
+hipError_t dot_typed(const DistillParams& p, hipStream_t stream) {
+  const int64_t waves = (int64_t)p.N * ((p.T + kDotIds - 1) / kDotIds);
+  const unsigned blocks = (unsigned)((waves + 3) / 4);
+  if constexpr (sizeof(T) == 2) {
+    if (p.h_f32 && p.w_f32)
+      distill_dot_kernel<T, float, float><<<blocks, 256, 0, stream>>>(p);
+    else if (p.h_f32)
+      distill_dot_kernel<T, float, T><<<blocks, 256, 0, stream>>>(p);
+    else if (p.w_f32)
+      distill_dot_kernel<T, T, float><<<blocks, 256, 0, stream>>>(p);
+    else
+      distill_dot_kernel<T, T, T><<<blocks, 256, 0, stream>>>(p);
+  } else {
+    distill_dot_kernel<T, T, T><<<blocks, 256, 0, stream>>>(p);
+  }
+  return hipGetLastError();
+}
+
+}  // namespace
+
+size_t distill_part_bytes(int64_t N) {
+  return (size_t)((N + kTokensPerBlock - 1) / kTokensPerBlock) * 2 * sizeof(float);
+}
+
+hipError_t distill_scale(const float* x, int64_t n, float s, float* y, hipStream_t stream) {
+  if (n == 0) return hipSuccess;
+  distill_scale_kernel<<<(unsigned)((n + 255) / 256), 256, 0, stream>>>(x, n, s, y);
+  return hipGetLastError();
+}
+
+hipError_t distill_loss(int dtype, const DistillParams& p, float* part, float* c, hipStream_t stream) {
+  const int n_blk = (p.N + kTokensPerBlock - 1) / kTokensPerBlock;
+  timing_begin(kKindDistill, stream);
+  hipError_t e = hipSuccess;
+  if (p.N > 0 && p.T > 0) {
+    e = dtype == kBF16 ? dot_typed<bf16_t>(p, stream) : dtype == kF16 ? dot_typed<f16_t>(p, stream)
+                                                                      : dot_typed<float>(p, stream);
+  }
+  if (e == hipSuccess && p.N > 0) {
+    distill_loss_kernel<<<n_blk, 256, 0, stream>>>(p, p.reduce ? part : nullptr, n_blk);
+    e = hipGetLastError();
+  }
+  if (e == hipSuccess && p.reduce) {
+    distill_reduce_kernel<<<1, 256, 0, stream>>>(part, n_blk, p.reduce == 2, p.out, c);
+    e = hipGetLastError();
+  }
+  timing_end(kKindDistill, stream);
+  return e;
+}
+
+hipError_t distill_prep(const DistillGradParams& p, hipStream_t stream) {
+  timing_begin(kKindDistill, stream);
+  distill_prep_kernel<<<(unsigned)((p.N + 3) / 4), 256, 0, stream>>>(p);
+  timing_end(kKindDistill, stream);
+  return hipGetLastError();
+}
+
+hipError_t distill_bias(const int* order, const int* seg, const float* t, int V, float inv_tau, float* gb,
+                        hipStream_t stream) {
+  timing_begin(kKindDistill, stream);
+  distill_bias_kernel<<<(unsigned)((V + 3) / 4), 256, 0, stream>>>(order, seg, t, V, inv_tau, gb);
+  timing_end(kKindDistill, stream);
+  return hipGetLastError();
+}
+
+}  // namespace swvr

@@ -1,0 +1,499 @@
+// Embedding lookup and its gradient (no counterpart in the reference, whose readout is the
+// soft lookup P E of a distribution P; this is that of a token).
+//
+//   out[n] = scale * E[ids[n]],         gE[v] = scale * sum over n with ids[n] = v of g[n]
+//
+// A negative id is no token: its row of out is 0 and it adds nothing to gE.  An id of V or more reads
+// nothing either; its row is NaN, so that it shows without a copy of the ids to the host.
+//
+// The lookup moves bytes: one 16-byte load and store per lane and step (8, 4 or one element's where rows
+// are not 16-byte aligned), a row's lanes consecutive.
+//
+// The gradient is a sum in token order, the same on every run, without atomics on values:
+//   sort_ids_kernel    the tokens in stable order of their id, and each id's segment of them (one launch);
+//   embed_sum_kernel   runs of kRun sorted tokens, whatever their ids, so that an id that half the batch
+//                      holds is split over many workgroups: a segment inside a run goes to its row of gE,
+//                      one that crosses a run's border leaves its part in fp32; beside them, the rows
+//                      without a token are written as zeros (most of gE's bytes, for a large table);
+//   embed_join_kernel  adds the parts of a segment that crosses borders, in order, and writes its row.
+#include <type_traits>
+
+#include "common.hpp"
+#include "launch.hpp"
+
+namespace swvr {
+
+namespace {
+
+template <class T> struct SumType { typedef float type; };
+template <> struct SumType<double> { typedef double type; };
+
+template <class T, int VB>
+struct alignas(VB) Vec {
+  static constexpr int n = VB / (int)sizeof(T);
+  T v[n];
+};
+
+__device__ __forceinline__ int64_t load_id(const void* ids, int id64, int64_t i) {
+  return id64 ? static_cast<const int64_t*>(ids)[i] : (int64_t)static_cast<const int*>(ids)[i];
+}
+
+// ---------------------------------------------------------------- lookup
+// LPR lanes (a power of two up to 256) per row; a lane takes every LPR-th vector of it.
+template <class T, int VB>
+__global__ __launch_bounds__(256) void embed_lookup_kernel(const void* __restrict__ ids, int id64, int64_t N, int V,
+                                                           const T* __restrict__ E, int64_t lde, int D, int lpr,
+                                                           double scale, T* __restrict__ out) {
+  typedef Vec<T, VB> X;
+  typedef typename SumType<T>::type A;
+  const int64_t n = (int64_t)blockIdx.x * (256 / lpr) + threadIdx.x / lpr;
+  if (n >= N) return;
+  const int64_t id = load_id(ids, id64, n);
+  const int cpr = D / X::n;
+  const A s = (A)scale;
+  X* dst = reinterpret_cast<X*>(out + n * D);
+  if (id < 0 || id >= V) {
+    X x;
+#pragma unroll
+    for (int i = 0; i < X::n; ++i) x.v[i] = (T)(id < 0 ? (A)0 : (A)__builtin_nanf(""));
+    for (int c = threadIdx.x % lpr; c < cpr; c += lpr) dst[c] = x;
+    return;
+  }
+  const X* src = reinterpret_cast<const X*>(E + id * lde);
+  for (int c = threadIdx.x % lpr; c < cpr; c += lpr) {
+    X x = src[c];
+#pragma unroll
+    for (int i = 0; i < X::n; ++i) x.v[i] = (T)((A)x.v[i] * s);
+    dst[c] = x;
+  }
+}
+
+// ---------------------------------------------------------------- sorting
+// Stable order of the tokens by id in one launch: a workgroup owns kSortRows consecutive ids and scans
+// every token for them, counting on the way the tokens of smaller ids, which is where its own begin; so no
+// workgroup waits for another, and there is no pass per digit.  Its 16 waves take equal runs of the tokens in
+// order.  Pass 1 counts per (wave, id) and keeps the hits (up to kSortHits a wave); a scan over ids and waves
+// turns the counts into positions; pass 2 places the hits, 64 at a time, a hit's rank among the equal ids of
+// its 64 by eight ballots (one per bit of the row), so the order does not depend on any atomic's.  A wave
+// with more hits than it kept scans its run again.
+// The scans read M ids per 256 rows, from L2: 16384 tokens on 151936 ids, 78 MB.
+constexpr int kSortRows = 256, kSortWaves = 16, kSortHits = 256, kSortUnroll = 8;
+
+template <class ID>
+__global__ __launch_bounds__(64 * kSortWaves) void sort_ids_kernel(const ID* __restrict__ ids, int M, int V,
+                                                                   int* __restrict__ order, int* __restrict__ sid,
+                                                                   int* __restrict__ seg) {
+  __shared__ int cnt[kSortWaves][kSortRows];
+  __shared__ int hit_i[kSortWaves][kSortHits];
+  __shared__ unsigned char hit_r[kSortWaves][kSortHits];
+  __shared__ int wless[kSortWaves], wtot[kSortRows / 64];
+  const int t = threadIdx.x, lane = lane_id(), w = wave_id();
+  const int v0 = blockIdx.x * kSortRows, rows = min(kSortRows, V - v0);
+  const uint64_t below = (1ull << lane) - 1;
+  for (int i = t; i < kSortWaves * kSortRows; i += 64 * kSortWaves) (&cnt[0][0])[i] = 0;
+  __syncthreads();
+  const int per = (int)(((int64_t)M + 64 * kSortWaves - 1) / (64 * kSortWaves)) * 64;
+  const int64_t i0 = (int64_t)w * per, i1 = i0 + per < M ? i0 + per : M;
+  int less = 0, hits = 0;
+  for (int64_t base = i0; base < i1; base += 64 * kSortUnroll) {
+    ID x[kSortUnroll];
+#pragma unroll
+    for (int u = 0; u < kSortUnroll; ++u) {
+      const int64_t i = base + u * 64 + lane;
+      x[u] = i < i1 ? ids[i] : (ID)-1;
+    }
+#pragma unroll
+    for (int u = 0; u < kSortUnroll; ++u) {
+      less += x[u] >= 0 && x[u] < v0;
+      const bool in = x[u] >= v0 && x[u] < v0 + rows;
+      const uint64_t m = __ballot(in);
+      if (m == 0) continue;
+      if (in) {
+        const int r = (int)(x[u] - v0), at = hits + __popcll(m & below);
+        atomicAdd(&cnt[w][r], 1);
+        if (at < kSortHits) {
+          hit_i[w][at] = (int)(base + u * 64 + lane);
+          hit_r[w][at] = (unsigned char)r;
+        }
+      }
+      hits += __popcll(m);
+    }
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) less += __shfl_xor(less, o);
+  if (lane == 0) wless[w] = less;
+  __syncthreads();
+  int first = 0;
+#pragma unroll
+  for (int j = 0; j < kSortWaves; ++j) first += wless[j];
+  int tot = 0, x = 0;
+  if (t < kSortRows) {
+#pragma unroll
+    for (int j = 0; j < kSortWaves; ++j) tot += cnt[j][t];
+    x = tot;  // inclusive scan over the wave's 64 rows
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int y = __shfl_up(x, o);
+      if (lane >= o) x += y;
+    }
+    if (lane == 63) wtot[w] = x;
+  }
+  __syncthreads();
+  if (t < kSortRows) {
+    int s = first + x - tot;
+    for (int j = 0; j < w; ++j) s += wtot[j];
+    if (t < rows) seg[v0 + t] = s;
+    if (t == rows - 1 && v0 + rows == V) seg[V] = s + tot;
+#pragma unroll
+    for (int j = 0; j < kSortWaves; ++j) {
+      const int c = cnt[j][t];
+      cnt[j][t] = s;
+      s += c;
+    }
+  }
+  __syncthreads();
+  volatile int* const next = cnt[w];
+  auto place = [&](int i, int r, bool in) {
+    uint64_t same = __ballot(in);
+#pragma unroll
+    for (int b = 0; b < 8; ++b) {
+      const uint64_t m = __ballot(in && ((r >> b) & 1));
+      same &= ((r >> b) & 1) ? m : ~m;
+    }
+    if (in) {
+      const int rank = __popcll(same & below), at = next[r] + rank;
+      order[at] = i;
+      sid[at] = v0 + r;
+      if (rank == 0) next[r] = at + __popcll(same);
+    }
+  };
+  if (hits <= kSortHits) {
+    for (int j = 0; j < hits; j += 64) {
+      const bool in = j + lane < hits;
+      place(in ? hit_i[w][j + lane] : 0, in ? hit_r[w][j + lane] : 0, in);
+    }
+  } else {
+    for (int64_t base = i0; base < i1; base += 64) {
+      const int64_t i = base + lane;
+      const ID id = i < i1 ? ids[i] : (ID)-1;
+      const bool in = id >= v0 && id < v0 + rows;
+      if (__ballot(in)) place((int)i, in ? (int)(id - v0) : 0, in);
+    }
+  }
+}
+
+// ---------------------------------------------------------------- gradient
+// Row of gE from an fp32 (fp64) sum.
+template <class T, int VB, class A>
+__device__ __forceinline__ void store_row(T* row, int c, const A (&acc)[Vec<T, VB>::n], A scale) {
+  Vec<T, VB> x;
+#pragma unroll
+  for (int i = 0; i < Vec<T, VB>::n; ++i) x.v[i] = (T)(acc[i] * scale);
+  reinterpret_cast<Vec<T, VB>*>(row)[c] = x;
+}
+
+struct EmbedGradKernelParams {
+  const void* g;
+  int64_t ldg;
+  const int* order;
+  const int* sid;
+  const int* seg;   // [V + 1]
+  int V, D, run;    // run: sorted tokens per run
+  int lpr, n_ct;    // lanes per run in a workgroup, vector tiles of lpr vectors
+  int n_sum;        // workgroups of the sums; the others write the rows without a token
+  int dpad;         // columns of a part
+  void* part;       // [runs][2][dpad]: slot 0, the segment that enters the run; slot 1, the one that leaves it
+  double scale;
+  void* gE;
+};
+
+// Rows without a token that one wave of the zero workgroups looks after.
+constexpr int kZeroRows = 16;
+
+template <class T, int VB>
+__global__ __launch_bounds__(256) void embed_sum_kernel(EmbedGradKernelParams p) {
+  typedef Vec<T, VB> X;
+  typedef typename SumType<T>::type A;
+  const int cpr = p.D / X::n;
+  T* const gE = static_cast<T*>(p.gE);
+  if ((int)blockIdx.x >= p.n_sum) {
+    const int v0 = (((int)blockIdx.x - p.n_sum) * 4 + wave_id()) * kZeroRows;
+    X z;
+#pragma unroll
+    for (int i = 0; i < X::n; ++i) z.v[i] = (T)0.f;
+    const int lane = lane_id();
+    // the rows' borders once, one lane each
+    const int b = v0 + lane <= p.V && lane <= kZeroRows ? p.seg[v0 + lane] : 0;
+    const int rows = min(kZeroRows, p.V - v0), end = __shfl_down(b, 1);  // (every lane takes part)
+    const uint32_t empty = (uint32_t)__ballot(lane < rows && b == end);
+    if (cpr >= 64) {
+      for (int r = 0; r < rows; ++r) {
+        if (!((empty >> r) & 1)) continue;
+        X* row = reinterpret_cast<X*>(gE + (int64_t)(v0 + r) * p.D);
+        for (int c = lane; c < cpr; c += 64) row[c] = z;
+      }
+    } else {
+      X* row0 = reinterpret_cast<X*>(gE + (int64_t)v0 * p.D);
+      for (int c = lane; c < rows * cpr; c += 64)
+        if ((empty >> ((uint32_t)c / (uint32_t)cpr)) & 1) row0[c] = z;
+    }
+    return;
+  }
+  const int rpb = 256 / p.lpr;
+  const int64_t run = (int64_t)((int)blockIdx.x / p.n_ct) * rpb + threadIdx.x / p.lpr;
+  const int c = ((int)blockIdx.x % p.n_ct) * p.lpr + threadIdx.x % p.lpr;
+  const int M = p.seg[p.V];
+  const int64_t p0 = run * p.run;
+  if (p0 >= M || c >= cpr) return;
+  const int64_t p1 = p0 + p.run < M ? p0 + p.run : M;
+  const T* const g = static_cast<const T*>(p.g);
+  int cur = p.sid[p0];
+  bool entered = p0 > 0 && p.sid[p0 - 1] == cur;
+  const bool leaves = p1 < M && p.sid[p1] == p.sid[p1 - 1];
+  A acc[X::n];
+#pragma unroll
+  for (int i = 0; i < X::n; ++i) acc[i] = 0;
+  auto part = [&](int slot) {
+    A* dst = static_cast<A*>(p.part) + (run * 2 + slot) * p.dpad + (int64_t)c * X::n;
+#pragma unroll
+    for (int i = 0; i < X::n; ++i) dst[i] = acc[i];
+  };
+  constexpr int U = 8;
+  for (int64_t q = p0; q < p1; q += U) {
+    X x[U];
+    int id[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t at = q + u < p1 ? q + u : p1 - 1;
+      id[u] = p.sid[at];
+      x[u] = reinterpret_cast<const X*>(g + (int64_t)p.order[at] * p.ldg)[c];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (q + u >= p1) break;
+      if (id[u] != cur) {
+        if (entered)
+          part(0);
+        else
+          store_row<T, VB, A>(gE + (int64_t)cur * p.D, c, acc, (A)p.scale);
+#pragma unroll
+        for (int i = 0; i < X::n; ++i) acc[i] = 0;
+        cur = id[u];
+        entered = false;
+      }
+#pragma unroll
+      for (int i = 0; i < X::n; ++i) acc[i] += (A)x[u].v[i];
+    }
+  }
+  if (entered)
+    part(0);
+  else if (leaves)
+    part(1);
+  else
+    store_row<T, VB, A>(gE + (int64_t)cur * p.D, c, acc, (A)p.scale);
+}
+
+// Parts of segments that cross runs, joined in run order.  A wave takes the run in which such a segment
+// begins, 64 columns; a workgroup's 4 waves share a segment of more than kJoinAlone parts (an id that fills a
+// large share of the tokens), a quarter of its parts each.
+constexpr int kJoinAlone = 32;
+template <class T>
+__global__ __launch_bounds__(256) void embed_join_kernel(EmbedGradKernelParams p, int n_ct) {
+  typedef typename SumType<T>::type A;
+  __shared__ int s_last[4];
+  __shared__ A s_sum[4][64];
+  const int lane = lane_id(), w = wave_id();
+  const int64_t j0 = (int64_t)((int)blockIdx.x / n_ct) * 4;
+  const int d = ((int)blockIdx.x % n_ct) * 64 + lane;
+  const int M = p.seg[p.V];
+  const A* const part = static_cast<const A*>(p.part);
+  T* const gE = static_cast<T*>(p.gE);
+  // the sum of the parts of runs a .. b of the segment that begins in run j
+  auto sum = [&](int64_t j, int64_t a, int64_t b) {
+    A acc = 0;
+    for (int64_t q0 = a; q0 <= b; q0 += 16) {
+      A x[16];
+#pragma unroll
+      for (int u = 0; u < 16; ++u) {
+        const int64_t q = q0 + u <= b ? q0 + u : b;
+        x[u] = part[(q * 2 + (q == j)) * p.dpad + d];
+      }
+#pragma unroll
+      for (int u = 0; u < 16; ++u)
+        if (q0 + u <= b) acc += x[u];
+    }
+    return acc;
+  };
+  // the last run of the segment that begins in run j and crosses its end, or -1
+  auto last_run = [&](int64_t j, int* v) -> int {
+    const int64_t p0 = j * p.run, p1 = p0 + p.run;
+    if (p1 >= M) return -1;
+    *v = p.sid[p1 - 1];
+    return p.sid[p1] == *v && p.seg[*v] >= p0 ? (p.seg[*v + 1] - 1) / p.run : -1;
+  };
+  int v = 0;
+  const int last = last_run(j0 + w, &v);
+  if (last >= 0 && last - (j0 + w) < kJoinAlone) {
+    if (d < p.D) gE[(int64_t)v * p.D + d] = (T)(sum(j0 + w, j0 + w, last) * (A)p.scale);
+  }
+  if (lane == 0) s_last[w] = last;
+  __syncthreads();
+  for (int i = 0; i < 4; ++i) {
+    const int64_t j = j0 + i;
+    const int b = s_last[i];
+    if (b < 0 || b - j < kJoinAlone) continue;  // the same for the whole workgroup
+    const int64_t n = b - j + 1, a0 = j + n * w / 4, a1 = j + n * (w + 1) / 4 - 1;
+    __syncthreads();  // the sums of the segment before have been read
+    s_sum[w][lane] = d < p.D ? sum(j, a0, a1) : (A)0;
+    __syncthreads();
+    if (w == 0 && d < p.D) {
+      const int id = p.sid[(j + 1) * p.run];
+      gE[(int64_t)id * p.D + d] = (T)((((s_sum[0][lane] + s_sum[1][lane]) + s_sum[2][lane]) + s_sum[3][lane]) *
+                                      (A)p.scale);
+    }
+  }
+}
+
+size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
+
+int elem_bytes(int dtype) { return dtype == kF64 ? 8 : dtype == kF32 ? 4 : 2; }
+
+// Largest vector (16, 8, 4, ... bytes) that divides every row and base.
+int vec_bytes(int eb, int64_t D, int64_t ld, const void* a, const void* b) {
+  int vb = 16;
+  const uintptr_t x = (uintptr_t)(D * eb) | (uintptr_t)(ld * eb) | (uintptr_t)a | (uintptr_t)b;
+  while (vb > eb && (x & (vb - 1))) vb /= 2;
+  return vb;
+}
+
+// Lanes per row: the most (up to 256, a wave at least for rows of 64 vectors) that leave under a tenth idle,
+// or the fewest idle.
+int lanes_per_row(int cpr) {
+  int best = 8, waste = 1 << 30;
+  for (int l = 256; l >= 8; l /= 2) {
+    const int idle = (cpr + l - 1) / l * l - cpr;
+    if (idle * 10 <= cpr) return l;
+    if (idle < waste) {
+      waste = idle;
+      best = l;
+    }
+  }
+  return best;
+}
+
+// f(element type, vector bytes) for a dtype tag and vector width.
+template <class F>
+hipError_t dispatch(int dtype, int vb, F&& f) {
+  auto by_vb = [&](auto t) -> hipError_t {
+    typedef decltype(t) T;
+    if (vb == 16) return f(t, std::integral_constant<int, 16>());
+    if (vb == 8) return f(t, std::integral_constant<int, 8>());
+    if constexpr (sizeof(T) <= 4)
+      if (vb == 4) return f(t, std::integral_constant<int, 4>());
+    if constexpr (sizeof(T) == 2)
+      if (vb == 2) return f(t, std::integral_constant<int, 2>());
+    return hipErrorInvalidValue;
+  };
+  switch (dtype) {
+    case kBF16: return by_vb((bf16_t)0.f);
+    case kF16: return by_vb((f16_t)0.f);
+    case kF32: return by_vb(0.f);
+    case kF64: return by_vb(0.0);
+    default: return hipErrorInvalidValue;
+  }
+}
+
+// Sorted tokens per run: 32, and 8 for the few tokens that would not fill the chip so.
+int run_of(int64_t M) { return M >= 4096 ? 32 : 8; }
+
+}  // namespace
+
+hipError_t embed_lookup_launch(const EmbedParams& p, hipStream_t stream) {
+  if (p.N == 0 || p.D == 0) return hipSuccess;
+  const int eb = elem_bytes(p.dtype), vb = vec_bytes(eb, p.D, p.lde, p.E, p.out);
+  return dispatch(p.dtype, vb, [&](auto t, auto w) -> hipError_t {
+    typedef decltype(t) T;
+    constexpr int VB = decltype(w)::value;
+    const int lpr = lanes_per_row(p.D / (VB / (int)sizeof(T))), rpb = 256 / lpr;
+    timing_begin(kKindEmbed, stream);
+    embed_lookup_kernel<T, VB><<<(unsigned)((p.N + rpb - 1) / rpb), 256, 0, stream>>>(
+        p.ids, p.id64, p.N, p.V, static_cast<const T*>(p.E), p.lde, p.D, lpr, p.scale, static_cast<T*>(p.out));
+    timing_end(kKindEmbed, stream);
+    return hipGetLastError();
+  });
+}
+
+hipError_t sort_ids(const void* ids, int id64, int M, int V, int* order, int* sid, int* seg, hipStream_t stream) {
+  if (V == 0) return hipSuccess;
+  const unsigned blocks = (unsigned)(((int64_t)V + kSortRows - 1) / kSortRows);
+  timing_begin(kKindSortIds, stream);
+  if (id64)
+    sort_ids_kernel<int64_t><<<blocks, 64 * kSortWaves, 0, stream>>>(static_cast<const int64_t*>(ids), M, V, order,
+                                                                      sid, seg);
+  else
+    sort_ids_kernel<int><<<blocks, 64 * kSortWaves, 0, stream>>>(static_cast<const int*>(ids), M, V, order, sid, seg);
+  timing_end(kKindSortIds, stream);
+  return hipGetLastError();
+}
+
+size_t embed_grad_workspace_bytes(int dtype, int64_t N, int64_t V, int64_t D) {
+  const int64_t run = run_of(N), runs = (N + run - 1) / run, dpad = (D + 7) / 8 * 8;
+  return 2 * align256((size_t)N * 4) + align256((size_t)(V + 1) * 4) +
+         align256((size_t)runs * 2 * dpad * (dtype == kF64 ? 8 : 4));
+}
+
+hipError_t embed_grad_launch(const EmbedParams& p, char* ws, hipStream_t stream) {
+  if (p.V == 0 || p.D == 0) return hipSuccess;
+  int* order = reinterpret_cast<int*>(ws);
+  int* sid = reinterpret_cast<int*>(ws += align256((size_t)p.N * 4));
+  int* seg = reinterpret_cast<int*>(ws += align256((size_t)p.N * 4));
+  ws += align256((size_t)(p.V + 1) * 4);
+  hipError_t e = sort_ids(p.ids, p.id64, (int)p.N, p.V, order, sid, seg, stream);
+  if (e != hipSuccess) return e;
+  const int eb = elem_bytes(p.dtype), vb = vec_bytes(eb, p.D, p.ldg, p.g, p.gE);
+  EmbedGradKernelParams k{};
+  k.g = p.g;
+  k.ldg = p.ldg;
+  k.order = order;
+  k.sid = sid;
+  k.seg = seg;
+  k.V = p.V;
+  k.D = p.D;
+  k.run = run_of(p.N);
+  k.dpad = (p.D + 7) / 8 * 8;
+  k.part = ws;
+  k.scale = p.scale;
+  k.gE = p.gE;
+  const int64_t runs = (p.N + k.run - 1) / k.run;
+  e = dispatch(p.dtype, vb, [&](auto t, auto w) -> hipError_t {
+    typedef decltype(t) T;
+    constexpr int VB = decltype(w)::value;
+    const int cpr = p.D / (VB / (int)sizeof(T));
+    const int l = lanes_per_row(cpr);
+    k.lpr = l;
+    k.n_ct = (cpr + l - 1) / l;
+    const int64_t sums = (runs + 256 / l - 1) / (256 / l) * k.n_ct;
+    const int64_t zeros = ((int64_t)p.V + 4 * kZeroRows - 1) / (4 * kZeroRows);
+    if (sums + zeros > INT32_MAX) return hipErrorInvalidValue;
+    k.n_sum = (int)sums;
+    timing_begin(kKindEmbed, stream);
+    embed_sum_kernel<T, VB><<<(unsigned)(sums + zeros), 256, 0, stream>>>(k);
+    timing_end(kKindEmbed, stream);
+    return hipGetLastError();
+  });
+  if (e != hipSuccess || runs < 2) return e;
+  const int n_ct = (p.D + 63) / 64;
+  const int64_t blocks = (runs + 3) / 4 * n_ct;
+  if (blocks > INT32_MAX) return hipErrorInvalidValue;
+  timing_begin(kKindEmbed, stream);
+  switch (p.dtype) {
+    case kBF16: embed_join_kernel<bf16_t><<<(unsigned)blocks, 256, 0, stream>>>(k, n_ct); break;
+    case kF16: embed_join_kernel<f16_t><<<(unsigned)blocks, 256, 0, stream>>>(k, n_ct); break;
+    case kF32: embed_join_kernel<float><<<(unsigned)blocks, 256, 0, stream>>>(k, n_ct); break;
+    default: embed_join_kernel<double><<<(unsigned)blocks, 256, 0, stream>>>(k, n_ct); break;
+  }
+  timing_end(kKindEmbed, stream);
+  return hipGetLastError();
+}
+
+}  // namespace swvr

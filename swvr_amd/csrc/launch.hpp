@@ -21,6 +21,10 @@ enum KernelKind {
   kKindQuant,
   kKindF64,
   kKindProbe,
+  kKindEmbed,
+  kKindSortIds,
+  kKindDistill,
+  kKindSample,
   kNumKinds
 };
 
@@ -303,6 +307,12 @@ struct BwdParams {
   const float* h_scale;
   const float* w_scale;
   int K8;
+  // elements of dS given by the caller (null pt_id: none): entry e of token e / pt_T has its value at vocabulary
+  // row pt_id[e] (-1: none; a row at most once per token)
+  const int* pt_id;
+  const float* pt_val;
+  int64_t n_pt;
+  int pt_T;
 };
 
 hipError_t bwd_launch(int dtype, const BwdPlan& plan, const BwdParams& p, hipStream_t stream);
@@ -372,6 +382,102 @@ struct F64Params {
 void f64_plan(int64_t N, int64_t V, int64_t D, int64_t chunk, int64_t* C, size_t* fwd_bytes, size_t* bwd_bytes);
 hipError_t f64_fwd(const F64Params& p, hipStream_t stream);
 hipError_t f64_bwd(const F64Params& p, hipStream_t stream);
+
+// ---------------------------------------------------------------- embedding lookup
+struct EmbedParams {
+  int dtype;           // of E, out, g and gE: 0 bf16, 1 f16, 2 f32, 4 f64
+  const void* ids;     // [N] int64 (id64) or int32
+  int id64;
+  int64_t N;
+  int V, D;
+  const void* E;       // lookup: [V][lde]
+  int64_t lde;
+  double scale;
+  void* out;           // lookup: [N][D]
+  const void* g;       // gradient: [N][ldg]
+  int64_t ldg;
+  void* gE;            // gradient: [V][D]
+};
+hipError_t embed_lookup_launch(const EmbedParams& p, hipStream_t stream);
+size_t embed_grad_workspace_bytes(int dtype, int64_t N, int64_t V, int64_t D);
+hipError_t embed_grad_launch(const EmbedParams& p, char* ws, hipStream_t stream);
+// Positions 0 .. M - 1 in stable order of their id (those with an id in 0 .. V - 1): order, their ids (sid) and
+// each id's segment, seg[v] .. seg[v + 1].
+hipError_t sort_ids(const void* ids, int id64, int M, int V, int* order, int* sid, int* seg, hipStream_t stream);
+
+// ---------------------------------------------------------------- distillation
+struct DistillParams {
+  const void* h;
+  int64_t ldh;
+  const void* W;
+  int64_t ldw;
+  int h_f32, w_f32;      // stored in fp32 under a 2-byte compute dtype
+  const float* bias;     // [V], divided by tau, or null
+  float scale;           // logit_scale / tau
+  float inv_tau;
+  int N, K, V, T;
+  const void* ids;       // [N][ldi] int64 (id64) or int32
+  int id64;
+  int64_t ldi;
+  const void* teacher;   // [N][ldt], t_dtype
+  int t_dtype;
+  int64_t ldt;
+  const float* weight;   // [N] or null
+  const float* lse;      // [N]
+  float zw;              // z-loss weight
+  int reduce;            // 0 none, 1 sum, 2 mean
+  float* z;              // [N][T] workspace
+  float* out;            // [N] (reduce == 0) or [1]
+  float* p;              // [N][T] teacher probabilities, or null (no gradient will be asked for)
+  float* q;              // [N][T] student probabilities at the ids (with p)
+  float* coef;           // [N] weights of the tokens that count (with p)
+};
+size_t distill_part_bytes(int64_t N);
+hipError_t distill_scale(const float* x, int64_t n, float s, float* y, hipStream_t stream);
+// The loss from the log-sum-exps; c: [1], the reduction's factor (reduce != 0).
+hipError_t distill_loss(int dtype, const DistillParams& p, float* part, float* c, hipStream_t stream);
+struct DistillGradParams {
+  int N, V, T;
+  const void* ids;
+  int id64;
+  int64_t ldi;
+  const float* g;        // [N] (reduce == 0) or [1]
+  int reduce;
+  const float* c;        // [1]
+  const float* lse;
+  const float* p;
+  const float* q;
+  const float* coef;
+  float zw;
+  float* glse;           // [N]
+  int* pt_id;            // [N][T]
+  float* pt_val;         // [N][T]
+  float* pt_t;           // [N][T] or null
+};
+hipError_t distill_prep(const DistillGradParams& p, hipStream_t stream);
+hipError_t distill_bias(const int* order, const int* seg, const float* t, int V, float inv_tau, float* gb,
+                        hipStream_t stream);
+
+// ---------------------------------------------------------------- sampling
+struct SampleParams {
+  int64_t R;             // rows
+  int64_t V;
+  const void* logits;    // [R][ld]
+  int64_t ld;
+  const void* u;         // [R] fp64 (u64) or fp32
+  int u64;
+  // a setting for all rows, or [R] one for each
+  double tau, p, min_p;
+  int64_t k;
+  const float* tau_rows;
+  const int* k_rows;
+  const float* p_rows;
+  const float* min_p_rows;
+  double one;            // 2^shift of the weights (set by the launcher)
+  int64_t* token;        // [R]
+  float* logprob;        // [R]
+};
+hipError_t sample_launch(int dtype, SampleParams p, hipStream_t stream);
 
 // Matrix-core throughput probe (probe.hip): workgroups of 8 waves, iters k16 steps of
 // 8 MFMAs per wave; out receives workgroups * 512 floats.

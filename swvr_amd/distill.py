@@ -1,0 +1,251 @@
+"""Distillation of the head from a teacher's top logits, without the [tokens, V] scores.
+
+Where ``softmax_readout_mse`` trains the readout O against target vectors, ``softmax_distill`` trains the
+distribution itself against the part of a teacher's that is kept: its largest logits and their ids, the way
+teacher outputs are stored.  One entry per token is cross entropy.  The log-normaliser and the dense part of
+the gradients run on the readout's kernels (no embedding), the teacher's entries on their own (C ABI:
+swvr_distill, swvr_distill_bwd).
+"""
+from typing import List, Optional, Tuple
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from ._ops import (DEFAULT_CHUNK, REDUCTIONS, _f32, _grad_buffer, _kpad, _lead_stride, _needs_grad, _operand, _plain,
+                   _require_device, _rows_staged, eager)
+from .api import _chunk, _compute_dtype
+
+MAX_TEACHER = 1024
+
+
+def _lists(x, keep, other):
+    """Teacher logits or ids as [N, T] with unit inner stride, in one of the dtypes ``keep`` or as ``other``."""
+    x = _plain(x)
+    x = x if x.dtype in keep else x.to(other)
+    return x if x.stride(1) == 1 and x.stride(0) >= 0 else x.contiguous()
+
+
+def _forward(h, W, bias, teacher, ids, weight, tau, z, reduction, scale, cdt, need_grad):
+    """The loss, and for the gradient (empty tensors without) c, lse, p, q, coef of swvr_distill."""
+    lib = _lib.load()
+    N, K = h.shape
+    V, T = W.shape[0], ids.shape[1]
+    Kp = _kpad(K)
+    (hc, h_tag), (Wc, w_tag) = _operand(h, cdt, Kp), _operand(W, cdt, Kp)
+    b, w = _f32(bias), _f32(weight)
+    t = _lists(teacher, _lib.DTYPE_TAG, torch.float32)
+    i = _lists(ids, (torch.int64, torch.int32), torch.int64)
+    tag = _lib.DTYPE_TAG[cdt]
+
+    def new(*shape):
+        return torch.empty(shape, dtype=torch.float32, device=h.device)
+
+    out, c, lse = new(*((N,) if reduction == 0 else ())), new(), new(N)
+    p, q, coef = (new(N, T), new(N, T), new(N)) if need_grad else (new(0), new(0), new(0))
+    ws_bytes = lib.swvr_distill_workspace_size(tag, N, Kp, V, T, int(w is not None))
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=h.device)
+    a = _lib.address
+    _lib.call(lib.swvr_distill, h.device, tag, h_tag, w_tag, N, Kp, V, T, hc.data_ptr(), _lead_stride(hc),
+              Wc.data_ptr(), _lead_stride(Wc), a(b), scale, i.data_ptr(), i.dtype == torch.int64, i.stride(0),
+              t.data_ptr(), _lib.DTYPE_TAG[t.dtype], t.stride(0), tau, a(w), z, reduction, out.data_ptr(), c.data_ptr(),
+              lse.data_ptr(), *(map(a, (p, q, coef)) if need_grad else (None,) * 3), ws.data_ptr(), ws_bytes)
+    return out, c, lse, p, q, coef
+
+
+def _backward(g, h, W, bias, ids, c, lse, p, q, coef, tau, z, reduction, scale, chunk, cdt, need_h, need_W, need_b):
+    lib = _lib.load()
+    N, K = h.shape
+    V, T = W.shape[0], ids.shape[1]
+    Kp = _kpad(K)
+    (hc, h_tag), (Wc, w_tag) = _operand(h, cdt, Kp), _operand(W, cdt, Kp)
+    b, g32 = _f32(bias), _f32(g)
+    i = _lists(ids, (torch.int64, torch.int32), torch.int64)
+    dev = h.device
+    gh = _grad_buffer((N, Kp), h.dtype, dev) if need_h else None
+    gW = _grad_buffer((V, Kp), W.dtype, dev) if need_W else None
+    gb = torch.empty(V, dtype=torch.float32, device=dev) if need_b else None
+    tag = _lib.DTYPE_TAG[cdt]
+    chunk = _rows_staged(chunk, tag, w_tag, N, Kp, V, 0, need_h)
+    ws_bytes = lib.swvr_distill_bwd_workspace_size(tag, w_tag, N, Kp, V, T, chunk, int(need_h))
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+
+    def tag_of(x):
+        return _lib.DTYPE_TAG[x.dtype] if x is not None else 0
+
+    a = _lib.address
+    _lib.call(lib.swvr_distill_bwd, dev, tag, h_tag, w_tag, N, Kp, V, T, hc.data_ptr(), _lead_stride(hc),
+              Wc.data_ptr(), _lead_stride(Wc), a(b), scale, i.data_ptr(), i.dtype == torch.int64, i.stride(0), tau, z,
+              reduction, g32.data_ptr(), c.data_ptr(), lse.data_ptr(), p.data_ptr(), q.data_ptr(), coef.data_ptr(),
+              chunk, a(gh), tag_of(gh), a(gW), tag_of(gW), a(gb), ws.data_ptr(), ws_bytes)
+    if gh is not None:
+        gh = gh[:, :K] if Kp != K else gh
+        gh = gh.to(h.dtype) if gh.dtype != h.dtype else gh
+    if gW is not None:
+        gW = gW[:, :K].contiguous() if Kp != K else gW
+        gW = gW.to(W.dtype) if gW.dtype != W.dtype else gW
+    if gb is not None and gb.dtype != bias.dtype:
+        gb = gb.to(bias.dtype)
+    return gh, gW, gb
+
+
+@torch.library.custom_op("swvr::distill", mutates_args=())
+def _fwd_op(h: torch.Tensor, W: torch.Tensor, bias: Optional[torch.Tensor], teacher: torch.Tensor, ids: torch.Tensor,
+            weight: Optional[torch.Tensor], tau: float, z: float, reduction: int, scale: float, chunk: int,
+            cdt: torch.dtype, need_grad: bool) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor,
+                                                        torch.Tensor, torch.Tensor]:
+    return _forward(h, W, bias, teacher, ids, weight, tau, z, reduction, scale, cdt, need_grad)
+
+
+@_fwd_op.register_fake
+def _(h, W, bias, teacher, ids, weight, tau, z, reduction, scale, chunk, cdt, need_grad):
+    N, T = ids.shape
+
+    def new(*shape):
+        return h.new_empty(shape, dtype=torch.float32)
+
+    kept = (new(N, T), new(N, T), new(N)) if need_grad else (new(0), new(0), new(0))
+    return (new(*((N,) if reduction == 0 else ())), new(), new(N), *kept)
+
+
+@torch.library.custom_op("swvr::distill_bwd", mutates_args=())
+def _bwd_op(g: torch.Tensor, h: torch.Tensor, W: torch.Tensor, bias: Optional[torch.Tensor], ids: torch.Tensor,
+            c: torch.Tensor, lse: torch.Tensor, p: torch.Tensor, q: torch.Tensor, coef: torch.Tensor, tau: float,
+            z: float, reduction: int, scale: float, chunk: int, cdt: torch.dtype, need_h: bool, need_W: bool,
+            need_b: bool) -> List[torch.Tensor]:
+    grads = _backward(g, h, W, bias, ids, c, lse, p, q, coef, tau, z, reduction, scale, chunk, cdt, need_h, need_W,
+                      need_b)
+    # a custom op cannot return None: an empty tensor stands for "no gradient"
+    return [x if x is not None else h.new_empty(0) for x in grads]
+
+
+@_bwd_op.register_fake
+def _(g, h, W, bias, ids, c, lse, p, q, coef, tau, z, reduction, scale, chunk, cdt, need_h, need_W, need_b):
+    return [torch.empty_like(x) if need else h.new_empty(0) for need, x in ((need_h, h), (need_W, W), (need_b, bias))]
+
+
+def _setup_context(ctx, inputs, output):
+    h, W, bias, _, ids, _, tau, z, reduction, scale, chunk, cdt, _ = inputs
+    _, c, lse, p, q, coef = output
+    ctx.mark_non_differentiable(c, lse, p, q, coef)
+    ctx.save_for_backward(h, W, bias, ids, c, lse, p, q, coef)
+    ctx.args = (tau, z, reduction, scale, chunk, cdt)
+
+
+def _needs(ctx, bias):
+    need_h, need_W, need_b = (bool(x) for x in ctx.needs_input_grad[:3])
+    return need_h, need_W, need_b and bias is not None
+
+
+def _op_grads(g, saved, args, needs):
+    *args, chunk, cdt = args
+    grads = _bwd_op(g, *saved, *args, chunk or DEFAULT_CHUNK, cdt, *needs)
+    return [x if need else None for x, need in zip(grads, needs)]
+
+
+def _autograd_backward(ctx, g, *_):
+    saved = ctx.saved_tensors
+    return (*_op_grads(g, saved, ctx.args, _needs(ctx, saved[2])), *[None] * 10)
+
+
+_fwd_op.register_autograd(_autograd_backward, setup_context=_setup_context)
+
+
+class _Distill(torch.autograd.Function):
+    """swvr::distill / distill_bwd as one node, returning the loss."""
+
+    @staticmethod
+    def forward(ctx, h, W, bias, teacher, ids, weight, tau, z, reduction, scale, chunk, cdt):
+        out, *kept = _forward(h, W, bias, teacher, ids, weight, tau, z, reduction, scale, cdt, True)
+        ctx.save_for_backward(h, W, bias, ids, *kept)
+        ctx.args = (tau, z, reduction, scale, chunk, cdt)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        saved = ctx.saved_tensors
+        needs = _needs(ctx, saved[2])
+        if eager(g, *saved):
+            grads = _backward(g, *saved, *ctx.args, *needs)
+        else:
+            grads = _op_grads(g, saved, ctx.args, needs)
+        return (*grads, *[None] * 9)
+
+
+def _check(h, W, teacher, ids, bias, weight, temperature, reduction):
+    if W.dim() != 2 or W.shape[0] < 1:
+        raise ValueError(f"W must be 2-D with at least one row, got {tuple(W.shape)}")
+    if h.dim() < 1 or h.shape[-1] != W.shape[1]:
+        raise ValueError(f"h has shape {tuple(h.shape)} but W is {tuple(W.shape)}")
+    if bias is not None and bias.shape != (W.shape[0],):
+        raise ValueError(f"bias must have shape ({W.shape[0]},), got {tuple(bias.shape)}")
+    lead = h.shape[:-1]
+    if ids.shape != teacher.shape or ids.dim() < 1 or ids.shape[:-1] != lead:
+        raise ValueError(f"teacher_logits and teacher_ids must both be {tuple(lead)} + (T,), got "
+                         f"{tuple(teacher.shape)} and {tuple(ids.shape)}")
+    if not 1 <= ids.shape[-1] <= MAX_TEACHER:
+        raise ValueError(f"a teacher's list holds 1 to {MAX_TEACHER} entries, got {ids.shape[-1]}")
+    if ids.dtype.is_floating_point or ids.dtype.is_complex or ids.dtype == torch.bool:
+        raise ValueError(f"teacher_ids must be integers, got {ids.dtype}")
+    if not teacher.dtype.is_floating_point:
+        raise ValueError(f"teacher_logits must be floating point, got {teacher.dtype}")
+    if weight is not None and weight.shape != lead:
+        raise ValueError(f"weight must have shape {tuple(lead)}, got {tuple(weight.shape)}")
+    for name, x in (("W", W), ("teacher_logits", teacher), ("teacher_ids", ids), ("bias", bias), ("weight", weight)):
+        if x is not None and x.device != h.device:
+            raise ValueError(f"{name} is on {x.device} but h on {h.device}")
+    for name, x in (("teacher_logits", teacher), ("weight", weight)):
+        if x is not None and x.requires_grad:
+            raise ValueError(f"{name} gets no gradient: detach it")
+    if not 0 < temperature < 3e38:
+        raise ValueError(f"temperature must be positive and finite, got {temperature}")
+    if reduction not in REDUCTIONS:
+        raise ValueError(f"unknown reduction {reduction!r}")
+
+
+def softmax_distill(h, W, teacher_logits, teacher_ids, bias=None, *, temperature=1.0, weight=None, reduction="mean",
+                    z_loss_weight=0.0, logit_scale=1.0, chunk_size=None):
+    """Divergence of the head's distribution from a teacher's top logits.
+
+    With student scores ``S = (logit_scale * h W^T + bias) / temperature`` over the V vocabulary rows (h ``[..., K]``,
+    W ``[V, K]``, optional bias ``[V]``), ``LSE = logsumexp(S)``, and the teacher's distribution
+    ``p = softmax(teacher_logits / temperature)`` over the T (1 to 1024) entries it gives for a token
+    (``teacher_logits`` and integer ``teacher_ids``, both ``[..., T]``), each token contributes
+    ``sum_k p_k (log p_k - S[id_k] + LSE)``, plus ``z_loss_weight * LSE^2``.  One entry per token is cross entropy.
+    An entry with a negative id or a logit of -inf is absent; ids may repeat.  A token without entries
+    contributes nothing, and an id of V or more makes its token's term NaN.
+
+    ``weight`` (``[...]``) multiplies each term; a zero drops the token, whatever its inputs hold.  ``reduction``:
+    "mean" (the weighted sum over the sum of the weights of the tokens that have an entry; 0 without any),
+    "sum" or "none" (the per-token terms).  The loss is fp32; there is no factor of ``temperature ** 2``.  The
+    products run in autocast's dtype or the promotion of h's and W's (bf16, fp16 or fp32), and the backward
+    recomputes the scores ``chunk_size`` vocabulary rows at a time, as ``softmax_readout`` does.  Autograd
+    reaches h, W and bias; the teacher and the weight get none.
+    """
+    _check(h, W, teacher_logits, teacher_ids, bias, weight, temperature, reduction)
+    chunk = _chunk(chunk_size)
+    cdt = _compute_dtype(h, W)
+    if cdt not in _lib.DTYPE_TAG:
+        raise NotImplementedError(f"swvr_amd: compute dtype {cdt} is not supported here (bf16, fp16, fp32)")
+    lead, T = h.shape[:-1], teacher_ids.shape[-1]
+    h2 = h.reshape(-1, h.shape[-1]) if h.dim() != 2 else h
+    t2, i2 = teacher_logits.reshape(-1, T), teacher_ids.reshape(-1, T)
+    w1 = weight.reshape(-1) if weight is not None else None
+    red = REDUCTIONS[reduction]
+    args = (float(temperature), float(z_loss_weight), red, float(logit_scale))
+    need = _needs_grad(h, W, bias)
+    if eager(h, W, teacher_logits, teacher_ids, bias, weight):
+        if need:
+            out = _Distill.apply(h2, W, bias, t2, i2, w1, *args, chunk, cdt)
+        else:
+            out = _forward(h2, W, bias, t2, i2, w1, *args, cdt, False)[0]
+    else:
+        if h.device.type == "cpu":
+            _require_device(h)
+        if h.device.type == "cuda":
+            with torch.autocast(h.device.type, enabled=False):
+                out = _fwd_op(h2, W, bias, t2, i2, w1, *args, chunk or DEFAULT_CHUNK, cdt, need)[0]
+        else:  # meta / fake tracing: no autocast state
+            out = _fwd_op(h2, W, bias, t2, i2, w1, *args, chunk or DEFAULT_CHUNK, cdt, need)[0]
+    return out.view(lead) if red == 0 else out
