@@ -369,10 +369,11 @@ int swvr_distill_bwd(int dtype, int h_dtype, int w_dtype, int64_t N, int64_t K, 
  * and logprob -inf.  A setting is one value, or with its _rows pointer one per row.  w is held
  * as a whole number of 2^-44 (V up to 2^18; a bit less per doubling of V), so sums are exact,
  * and a token of smaller weight than half of that is never drawn. */
+size_t swvr_sample_workspace_size(int64_t R, int64_t V);
 int swvr_sample(int dtype, int64_t R, int64_t V, const void* logits, int64_t ld, const void* u, int u64,
                 double temperature, const float* temperature_rows, int64_t top_k, const int* top_k_rows,
                 double top_p, const float* top_p_rows, double min_p, const float* min_p_rows,
-                int64_t* token, float* logprob, void* stream);
+                int64_t* token, float* logprob, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Matrix-core throughput probe (measurement only; no reference counterpart):
  * `workgroups` workgroups of 8 waves, each wave `iters` steps of a 4 x 2 grid

@@ -69,7 +69,8 @@ SIGNATURES = {
     "swvr_distill_bwd": (_i, [_i, _i, _i, _i64, _i64, _i64, _i64, _p, _i64, _p, _i64, _p, _f, _p, _i, _i64, _f, _f, _i,
                               _p, _p, _p, _p, _p, _p, _i64, _p, _i, _p, _i, _p, _p, _sz, _p]),
     "swvr_sample": (_i, [_i, _i64, _i64, _p, _i64, _p, _i, ctypes.c_double, _p, _i64, _p, ctypes.c_double, _p,
-                         ctypes.c_double, _p, _p, _p, _p]),
+                         ctypes.c_double, _p, _p, _p, _p, _sz, _p]),
+    "swvr_sample_workspace_size": (_sz, [_i64, _i64]),
     "swvr_probe_mfma": (_i, [_i64, _i64, _i, _p, _p]),
     "swvr_timing_enable": (_i, [_i]),
     "swvr_timing_collect": (_i, [ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_int64), _i]),

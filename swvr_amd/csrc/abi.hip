@@ -635,10 +635,15 @@ int swvr_distill_bwd(int dtype, int h_dtype, int w_dtype, int64_t N, int64_t K, 
 }
 
 // ---------------------------------------------------------------- sampling
+size_t swvr_sample_workspace_size(int64_t R, int64_t V) {
+  if (R < 0 || V < 1 || R > INT32_MAX || V > INT32_MAX) return 0;
+  return swvr::sample_workspace_bytes(R, V);
+}
+
 int swvr_sample(int dtype, int64_t R, int64_t V, const void* logits, int64_t ld, const void* u, int u64,
                 double temperature, const float* temperature_rows, int64_t top_k, const int* top_k_rows, double top_p,
                 const float* top_p_rows, double min_p, const float* min_p_rows, int64_t* token, float* logprob,
-                void* stream) {
+                void* workspace, size_t workspace_bytes, void* stream) {
   g_err[0] = 0;
   if (!is_dtype(dtype)) return fail(SWVR_EDTYPE, "unsupported logits dtype tag %d", dtype);
   if (R < 0 || V < 1 || R > INT32_MAX || V > INT32_MAX)
@@ -649,6 +654,9 @@ int swvr_sample(int dtype, int64_t R, int64_t V, const void* logits, int64_t ld,
     return fail(SWVR_EINVAL, "temperature must not be negative, got %g", temperature);
   if (R == 0) return SWVR_OK;
   if (!logits || !u || !token || !logprob) return fail(SWVR_EINVAL, "logits, u, token and logprob must be non-null");
+  const size_t need = swvr::sample_workspace_bytes(R, V);
+  if (workspace_bytes < need || (need > 0 && !workspace))
+    return fail(SWVR_EWORKSPACE, "sampling workspace of %zu bytes needed, %zu given", need, workspace_bytes);
   const uintptr_t eb = dtype == SWVR_F32 ? 4 : 2;
   if (reinterpret_cast<uintptr_t>(logits) % eb) return fail(SWVR_EINVAL, "logits must be aligned to their elements");
   swvr::SampleParams p{};
@@ -668,7 +676,7 @@ int swvr_sample(int dtype, int64_t R, int64_t V, const void* logits, int64_t ld,
   p.min_p_rows = min_p_rows;
   p.token = token;
   p.logprob = logprob;
-  hipError_t e = swvr::sample_launch(dtype, p, static_cast<hipStream_t>(stream));
+  hipError_t e = swvr::sample_launch(dtype, p, static_cast<char*>(workspace), static_cast<hipStream_t>(stream));
   if (e != hipSuccess) return hip_fail(e, "sampling launch");
   return SWVR_OK;
 }

@@ -477,7 +477,8 @@ struct SampleParams {
   int64_t* token;        // [R]
   float* logprob;        // [R]
 };
-hipError_t sample_launch(int dtype, SampleParams p, hipStream_t stream);
+size_t sample_workspace_bytes(int64_t R, int64_t V);
+hipError_t sample_launch(int dtype, SampleParams p, char* ws, hipStream_t stream);
 
 // Matrix-core throughput probe (probe.hip): workgroups of 8 waves, iters k16 steps of
 // 8 MFMAs per wave; out receives workgroups * 512 floats.

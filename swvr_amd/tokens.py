@@ -148,10 +148,12 @@ def _sample(logits, u, tau, k, p, min_p, tau_r, k_r, p_r, min_p_r):
     tau_r, k_r = _per_row(tau_r, torch.float32, R), _per_row(k_r, torch.int32, R)
     p_r, min_p_r = _per_row(p_r, torch.float32, R), _per_row(min_p_r, torch.float32, R)
     token, logprob = x.new_empty(u.shape, dtype=torch.int64), x.new_empty(u.shape, dtype=torch.float32)
-    a = _lib.address
-    _lib.call(_lib.load().swvr_sample, x.device, _lib.DTYPE_TAG[x.dtype], R, V, x.data_ptr(), x.stride(0),
+    a, lib = _lib.address, _lib.load()
+    ws_bytes = lib.swvr_sample_workspace_size(R, V)
+    ws = x.new_empty(ws_bytes, dtype=torch.uint8)
+    _lib.call(lib.swvr_sample, x.device, _lib.DTYPE_TAG[x.dtype], R, V, x.data_ptr(), x.stride(0),
               u1.data_ptr(), u1.dtype == torch.float64, tau, a(tau_r), k, a(k_r), p, a(p_r), min_p, a(min_p_r),
-              token.data_ptr(), logprob.data_ptr())
+              token.data_ptr(), logprob.data_ptr(), ws.data_ptr(), ws_bytes)
     return token, logprob
 
 

@@ -100,8 +100,8 @@ def test_ties_at_every_cut(kw):
 
 @pytest.mark.parametrize("kw", [dict(), dict(top_k=4), dict(top_p=0.8), dict(min_p=0.3), dict(temperature=0.0)], ids=str)
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
-def test_masked_infinite_and_nan_logits(kw, dtype):
-    V = 3001
+@pytest.mark.parametrize("V", [3001, 20011])   # a row in one launch, and in several
+def test_masked_infinite_and_nan_logits(kw, dtype, V):
     x = torch.randn(10, V, device=DEV, generator=gen(9)).to(dtype)
     x[0] = -math.inf                                # nothing to draw
     x[1] = math.nan                                 # nothing to draw
@@ -157,11 +157,14 @@ def test_views_off_every_alignment(dtype):
     big = (3 * torch.randn(6, 9000, device=DEV, generator=gen(12))).to(dtype)
     u = torch.rand(6, device=DEV, generator=gen(13))
     for lo in range(9):
-        for n in (1, 5, 4093, 8990):
+        for n in (1, 5, 4093, 4097, 8990):
             check(big[:, lo:lo + n], u, top_p=0.9)
     check(big[:, ::3], u, top_k=9)
     check(big[::2], u[::2])
     check(big[:1].expand(6, 9000), u, top_p=0.7)
+    for kw in (dict(), dict(top_k=30), dict(top_p=0.5), dict(min_p=0.01)):
+        for lo in (1, 3, 8):
+            check(big[:, lo:lo + 8200], u, **kw)
     check(torch.randn(300, 6, device=DEV, generator=gen(14)).to(dtype).t(), u)
 
 

@@ -122,9 +122,9 @@ def embedding_bwd(dtype=_lib.BF16, id64=1, N=4, V=8, D=4, ids=P, g=P, ldg=4, gE=
     return _lib.load().swvr_embedding_bwd(dtype, id64, N, V, D, ids, g, ldg, 1.0, gE, ws, nbytes, None)
 
 
-def sample(dtype=_lib.BF16, R=4, V=8, logits=P, ld=8, u=P, u64=0, tau=1.0, token=P, logprob=P):
+def sample(dtype=_lib.BF16, R=4, V=8, logits=P, ld=8, u=P, u64=0, tau=1.0, token=P, logprob=P, ws=P, nbytes=1 << 30):
     return _lib.load().swvr_sample(dtype, R, V, logits, ld, u, u64, tau, None, 0, None, 1.0, None, 0.0, None, token,
-                                   logprob, None)
+                                   logprob, ws, nbytes, None)
 
 
 def distill_abi(dtype=_lib.BF16, N=4, K=16, V=8, T=2, h=P, ids=P, id64=1, teacher=P, t_dtype=_lib.F32, tau=1.0, red=2,
@@ -163,6 +163,8 @@ def distill_bwd_abi(dtype=_lib.BF16, N=4, V=8, T=2, tau=1.0, chunk=8192, g=P, gb
     (sample, dict(tau=float("nan")), _lib.EINVAL),
     (sample, dict(logits=ctypes.c_void_p(17)), _lib.EINVAL),
     (sample, dict(token=None), _lib.EINVAL),
+    (sample, dict(V=50000, nbytes=1000), _lib.EWORKSPACE),
+    (sample, dict(V=50000, ws=None), _lib.EWORKSPACE),
     (distill_abi, dict(dtype=_lib.F64), _lib.EDTYPE),
     (distill_abi, dict(t_dtype=5), _lib.EDTYPE),
     (distill_abi, dict(T=0), _lib.EINVAL),
