@@ -14,8 +14,6 @@
 // 151936 tokens), whose sums are exact in 64-bit integers in any order, atomics included.  A token whose w rounds to
 // 0 (below 2^-45 of the largest) is never drawn.  The logarithm of the drawn token's probability comes from the
 // fp64 exponent, not from the rounded w.
-#include <cfloat>
-
 #include "common.hpp"
 #include "launch.hpp"
 
@@ -42,21 +40,28 @@ __device__ __forceinline__ float logit_of(uint32_t key) {
   return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
 
-// Logits i0 .. i0 + L - 1 of a row as keys (0 outside 0 .. V - 1), in one load (fp32: 16 bytes each).  A row may begin
+// Logits i0 .. i0 + L - 1 of a row (-inf outside 0 .. V - 1), in one load (fp32: 16 bytes each).  A row may begin
 // anywhere: i0 + lead is a multiple of L, lead the row's distance from a border of L elements.
 template <class T, int L>
-__device__ __forceinline__ void load_keys(const T* row, int64_t i0, int64_t V, uint32_t (&key)[L]) {
+__device__ __forceinline__ void load_logits(const T* row, int64_t i0, int64_t V, float (&x_)[L]) {
   if (i0 >= 0 && i0 + L <= V) {
     struct alignas(L * sizeof(T) < 16 ? L * sizeof(T) : 16) X {
       T v[L];
     };
     const X x = *reinterpret_cast<const X*>(row + i0);
 #pragma unroll
-    for (int u = 0; u < L; ++u) key[u] = key_of((float)x.v[u]);
+    for (int u = 0; u < L; ++u) x_[u] = (float)x.v[u];
   } else {
 #pragma unroll
-    for (int u = 0; u < L; ++u) key[u] = i0 + u >= 0 && i0 + u < V ? key_of((float)row[i0 + u]) : 0;
+    for (int u = 0; u < L; ++u) x_[u] = i0 + u >= 0 && i0 + u < V ? (float)row[i0 + u] : kNegInf;
   }
+}
+template <class T, int L>
+__device__ __forceinline__ void load_keys(const T* row, int64_t i0, int64_t V, uint32_t (&key)[L]) {
+  float x[L];
+  load_logits(row, i0, V, x);
+#pragma unroll
+  for (int u = 0; u < L; ++u) key[u] = key_of(x[u]);
 }
 
 // Weights of a row: w = 2^t, t = (l - m) to_log2, to_log2 = log2(e) / tau, in fp64: with n the whole number next to
@@ -71,10 +76,12 @@ __device__ __forceinline__ void fill_powers(double* s) {  // no barrier
 struct Weigh {
   const double* powers;  // [kPowers], LDS
   double m, to_log2, one;  // one: 2^shift
+  float m_f;
   uint32_t key_m;
-  __device__ __forceinline__ double rel(uint32_t key) const {
+  __device__ __forceinline__ double rel(uint32_t key) const { return rel(logit_of(key)); }
+  __device__ __forceinline__ double rel(float l) const {
     constexpr double kRound = 6755399441055744.0;  // 1.5 2^52: sums with it are whole numbers, in the low bits
-    const double t = ((double)logit_of(key) - m) * to_log2;
+    const double t = ((double)l - m) * to_log2;
     const double y = fma(t, (double)kPowers, kRound);
     const int n = (int)__double_as_longlong(y);
     const double f = fma(y - kRound, -1.0 / kPowers, t);
@@ -85,8 +92,8 @@ struct Weigh {
     x = fma(x, f, 1.0);
     const double w = x * __longlong_as_double(__double_as_longlong(powers[n & (kPowers - 1)]) +
                                               ((long long)(n >> 5) << 52));
-    // (t is NaN where the largest logit is infinite: tokens equal to it, or under an infinite tau)
-    return key == key_m ? 1.0 : key != 0 && t > -1000 ? w : 0.0;
+    // (t is NaN for a NaN, and where the largest logit is infinite for tokens equal to it)
+    return l == m_f ? 1.0 : t > -1000 ? w : 0.0;
   }
   // w in units of 2^-shift, to nearest: below 2^52, so the sum's low bits are the whole number
   __device__ __forceinline__ u64 fix(double w) const {
@@ -94,11 +101,37 @@ struct Weigh {
   }
 };
 
-__device__ __forceinline__ u64 wave_sum64(u64 x) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o);
-  return x;
+// x of the lane that DPP control CTRL names, 0 where there is none or the row is not in RM.
+template <int CTRL, int RM = 0xf>
+__device__ __forceinline__ u64 dpp64(u64 x) {
+  const int lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)x, CTRL, RM, 0xf, false);
+  const int hi = __builtin_amdgcn_update_dpp(0, (int)(x >> 32), CTRL, RM, 0xf, false);
+  return (u64)(uint32_t)hi << 32 | (uint32_t)lo;
 }
+// Inclusive scan over the wave under an operation with identity 0: within rows of 16 lanes (row_shr 1, 2, 4, 8),
+// then the last lane of row 0 and 2 into rows 1 and 3 (row_bcast 15), and lane 31 into the upper half (row_bcast 31).
+// (DPP moves cost a few cycles where __shfl goes through LDS: a workgroup's scan of 1024 threads 0.85 -> 0.5 us.)
+template <class Op>
+__device__ __forceinline__ u64 wave_scan64(u64 x, Op op) {
+  x = op(x, dpp64<0x111>(x));
+  x = op(x, dpp64<0x112>(x));
+  x = op(x, dpp64<0x114>(x));
+  x = op(x, dpp64<0x118>(x));
+  x = op(x, dpp64<0x142, 0xa>(x));
+  return op(x, dpp64<0x143, 0xc>(x));
+}
+struct Sum64 {
+  __device__ __forceinline__ u64 operator()(u64 a, u64 b) const { return a + b; }
+};
+struct Max64 {
+  __device__ __forceinline__ u64 operator()(u64 a, u64 b) const { return a > b ? a : b; }
+};
+__device__ __forceinline__ u64 last_lane64(u64 x) {
+  return (u64)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), 63) << 32 |
+         (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)x, 63);
+}
+__device__ __forceinline__ u64 wave_sum64(u64 x) { return last_lane64(wave_scan64(x, Sum64())); }
+__device__ __forceinline__ u64 wave_max64(u64 x) { return last_lane64(wave_scan64(x, Max64())); }
 
 // Sum over a workgroup of NW waves, in every thread; s: NW words of LDS, free again at the next barrier after.
 template <int NW>
@@ -116,12 +149,7 @@ __device__ __forceinline__ u64 block_sum64(u64 x, u64* s) {
 // Sum of the threads before this one, and of all (total).
 template <int NW>
 __device__ __forceinline__ u64 block_before64(u64 x, u64* s, u64* total) {
-  u64 y = x;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const u64 z = __shfl_up(y, o);
-    if (lane_id() >= o) y += z;
-  }
+  const u64 y = wave_scan64(x, Sum64());
   __syncthreads();
   if (lane_id() == 63) s[wave_id()] = y;
   __syncthreads();
@@ -384,20 +412,12 @@ __device__ __forceinline__ u64 place_of(uint32_t key, int64_t i) {
 }
 __device__ __forceinline__ uint32_t key_at(u64 place) { return (uint32_t)(place >> 32); }
 __device__ __forceinline__ int64_t index_at(u64 place) { return (int64_t)(uint32_t)~(uint32_t)place; }
-__device__ __forceinline__ u64 wave_max64(u64 x) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    const u64 y = __shfl_xor(x, o);
-    x = y > x ? y : x;
-  }
-  return x;
-}
-
 __device__ __forceinline__ Weigh weigh_of(const SampleParams& a, const RowSettings& s, uint32_t key_m,
                                           const double* powers) {
   Weigh w;
   w.powers = powers;
-  w.m = (double)logit_of(key_m);
+  w.m_f = logit_of(key_m);
+  w.m = (double)w.m_f;
   w.to_log2 = 1.4426950408889634074 / s.tau;
   w.one = a.one;
   w.key_m = key_m;
@@ -459,10 +479,10 @@ __global__ __launch_bounds__(kRowThreads) void sample_row_kernel(SampleParams a)
 // So a row is read once with top-k, twice with min-p or nothing, three times with top-p, and its logits never sorted.
 // A list that would pass kList tokens, or kSegList from one workgroup (equal logits, a nearly flat row) leaves its row to sample_row, in the same
 // launch, as does a k above kTopK.  Every sum is one of whole numbers, so its order does not matter.
-constexpr int kSub = 2048, kGroups = 4096, kList = 4096, kSegList = 2048, kTopK = 1024;
+constexpr int kSub = 2048, kGroups = 4096, kList = 4096, kSegList = 2048, kTopK = 1024, kFew = 128;
 constexpr int64_t kRowMost = 4096, kStagedMost = ((int64_t)1 << 21) - 8;  // (groups of at most a wave's 512)
 constexpr int kSubsMost = (int)(((int64_t)1 << 21) / kSub);
-constexpr int kWaveLoad = 8;
+constexpr int kWaveLoad = 8, kCross = 3;
 
 enum RowKind { kGreedy, kTopKRow, kTopPRow, kSumRow, kWholeRow };
 __device__ __forceinline__ RowKind kind_of(const RowSettings& s, int64_t V) {
@@ -481,7 +501,8 @@ struct Staged {
   u64* list;        // [rows][kList] places
   int* n_list;      // [rows]
   u64* sums;        // [rows][n_sub]
-  u64* crossing;    // [rows][2]: the bin in which the prefix ends, the weight before it
+  u64* crossing;    // [rows][kCross]: the bin in which the prefix ends, the weight before it, the whole weight
+  int may_k, may_p, may_sum;  // whether a row may have top-k, top-p alone, no top-k (the host cannot see every setting)
 };
 
 template <class T>
@@ -495,20 +516,54 @@ struct RowView {
   }
 };
 
-// f(sub-block, first index of the lane's kWaveLoad logits, keys) over the sub-blocks of this wave.
-template <class T, class F, class G>
-__device__ __forceinline__ void each_sub(const Staged& p, const RowView<T>& v, F&& f, G&& done) {
-  constexpr int kSteps = kSub / (64 * kWaveLoad);
-  for (int sub = (int)(blockIdx.x % p.n_seg) * 4 + wave_id(); sub < p.n_sub; sub += 4 * p.n_seg) {
-    uint32_t key[kSteps][kWaveLoad];
-    const int64_t i0 = (int64_t)sub * kSub - v.lead + lane_id() * kWaveLoad;
-#pragma unroll
-    for (int j = 0; j < kSteps; ++j) load_keys(v.row, i0 + j * 64 * kWaveLoad, v.V, key[j]);
-#pragma unroll
-    for (int j = 0; j < kSteps; ++j) f(sub, j, i0 + j * 64 * kWaveLoad, key[j]);
-    done(sub);
-  }
+// Room for this lane's c entries at the end of a list of *n (LDS), in one atomic of the whole wave.
+__device__ __forceinline__ int append(int* n, int c) {
+  const int to = (int)wave_scan64((u64)c, Sum64());
+  int base = 0;
+  if (lane_id() == 63 && to > 0) base = atomicAdd(n, to);
+  return __builtin_amdgcn_readlane(base, 63) + to - c;
 }
+
+// kWaveLoad consecutive logits of a lane from i0 on (i0 + lead a multiple of kWaveLoad), as stored: loads of several go
+// out before the first is used (converted inside the branch of load_logits, each waited for the one before: the first
+// launch took 42 us for 512 rows of 151936).  Where they reach over an end of the row, fix() replaces them.
+template <class T>
+struct alignas(kWaveLoad * sizeof(T) < 16 ? kWaveLoad * sizeof(T) : 16) Chunk {
+  T v[kWaveLoad];
+};
+template <class T>
+__device__ __forceinline__ Chunk<T> load_chunk(const RowView<T>& v, int64_t i0) {
+  // the nearest chunk inside the row (V > 2 kWaveLoad)
+  const int64_t lo = v.lead == 0 ? 0 : kWaveLoad - v.lead;
+  const int64_t hi = lo + (v.V - lo) / kWaveLoad * kWaveLoad - kWaveLoad;
+  const int64_t at = i0 < lo ? lo : i0 > hi ? hi : i0;
+  return *reinterpret_cast<const Chunk<T>*>(v.row + at);
+}
+template <class T>
+__device__ __forceinline__ void chunk_logits(const RowView<T>& v, int64_t i0, const Chunk<T>& c, float (&x)[kWaveLoad]) {
+#pragma unroll
+  for (int u = 0; u < kWaveLoad; ++u) x[u] = (float)c.v[u];
+  if (i0 < 0 || i0 + kWaveLoad > v.V)
+#pragma unroll
+    for (int u = 0; u < kWaveLoad; ++u) x[u] = i0 + u >= 0 && i0 + u < v.V ? (float)v.row[i0 + u] : kNegInf;
+}
+
+// The logits of a wave's sub-block, step j of kSteps holding kWaveLoad consecutive ones of each lane from first(j) on
+// (outside the row: -inf).
+constexpr int kSteps = kSub / (64 * kWaveLoad);
+template <class T>
+struct SubBlock {
+  int sub;
+  int64_t i0;
+  Chunk<T> c[kSteps];
+  __device__ __forceinline__ SubBlock(const Staged& p, const RowView<T>& v, int seg, int waves) {
+    sub = seg * waves + wave_id();
+    i0 = (int64_t)sub * kSub - v.lead + lane_id() * kWaveLoad;
+#pragma unroll
+    for (int j = 0; j < kSteps; ++j) c[j] = load_chunk(v, first(j));
+  }
+  __device__ __forceinline__ int64_t first(int j) const { return i0 + j * 64 * kWaveLoad; }
+};
 
 // A row's first token in order, by each wave for itself.
 __device__ __forceinline__ u64 row_first(const Staged& p, int64_t q) {
@@ -523,9 +578,9 @@ __device__ __forceinline__ u64 row_first(const Staged& p, int64_t q) {
 // Bin of a key: its distance below the largest in units of 46 log2-steps of weight / kBins (past that, weights are 0),
 // in fp32: no smaller for a smaller logit.
 __device__ __forceinline__ float bin_scale(const Weigh& w) { return (float)(w.to_log2 * (kBins / 46.0)); }
-__device__ __forceinline__ int bin_of(uint32_t key, const Weigh& w, float scale) {
-  const float x = ((float)w.m - logit_of(key)) * scale;
-  return key == w.key_m ? 0 : x < kBins - 1 ? (int)x : kBins - 1;
+__device__ __forceinline__ int bin_of(float l, const Weigh& w, float scale) {
+  const float x = (w.m_f - l) * scale;
+  return l == w.m_f ? 0 : x < kBins - 1 ? (int)x : kBins - 1;
 }
 
 template <class T>
@@ -539,58 +594,63 @@ __global__ __launch_bounds__(256) void sample_max_kernel(Staged p) {
     if (seg == 0 && threadIdx.x == 0) p.n_list[q] = 0;
   }
   const int lanes = 1 << (p.gshift - 3);  // of a group
+  const RowView<T> v(p.a, r);
+  const SubBlock<T> b(p, v, (int)(blockIdx.x % p.n_seg), 4);
+  if (b.sub >= p.n_sub) return;
   u64 first = 0;
-  each_sub(
-      p, RowView<T>(p.a, r),
-      [&](int sub, int j, int64_t i0, const uint32_t(&key)[kWaveLoad]) {
-        uint32_t k = 0;
-        int at = 0;
 #pragma unroll
-        for (int u = 0; u < kWaveLoad; ++u)
-          if (key[u] > k) {
-            k = key[u];
-            at = u;
-          }
-        const u64 x = place_of(k, i0 + at);
-        first = x > first ? x : first;
-        if (kind != kTopKRow) return;
-        for (int o = 1; o < lanes; o <<= 1) {
-          const uint32_t y = __shfl_xor(k, o);
-          k = y > k ? y : k;
-        }
-        if ((lane_id() & (lanes - 1)) == 0)
-          p.group[q * kGroups + (((int64_t)sub * kSub + j * 64 * kWaveLoad + lane_id() * kWaveLoad) >> p.gshift)] = k;
-      },
-      [&](int sub) {
-        first = wave_max64(first);
-        if (lane_id() == 0) p.first[q * p.n_sub + sub] = first;
-        first = 0;
-      });
+  for (int j = 0; j < kSteps; ++j) {
+    uint32_t k = 0;
+    int at = 0;
+    float l[kWaveLoad];
+    chunk_logits(v, b.first(j), b.c[j], l);
+#pragma unroll
+    for (int u = 0; u < kWaveLoad; ++u) {
+      const uint32_t key = key_of(l[u]);
+      at = key > k ? u : at;
+      k = key > k ? key : k;
+    }
+    const u64 x = place_of(k, b.first(j) + at);
+    first = x > first ? x : first;
+    if (kind != kTopKRow) continue;
+    for (int o = 1; o < lanes; o <<= 1) {
+      const uint32_t y = __shfl_xor(k, o);
+      k = y > k ? y : k;
+    }
+    if ((lane_id() & (lanes - 1)) == 0)
+      p.group[q * kGroups + (((int64_t)b.sub * kSub + (j * 64 + lane_id()) * kWaveLoad) >> p.gshift)] = k;
+  }
+  first = wave_max64(first);
+  if (lane_id() == 0) p.first[q * p.n_sub + b.sub] = first;
 }
 
+// (Workgroups of 16 waves add a quarter as many bins to the rows', and take longer: 47 us for 40.)
 template <class T>
 __global__ __launch_bounds__(256) void sample_hist_kernel(Staged p) {
   __shared__ u64 s_hist[kBins];
   __shared__ double s_powers[kPowers];
   const int64_t q = blockIdx.x / p.n_seg, r = p.r0 + q;
   const RowSettings s = settings_of(p.a, r);
+  if (kind_of(s, p.a.V) != kTopPRow) return;
+  const RowView<T> v(p.a, r);
+  const SubBlock<T> b(p, v, (int)(blockIdx.x % p.n_seg), 4);
   const u64 first = row_first(p, q);
-  if (kind_of(s, p.a.V) != kTopPRow || first == 0) return;
+  if (first == 0) return;
   fill_powers(s_powers);
   for (int i = threadIdx.x; i < kBins; i += 256) s_hist[i] = 0;
   __syncthreads();
   const Weigh wt = weigh_of(p.a, s, key_at(first), s_powers);
   const float scale = bin_scale(wt);
-  each_sub(
-      p, RowView<T>(p.a, r),
-      [&](int, int, int64_t, const uint32_t(&key)[kWaveLoad]) {
 #pragma unroll
-        for (int u = 0; u < kWaveLoad; ++u) {
-          const u64 w = wt.fix(wt.rel(key[u]));
-          if (w) atomicAdd(&s_hist[bin_of(key[u], wt, scale)], w);
-        }
-      },
-      [](int) {});
+  for (int j = 0; j < kSteps; ++j) {
+    float l[kWaveLoad];
+    chunk_logits(v, b.first(j), b.c[j], l);
+#pragma unroll
+    for (int u = 0; u < kWaveLoad; ++u) {
+      const u64 w = wt.fix(wt.rel(l[u]));
+      if (w) atomicAdd(&s_hist[bin_of(l[u], wt, scale)], w);
+    }
+  }
   __syncthreads();
   for (int i = threadIdx.x; i < kBins; i += 256)
     if (s_hist[i]) atomicAdd(&p.hist[q * kBins + i], s_hist[i]);
@@ -598,14 +658,17 @@ __global__ __launch_bounds__(256) void sample_hist_kernel(Staged p) {
 
 template <class T>
 __global__ __launch_bounds__(256) void sample_sums_kernel(Staged p) {
-  __shared__ u64 s_sum[4], s_cross[2], s_list[kSegList];
+  __shared__ u64 s_sum[4], s_cross[kCross], s_list[kSegList];
   __shared__ double s_powers[kPowers];
   __shared__ int s_n, s_at;
   const int64_t q = blockIdx.x / p.n_seg, r = p.r0 + q;
   const RowSettings s = settings_of(p.a, r);
   const RowKind kind = kind_of(s, p.a.V);
+  if (kind != kTopPRow && kind != kSumRow) return;
+  const RowView<T> v(p.a, r);
+  const SubBlock<T> b(p, v, (int)(blockIdx.x % p.n_seg), 4);
   const u64 first = row_first(p, q);
-  if ((kind != kTopPRow && kind != kSumRow) || first == 0) return;
+  if (first == 0) return;
   fill_powers(s_powers);
   if (threadIdx.x == 0) s_n = 0;
   int cross = kBins;
@@ -621,37 +684,44 @@ __global__ __launch_bounds__(256) void sample_sums_kernel(Staged p) {
       if (w[i] && (double)at < limit && (double)(at + w[i]) >= limit) {
         s_cross[0] = threadIdx.x * kPer + i;
         s_cross[1] = at;
+        s_cross[2] = total;
       }
       at += w[i];
     }
     __syncthreads();
     cross = (int)s_cross[0];
-    if (blockIdx.x % p.n_seg == 0 && threadIdx.x < 2) p.crossing[q * 2 + threadIdx.x] = s_cross[threadIdx.x];
+    if (blockIdx.x % p.n_seg == 0 && threadIdx.x < kCross)
+      p.crossing[q * kCross + threadIdx.x] = s_cross[threadIdx.x];
   }
   __syncthreads();
   const Weigh wt = weigh_of(p.a, s, key_at(first), s_powers);
   const float scale = bin_scale(wt);
+  // the sum, and a bit for each token of the bin: those, few, are read again (kept apart, they hold no registers)
   u64 sum = 0;
-  each_sub(
-      p, RowView<T>(p.a, r),
-      [&](int, int, int64_t i0, const uint32_t(&key)[kWaveLoad]) {
+  uint32_t hits = 0;
 #pragma unroll
-        for (int u = 0; u < kWaveLoad; ++u) {
-          const int b = bin_of(key[u], wt, scale);
-          if (b < cross) {
-            const double w = wt.rel(key[u]);
-            sum += w >= s.min_p ? wt.fix(w) : 0;
-          } else if (b == cross && key[u] != 0) {
-            const int at = atomicAdd(&s_n, 1);
-            if (at < kSegList) s_list[at] = place_of(key[u], i0 + u);
-          }
-        }
-      },
-      [&](int sub) {
-        sum = wave_sum64(sum);
-        if (lane_id() == 0) p.sums[q * p.n_sub + sub] = sum;
-        sum = 0;
-      });
+  for (int j = 0; j < kSteps; ++j) {
+    float x[kWaveLoad];
+    chunk_logits(v, b.first(j), b.c[j], x);
+#pragma unroll
+    for (int u = 0; u < kWaveLoad; ++u) {
+      const float l = x[u];
+      const int bin = bin_of(l, wt, scale);
+      const double w = wt.rel(l);
+      sum += bin < cross && w >= s.min_p ? wt.fix(w) : 0;
+      hits |= (bin == cross && l > kNegInf) ? 1u << (j * kWaveLoad + u) : 0u;
+      // one element after another: left to it, the compiler keeps all 32 in flight, in 245 registers (60 + 20 -> 75 us)
+      asm volatile("" : "+v"(hits), "+v"(sum));
+    }
+  }
+  for (; hits != 0; hits &= hits - 1) {
+    const int i = __ffs((int)hits) - 1;
+    const int64_t at = b.first(i / kWaveLoad) + i % kWaveLoad;
+    const int n = atomicAdd(&s_n, 1);
+    if (n < kSegList) s_list[n] = place_of(key_of((float)v.row[at]), at);
+  }
+  sum = wave_sum64(sum);
+  if (lane_id() == 0 && b.sub < p.n_sub) p.sums[q * p.n_sub + b.sub] = sum;
   if (kind != kTopPRow) return;
   // the bin's tokens of this workgroup to the row's list, whose order does not matter
   __syncthreads();
@@ -662,38 +732,96 @@ __global__ __launch_bounds__(256) void sample_sums_kernel(Staged p) {
     if (s_at + i < kList) p.list[q * kList + s_at + i] = s_list[i];
 }
 
-// s[0 .. n2), n2 a power of two, into descending (or ascending) order by kRowThreads threads.  A wave's pairs of
-// a step of up to 64 lie in 128 elements of its own.
-template <bool DESC>
-__device__ __forceinline__ void bitonic_sort(u64* s, int n2) {
-  for (int k = 2; k <= n2; k <<= 1)
-    for (int j = k >> 1; j > 0; j >>= 1) {
-      if (j >= 128 || (j == 64 && k > 128) || k == 2)
+// s[0 .. n2), n2 a power of two up to kList, into descending order by kRowThreads threads: a bitonic network, of
+// which a thread holds 4 consecutive elements in registers.  Steps over 1 and 2 elements stay in the thread, those over
+// up to 128 in the wave (lane moves), and only wider ones go through LDS between barriers: 2048 elements, 66 steps,
+// took 18 us with all steps in LDS.
+__device__ __forceinline__ void order2(u64& a, u64& b, bool desc) {
+  const bool swap = (a < b) == desc && a != b;
+  const u64 x = a;
+  a = swap ? b : a;
+  b = swap ? x : b;
+}
+__device__ __forceinline__ void sort_descending(u64* s, int n2) {
+  const int i0 = threadIdx.x * 4;
+  const bool in = i0 < n2;
+  u64 x[4];
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = in && i0 + i < n2 ? s[i0 + i] : 0;
+#pragma unroll 1
+  for (int k = 2; k <= n2; k <<= 1) {
+#pragma unroll 1
+    for (int j = k >> 1; j >= 4; j >>= 1) {
+      const bool lower = (i0 & j) == 0, desc = (i0 & k) == 0;
+      u64 y[4];
+      if (j >= 256) {
         __syncthreads();
-      else
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      for (int t = threadIdx.x; t < n2 / 2; t += kRowThreads) {
-        const int i = (t & ~(j - 1)) * 2 + (t & (j - 1));
-        const u64 a = s[i], b = s[i + j];
-        const bool up = ((i & k) == 0) != DESC;  // this pair ascending
-        if ((a > b) == up) {
-          s[i] = b;
-          s[i + j] = a;
-        }
+        if (in)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[i0 + i] = x[i];
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] = in ? s[(i0 ^ j) + i] : 0;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] = __shfl_xor(x[i], j / 4);
       }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = (x[i] > y[i]) == (lower == desc) ? x[i] : y[i];
     }
+    if (k >= 4) {
+      const bool desc = (i0 & k) == 0;
+      order2(x[0], x[2], desc);
+      order2(x[1], x[3], desc);
+      order2(x[0], x[1], desc);
+      order2(x[2], x[3], desc);
+    } else {
+      order2(x[0], x[1], true);
+      order2(x[2], x[3], false);
+    }
+  }
+  __syncthreads();
+  if (in)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i0 + i < n2) s[i0 + i] = x[i];
   __syncthreads();
 }
 
-__device__ __forceinline__ int pow2_at_least(int n) { return n <= 2 ? 2 : 1 << (32 - __clz(n - 1)); }
+__device__ __forceinline__ int pow2_at_least(int n) { return n <= 4 ? 4 : 1 << (32 - __clz(n - 1)); }
+
+// Bin of a key's distance d below the largest: 64 per octave of d (the upper bits of d as a float), so that the
+// largest keys, whatever they are, spread over many.
+constexpr uint32_t kOneBits = 127u << 6;  // 1.f's upper bits
+__device__ __forceinline__ int distance_bin(uint32_t d) {
+  const uint32_t x = d == 0 ? 0 : (__float_as_uint((float)d) >> 17) - kOneBits;
+  return x < kBins ? (int)x : kBins - 1;
+}
 
 template <class T>
 __global__ __launch_bounds__(kRowThreads) void sample_finish_kernel(Staged p) {
   __shared__ u64 s_list[kList], s_w[kList], s_sub[kSubsMost], s_sum[kRowWaves], s_out[4];
   __shared__ double s_powers[kPowers];
-  __shared__ int s_n;
+  __shared__ int s_n, s_m;
   const SampleParams& a = p.a;
   const int64_t q = blockIdx.x, r = p.r0 + q;
+  // what any kind of row may need goes out together (a row of another kind leaves it unread)
+  constexpr int kPerGroup = kGroups / kRowThreads;
+  const int groups = (int)(((int64_t)p.n_sub * kSub) >> p.gshift), j0 = 2 * threadIdx.x;
+  uint32_t g[kPerGroup];
+#pragma unroll
+  for (int i = 0; i < kPerGroup; ++i) {
+    const int at = threadIdx.x + i * kRowThreads;
+    g[i] = p.may_k && at < groups ? p.group[q * kGroups + at] : 0;
+  }
+  u64 sub[2], crossing[kCross];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) sub[i] = p.may_sum && j0 + i < p.n_sub ? p.sums[q * p.n_sub + j0 + i] : 0;
+#pragma unroll
+  for (int i = 0; i < kCross; ++i) crossing[i] = p.may_p ? p.crossing[q * kCross + i] : 0;
+  const int n_list = p.may_p ? p.n_list[q] : 0;
+  const u64 list0 = p.may_p ? p.list[q * kList + threadIdx.x] : 0;
   const RowSettings s = settings_of(a, r);
   const u64 first = row_first(p, q);
   if (settled(a, r, s, first)) return;
@@ -703,205 +831,330 @@ __global__ __launch_bounds__(kRowThreads) void sample_finish_kernel(Staged p) {
   const Weigh wt = weigh_of(a, s, key_at(first), s_powers);
   constexpr int kPer = kList / kRowThreads;  // list entries of a thread
   const int t0 = threadIdx.x * kPer;
-  if (threadIdx.x == 0) s_n = 0;
-  __syncthreads();
+  auto draw = [&](u64 place, u64 total) {  // by one thread
+    const uint32_t key = key_at(place);
+    const double rel = key == wt.key_m ? 0.0 : ((double)logit_of(key) - wt.m) / s.tau;
+    a.token[r] = index_at(place);
+    a.logprob[r] = (float)(rel - log((double)total / a.one));
+  };
+  auto target_of = [&](u64 total) {
+    const double uz = s.u * (double)total;
+    return uz < (double)(total - 1) ? (u64)uz : total - 1;
+  };
 
   int n = 0;  // list entries
   if (kind == kTopKRow) {
-    // a key that at least k tokens reach, from its upper 22 bits
+    // A key that at least k groups reach: a histogram of the groups' distances below the largest key; the bin of the
+    // k-th from the top by one wave (32 bins a lane, read in an order that meets every LDS bank).
     uint32_t* const s_cnt = reinterpret_cast<uint32_t*>(s_list);
-    const int groups = (int)(((int64_t)p.n_sub * kSub) >> p.gshift);
-    uint32_t g[kGroups / kRowThreads];
+    for (int i = threadIdx.x; i < kBins; i += kRowThreads) s_cnt[i] = 0;
+    if (threadIdx.x == 0) s_n = s_m = 0;
+    __syncthreads();
 #pragma unroll
-    for (int i = 0; i < kGroups / kRowThreads; ++i) {
-      const int at = threadIdx.x + i * kRowThreads;
-      g[i] = at < groups ? p.group[q * kGroups + at] : 0;
-    }
-    uint32_t bound = 0, before = 0;
-    bool found = true;
-#pragma unroll 1
-    for (int sh = 21; sh >= 10 && found; sh -= 11) {
-      for (int i = threadIdx.x; i < kBins; i += kRowThreads) s_cnt[i] = 0;
-      if (threadIdx.x == 0) s_out[0] = ~0ull;
-      __syncthreads();
-#pragma unroll
-      for (int i = 0; i < kGroups / kRowThreads; ++i)
-        if (g[i] != 0 && (sh == 21 || (g[i] >> 21) == (bound >> 21)))
-          atomicAdd(&s_cnt[(g[i] >> sh) & (kBins - 1)], 1u);
-      __syncthreads();
-      const int b1 = kBins - 1 - 2 * (int)threadIdx.x;
-      const uint32_t n1 = s_cnt[b1], n0 = s_cnt[b1 - 1];
-      u64 all;
-      const uint32_t at = before + (uint32_t)block_before64<kRowWaves>(n1 + n0, s_sum, &all);
-      if (at < s.k && at + n1 >= s.k) {
-        s_out[0] = b1;
-        s_out[1] = at;
-      } else if (at + n1 < s.k && at + n1 + n0 >= s.k) {
-        s_out[0] = b1 - 1;
-        s_out[1] = at + n1;
+    for (int i = 0; i < kPerGroup; ++i)
+      if (g[i] != 0) {
+        atomicAdd(&s_cnt[distance_bin(wt.key_m - g[i])], 1u);
       }
-      __syncthreads();
-      found = s_out[0] != ~0ull;
-      if (found) {
-        bound |= (uint32_t)s_out[0] << sh;
-        before = (uint32_t)s_out[1];
+    __syncthreads();
+    if (wave_id() == 0) {
+      const int lane = lane_id(), b0 = 32 * lane;
+      uint32_t sum = 0;
+#pragma unroll 8
+      for (int i = 0; i < 32; ++i) sum += s_cnt[b0 + ((i + lane) & 31)];
+      const uint32_t to = (uint32_t)wave_scan64(sum, Sum64());
+      uint32_t at = to - sum;
+      if (lane == 63 && to < s.k) s_out[0] = kBins;
+      if (at < s.k && to >= s.k) {
+        int b = b0;
+        while (at + s_cnt[b] < s.k) at += s_cnt[b++];
+        s_out[0] = b;
       }
-      __syncthreads();
     }
-    if (bound == 0) bound = 1;
+    __syncthreads();
+    // d is below the bin's upper edge
+    const uint32_t bin = (uint32_t)s_out[0];
+    const float edge = __uint_as_float((bin + 1 + kOneBits) << 17);
+    const uint32_t bound = bin < kBins && edge < (float)wt.key_m ? wt.key_m - (uint32_t)edge : 1;
     // the groups that reach it, then their tokens
     int* const s_group = reinterpret_cast<int*>(s_w);
+    {
+      int c = 0;
 #pragma unroll
-    for (int i = 0; i < kGroups / kRowThreads; ++i)
-      if (g[i] >= bound) s_group[atomicAdd(&s_n, 1)] = threadIdx.x + i * kRowThreads;
-    __syncthreads();
-    const int n_group = s_n;
-    __syncthreads();
-    if (threadIdx.x == 0) s_n = 0;
-    __syncthreads();
-    const int lanes = 1 << (p.gshift - 3), per = kRowThreads / lanes;
-#pragma unroll 2
-    for (int i = threadIdx.x / lanes; i < n_group; i += per) {
-      const int64_t i0 = ((int64_t)s_group[i] << p.gshift) - v.lead + (threadIdx.x % lanes) * kWaveLoad;
-      uint32_t key[kWaveLoad];
-      load_keys(v.row, i0, v.V, key);
+      for (int i = 0; i < kPerGroup; ++i) c += g[i] >= bound;
+      int at = append(&s_m, c);
 #pragma unroll
-      for (int u = 0; u < kWaveLoad; ++u)
-        if (key[u] >= bound) {
-          const int at = atomicAdd(&s_n, 1);
-          if (at < kList) s_list[at] = place_of(key[u], i0 + u);
-        }
+      for (int i = 0; i < kPerGroup; ++i)
+        if (g[i] >= bound) s_group[at++] = threadIdx.x + i * kRowThreads;
+    }
+    __syncthreads();
+    const int n_group = s_m, lanes = 1 << (p.gshift - 3), per = kRowThreads / lanes;
+    for (int first_i = 0; first_i < n_group; first_i += 4 * per) {
+      const int i0 = first_i + threadIdx.x / lanes;
+      Chunk<T> c[4];
+      int64_t at0[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int i = i0 + j * per;
+        at0[j] = ((int64_t)(i < n_group ? s_group[i] : 0) << p.gshift) - v.lead + (threadIdx.x % lanes) * kWaveLoad;
+        c[j] = load_chunk(v, at0[j]);
+      }
+      uint32_t hits = 0;  // a bit for each that reaches the bound; they are few
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float l[kWaveLoad];
+        chunk_logits(v, at0[j], c[j], l);
+#pragma unroll
+        for (int u = 0; u < kWaveLoad; ++u)
+          hits |= i0 + j * per < n_group && key_of(l[u]) >= bound ? 1u << (j * kWaveLoad + u) : 0u;
+      }
+      int at = append(&s_n, __popc(hits));
+      for (; hits != 0; hits &= hits - 1, ++at) {
+        const int b = __ffs((int)hits) - 1, j = b / kWaveLoad;
+        const int64_t i = (j == 0 ? at0[0] : j == 1 ? at0[1] : j == 2 ? at0[2] : at0[3]) + b % kWaveLoad;
+        if (at < kList) s_list[at] = place_of(key_of((float)v.row[i]), i);
+      }
     }
     __syncthreads();
     n = s_n;
+    if (n <= kFew) {
+      // few tokens, by one wave without barriers: each against all, for its place in the order and the weight before
+      // it, then for the kept weight before it by index
+      if (wave_id() != 0) return;
+      const int lane = lane_id();
+      u64 place[2], w[2], at[2] = {0, 0};
+      double rel[2];
+      int rank[2] = {0, 0};
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        place[i] = lane + 64 * i < n ? s_list[lane + 64 * i] : 0;
+        rel[i] = place[i] != 0 ? wt.rel(key_at(place[i])) : 0;
+        s_w[lane + 64 * i] = w[i] = wt.fix(rel[i]);
+      }
+      if (lane < 4) s_list[n + lane] = s_w[kFew + lane] = 0;  // to a multiple of 4
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      for (int j = 0; j < n; j += 4)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const u64 y = s_list[j + u], wy = s_w[j + u];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            rank[i] += y > place[i];
+            at[i] += y > place[i] ? wy : 0;
+          }
+        }
+      u64 z = 0, total = 0;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) z += place[i] != 0 && rank[i] < s.k ? w[i] : 0;
+      z = wave_sum64(z);
+      const double pz = s.p < 1 ? s.p * (double)z : kPosInf, limit = pz > 0 ? pz : 0.5;
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const bool keep = place[i] != 0 && rank[i] < s.k && (double)at[i] < limit && rel[i] >= s.min_p;
+        w[i] = keep ? w[i] : 0;
+        s_w[lane + 64 * i] = w[i];
+        total += w[i];
+        at[i] = 0;
+      }
+      total = wave_sum64(total);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      for (int j = 0; j < n; j += 4)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const u64 y = s_list[j + u], wy = s_w[j + u];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) at[i] += (uint32_t)y > (uint32_t)place[i] ? wy : 0;
+        }
+      const u64 target = target_of(total);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (at[i] <= target && at[i] + w[i] > target) draw(place[i], total);
+      return;
+    }
   } else if (kind == kTopPRow) {
-    n = p.n_list[q];
-    for (int i = threadIdx.x; i < n && i < kList; i += kRowThreads) s_list[i] = p.list[q * kList + i];
+    n = n_list;
+    if ((int)threadIdx.x < n) s_list[threadIdx.x] = list0;
+    for (int i = threadIdx.x + kRowThreads; i < n && i < kList; i += kRowThreads) s_list[i] = p.list[q * kList + i];
   }
+  __syncthreads();
   if (kind == kWholeRow || n > kList) {
-    __syncthreads();
     sample_row<T>(a, r, s, wt, RowShared{s_sum, s_out, s_w, reinterpret_cast<uint32_t*>(s_list)});
     return;
   }
 
-  u64 cut = 0, total = 0;  // the last token of the prefix (0: every token), the kept weight
-  int kept = 0;            // entries of the list up to the last that is in the prefix and not below min_p
+  u64 cut = 0;  // the last token of the prefix (0: every token)
+  for (int i = threadIdx.x; i < p.n_sub; i += kRowThreads) s_sub[i] = 0;
   if (n > 0) {
-    const int n2 = pow2_at_least(n);
+    // The cut: counts and weights of the list's tokens per bin of their distance below the largest key; with top-k the
+    // bin in which the k-th lies, and in it the cut and the weight up to it; then the bin in which the weight passes
+    // the limit of top-p.  A bin holds few tokens, each compared with all; one that holds over kFew (equal
+    // logits) has the whole list sorted instead.
+    const u64 before_list = kind == kTopPRow ? crossing[1] : 0;
+    u64* const bin_w = s_w;                                                     // [kBins]
+    uint32_t* const bin_n = reinterpret_cast<uint32_t*>(s_w + kBins);           // [kBins]
+    u64* const few = s_w + kBins + kBins / 2;                                   // [kFew] places, then weights
+    if (threadIdx.x == 0) s_n = s_m = 0;
+    for (int i = threadIdx.x; i < kBins + kBins / 2; i += kRowThreads) s_w[i] = 0;
     __syncthreads();
-    for (int i = n + threadIdx.x; i < n2; i += kRowThreads) s_list[i] = 0;
-    bitonic_sort<true>(s_list, n2);
-    u64 place[kPer], w[kPer], sum = 0, all;
-    double rel[kPer];
+    u64 place[kPer], w[kPer];
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      const bool in = t0 + i < n && (kind != kTopKRow || t0 + i < s.k);
-      place[i] = in ? s_list[t0 + i] : 0;
-      rel[i] = in ? wt.rel(key_at(place[i])) : 0;
-      sum += w[i] = wt.fix(rel[i]);
+      const int at = threadIdx.x + i * kRowThreads;
+      place[i] = at < n ? s_list[at] : 0;
+      const double rel = place[i] != 0 ? wt.rel(key_at(place[i])) : 0;
+      w[i] = wt.fix(rel);
+      if (place[i] != 0) {
+        const int bin = distance_bin(wt.key_m - key_at(place[i]));
+        atomicAdd(&bin_n[bin], 1u);
+        if (w[i]) atomicAdd(&bin_w[bin], w[i]);
+      }
+      if (!(rel >= s.min_p)) w[i] = 0;  // from here on: the weight it is drawn with
     }
-    u64 at = block_before64<kRowWaves>(sum, s_sum, &all);
-    double limit = s.p < 1 ? s.p * (double)all : kPosInf;
-    if (kind == kTopPRow) {
-      at += p.crossing[q * 2 + 1];
-      u64 z = 0, x;
-      for (int i = threadIdx.x; i < kBins; i += kRowThreads) z += p.hist[q * kBins + i];
-      x = block_sum64<kRowWaves>(z, s_sum);
-      limit = s.p * (double)x;
-    }
-    if (!(limit > 0)) limit = 0.5;
-    u64 n_prefix = 0, kept_w = 0;
-    if (threadIdx.x == 0) s_n = 0;
     __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const bool prefix = place[i] != 0 && (double)at < limit;
-      at += w[i];
-      const bool keep = prefix && rel[i] >= s.min_p;
-      n_prefix += prefix;
-      if (keep) atomicMax(&s_n, t0 + i + 1);
-      kept_w += keep ? w[i] : 0;
-      if (kind == kTopKRow) s_w[t0 + i] = keep ? w[i] : 0;
-      rel[i] = keep ? 1 : 0;
-    }
-    n_prefix = block_sum64<kRowWaves>(n_prefix, s_sum);
-    total = block_sum64<kRowWaves>(kept_w, s_sum);
-    kept = s_n;
-    cut = s_list[n_prefix - 1];
-    __syncthreads();
-    if (kind == kTopKRow) {
-      // the kept ones by index, each with its place in the order
+    const u64 w0 = bin_w[j0], w1 = bin_w[j0 + 1];
+    const uint32_t n0 = bin_n[j0], n1 = bin_n[j0 + 1];
+    u64 all_w, all_n;
+    const u64 at_w = before_list + block_before64<kRowWaves>(w0 + w1, s_sum, &all_w);
+    const u64 at_n = block_before64<kRowWaves>(n0 + n1, s_sum, &all_n);
+    const u64 k = kind == kTopKRow && (u64)s.k < all_n ? (u64)s.k : all_n;
+    double limit = kPosInf;
+    if (kind == kTopPRow) limit = s.p * (double)crossing[2] > 0 ? s.p * (double)crossing[2] : 0.5;
+    // the tokens of a bin whose count or weight passes a limit, resolved by the first wave: s_out = the last token of
+    // the prefix and the weight up to it; false: too many
+    auto resolve = [&](bool mine0, bool mine1) -> bool {
+      if (mine0 || mine1) {
+        s_out[0] = mine0 ? j0 : j0 + 1;
+        s_out[1] = mine0 ? at_w : at_w + w0;
+        s_out[2] = mine0 ? at_n : at_n + n0;
+      }
+      __syncthreads();
+      const int bin = (int)s_out[0];
+      const u64 b_w = s_out[1], b_n = s_out[2];
+      const int m = (int)bin_n[bin];
+      if (m > kFew) return false;
 #pragma unroll
       for (int i = 0; i < kPer; ++i)
-        if (t0 + i < pow2_at_least(kept))
-          s_list[t0 + i] = t0 + i < kept ? (u64)index_at(place[i]) << 32 | (u64)(t0 + i) : ~0ull;
-      bitonic_sort<false>(s_list, pow2_at_least(kept));
-      const double uz = s.u * (double)total;
-      const u64 target = uz < (double)(total - 1) ? (u64)uz : total - 1;
-      u64 x[kPer];
-      sum = 0;
+        if (place[i] != 0 && distance_bin(wt.key_m - key_at(place[i])) == bin) few[atomicAdd(&s_m, 1)] = place[i];
+      __syncthreads();
+      if (wave_id() == 0) {
+        const int lane = lane_id();
+        u64 x[2], y[2], at[2] = {b_w, b_w};
+        u64 rank[2] = {b_n, b_n};
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) sum += x[i] = t0 + i < kept ? s_w[(uint32_t)s_list[t0 + i]] : 0;
-      at = block_before64<kRowWaves>(sum, s_sum, &all);
+        for (int i = 0; i < 2; ++i) {
+          x[i] = lane + 64 * i < m ? few[lane + 64 * i] : 0;
+          y[i] = x[i] != 0 ? wt.fix(wt.rel(key_at(x[i]))) : 0;
+          few[kFew + lane + 64 * i] = y[i];
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll 4
+        for (int j = 0; j < m; ++j) {
+          const u64 z = few[j], wz = few[kFew + j];
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        if (at <= target && at + x[i] > target) s_out[0] = s_list[t0 + i] >> 32;
-        at += x[i];
+          for (int i = 0; i < 2; ++i) {
+            rank[i] += z > x[i];
+            at[i] += z > x[i] ? wz : 0;
+          }
+        }
+        u64 last = ~0ull, sum = 0;  // the smallest place of the prefix
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const bool in = x[i] != 0 && rank[i] < k && (double)at[i] < limit;
+          last = in && x[i] < last ? x[i] : last;
+          sum += in ? y[i] : 0;
+        }
+        last = ~wave_max64(~last);
+        sum = wave_sum64(sum);
+        if (lane == 0) {
+          s_out[0] = last;
+          s_out[1] = b_w + sum;
+          s_m = 0;
+        }
+      }
+      __syncthreads();
+      cut = s_out[0];
+      return true;
+    };
+    bool done = true;
+    if (kind == kTopKRow) {
+      const bool in0 = at_n < k && at_n + n0 >= k, in1 = at_n + n0 < k && at_n + n0 + n1 >= k;
+      done = resolve(in0, in1);
+      if (done && s.p < 1) {
+        const double pz = s.p * (double)s_out[1];
+        limit = pz > 0 ? pz : 0.5;
+        __syncthreads();
+        // the last bin that begins below the limit, of those up to the k-th's
+        const bool b0 = n0 > 0 && at_n < k && (double)at_w < limit;
+        const bool b1 = n1 > 0 && at_n + n0 < k && (double)(at_w + w0) < limit;
+        const bool e0 = b0 && ((double)(at_w + w0) >= limit || at_n + n0 >= k);
+        const bool e1 = b1 && ((double)(at_w + w0 + w1) >= limit || at_n + n0 + n1 >= k);
+        done = resolve(e0, e1 && !e0);
       }
     } else {
-      // their weights join their sub-blocks' sums
-      for (int i = threadIdx.x; i < p.n_sub; i += kRowThreads) s_sub[i] = 0;
+      const bool b0 = (double)at_w < limit && (double)(at_w + w0) >= limit;
+      const bool b1 = (double)(at_w + w0) < limit && (double)(at_w + w0 + w1) >= limit;
+      done = resolve(b0, b1);
+    }
+    if (!done) {
       __syncthreads();
+      const int n2 = pow2_at_least(n);
+      for (int i = n + threadIdx.x; i < n2; i += kRowThreads) s_list[i] = 0;
+      sort_descending(s_list, n2);
+      u64 sum = 0, x[kPer], all;
 #pragma unroll
-      for (int i = 0; i < kPer; ++i)
-        if (rel[i] != 0 && w[i]) atomicAdd(&s_sub[(index_at(place[i]) + v.lead) / kSub], w[i]);
-    }
-  }
-  if (kind != kTopKRow) {
-    // the sub-block that holds the token, then its place there
-    __syncthreads();
-    const int j0 = 2 * threadIdx.x;
-    u64 x[2], all;
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-      x[i] = j0 + i < p.n_sub ? p.sums[q * p.n_sub + j0 + i] + (n > 0 ? s_sub[j0 + i] : 0) : 0;
-    u64 at = block_before64<kRowWaves>(x[0] + x[1], s_sum, &all);
-    total = all;
-    const double uz = s.u * (double)total;
-    const u64 target = uz < (double)(total - 1) ? (u64)uz : total - 1;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      if (at <= target && at + x[i] > target) {
-        s_out[1] = j0 + i;
-        s_out[2] = at;
+      for (int i = 0; i < kPer; ++i) {
+        const bool in = t0 + i < n && (u64)(t0 + i) < k;
+        sum += x[i] = in ? wt.fix(wt.rel(key_at(s_list[t0 + i]))) : 0;
       }
-      at += x[i];
-    }
-    __syncthreads();
-    const int64_t i0 = (int64_t)s_out[1] * kSub - v.lead + 2 * threadIdx.x;
-    at = s_out[2];
-    u64 w[2];
+      u64 at = before_list + block_before64<kRowWaves>(sum, s_sum, &all);
+      if (kind == kTopKRow && s.p < 1) limit = s.p * (double)all > 0 ? s.p * (double)all : 0.5;
+      u64 prefix = 0;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const uint32_t key = i0 + i >= 0 && i0 + i < v.V ? key_of((float)v.row[i0 + i]) : 0;
-      const u64 place = place_of(key, i0 + i);
-      const double rel = wt.rel(key);
-      w[i] = place != 0 && place >= cut && rel >= s.min_p ? wt.fix(rel) : 0;
+      for (int i = 0; i < kPer; ++i) {
+        prefix += t0 + i < n && (u64)(t0 + i) < k && (double)at < limit;
+        at += x[i];
+      }
+      prefix = block_sum64<kRowWaves>(prefix, s_sum);
+      cut = s_list[prefix - 1];
     }
-    at += block_before64<kRowWaves>(w[0] + w[1], s_sum, &all);
+    // the prefix's tokens join the sub-blocks' sums (with top-k they are all there is)
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      if (at <= target && at + w[i] > target) s_out[0] = (u64)(i0 + i);
-      at += w[i];
+    for (int i = 0; i < kPer; ++i)
+      if (place[i] >= cut && w[i]) atomicAdd(&s_sub[(index_at(place[i]) + v.lead) / kSub], w[i]);
+  }
+  // the sub-block that holds the token, then its place there
+  __syncthreads();
+  u64 total;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    if (kind == kTopKRow) sub[i] = 0;
+    if (j0 + i < p.n_sub) sub[i] += s_sub[j0 + i];
+  }
+  u64 at = block_before64<kRowWaves>(sub[0] + sub[1], s_sum, &total);
+  const u64 target = target_of(total);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    if (at <= target && at + sub[i] > target) {
+      s_out[0] = j0 + i;
+      s_out[1] = at;
     }
+    at += sub[i];
   }
   __syncthreads();
-  if (threadIdx.x == 0) {
-    const int64_t token = (int64_t)s_out[0];
-    const uint32_t key = key_of((float)v.row[token]);
-    const double rel = key == wt.key_m ? 0.0 : ((double)logit_of(key) - wt.m) / s.tau;
-    a.token[r] = token;
-    a.logprob[r] = (float)(rel - log((double)total / a.one));
+  const int64_t i0 = (int64_t)s_out[0] * kSub - v.lead + 2 * threadIdx.x;
+  at = s_out[1];
+  u64 place[2], w[2], all;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    place[i] = i0 + i >= 0 && i0 + i < v.V ? place_of(key_of((float)v.row[i0 + i]), i0 + i) : 0;
+    const double rel = wt.rel(key_at(place[i]));
+    w[i] = place[i] != 0 && place[i] >= cut && rel >= s.min_p ? wt.fix(rel) : 0;
+  }
+  at += block_before64<kRowWaves>(w[0] + w[1], s_sum, &all);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    if (at <= target && at + w[i] > target) draw(place[i], total);
+    at += w[i];
   }
 }
 
@@ -921,7 +1174,7 @@ struct StagedSizes {
 StagedSizes staged_sizes(int64_t R, int64_t V) {
   const size_t rows = (size_t)(R < kRowsMost ? R : kRowsMost), subs = (size_t)subs_of(V);
   return {align256(rows * subs * 8), align256(rows * kGroups * 4), align256(rows * kBins * 8), align256(rows * kList * 8),
-          align256(rows * 4), align256(rows * subs * 8), align256(rows * 16)};
+          align256(rows * 4), align256(rows * subs * 8), align256(rows * kCross * 8)};
 }
 
 template <class T>
@@ -929,6 +1182,9 @@ hipError_t run_staged(const SampleParams& a, char* ws, hipStream_t stream) {
   Staged p{};
   p.a = a;
   p.n_sub = subs_of(a.V);
+  // A sub-block per wave.  With 2, 4 and 9 each, 512 rows of 151936 with settings of their own take the three launches
+  // 181, 206 and 269 us, so 151: a launch passes over many rows, and the others need workgroups enough for every CU.
+  p.n_seg = (p.n_sub + 3) / 4;
   p.gshift = 3;
   while (((int64_t)p.n_sub * kSub) >> p.gshift > kGroups) ++p.gshift;
   const StagedSizes z = staged_sizes(a.R, a.V);
@@ -942,16 +1198,15 @@ hipError_t run_staged(const SampleParams& a, char* ws, hipStream_t stream) {
   // rows' kinds, as far as the host knows them
   const bool greedy = !a.tau_rows && !(a.tau > 0);
   const bool all_k = !a.k_rows && a.k > 0 && a.k < a.V;
-  const bool may_p = !greedy && !all_k && (a.p_rows || a.p < 1), may_sum = !greedy && !all_k;
+  p.may_k = !greedy && (a.k_rows || (all_k && a.k <= kTopK));
+  p.may_p = !greedy && !all_k && (a.p_rows || a.p < 1);
+  p.may_sum = !greedy && !all_k;
   for (p.r0 = 0; p.r0 < a.R; p.r0 += kRowsMost) {
     const int64_t rows = a.R - p.r0 < kRowsMost ? a.R - p.r0 : kRowsMost;
-    // about 1024 workgroups for all rows, a sub-block at least per wave
-    const int64_t want = (1024 + rows - 1) / rows, most = (p.n_sub + 3) / 4;
-    p.n_seg = (int)(want < most ? want : most);
     const unsigned blocks = (unsigned)(rows * p.n_seg);
     sample_max_kernel<T><<<blocks, 256, 0, stream>>>(p);
-    if (may_p) sample_hist_kernel<T><<<blocks, 256, 0, stream>>>(p);
-    if (may_sum) sample_sums_kernel<T><<<blocks, 256, 0, stream>>>(p);
+    if (p.may_p) sample_hist_kernel<T><<<blocks, 256, 0, stream>>>(p);
+    if (p.may_sum) sample_sums_kernel<T><<<blocks, 256, 0, stream>>>(p);
     sample_finish_kernel<T><<<(unsigned)rows, kRowThreads, 0, stream>>>(p);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
