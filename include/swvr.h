@@ -332,17 +332,19 @@ int swvr_embedding_bwd(int dtype, int id64, int64_t N, int64_t V, int64_t D, con
  * stride ldt, t_dtype).  An entry with a negative id or a teacher logit of -inf is
  * absent; a token without entries, or of weight 0, has term 0.  An id of V or
  * more makes its token's term NaN.  Ids may repeat within a token.  weight: fp32
- * [N] or NULL (1).  T is 1 to SWVR_MAX_TEACHER.  h, W, bias as in swvr_fwd_mixed.
+ * [N] or NULL (1).  T is 1 to SWVR_MAX_TEACHER.  h, W as in swvr_fwd_mixed; bias [V] in
+ * its own dtype or NULL, and with it bias_scaled [V], which gets bias / temperature.
  * lse [N] is written, c [1] too (not for NONE).  For the gradient: p and q
  * ([N,T], the teacher's and the student's probabilities at the ids) and coef [N]
  * are written (all NULL: no gradient).
- * swvr_distill_bwd takes them back with g, the gradient of out ([N] or one
- * value), and writes gh [N,K], gW [V,K] (their dtype tags) and gb [V] (fp32);
+ * swvr_distill_bwd takes them and bias_scaled back with g, the gradient of out
+ * ([N] or one value), and writes gh [N,K], gW [V,K] and gb [V] (their dtype tags);
  * each may be NULL.  Only ids is read of the teacher's lists.  chunk as in swvr_bwd. */
 #define SWVR_MAX_TEACHER 1024
 size_t swvr_distill_workspace_size(int dtype, int64_t N, int64_t K, int64_t V, int64_t T, int weighted);
 int swvr_distill(int dtype, int h_dtype, int w_dtype, int64_t N, int64_t K, int64_t V, int64_t T,
-                 const void* h, int64_t ldh, const void* W, int64_t ldw, const float* bias, float logit_scale,
+                 const void* h, int64_t ldh, const void* W, int64_t ldw, const void* bias, int bias_dtype,
+                 float* bias_scaled, float logit_scale,
                  const void* ids, int id64, int64_t ldi, const void* teacher, int t_dtype, int64_t ldt,
                  float temperature, const float* weight, float z_loss_weight, int reduction,
                  float* out, float* c, float* lse, float* p, float* q, float* coef,
@@ -350,10 +352,12 @@ int swvr_distill(int dtype, int h_dtype, int w_dtype, int64_t N, int64_t K, int6
 size_t swvr_distill_bwd_workspace_size(int dtype, int w_dtype, int64_t N, int64_t K, int64_t V, int64_t T,
                                        int64_t chunk, int need_gh);
 int swvr_distill_bwd(int dtype, int h_dtype, int w_dtype, int64_t N, int64_t K, int64_t V, int64_t T,
-                     const void* h, int64_t ldh, const void* W, int64_t ldw, const float* bias, float logit_scale,
+                     const void* h, int64_t ldh, const void* W, int64_t ldw, const float* bias_scaled,
+                     float logit_scale,
                      const void* ids, int id64, int64_t ldi, float temperature, float z_loss_weight, int reduction,
                      const float* g, const float* c, const float* lse, const float* p, const float* q,
-                     const float* coef, int64_t chunk, void* gh, int gh_dtype, void* gW, int gW_dtype, float* gb,
+                     const float* coef, int64_t chunk, void* gh, int gh_dtype, void* gW, int gW_dtype,
+                     void* gb, int gb_dtype,
                      void* workspace, size_t workspace_bytes, void* stream);
 
 /* One token per row of logits [R,V] (row stride ld >= 0) from a uniform number u[r] in [0, 1)

@@ -185,7 +185,7 @@ int bwd_common(int dtype, int h_dtype, int w_dtype, int64_t N, int64_t K, int64_
   if (gW && !is_dtype(gW_dtype)) return fail(SWVR_EDTYPE, "unsupported gW dtype tag %d", gW_dtype);
   if (gE && !is_dtype(gE_dtype)) return fail(SWVR_EDTYPE, "unsupported gE dtype tag %d", gE_dtype);
   if (gb && !bias) return fail(SWVR_EINVAL, "gb requested without a bias");
-  if (N > 0 && (!lse || !glse || (D > 0 && (!O || !gO)))) return fail(SWVR_EINVAL, "O, lse, gO and glse must be non-null");
+  if (N > 0 && (!lse || (!glse && !pt_id) || (D > 0 && (!O || !gO)))) return fail(SWVR_EINVAL, "O, lse, gO and glse must be non-null");
   BwdPlan plan;
   if (!bwd_plan(dtype, N, K, V, D, chunk, gh != nullptr, &plan, w_dtype != dtype, hq ? K8 : 0))
     return fail(SWVR_EDTYPE, "no backward kernel for dtype %d, D=%lld", dtype, (long long)D);
@@ -479,17 +479,19 @@ static int check_distill(int dtype, int64_t N, int64_t V, int64_t T, int id64, c
 size_t swvr_distill_workspace_size(int dtype, int64_t N, int64_t K, int64_t V, int64_t T, int weighted) {
   FwdPlan plan;
   if (N < 0 || V < 0 || T < 0 || !fwd_plan(dtype, N, K, V, 0, &plan, weighted != 0)) return 0;
-  return up256(plan.ws_bytes) + up256((size_t)N * T * 4) + up256((size_t)V * 4) + up256(swvr::distill_part_bytes(N));
+  return up256(plan.ws_bytes) + up256((size_t)N * T * 4) + up256(swvr::distill_part_bytes(N));
 }
 
 int swvr_distill(int dtype, int h_dtype, int w_dtype, int64_t N, int64_t K, int64_t V, int64_t T, const void* h,
-                 int64_t ldh, const void* W, int64_t ldw, const float* bias, float logit_scale, const void* ids,
-                 int id64, int64_t ldi, const void* teacher, int t_dtype, int64_t ldt, float temperature,
-                 const float* weight, float z_loss_weight, int reduction, float* out, float* c, float* lse, float* p,
+                 int64_t ldh, const void* W, int64_t ldw, const void* bias, int bias_dtype, float* bias_scaled,
+                 float logit_scale, const void* ids, int id64, int64_t ldi, const void* teacher, int t_dtype, int64_t ldt,
+                 float temperature, const float* weight, float z_loss_weight, int reduction, float* out, float* c, float* lse, float* p,
                  float* q, float* coef, void* workspace, size_t workspace_bytes, void* stream) {
   int rc = check_distill(dtype, N, V, T, id64, ids, ldi, temperature, reduction);
   if (rc != SWVR_OK) return rc;
   if (!is_dtype(t_dtype)) return fail(SWVR_EDTYPE, "unsupported teacher dtype tag %d", t_dtype);
+  if (bias && !is_dtype(bias_dtype)) return fail(SWVR_EDTYPE, "unsupported bias dtype tag %d", bias_dtype);
+  if (bias && !bias_scaled) return fail(SWVR_EINVAL, "bias_scaled must be non-null with a bias");
   if (ldt < 0) return fail(SWVR_EINVAL, "ldt=%lld must not be negative", (long long)ldt);
   if (N > 0 && (!teacher || !lse)) return fail(SWVR_EINVAL, "teacher logits and lse must be non-null");
   if ((N > 0 || reduction) && !out) return fail(SWVR_EINVAL, "out must be non-null");
@@ -505,16 +507,14 @@ int swvr_distill(int dtype, int h_dtype, int w_dtype, int64_t N, int64_t K, int6
   fwd_plan(dtype, N, K, V, 0, &plan, weight != nullptr);
   const size_t fwd_bytes = plan.ws_bytes;
   float* z = reinterpret_cast<float*>(ws + up256(fwd_bytes));
-  float* sb = z + up256((size_t)N * T * 4) / 4;
-  float* part = sb + up256((size_t)V * 4) / 4;
+  float* part = z + up256((size_t)N * T * 4) / 4;
   const float inv_tau = 1.f / temperature, scale = logit_scale / temperature;
   hipError_t e = hipSuccess;
-  if (bias && temperature != 1.f) {
-    if ((e = swvr::distill_scale(bias, V, inv_tau, sb, s)) != hipSuccess) return hip_fail(e, "bias launch");
-    bias = sb;
-  }
+  if (bias && (e = swvr::distill_scale(bias, bias_dtype, V, inv_tau, bias_scaled, s)) != hipSuccess)
+    return hip_fail(e, "bias launch");
+  const float* const sb = bias ? bias_scaled : nullptr;
   // the log-sum-exps: a readout without columns
-  rc = fwd_common(dtype, h_dtype, w_dtype, N, K, V, 0, h, ldh, W, ldw, W, 0, bias, scale, nullptr, lse, nullptr, nullptr,
+  rc = fwd_common(dtype, h_dtype, w_dtype, N, K, V, 0, h, ldh, W, ldw, W, 0, sb, scale, nullptr, lse, nullptr, nullptr,
                   workspace, fwd_bytes, stream, weight != nullptr, weight);
   if (rc != SWVR_OK) return rc;
   swvr::DistillParams d{};
@@ -524,7 +524,7 @@ int swvr_distill(int dtype, int h_dtype, int w_dtype, int64_t N, int64_t K, int6
   d.ldw = ldw;
   d.h_f32 = h_dtype != dtype;
   d.w_f32 = w_dtype != dtype;
-  d.bias = bias;
+  d.bias = sb;
   d.scale = scale;
   d.inv_tau = inv_tau;
   d.N = (int)N;
@@ -556,22 +556,22 @@ size_t swvr_distill_bwd_workspace_size(int dtype, int w_dtype, int64_t N, int64_
   BwdPlan plan;
   if (N < 0 || V < 0 || T < 0 || chunk <= 0 || !bwd_plan(dtype, N, K, V, 0, chunk, need_gh != 0, &plan, w_dtype != dtype))
     return 0;
-  return up256(plan.ws_bytes) + up256((size_t)V * 4) + up256((size_t)N * 4) + 5 * up256((size_t)N * T * 4) +
-         up256((size_t)(V + 1) * 4);
+  return up256(plan.ws_bytes) + up256((size_t)V * 4) + 5 * up256((size_t)N * T * 4) + up256((size_t)(V + 1) * 4);
 }
 
 int swvr_distill_bwd(int dtype, int h_dtype, int w_dtype, int64_t N, int64_t K, int64_t V, int64_t T, const void* h,
-                     int64_t ldh, const void* W, int64_t ldw, const float* bias, float logit_scale, const void* ids,
-                     int id64, int64_t ldi, float temperature, float z_loss_weight, int reduction, const float* g,
+                     int64_t ldh, const void* W, int64_t ldw, const float* bias_scaled, float logit_scale,
+                     const void* ids, int id64, int64_t ldi, float temperature, float z_loss_weight, int reduction, const float* g,
                      const float* c, const float* lse, const float* p, const float* q, const float* coef,
-                     int64_t chunk, void* gh, int gh_dtype, void* gW, int gW_dtype, float* gb, void* workspace,
-                     size_t workspace_bytes, void* stream) {
+                     int64_t chunk, void* gh, int gh_dtype, void* gW, int gW_dtype, void* gb, int gb_dtype,
+                     void* workspace, size_t workspace_bytes, void* stream) {
   int rc = check_distill(dtype, N, V, T, id64, ids, ldi, temperature, reduction);
   if (rc != SWVR_OK) return rc;
   if (chunk <= 0) return fail(SWVR_EINVAL, "chunk must be positive, got %lld", (long long)chunk);
   if (N > 0 && (!g || !lse || !p || !q || !coef || (reduction && !c)))
     return fail(SWVR_EINVAL, "g, c, lse, p, q and coef must be non-null");
-  if (gb && !bias) return fail(SWVR_EINVAL, "gb requested without a bias");
+  if (gb && !bias_scaled) return fail(SWVR_EINVAL, "gb requested without a bias");
+  if (gb && !is_dtype(gb_dtype)) return fail(SWVR_EDTYPE, "unsupported gb dtype tag %d", gb_dtype);
   const size_t need = swvr_distill_bwd_workspace_size(dtype, w_dtype, N, K, V, T, chunk, gh != nullptr);
   if (!workspace || workspace_bytes < need)
     return fail(SWVR_EWORKSPACE, "distillation workspace of %zu bytes needed, %zu given", need, workspace_bytes);
@@ -584,8 +584,7 @@ int swvr_distill_bwd(int dtype, int h_dtype, int w_dtype, int64_t N, int64_t K, 
     at += up256(bytes);
     return x;
   };
-  float* sb = reinterpret_cast<float*>(take((size_t)V * 4));
-  float* glse = reinterpret_cast<float*>(take((size_t)N * 4));
+  float* dense = reinterpret_cast<float*>(take((size_t)V * 4));
   const size_t nt = (size_t)N * T * 4;
   int* pt_id = reinterpret_cast<int*>(take(nt));
   float* pt_val = reinterpret_cast<float*>(take(nt));
@@ -595,10 +594,6 @@ int swvr_distill_bwd(int dtype, int h_dtype, int w_dtype, int64_t N, int64_t K, 
   int* seg = reinterpret_cast<int*>(take((size_t)(V + 1) * 4));
   const float inv_tau = 1.f / temperature;
   hipError_t e = hipSuccess;
-  if (bias && temperature != 1.f) {
-    if ((e = swvr::distill_scale(bias, V, inv_tau, sb, s)) != hipSuccess) return hip_fail(e, "bias launch");
-    bias = sb;
-  }
   if (N > 0) {
     swvr::DistillGradParams d{};
     d.N = (int)N;
@@ -615,20 +610,21 @@ int swvr_distill_bwd(int dtype, int h_dtype, int w_dtype, int64_t N, int64_t K, 
     d.q = q;
     d.coef = coef;
     d.zw = z_loss_weight;
-    d.glse = glse;
+    d.delta = reinterpret_cast<float*>(static_cast<char*>(workspace) + plan.off_delta);
+    d.flag = reinterpret_cast<int*>(static_cast<char*>(workspace) + plan.off_flag);
     d.pt_id = pt_id;
     d.pt_val = pt_val;
     d.pt_t = gb ? pt_t : nullptr;
     if ((e = swvr::distill_prep(d, s)) != hipSuccess) return hip_fail(e, "distillation launch");
   }
-  rc = bwd_common(dtype, h_dtype, w_dtype, N, K, V, 0, h, ldh, W, ldw, W, 0, bias, logit_scale / temperature, nullptr,
-                  lse, nullptr, glse, chunk, gh, gh_dtype, gW, gW_dtype, nullptr, 0, gb, workspace,
+  rc = bwd_common(dtype, h_dtype, w_dtype, N, K, V, 0, h, ldh, W, ldw, W, 0, bias_scaled, logit_scale / temperature,
+                  nullptr, lse, nullptr, nullptr, chunk, gh, gh_dtype, gW, gW_dtype, nullptr, 0, gb ? dense : nullptr, workspace,
                   up256(plan.ws_bytes), stream, nullptr, 0, 0, nullptr, nullptr, 0, nullptr, pt_id, pt_val, N * T,
                   (int)T);
   if (rc != SWVR_OK) return rc;
-  if (gb && N > 0 && V > 0) {
+  if (gb && V > 0) {
     if ((e = swvr::sort_ids(pt_id, 0, (int)(N * T), (int)V, order, sid, seg, s)) != hipSuccess ||
-        (e = swvr::distill_bias(order, seg, pt_t, (int)V, inv_tau, gb, s)) != hipSuccess)
+        (e = swvr::distill_bias(order, seg, pt_t, dense, (int)V, inv_tau, gb, gb_dtype, s)) != hipSuccess)
       return hip_fail(e, "bias gradient launch");
   }
   return SWVR_OK;

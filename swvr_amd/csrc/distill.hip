@@ -44,17 +44,16 @@ __device__ __forceinline__ int64_t id_at(const DistillParams& p, int n, int k) {
   return p.id64 ? static_cast<const int64_t*>(p.ids)[i] : (int64_t)static_cast<const int*>(p.ids)[i];
 }
 
-__device__ __forceinline__ float teacher_at(const DistillParams& p, int n, int k) {
-  const int64_t i = (int64_t)n * p.ldt + k;
-  return p.t_dtype == kBF16  ? (float)static_cast<const bf16_t*>(p.teacher)[i]
-         : p.t_dtype == kF16 ? (float)static_cast<const f16_t*>(p.teacher)[i]
-                             : static_cast<const float*>(p.teacher)[i];
+__device__ __forceinline__ float load_as(const void* x, int64_t i, int dtype) {
+  return dtype == kBF16  ? (float)static_cast<const bf16_t*>(x)[i]
+         : dtype == kF16 ? (float)static_cast<const f16_t*>(x)[i]
+                         : static_cast<const float*>(x)[i];
 }
 
-__global__ __launch_bounds__(256) void distill_scale_kernel(const float* __restrict__ x, int64_t n, float s,
+__global__ __launch_bounds__(256) void distill_scale_kernel(const void* __restrict__ x, int dtype, int64_t n, float s,
                                                             float* __restrict__ y) {
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i < n) y[i] = x[i] * s;
+  if (i < n) y[i] = load_as(x, i, dtype) * s;
 }
 
 // 8 consecutive values of a row stored as S, rounded to the compute dtype T.
@@ -112,71 +111,80 @@ __global__ __launch_bounds__(256) void distill_dot_kernel(DistillParams p) {
   }
 }
 
-// One wave per token, 16 tokens per workgroup; the workgroup's sums of the terms and of the weights in token
-// order (mse_loss's reduction).
-constexpr int kTokensPerWave = 4, kTokensPerBlock = 4 * kTokensPerWave;
+// One wave per token, 4 tokens per workgroup, the workgroup's sums of the terms and of the weights in token order.  The
+// first 64 entries stay in registers; longer lists are read again for each of the three passes (the largest, the sum of
+// exponentials, the terms).  (4 tokens per wave, one after another, took 11 us for 500 tokens.)
+constexpr int kTokensPerBlock = 4;
 __global__ __launch_bounds__(256) void distill_loss_kernel(DistillParams p, float* __restrict__ part, int n_blk) {
   __shared__ float s_loss[4], s_w[4];
   const int lane = lane_id(), wv = wave_id();
-  float wave_loss = 0.f, wave_w = 0.f;
-  for (int j = 0; j < kTokensPerWave; ++j) {
-    const int n = blockIdx.x * kTokensPerBlock + wv * kTokensPerWave + j;
-    if (n >= p.N) break;  // uniform across the wave
-    const float w = p.weight ? p.weight[n] : 1.f;
-    float m = kNegInf;
-    bool has = false;
-    for (int k = lane; k < p.T; k += 64) {
-      const float t = teacher_at(p, n, k) * p.inv_tau;
-      if (id_at(p, n, k) < 0 || t == kNegInf) continue;
-      has = true;
-      m = fmaxf(m, t);
+  const int n = blockIdx.x * kTokensPerBlock + wv;
+  float tok = 0.f, w = 0.f;
+  if (n < p.N) {
+    struct Entry {
+      int64_t id;
+      float t;  // -inf: absent
+    };
+    auto entry = [&](int k) {
+      Entry e;
+      e.id = id_at(p, n, k);
+      const float t = load_as(p.teacher, (int64_t)n * p.ldt + k, p.t_dtype) * p.inv_tau;
+      e.t = e.id < 0 ? kNegInf : t;
+      return e;
+    };
+    const Entry none{-1, kNegInf};
+    const Entry mine = lane < p.T ? entry(lane) : none;
+    const float z0 = lane < p.T && mine.id >= 0 && mine.id < p.V ? p.z[(int64_t)n * p.T + lane] : 0.f;
+    const float lse = p.lse[n];
+    w = p.weight ? p.weight[n] : 1.f;
+    // fmaxf leaves a NaN out; it comes back with the exponentials
+    float m = mine.t;
+    bool has = mine.t != kNegInf;
+    for (int k = lane + 64; k < p.T; k += 64) {
+      const Entry e = entry(k);
+      has |= e.t != kNegInf;
+      m = fmaxf(m, e.t);
     }
     m = wave_max(m);
-    const bool live = w != 0.f && __ballot(has) != 0;
-    if (!live) {
-      if (lane == 0) {
-        if (p.coef) p.coef[n] = 0.f;
-        if (p.reduce == 0) p.out[n] = 0.f;
+    if (w == 0.f || __ballot(has) == 0) w = 0.f;
+    if (w != 0.f) {
+      auto mass = [&](float t) { return t != kNegInf ? expf(t - m) : 0.f; };
+      float sum = mass(mine.t);
+      for (int k = lane + 64; k < p.T; k += 64) sum += mass(entry(k).t);
+      const float lp = m + logf(wave_sum(sum));
+      float kl = 0.f;
+      auto term = [&](const Entry& e, int k, float z) {
+        const float logq = e.id >= p.V ? __builtin_nanf("") : e.id >= 0 ? z - lse : kNegInf;
+        const float logp = e.t - lp, pk = e.t != kNegInf ? expf(logp) : 0.f;
+        if (pk != 0.f) kl += pk * (logp - logq);  // NaN != 0
+        if (p.p) {
+          p.p[(int64_t)n * p.T + k] = pk;
+          p.q[(int64_t)n * p.T + k] = e.id >= p.V ? 0.f : expf(logq);
+        }
+      };
+      if (lane < p.T) term(mine, lane, z0);
+      for (int k = lane + 64; k < p.T; k += 64) {
+        const Entry e = entry(k);
+        term(e, k, e.id >= 0 && e.id < p.V ? p.z[(int64_t)n * p.T + k] : 0.f);
       }
-      if (p.p)
-        for (int k = lane; k < p.T; k += 64) p.p[(int64_t)n * p.T + k] = p.q[(int64_t)n * p.T + k] = 0.f;
-      continue;
+      tok = wave_sum(kl);
+      if (p.zw != 0.f) tok += p.zw * (lse * lse);
+      tok *= w;
+    } else if (p.p) {
+      for (int k = lane; k < p.T; k += 64) p.p[(int64_t)n * p.T + k] = p.q[(int64_t)n * p.T + k] = 0.f;
     }
-    float sum = 0.f;
-    for (int k = lane; k < p.T; k += 64) {
-      const float t = teacher_at(p, n, k) * p.inv_tau;
-      if (id_at(p, n, k) >= 0 && t != kNegInf) sum += expf(t - m);
-    }
-    const float lp = m + logf(wave_sum(sum)), lse = p.lse[n];
-    float kl = 0.f;
-    for (int k = lane; k < p.T; k += 64) {
-      const int64_t id = id_at(p, n, k);
-      const float t = teacher_at(p, n, k) * p.inv_tau;
-      const float logq = id >= p.V ? __builtin_nanf("") : id >= 0 ? p.z[(int64_t)n * p.T + k] - lse : kNegInf;
-      const float logp = t - lp, pk = id >= 0 && t != kNegInf ? expf(logp) : 0.f;
-      if (pk != 0.f) kl += pk * (logp - logq);  // NaN != 0
-      if (p.p) {
-        p.p[(int64_t)n * p.T + k] = pk;
-        p.q[(int64_t)n * p.T + k] = id >= p.V ? 0.f : expf(logq);
-      }
-    }
-    kl = wave_sum(kl);
-    float tok = kl;
-    if (p.zw != 0.f) tok += p.zw * (lse * lse);
-    tok *= w;
     if (lane == 0) {
       if (p.coef) p.coef[n] = w;
       if (p.reduce == 0) p.out[n] = tok;
     }
-    wave_loss += tok;
-    wave_w += w;
   }
+  if (!part) return;
   if (lane == 0) {
-    s_loss[wv] = wave_loss;
-    s_w[wv] = wave_w;
+    s_loss[wv] = tok;
+    s_w[wv] = w;
   }
   __syncthreads();
-  if (threadIdx.x == 0 && part) {
+  if (threadIdx.x == 0) {
     part[blockIdx.x] = ((s_loss[0] + s_loss[1]) + s_loss[2]) + s_loss[3];
     part[n_blk + blockIdx.x] = ((s_w[0] + s_w[1]) + s_w[2]) + s_w[3];
   }
@@ -208,44 +216,60 @@ __global__ __launch_bounds__(256) void distill_reduce_kernel(const float* __rest
   }
 }
 
-// One wave per token: gLSE = c_n, and per entry the id (-1: no element of its own), dS there, and g_n p.
-// Entries of a token that repeat an id share one element of dS: the first of them holds their sum.
+// One wave per token: what the backward's first kernel would make of O = gO = 0 and gLSE = c_n (delta = -c_n and the
+// flag of an active token), and per entry the id (-1: no element of its own), dS there, and g_n p.  Entries of a
+// token that repeat an id share one element of dS: the first of them holds their sum.  The entries are compared 64
+// against 64, one side from a lane's registers at a time.
 __global__ __launch_bounds__(256) void distill_prep_kernel(DistillGradParams p) {
   const int n = blockIdx.x * 4 + wave_id();
   if (n >= p.N) return;
   const int lane = lane_id();
   const float w = p.coef[n];
   const float gn = w == 0.f ? 0.f : p.g[p.reduce == 0 ? n : 0] * w * (p.reduce == 0 ? 1.f : p.c[0]);
-  float cn = p.zw != 0.f ? gn * (1.f + 2.f * p.zw * p.lse[n]) : gn;
+  float cn = p.zw != 0.f && w != 0.f ? gn * (1.f + 2.f * p.zw * p.lse[n]) : gn;
   // the backward leaves out tokens of gLSE = 0: one whose two terms cancel stays
   if (cn == 0.f && gn != 0.f) cn = FLT_MIN;
-  if (w == 0.f) cn = 0.f;
-  if (lane == 0) p.glse[n] = cn;
-  for (int k = lane; k < p.T; k += 64) {
+  if (lane == 0) {
+    p.delta[n] = -cn;
+    p.flag[n] = cn != 0.f;  // NaN != 0
+  }
+  // ids as the matrix has them, -1 outside it
+  auto id_of = [&](int k) -> int {
+    if (k >= p.T || w == 0.f) return -1;
+    const int64_t i = (int64_t)n * p.ldi + k;
+    const int64_t id = p.id64 ? static_cast<const int64_t*>(p.ids)[i] : (int64_t)static_cast<const int*>(p.ids)[i];
+    return id >= 0 && id < p.V ? (int)id : -1;
+  };
+  for (int k = lane; k < (p.T + 63) / 64 * 64; k += 64) {
     const int64_t e = (int64_t)n * p.T + k;
-    const int64_t at = (int64_t)n * p.ldi;
-    auto id_of = [&](int j) {
-      return p.id64 ? static_cast<const int64_t*>(p.ids)[at + j] : (int64_t)static_cast<const int*>(p.ids)[at + j];
-    };
-    const int64_t id = id_of(k);
-    bool own = w != 0.f && id >= 0 && id < p.V;
+    const int id = id_of(k);
+    const float q = k < p.T ? p.q[e] : 0.f;
+    bool own = id >= 0;
     float sum = 0.f;
-    for (int j = 0; j < p.T; ++j) {
-      const bool same = id_of(j) == id;
-      if (same && j < k) own = false;
-      if (same) sum += p.p[(int64_t)n * p.T + j];
+    for (int j0 = 0; j0 < p.T; j0 += 64) {
+      const int id_j = j0 == k - lane ? id : id_of(j0 + lane);
+      const float p_j = j0 + lane < p.T ? p.p[(int64_t)n * p.T + j0 + lane] : 0.f;
+      const int most = min(64, p.T - j0);
+      for (int j = 0; j < most; ++j) {
+        const bool same = __builtin_amdgcn_readlane(id_j, j) == id;
+        own = own && !(same && j0 + j < k);
+        sum += same ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(p_j), j)) : 0.f;
+      }
     }
-    const float t = gn * sum;
-    p.pt_id[e] = own ? (int)id : -1;
-    p.pt_val[e] = cn * p.q[e] - t;
-    if (p.pt_t) p.pt_t[e] = t;
+    if (k < p.T) {
+      const float t = gn * sum;
+      p.pt_id[e] = own ? id : -1;
+      p.pt_val[e] = cn * q - t;
+      if (p.pt_t) p.pt_t[e] = t;
+    }
   }
 }
 
-// gb[v] = (gb[v] - sum of t over the entries of v) / tau, a wave per id.
+// gb[v] = (dense[v] - sum of t over the entries of v) / tau, a wave per id, in gb's dtype.
 __global__ __launch_bounds__(256) void distill_bias_kernel(const int* __restrict__ order, const int* __restrict__ seg,
-                                                           const float* __restrict__ t, int V, float inv_tau,
-                                                           float* __restrict__ gb) {
+                                                           const float* __restrict__ t,
+                                                           const float* __restrict__ dense, int V, float inv_tau,
+                                                           void* __restrict__ gb, int gb_dtype) {
   const int v = blockIdx.x * 4 + wave_id();
   if (v >= V) return;
   const int lane = lane_id(), i1 = seg[v + 1];
@@ -257,7 +281,14 @@ __global__ __launch_bounds__(256) void distill_bias_kernel(const int* __restrict
     s += (x[0] + x[1]) + (x[2] + x[3]);
   }
   s = wave_sum(s);
-  if (lane == 0) gb[v] = (gb[v] - s) * inv_tau;
+  if (lane != 0) return;
+  const float y = (dense[v] - s) * inv_tau;
+  if (gb_dtype == kBF16)
+    static_cast<bf16_t*>(gb)[v] = (bf16_t)y;
+  else if (gb_dtype == kF16)
+    static_cast<f16_t*>(gb)[v] = (f16_t)y;
+  else
+    static_cast<float*>(gb)[v] = y;
 }
 
 template <class T>
@@ -285,9 +316,9 @@ size_t distill_part_bytes(int64_t N) {
   return (size_t)((N + kTokensPerBlock - 1) / kTokensPerBlock) * 2 * sizeof(float);
 }
 
-hipError_t distill_scale(const float* x, int64_t n, float s, float* y, hipStream_t stream) {
+hipError_t distill_scale(const void* x, int dtype, int64_t n, float s, float* y, hipStream_t stream) {
   if (n == 0) return hipSuccess;
-  distill_scale_kernel<<<(unsigned)((n + 255) / 256), 256, 0, stream>>>(x, n, s, y);
+  distill_scale_kernel<<<(unsigned)((n + 255) / 256), 256, 0, stream>>>(x, dtype, n, s, y);
   return hipGetLastError();
 }
 
@@ -318,10 +349,10 @@ hipError_t distill_prep(const DistillGradParams& p, hipStream_t stream) {
   return hipGetLastError();
 }
 
-hipError_t distill_bias(const int* order, const int* seg, const float* t, int V, float inv_tau, float* gb,
-                        hipStream_t stream) {
+hipError_t distill_bias(const int* order, const int* seg, const float* t, const float* dense, int V, float inv_tau,
+                        void* gb, int gb_dtype, hipStream_t stream) {
   timing_begin(kKindDistill, stream);
-  distill_bias_kernel<<<(unsigned)((V + 3) / 4), 256, 0, stream>>>(order, seg, t, V, inv_tau, gb);
+  distill_bias_kernel<<<(unsigned)((V + 3) / 4), 256, 0, stream>>>(order, seg, t, dense, V, inv_tau, gb, gb_dtype);
   timing_end(kKindDistill, stream);
   return hipGetLastError();
 }

@@ -308,7 +308,8 @@ struct BwdParams {
   const float* w_scale;
   int K8;
   // elements of dS given by the caller (null pt_id: none): entry e of token e / pt_T has its value at vocabulary
-  // row pt_id[e] (-1: none; a row at most once per token)
+  // row pt_id[e] (-1: none; a row at most once per token).  With them, delta and the active flags are in the
+  // workspace already (D = 0: they follow from gLSE, which the caller forms)
   const int* pt_id;
   const float* pt_val;
   int64_t n_pt;
@@ -433,7 +434,8 @@ struct DistillParams {
   float* coef;           // [N] weights of the tokens that count (with p)
 };
 size_t distill_part_bytes(int64_t N);
-hipError_t distill_scale(const float* x, int64_t n, float s, float* y, hipStream_t stream);
+// y = x s in fp32.
+hipError_t distill_scale(const void* x, int dtype, int64_t n, float s, float* y, hipStream_t stream);
 // The loss from the log-sum-exps; c: [1], the reduction's factor (reduce != 0).
 hipError_t distill_loss(int dtype, const DistillParams& p, float* part, float* c, hipStream_t stream);
 struct DistillGradParams {
@@ -449,14 +451,15 @@ struct DistillGradParams {
   const float* q;
   const float* coef;
   float zw;
-  float* glse;           // [N]
+  float* delta;          // [N] -gLSE
+  int* flag;             // [N] whether the token is active
   int* pt_id;            // [N][T]
   float* pt_val;         // [N][T]
   float* pt_t;           // [N][T] or null
 };
 hipError_t distill_prep(const DistillGradParams& p, hipStream_t stream);
-hipError_t distill_bias(const int* order, const int* seg, const float* t, int V, float inv_tau, float* gb,
-                        hipStream_t stream);
+hipError_t distill_bias(const int* order, const int* seg, const float* t, const float* dense, int V, float inv_tau,
+                        void* gb, int gb_dtype, hipStream_t stream);
 
 // ---------------------------------------------------------------- sampling
 struct SampleParams {

@@ -26,58 +26,71 @@ def _lists(x, keep, other):
     return x if x.stride(1) == 1 and x.stride(0) >= 0 else x.contiguous()
 
 
+def _kept(kept, N, T, need_grad):
+    """Addresses in the fp32 buffer a call keeps: c [1], lse [N], and for the gradient coef [N], p [N, T], q [N, T]."""
+    at = kept.data_ptr()
+    lse, coef = at + 4, at + 4 * (1 + N)
+    return (at, lse, coef, coef + 4 * N, coef + 4 * (N + N * T)) if need_grad else (at, lse, None, None, None)
+
+
 def _forward(h, W, bias, teacher, ids, weight, tau, z, reduction, scale, cdt, need_grad):
-    """The loss, and for the gradient (empty tensors without) c, lse, p, q, coef of swvr_distill."""
+    """The loss, what ``_kept`` names, and the bias over tau in fp32 (empty without a bias)."""
     lib = _lib.load()
     N, K = h.shape
     V, T = W.shape[0], ids.shape[1]
     Kp = _kpad(K)
     (hc, h_tag), (Wc, w_tag) = _operand(h, cdt, Kp), _operand(W, cdt, Kp)
-    b, w = _f32(bias), _f32(weight)
+    b, w = _bias(bias), _f32(weight)
     t = _lists(teacher, _lib.DTYPE_TAG, torch.float32)
     i = _lists(ids, (torch.int64, torch.int32), torch.int64)
     tag = _lib.DTYPE_TAG[cdt]
-
-    def new(*shape):
-        return torch.empty(shape, dtype=torch.float32, device=h.device)
-
-    out, c, lse = new(*((N,) if reduction == 0 else ())), new(), new(N)
-    p, q, coef = (new(N, T), new(N, T), new(N)) if need_grad else (new(0), new(0), new(0))
-    ws_bytes = lib.swvr_distill_workspace_size(tag, N, Kp, V, T, int(w is not None))
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=h.device)
+    out = hc.new_empty((N,) if reduction == 0 else (), dtype=torch.float32)
+    kept = hc.new_empty(1 + N * (2 * T + 2) if need_grad else 1 + N, dtype=torch.float32)
+    sb = hc.new_empty(V if b is not None else 0, dtype=torch.float32)
+    ws_bytes = lib.swvr_distill_workspace_size(tag, N, Kp, V, T, w is not None)
+    ws = hc.new_empty(ws_bytes, dtype=torch.uint8)
     a = _lib.address
+    c, lse, coef, p, q = _kept(kept, N, T, need_grad)
     _lib.call(lib.swvr_distill, h.device, tag, h_tag, w_tag, N, Kp, V, T, hc.data_ptr(), _lead_stride(hc),
-              Wc.data_ptr(), _lead_stride(Wc), a(b), scale, i.data_ptr(), i.dtype == torch.int64, i.stride(0),
-              t.data_ptr(), _lib.DTYPE_TAG[t.dtype], t.stride(0), tau, a(w), z, reduction, out.data_ptr(), c.data_ptr(),
-              lse.data_ptr(), *(map(a, (p, q, coef)) if need_grad else (None,) * 3), ws.data_ptr(), ws_bytes)
-    return out, c, lse, p, q, coef
+              Wc.data_ptr(), _lead_stride(Wc), a(b), _lib.DTYPE_TAG[b.dtype] if b is not None else 0, sb.data_ptr(),
+              scale, i.data_ptr(), i.dtype == torch.int64, i.stride(0), t.data_ptr(), _lib.DTYPE_TAG[t.dtype],
+              t.stride(0), tau, a(w), z, reduction, out.data_ptr(), c, lse, p, q, coef, ws.data_ptr(), ws_bytes)
+    return out, kept, sb
 
 
-def _backward(g, h, W, bias, ids, c, lse, p, q, coef, tau, z, reduction, scale, chunk, cdt, need_h, need_W, need_b):
+def _bias(bias):
+    """``bias`` dense, in a dtype the library reads (or None)."""
+    if bias is None:
+        return None
+    b = _plain(bias)
+    return (b if b.dtype in _lib.DTYPE_TAG else b.to(torch.float32)).contiguous()
+
+
+def _backward(g, h, W, bias, ids, kept, sb, tau, z, reduction, scale, chunk, cdt, need_h, need_W, need_b):
     lib = _lib.load()
     N, K = h.shape
     V, T = W.shape[0], ids.shape[1]
     Kp = _kpad(K)
     (hc, h_tag), (Wc, w_tag) = _operand(h, cdt, Kp), _operand(W, cdt, Kp)
-    b, g32 = _f32(bias), _f32(g)
+    g32 = _f32(g)
     i = _lists(ids, (torch.int64, torch.int32), torch.int64)
     dev = h.device
     gh = _grad_buffer((N, Kp), h.dtype, dev) if need_h else None
     gW = _grad_buffer((V, Kp), W.dtype, dev) if need_W else None
-    gb = torch.empty(V, dtype=torch.float32, device=dev) if need_b else None
+    gb = _grad_buffer((V,), bias.dtype, dev) if need_b else None
     tag = _lib.DTYPE_TAG[cdt]
     chunk = _rows_staged(chunk, tag, w_tag, N, Kp, V, 0, need_h)
-    ws_bytes = lib.swvr_distill_bwd_workspace_size(tag, w_tag, N, Kp, V, T, chunk, int(need_h))
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+    ws_bytes = lib.swvr_distill_bwd_workspace_size(tag, w_tag, N, Kp, V, T, chunk, need_h)
+    ws = hc.new_empty(ws_bytes, dtype=torch.uint8)
 
-    def tag_of(x):
-        return _lib.DTYPE_TAG[x.dtype] if x is not None else 0
+    def of(x):
+        return (x.data_ptr(), _lib.DTYPE_TAG[x.dtype]) if x is not None else (None, 0)
 
-    a = _lib.address
+    c, lse, coef, p, q = _kept(kept, N, T, True)
     _lib.call(lib.swvr_distill_bwd, dev, tag, h_tag, w_tag, N, Kp, V, T, hc.data_ptr(), _lead_stride(hc),
-              Wc.data_ptr(), _lead_stride(Wc), a(b), scale, i.data_ptr(), i.dtype == torch.int64, i.stride(0), tau, z,
-              reduction, g32.data_ptr(), c.data_ptr(), lse.data_ptr(), p.data_ptr(), q.data_ptr(), coef.data_ptr(),
-              chunk, a(gh), tag_of(gh), a(gW), tag_of(gW), a(gb), ws.data_ptr(), ws_bytes)
+              Wc.data_ptr(), _lead_stride(Wc), sb.data_ptr() if bias is not None else None, scale, i.data_ptr(),
+              i.dtype == torch.int64, i.stride(0), tau, z, reduction, g32.data_ptr(), c, lse, p, q, coef, chunk, *of(gh),
+              *of(gW), *of(gb), ws.data_ptr(), ws_bytes)
     if gh is not None:
         gh = gh[:, :K] if Kp != K else gh
         gh = gh.to(h.dtype) if gh.dtype != h.dtype else gh
@@ -92,8 +105,7 @@ def _backward(g, h, W, bias, ids, c, lse, p, q, coef, tau, z, reduction, scale, 
 @torch.library.custom_op("swvr::distill", mutates_args=())
 def _fwd_op(h: torch.Tensor, W: torch.Tensor, bias: Optional[torch.Tensor], teacher: torch.Tensor, ids: torch.Tensor,
             weight: Optional[torch.Tensor], tau: float, z: float, reduction: int, scale: float, chunk: int,
-            cdt: torch.dtype, need_grad: bool) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor,
-                                                        torch.Tensor, torch.Tensor]:
+            cdt: torch.dtype, need_grad: bool) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     return _forward(h, W, bias, teacher, ids, weight, tau, z, reduction, scale, cdt, need_grad)
 
 
@@ -104,36 +116,34 @@ def _(h, W, bias, teacher, ids, weight, tau, z, reduction, scale, chunk, cdt, ne
     def new(*shape):
         return h.new_empty(shape, dtype=torch.float32)
 
-    kept = (new(N, T), new(N, T), new(N)) if need_grad else (new(0), new(0), new(0))
-    return (new(*((N,) if reduction == 0 else ())), new(), new(N), *kept)
+    return (new(N) if reduction == 0 else new(), new(1 + N * (2 * T + 2) if need_grad else 1 + N),
+            new(W.shape[0] if bias is not None else 0))
 
 
 @torch.library.custom_op("swvr::distill_bwd", mutates_args=())
 def _bwd_op(g: torch.Tensor, h: torch.Tensor, W: torch.Tensor, bias: Optional[torch.Tensor], ids: torch.Tensor,
-            c: torch.Tensor, lse: torch.Tensor, p: torch.Tensor, q: torch.Tensor, coef: torch.Tensor, tau: float,
-            z: float, reduction: int, scale: float, chunk: int, cdt: torch.dtype, need_h: bool, need_W: bool,
-            need_b: bool) -> List[torch.Tensor]:
-    grads = _backward(g, h, W, bias, ids, c, lse, p, q, coef, tau, z, reduction, scale, chunk, cdt, need_h, need_W,
-                      need_b)
+            kept: torch.Tensor, sb: torch.Tensor, tau: float, z: float, reduction: int, scale: float, chunk: int,
+            cdt: torch.dtype, need_h: bool, need_W: bool, need_b: bool) -> List[torch.Tensor]:
+    grads = _backward(g, h, W, bias, ids, kept, sb, tau, z, reduction, scale, chunk, cdt, need_h, need_W, need_b)
     # a custom op cannot return None: an empty tensor stands for "no gradient"
     return [x if x is not None else h.new_empty(0) for x in grads]
 
 
 @_bwd_op.register_fake
-def _(g, h, W, bias, ids, c, lse, p, q, coef, tau, z, reduction, scale, chunk, cdt, need_h, need_W, need_b):
+def _(g, h, W, bias, ids, kept, sb, tau, z, reduction, scale, chunk, cdt, need_h, need_W, need_b):
     return [torch.empty_like(x) if need else h.new_empty(0) for need, x in ((need_h, h), (need_W, W), (need_b, bias))]
 
 
 def _setup_context(ctx, inputs, output):
     h, W, bias, _, ids, _, tau, z, reduction, scale, chunk, cdt, _ = inputs
-    _, c, lse, p, q, coef = output
-    ctx.mark_non_differentiable(c, lse, p, q, coef)
-    ctx.save_for_backward(h, W, bias, ids, c, lse, p, q, coef)
+    _, kept, sb = output
+    ctx.mark_non_differentiable(kept, sb)
+    ctx.save_for_backward(h, W, bias, ids, kept, sb)
     ctx.args = (tau, z, reduction, scale, chunk, cdt)
 
 
 def _needs(ctx, bias):
-    need_h, need_W, need_b = (bool(x) for x in ctx.needs_input_grad[:3])
+    need_h, need_W, need_b = ctx.needs_input_grad[:3]
     return need_h, need_W, need_b and bias is not None
 
 
@@ -156,8 +166,8 @@ class _Distill(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, h, W, bias, teacher, ids, weight, tau, z, reduction, scale, chunk, cdt):
-        out, *kept = _forward(h, W, bias, teacher, ids, weight, tau, z, reduction, scale, cdt, True)
-        ctx.save_for_backward(h, W, bias, ids, *kept)
+        out, kept, sb = _forward(h, W, bias, teacher, ids, weight, tau, z, reduction, scale, cdt, True)
+        ctx.save_for_backward(h, W, bias, ids, kept, sb)
         ctx.args = (tau, z, reduction, scale, chunk, cdt)
         return out
 
