@@ -69,28 +69,30 @@ __global__ __launch_bounds__(256) void embed_lookup_kernel(const void* __restric
 }
 
 // ---------------------------------------------------------------- sorting
-// Stable order of the tokens by id in one launch: a workgroup owns kSortRows consecutive ids and scans
-// every token for them, counting on the way the tokens of smaller ids, which is where its own begin; so no
-// workgroup waits for another, and there is no pass per digit.  Its 16 waves take equal runs of the tokens in
-// order.  Pass 1 counts per (wave, id) and keeps the hits (up to kSortHits a wave); a scan over ids and waves
-// turns the counts into positions; pass 2 places the hits, 64 at a time, a hit's rank among the equal ids of
-// its 64 by eight ballots (one per bit of the row), so the order does not depend on any atomic's.  A wave
-// with more hits than it kept scans its run again.
-// The scans read M ids per 256 rows, from L2: 16384 tokens on 151936 ids, 78 MB.
-constexpr int kSortRows = 256, kSortWaves = 16, kSortHits = 256, kSortUnroll = 8;
+// Stable order of the tokens by id in one launch: a workgroup owns consecutive ids (its rows) and scans every
+// token for them, counting on the way the tokens of smaller ids, which is where its own begin; so no workgroup
+// waits for another, and there is no pass per digit.  Its 16 waves take equal runs of the tokens in order.  Pass 1
+// counts per (wave, row) and keeps the hits (up to kSortHits a wave); a scan over rows and waves turns the counts
+// into positions; pass 2 places the hits, 64 at a time, a hit's rank among the equal ids of its 64 by ten ballots
+// (one per bit of the row), so the order does not depend on any atomic's.  A wave with more hits than it kept
+// scans its run again.
+// The scans read every id once per workgroup, from L2, so there are few: rows for about one workgroup per CU, 256
+// to 1024 (what the counts' LDS holds).  32768 tokens on 256000 ids with 256 rows each, 25 us; so, 12.
+constexpr int kSortRows = 1024, kSortRowsFewest = 256, kSortWaves = 16, kSortHits = 256, kSortUnroll = 8;
 
 template <class ID>
-__global__ __launch_bounds__(64 * kSortWaves) void sort_ids_kernel(const ID* __restrict__ ids, int M, int V,
+__global__ __launch_bounds__(64 * kSortWaves) void sort_ids_kernel(const ID* __restrict__ ids, int M, int V, int R,
                                                                    int* __restrict__ order, int* __restrict__ sid,
                                                                    int* __restrict__ seg) {
-  __shared__ int cnt[kSortWaves][kSortRows];
+  __shared__ int cnt[kSortWaves * kSortRows];  // [wave][R]
   __shared__ int hit_i[kSortWaves][kSortHits];
-  __shared__ unsigned char hit_r[kSortWaves][kSortHits];
+  __shared__ unsigned short hit_r[kSortWaves][kSortHits];
   __shared__ int wless[kSortWaves], wtot[kSortRows / 64];
   const int t = threadIdx.x, lane = lane_id(), w = wave_id();
-  const int v0 = blockIdx.x * kSortRows, rows = min(kSortRows, V - v0);
+  const int v0 = blockIdx.x * R, rows = min(R, V - v0);
   const uint64_t below = (1ull << lane) - 1;
-  for (int i = t; i < kSortWaves * kSortRows; i += 64 * kSortWaves) (&cnt[0][0])[i] = 0;
+  int* const mine = cnt + w * R;
+  for (int i = t; i < kSortWaves * R; i += 64 * kSortWaves) cnt[i] = 0;
   __syncthreads();
   const int per = (int)(((int64_t)M + 64 * kSortWaves - 1) / (64 * kSortWaves)) * 64;
   const int64_t i0 = (int64_t)w * per, i1 = i0 + per < M ? i0 + per : M;
@@ -110,10 +112,10 @@ __global__ __launch_bounds__(64 * kSortWaves) void sort_ids_kernel(const ID* __r
       if (m == 0) continue;
       if (in) {
         const int r = (int)(x[u] - v0), at = hits + __popcll(m & below);
-        atomicAdd(&cnt[w][r], 1);
+        atomicAdd(&mine[r], 1);
         if (at < kSortHits) {
           hit_i[w][at] = (int)(base + u * 64 + lane);
-          hit_r[w][at] = (unsigned char)r;
+          hit_r[w][at] = (unsigned short)r;
         }
       }
       hits += __popcll(m);
@@ -127,9 +129,9 @@ __global__ __launch_bounds__(64 * kSortWaves) void sort_ids_kernel(const ID* __r
 #pragma unroll
   for (int j = 0; j < kSortWaves; ++j) first += wless[j];
   int tot = 0, x = 0;
-  if (t < kSortRows) {
+  if (t < R) {  // whole waves
 #pragma unroll
-    for (int j = 0; j < kSortWaves; ++j) tot += cnt[j][t];
+    for (int j = 0; j < kSortWaves; ++j) tot += cnt[j * R + t];
     x = tot;  // inclusive scan over the wave's 64 rows
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -139,24 +141,24 @@ __global__ __launch_bounds__(64 * kSortWaves) void sort_ids_kernel(const ID* __r
     if (lane == 63) wtot[w] = x;
   }
   __syncthreads();
-  if (t < kSortRows) {
+  if (t < R) {
     int s = first + x - tot;
     for (int j = 0; j < w; ++j) s += wtot[j];
     if (t < rows) seg[v0 + t] = s;
     if (t == rows - 1 && v0 + rows == V) seg[V] = s + tot;
 #pragma unroll
     for (int j = 0; j < kSortWaves; ++j) {
-      const int c = cnt[j][t];
-      cnt[j][t] = s;
+      const int c = cnt[j * R + t];
+      cnt[j * R + t] = s;
       s += c;
     }
   }
   __syncthreads();
-  volatile int* const next = cnt[w];
+  volatile int* const next = mine;
   auto place = [&](int i, int r, bool in) {
     uint64_t same = __ballot(in);
 #pragma unroll
-    for (int b = 0; b < 8; ++b) {
+    for (int b = 0; b < 10; ++b) {
       const uint64_t m = __ballot(in && ((r >> b) & 1));
       same &= ((r >> b) & 1) ? m : ~m;
     }
@@ -192,6 +194,21 @@ __device__ __forceinline__ void store_row(T* row, int c, const A (&acc)[Vec<T, V
   reinterpret_cast<Vec<T, VB>*>(row)[c] = x;
 }
 
+// VB zero bytes; whole 16-byte vectors past the caches, as nothing reads them soon (V = 151936, D = 2560 in bf16: the
+// launch 156 -> 152 us; rows of 8-byte vectors, D = 300 on 256000, take 31 us through the caches and 41 past them).
+template <int VB>
+__device__ __forceinline__ void store_zero(void* p) {
+  typedef typename std::conditional<VB == 2, unsigned short, unsigned int>::type E;
+  typedef E V __attribute__((ext_vector_type(VB / sizeof(E))));
+  V z;
+#pragma unroll
+  for (int i = 0; i < (int)(VB / sizeof(E)); ++i) z[i] = 0;
+  if constexpr (VB == 16)
+    __builtin_nontemporal_store(z, static_cast<V*>(p));
+  else
+    *static_cast<V*>(p) = z;
+}
+
 struct EmbedGradKernelParams {
   const void* g;
   int64_t ldg;
@@ -218,9 +235,6 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(EmbedGradKernelParams p)
   T* const gE = static_cast<T*>(p.gE);
   if ((int)blockIdx.x >= p.n_sum) {
     const int v0 = (((int)blockIdx.x - p.n_sum) * 4 + wave_id()) * kZeroRows;
-    X z;
-#pragma unroll
-    for (int i = 0; i < X::n; ++i) z.v[i] = (T)0.f;
     const int lane = lane_id();
     // the rows' borders once, one lane each
     const int b = v0 + lane <= p.V && lane <= kZeroRows ? p.seg[v0 + lane] : 0;
@@ -230,12 +244,12 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(EmbedGradKernelParams p)
       for (int r = 0; r < rows; ++r) {
         if (!((empty >> r) & 1)) continue;
         X* row = reinterpret_cast<X*>(gE + (int64_t)(v0 + r) * p.D);
-        for (int c = lane; c < cpr; c += 64) row[c] = z;
+        for (int c = lane; c < cpr; c += 64) store_zero<VB>(row + c);
       }
     } else {
       X* row0 = reinterpret_cast<X*>(gE + (int64_t)v0 * p.D);
       for (int c = lane; c < rows * cpr; c += 64)
-        if ((empty >> ((uint32_t)c / (uint32_t)cpr)) & 1) row0[c] = z;
+        if ((empty >> ((uint32_t)c / (uint32_t)cpr)) & 1) store_zero<VB>(row0 + c);
     }
     return;
   }
@@ -294,35 +308,45 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(EmbedGradKernelParams p)
 }
 
 // Parts of segments that cross runs, joined in run order.  A wave takes the run in which such a segment
-// begins, 64 columns; a workgroup's 4 waves share a segment of more than kJoinAlone parts (an id that fills a
-// large share of the tokens), a quarter of its parts each.
-constexpr int kJoinAlone = 32;
+// begins, 256 columns, 4 consecutive ones a lane; a workgroup's 4 waves share a segment of more than kJoinAlone parts
+// (an id that fills a large share of the tokens), a quarter of its parts each.
+constexpr int kJoinAlone = 16, kJoinCols = 256;
 template <class T>
 __global__ __launch_bounds__(256) void embed_join_kernel(EmbedGradKernelParams p, int n_ct) {
   typedef typename SumType<T>::type A;
+  struct alignas(16) A4 {
+    A v[4];
+  };
   __shared__ int s_last[4];
-  __shared__ A s_sum[4][64];
+  __shared__ A4 s_sum[4][64];
   const int lane = lane_id(), w = wave_id();
   const int64_t j0 = (int64_t)((int)blockIdx.x / n_ct) * 4;
-  const int d = ((int)blockIdx.x % n_ct) * 64 + lane;
+  const int d = ((int)blockIdx.x % n_ct) * kJoinCols + 4 * lane;
   const int M = p.seg[p.V];
   const A* const part = static_cast<const A*>(p.part);
-  T* const gE = static_cast<T*>(p.gE);
-  // the sum of the parts of runs a .. b of the segment that begins in run j
+  // the sum of the parts of runs a .. b of the segment that begins in run j (parts are dpad wide, a multiple of 8)
   auto sum = [&](int64_t j, int64_t a, int64_t b) {
-    A acc = 0;
-    for (int64_t q0 = a; q0 <= b; q0 += 16) {
-      A x[16];
+    A4 acc{{0, 0, 0, 0}};
+    for (int64_t q0 = a; q0 <= b; q0 += 8) {
+      A4 x[8];
 #pragma unroll
-      for (int u = 0; u < 16; ++u) {
+      for (int u = 0; u < 8; ++u) {
         const int64_t q = q0 + u <= b ? q0 + u : b;
-        x[u] = part[(q * 2 + (q == j)) * p.dpad + d];
+        x[u] = *reinterpret_cast<const A4*>(part + (q * 2 + (q == j)) * p.dpad + d);
       }
 #pragma unroll
-      for (int u = 0; u < 16; ++u)
-        if (q0 + u <= b) acc += x[u];
+      for (int u = 0; u < 8; ++u)
+        if (q0 + u <= b)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc.v[i] += x[u].v[i];
     }
     return acc;
+  };
+  auto store = [&](int v, const A4& x) {
+    T* const row = static_cast<T*>(p.gE) + (int64_t)v * p.D;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (d + i < p.D) row[d + i] = (T)(x.v[i] * (A)p.scale);
   };
   // the last run of the segment that begins in run j and crosses its end, or -1
   auto last_run = [&](int64_t j, int* v) -> int {
@@ -333,9 +357,7 @@ __global__ __launch_bounds__(256) void embed_join_kernel(EmbedGradKernelParams p
   };
   int v = 0;
   const int last = last_run(j0 + w, &v);
-  if (last >= 0 && last - (j0 + w) < kJoinAlone) {
-    if (d < p.D) gE[(int64_t)v * p.D + d] = (T)(sum(j0 + w, j0 + w, last) * (A)p.scale);
-  }
+  if (last >= 0 && last - (j0 + w) < kJoinAlone && d < p.D) store(v, sum(j0 + w, j0 + w, last));
   if (lane == 0) s_last[w] = last;
   __syncthreads();
   for (int i = 0; i < 4; ++i) {
@@ -344,12 +366,14 @@ __global__ __launch_bounds__(256) void embed_join_kernel(EmbedGradKernelParams p
     if (b < 0 || b - j < kJoinAlone) continue;  // the same for the whole workgroup
     const int64_t n = b - j + 1, a0 = j + n * w / 4, a1 = j + n * (w + 1) / 4 - 1;
     __syncthreads();  // the sums of the segment before have been read
-    s_sum[w][lane] = d < p.D ? sum(j, a0, a1) : (A)0;
+    if (d < p.D) s_sum[w][lane] = sum(j, a0, a1);
     __syncthreads();
     if (w == 0 && d < p.D) {
-      const int id = p.sid[(j + 1) * p.run];
-      gE[(int64_t)id * p.D + d] = (T)((((s_sum[0][lane] + s_sum[1][lane]) + s_sum[2][lane]) + s_sum[3][lane]) *
-                                      (A)p.scale);
+      A4 x;
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        x.v[c] = ((s_sum[0][lane].v[c] + s_sum[1][lane].v[c]) + s_sum[2][lane].v[c]) + s_sum[3][lane].v[c];
+      store(p.sid[(j + 1) * p.run], x);
     }
   }
 }
@@ -403,8 +427,8 @@ hipError_t dispatch(int dtype, int vb, F&& f) {
   }
 }
 
-// Sorted tokens per run: 32, and 8 for the few tokens that would not fill the chip so.
-int run_of(int64_t M) { return M >= 4096 ? 32 : 8; }
+// Sorted tokens per run: 64, and 32 and 8 for the fewer tokens that would not fill the chip so.
+int run_of(int64_t M) { return M >= 16384 ? 64 : M >= 4096 ? 32 : 8; }
 
 }  // namespace
 
@@ -425,13 +449,16 @@ hipError_t embed_lookup_launch(const EmbedParams& p, hipStream_t stream) {
 
 hipError_t sort_ids(const void* ids, int id64, int M, int V, int* order, int* sid, int* seg, hipStream_t stream) {
   if (V == 0) return hipSuccess;
-  const unsigned blocks = (unsigned)(((int64_t)V + kSortRows - 1) / kSortRows);
+  int R = kSortRowsFewest;
+  while (R < kSortRows && (int64_t)R * 256 < V) R *= 2;
+  const unsigned blocks = (unsigned)(((int64_t)V + R - 1) / R);
   timing_begin(kKindSortIds, stream);
   if (id64)
-    sort_ids_kernel<int64_t><<<blocks, 64 * kSortWaves, 0, stream>>>(static_cast<const int64_t*>(ids), M, V, order,
-                                                                      sid, seg);
+    sort_ids_kernel<int64_t><<<blocks, 64 * kSortWaves, 0, stream>>>(static_cast<const int64_t*>(ids), M, V, R,
+                                                                      order, sid, seg);
   else
-    sort_ids_kernel<int><<<blocks, 64 * kSortWaves, 0, stream>>>(static_cast<const int*>(ids), M, V, order, sid, seg);
+    sort_ids_kernel<int><<<blocks, 64 * kSortWaves, 0, stream>>>(static_cast<const int*>(ids), M, V, R, order, sid,
+                                                                 seg);
   timing_end(kKindSortIds, stream);
   return hipGetLastError();
 }
@@ -482,7 +509,7 @@ hipError_t embed_grad_launch(const EmbedParams& p, char* ws, hipStream_t stream)
     return hipGetLastError();
   });
   if (e != hipSuccess || runs < 2) return e;
-  const int n_ct = (p.D + 63) / 64;
+  const int n_ct = (p.D + kJoinCols - 1) / kJoinCols;
   const int64_t blocks = (runs + 3) / 4 * n_ct;
   if (blocks > INT32_MAX) return hipErrorInvalidValue;
   timing_begin(kKindEmbed, stream);
