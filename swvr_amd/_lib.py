@@ -59,9 +59,10 @@ SIGNATURES = {
     "swvr_mse_loss_workspace_size": (_sz, [_i64]),
     "swvr_mse_loss": (_i, [_i64, _i64, _p, _p, _p, _i, _i64, _p, _f, _i, _p, _p, _p, _p, _p, _sz, _p]),
     "swvr_mse_loss_noalloc": (_i, [_i64, _i64, _p, _p, _p, _i, _i64, _p, _f, _i, _p, _p, _p, _p, _p]),
-    "swvr_embedding": (_i, [_i, _i, _i64, _i64, _i64, _p, _p, _i64, ctypes.c_double, _p, _p]),
+    "swvr_embedding": (_i, [_i, _i, _i64, _i64, _i64, _p, _p, _i64, ctypes.c_double, _p, _p, _p]),
+    "swvr_embedding_sorted_size": (_sz, [_i64, _i64]),
     "swvr_embedding_bwd_workspace_size": (_sz, [_i, _i64, _i64, _i64]),
-    "swvr_embedding_bwd": (_i, [_i, _i, _i64, _i64, _i64, _p, _p, _i64, ctypes.c_double, _p, _p, _sz, _p]),
+    "swvr_embedding_bwd": (_i, [_i, _i, _i64, _i64, _i64, _p, _p, _i64, ctypes.c_double, _p, _p, _p, _sz, _p]),
     "swvr_distill_workspace_size": (_sz, [_i, _i64, _i64, _i64, _i64, _i]),
     "swvr_distill": (_i, [_i, _i, _i, _i64, _i64, _i64, _i64, _p, _i64, _p, _i64, _p, _i, _p, _f, _p, _i, _i64, _p, _i, _i64,
                           _f, _p, _f, _i, _p, _p, _p, _p, _p, _p, _p, _sz, _p]),

@@ -405,7 +405,7 @@ static int check_embed(int dtype, int id64, int64_t N, int64_t V, int64_t D, con
 }
 
 int swvr_embedding(int dtype, int id64, int64_t N, int64_t V, int64_t D, const void* ids, const void* E, int64_t lde,
-                   double scale, void* out, void* stream) {
+                   double scale, void* out, int* sorted, void* stream) {
   const int rc = check_embed(dtype, id64, N, V, D, ids);
   if (rc != SWVR_OK) return rc;
   if (lde < D) return fail(SWVR_EINVAL, "lde=%lld must be >= D", (long long)lde);
@@ -422,8 +422,14 @@ int swvr_embedding(int dtype, int id64, int64_t N, int64_t V, int64_t D, const v
   p.scale = scale;
   p.out = out;
   hipError_t e = swvr::embed_lookup_launch(p, static_cast<hipStream_t>(stream));
+  if (e == hipSuccess && sorted) e = swvr::embed_sort(p, sorted, static_cast<hipStream_t>(stream));
   if (e != hipSuccess) return hip_fail(e, "embedding launch");
   return SWVR_OK;
+}
+
+size_t swvr_embedding_sorted_size(int64_t N, int64_t V) {
+  if (N < 0 || V < 0 || N > INT32_MAX || V > INT32_MAX - 1) return 0;
+  return swvr::embed_sorted_ints(N, V) * sizeof(int);
 }
 
 size_t swvr_embedding_bwd_workspace_size(int dtype, int64_t N, int64_t V, int64_t D) {
@@ -432,13 +438,14 @@ size_t swvr_embedding_bwd_workspace_size(int dtype, int64_t N, int64_t V, int64_
 }
 
 int swvr_embedding_bwd(int dtype, int id64, int64_t N, int64_t V, int64_t D, const void* ids, const void* g,
-                       int64_t ldg, double scale, void* gE, void* workspace, size_t workspace_bytes, void* stream) {
+                       int64_t ldg, double scale, const int* sorted, void* gE, void* workspace, size_t workspace_bytes,
+                       void* stream) {
   const int rc = check_embed(dtype, id64, N, V, D, ids);
   if (rc != SWVR_OK) return rc;
   if (ldg < 0) return fail(SWVR_EINVAL, "ldg=%lld must not be negative", (long long)ldg);
   if (V > 0 && D > 0 && ((N > 0 && !g) || !gE)) return fail(SWVR_EINVAL, "g and gE must be non-null");
   const size_t need = swvr::embed_grad_workspace_bytes(dtype, N, V, D);
-  if (!workspace || workspace_bytes < need)
+  if ((need > 0 && !workspace) || workspace_bytes < need)
     return fail(SWVR_EWORKSPACE, "embedding workspace of %zu bytes needed, %zu given", need, workspace_bytes);
   swvr::EmbedParams p{};
   p.dtype = dtype;
@@ -451,7 +458,7 @@ int swvr_embedding_bwd(int dtype, int id64, int64_t N, int64_t V, int64_t D, con
   p.g = g;
   p.ldg = ldg;
   p.gE = gE;
-  hipError_t e = swvr::embed_grad_launch(p, static_cast<char*>(workspace), static_cast<hipStream_t>(stream));
+  hipError_t e = swvr::embed_grad_launch(p, sorted, static_cast<char*>(workspace), static_cast<hipStream_t>(stream));
   if (e != hipSuccess) return hip_fail(e, "embedding gradient launch");
   return SWVR_OK;
 }

@@ -16,6 +16,7 @@
 //                      one that crosses a run's border leaves its part in fp32; beside them, the rows
 //                      without a token are written as zeros (most of gE's bytes, for a large table);
 //   embed_join_kernel  adds the parts of a segment that crosses borders, in order, and writes its row.
+// Up to 2048 tokens one launch does all of it, embed_direct_kernel.
 #include <type_traits>
 
 #include "common.hpp"
@@ -378,6 +379,149 @@ __global__ __launch_bounds__(256) void embed_join_kernel(EmbedGradKernelParams p
   }
 }
 
+// ---------------------------------------------------------------- gradient of few tokens
+// Up to kDirectMost tokens in one launch: a workgroup owns R rows of gE, sorts their tokens in LDS as sort_ids_kernel
+// does (4 waves, each with a quarter of the tokens), and writes the rows, a wave each: zeros, or the sum in
+// token order.  A row of more than kDirectAlone tokens is shared by the 4 waves, a quarter of its tokens each.
+constexpr int kDirectMost = 2048, kDirectRows = 128, kDirectAlone = 32;
+template <class T, int VB, class ID>
+__global__ __launch_bounds__(256) void embed_direct_kernel(const ID* __restrict__ ids, int M, const T* __restrict__ g,
+                                                           int64_t ldg, int V, int D, int R, double scale,
+                                                           T* __restrict__ gE) {
+  typedef Vec<T, VB> X;
+  typedef typename SumType<T>::type A;
+  constexpr int kMine = kDirectMost / 4;
+  struct Sum {
+    A v[X::n];
+  };
+  __shared__ int cnt[4][kDirectRows], seg[kDirectRows + 1], wtot[2];
+  __shared__ unsigned short hit[4][kMine], order[kDirectMost];
+  __shared__ unsigned char hit_r[4][kMine];
+  __shared__ Sum s_sum[4][64];
+  const int t = threadIdx.x, lane = lane_id(), w = wave_id();
+  const int v0 = blockIdx.x * R, rows = min(R, V - v0);
+  const uint64_t below = (1ull << lane) - 1;
+  for (int i = t; i < 4 * kDirectRows; i += 256) (&cnt[0][0])[i] = 0;
+  __syncthreads();
+  const int per = (M + 255) / 256 * 64, i0 = w * per, i1 = min(i0 + per, M);
+  int hits = 0;
+  for (int base = i0; base < i1; base += 256) {
+    ID x[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) x[u] = base + u * 64 + lane < i1 ? ids[base + u * 64 + lane] : (ID)-1;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const bool in = x[u] >= v0 && x[u] < v0 + rows;
+      const uint64_t m = __ballot(in);
+      if (m == 0) continue;
+      if (in) {
+        const int r = (int)(x[u] - v0), at = hits + __popcll(m & below);
+        atomicAdd(&cnt[w][r], 1);
+        hit[w][at] = (unsigned short)(base + u * 64 + lane);
+        hit_r[w][at] = (unsigned char)r;
+      }
+      hits += __popcll(m);
+    }
+  }
+  __syncthreads();
+  int tot = 0, x = 0;
+  if (t < kDirectRows) {
+    x = tot = cnt[0][t] + cnt[1][t] + cnt[2][t] + cnt[3][t];
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int y = __shfl_up(x, o);
+      if (lane >= o) x += y;
+    }
+    if (lane == 63) wtot[w] = x;
+  }
+  __syncthreads();
+  if (t < kDirectRows) {
+    int s = x - tot + (w == 1 ? wtot[0] : 0);
+    seg[t] = s;
+    if (t == kDirectRows - 1) seg[kDirectRows] = s + tot;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int c = cnt[j][t];
+      cnt[j][t] = s;
+      s += c;
+    }
+  }
+  __syncthreads();
+  volatile int* const next = cnt[w];
+  for (int j = 0; j < hits; j += 64) {
+    const bool in = j + lane < hits;
+    const int r = in ? hit_r[w][j + lane] : 0;
+    uint64_t same = __ballot(in);
+#pragma unroll
+    for (int b = 0; b < 7; ++b) {
+      const uint64_t m = __ballot(in && ((r >> b) & 1));
+      same &= ((r >> b) & 1) ? m : ~m;
+    }
+    if (in) {
+      const int rank = __popcll(same & below), at = next[r] + rank;
+      order[at] = hit[w][j + lane];
+      if (rank == 0) next[r] = at + __popcll(same);
+    }
+  }
+  __syncthreads();
+  const int cpr = D / X::n;
+  // the sum of the tokens a .. b - 1 of the order in vector c
+  auto sum = [&](int a, int b, int c) {
+    Sum acc;
+#pragma unroll
+    for (int i = 0; i < X::n; ++i) acc.v[i] = 0;
+    for (int q = a; q < b; q += 8) {
+      X y[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        y[u] = reinterpret_cast<const X*>(g + (int64_t)order[q + u < b ? q + u : b - 1] * ldg)[c];
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        if (q + u < b)
+#pragma unroll
+          for (int i = 0; i < X::n; ++i) acc.v[i] += (A)y[u].v[i];
+    }
+    return acc;
+  };
+  bool shared_rows = false;
+  for (int r = w; r < rows; r += 4) {
+    const int a = seg[r], b = seg[r + 1];
+    if (b - a > kDirectAlone) {
+      shared_rows = true;
+      continue;
+    }
+    T* const row = gE + (int64_t)(v0 + r) * D;
+    if (a == b) {
+      for (int c = lane; c < cpr; c += 64) store_zero<VB>(row + (int64_t)c * X::n);
+      continue;
+    }
+    for (int c = lane; c < cpr; c += 64) {
+      const Sum acc = sum(a, b, c);
+      store_row<T, VB, A>(row, c, acc.v, (A)scale);
+    }
+  }
+  if (!__syncthreads_or(shared_rows)) return;
+  for (int r = 0; r < rows; ++r) {
+    const int a = seg[r], n = seg[r + 1] - a;
+    if (n <= kDirectAlone) continue;  // the same for the whole workgroup
+    T* const row = gE + (int64_t)(v0 + r) * D;
+    for (int c0 = 0; c0 < cpr; c0 += 64) {
+      const int c = c0 + lane;
+      if (c < cpr) s_sum[w][lane] = sum(a + n * w / 4, a + n * (w + 1) / 4, c);
+      __syncthreads();
+      if (w == 0 && c < cpr) {
+        Sum acc = s_sum[0][lane];
+#pragma unroll
+        for (int j = 1; j < 4; ++j)
+#pragma unroll
+          for (int i = 0; i < X::n; ++i) acc.v[i] += s_sum[j][lane].v[i];
+        store_row<T, VB, A>(row, c, acc.v, (A)scale);
+      }
+      __syncthreads();
+    }
+  }
+}
+
 size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
 
 int elem_bytes(int dtype) { return dtype == kF64 ? 8 : dtype == kF32 ? 4 : 2; }
@@ -427,8 +571,8 @@ hipError_t dispatch(int dtype, int vb, F&& f) {
   }
 }
 
-// Sorted tokens per run: 64, and 32 and 8 for the fewer tokens that would not fill the chip so.
-int run_of(int64_t M) { return M >= 16384 ? 64 : M >= 4096 ? 32 : 8; }
+// Sorted tokens per run: 64, and 32 and 16 for the fewer tokens that would not fill the chip so.
+int run_of(int64_t M) { return M >= 16384 ? 64 : M >= 4096 ? 32 : 16; }
 
 }  // namespace
 
@@ -463,35 +607,75 @@ hipError_t sort_ids(const void* ids, int id64, int M, int V, int* order, int* si
   return hipGetLastError();
 }
 
-size_t embed_grad_workspace_bytes(int dtype, int64_t N, int64_t V, int64_t D) {
-  const int64_t run = run_of(N), runs = (N + run - 1) / run, dpad = (D + 7) / 8 * 8;
-  return 2 * align256((size_t)N * 4) + align256((size_t)(V + 1) * 4) +
-         align256((size_t)runs * 2 * dpad * (dtype == kF64 ? 8 : 4));
+namespace {
+// order [N], sid [N], seg [V + 1] in one buffer
+struct Sorted {
+  int *order, *sid, *seg;
+};
+Sorted sorted_in(int* p, int64_t N) { return {p, p + N, p + 2 * N}; }
+
+template <class T, int VB>
+hipError_t launch_direct(const EmbedParams& p, hipStream_t stream) {
+  // rows for about 1024 workgroups, up to what a workgroup's LDS holds
+  int R = 4;
+  while (R < kDirectRows && (int64_t)R * 1024 < p.V) R *= 2;
+  const unsigned blocks = (unsigned)(((int64_t)p.V + R - 1) / R);
+  const T* const g = static_cast<const T*>(p.g);
+  T* const gE = static_cast<T*>(p.gE);
+  timing_begin(kKindEmbed, stream);
+  if (p.id64)
+    embed_direct_kernel<T, VB, int64_t><<<blocks, 256, 0, stream>>>(static_cast<const int64_t*>(p.ids), (int)p.N, g,
+                                                                     p.ldg, p.V, p.D, R, p.scale, gE);
+  else
+    embed_direct_kernel<T, VB, int><<<blocks, 256, 0, stream>>>(static_cast<const int*>(p.ids), (int)p.N, g, p.ldg,
+                                                                 p.V, p.D, R, p.scale, gE);
+  timing_end(kKindEmbed, stream);
+  return hipGetLastError();
+}
+}  // namespace
+
+size_t embed_sorted_ints(int64_t N, int64_t V) { return N <= kDirectMost ? 0 : (size_t)(2 * N + V + 1); }
+
+hipError_t embed_sort(const EmbedParams& p, int* sorted, hipStream_t stream) {
+  if (p.N <= kDirectMost) return hipSuccess;
+  const Sorted z = sorted_in(sorted, p.N);
+  return sort_ids(p.ids, p.id64, (int)p.N, p.V, z.order, z.sid, z.seg, stream);
 }
 
-hipError_t embed_grad_launch(const EmbedParams& p, char* ws, hipStream_t stream) {
+size_t embed_grad_workspace_bytes(int dtype, int64_t N, int64_t V, int64_t D) {
+  if (N <= kDirectMost) return 0;
+  const int64_t run = run_of(N), runs = (N + run - 1) / run, dpad = (D + 7) / 8 * 8;
+  return align256(embed_sorted_ints(N, V) * 4) + align256((size_t)runs * 2 * dpad * (dtype == kF64 ? 8 : 4));
+}
+
+hipError_t embed_grad_launch(const EmbedParams& p, const int* sorted, char* ws, hipStream_t stream) {
   if (p.V == 0 || p.D == 0) return hipSuccess;
-  int* order = reinterpret_cast<int*>(ws);
-  int* sid = reinterpret_cast<int*>(ws += align256((size_t)p.N * 4));
-  int* seg = reinterpret_cast<int*>(ws += align256((size_t)p.N * 4));
-  ws += align256((size_t)(p.V + 1) * 4);
-  hipError_t e = sort_ids(p.ids, p.id64, (int)p.N, p.V, order, sid, seg, stream);
-  if (e != hipSuccess) return e;
   const int eb = elem_bytes(p.dtype), vb = vec_bytes(eb, p.D, p.ldg, p.g, p.gE);
+  hipError_t e;
+  if (p.N <= kDirectMost)
+    return dispatch(p.dtype, vb, [&](auto t, auto w) { return launch_direct<decltype(t), decltype(w)::value>(p, stream); });
+  // the workspace: the parts, then the sorted order of a caller that has none
+  const int64_t run = run_of(p.N), runs = (p.N + run - 1) / run;
+  const int dpad = (p.D + 7) / 8 * 8;
+  if (!sorted) {
+    int* const own = reinterpret_cast<int*>(ws + align256((size_t)runs * 2 * dpad * (p.dtype == kF64 ? 8 : 4)));
+    if ((e = embed_sort(p, own, stream)) != hipSuccess) return e;
+    sorted = own;
+  }
+  const Sorted z = sorted_in(const_cast<int*>(sorted), p.N);
   EmbedGradKernelParams k{};
   k.g = p.g;
   k.ldg = p.ldg;
-  k.order = order;
-  k.sid = sid;
-  k.seg = seg;
+  k.order = z.order;
+  k.sid = z.sid;
+  k.seg = z.seg;
   k.V = p.V;
   k.D = p.D;
-  k.run = run_of(p.N);
-  k.dpad = (p.D + 7) / 8 * 8;
+  k.run = (int)run;
+  k.dpad = dpad;
   k.part = ws;
   k.scale = p.scale;
   k.gE = p.gE;
-  const int64_t runs = (p.N + k.run - 1) / k.run;
   e = dispatch(p.dtype, vb, [&](auto t, auto w) -> hipError_t {
     typedef decltype(t) T;
     constexpr int VB = decltype(w)::value;

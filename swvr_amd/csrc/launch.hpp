@@ -401,7 +401,11 @@ struct EmbedParams {
 };
 hipError_t embed_lookup_launch(const EmbedParams& p, hipStream_t stream);
 size_t embed_grad_workspace_bytes(int dtype, int64_t N, int64_t V, int64_t D);
-hipError_t embed_grad_launch(const EmbedParams& p, char* ws, hipStream_t stream);
+// sorted: embed_sort's, or null (the order is made in the workspace).
+hipError_t embed_grad_launch(const EmbedParams& p, const int* sorted, char* ws, hipStream_t stream);
+// The tokens' order for the gradient, embed_sorted_ints ints (0: the gradient of so few needs none).
+size_t embed_sorted_ints(int64_t N, int64_t V);
+hipError_t embed_sort(const EmbedParams& p, int* sorted, hipStream_t stream);
 // Positions 0 .. M - 1 in stable order of their id (those with an id in 0 .. V - 1): order, their ids (sid) and
 // each id's segment, seg[v] .. seg[v + 1].
 hipError_t sort_ids(const void* ids, int id64, int M, int V, int* order, int* sid, int* seg, hipStream_t stream);

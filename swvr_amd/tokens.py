@@ -18,6 +18,7 @@ from . import _lib
 from ._ops import _needs_grad, _plain, _require_device, eager
 
 _EMBED_TAG = {**_lib.DTYPE_TAG, torch.float64: _lib.F64}
+_SORT_FREE = 2048  # tokens up to which the gradient needs neither order nor workspace (their sizes are 0)
 
 
 # ---------------------------------------------------------------- embedding lookup
@@ -29,18 +30,25 @@ def _ids(ids):
     return ids if ids.is_contiguous() else ids.contiguous()
 
 
-def _lookup(ids, E, scale):
+def _lookup(ids, E, scale, sort=False):
+    """The rows, and with ``sort`` (for the gradient) the tokens' order that ``_lookup_grad`` takes, else None (few
+    tokens need none)."""
+    lib = _lib.load()
     i, x = _ids(ids), _plain(E)
     V, D = x.shape
     if not x.is_contiguous() and (x.stride(1) != 1 or (V > 1 and x.stride(0) < D)):
         x = x.contiguous()
+    N = i.numel()
     out = x.new_empty(*ids.shape, D)
-    _lib.call(_lib.load().swvr_embedding, x.device, _EMBED_TAG[x.dtype], i.dtype == torch.int64, i.numel(), V, D,
-              i.data_ptr(), x.data_ptr(), x.stride(0) if V > 1 else D, scale, out.data_ptr())
-    return out
+    order = None
+    if sort and N > _SORT_FREE:
+        order = x.new_empty(lib.swvr_embedding_sorted_size(N, V), dtype=torch.uint8)
+    _lib.call(lib.swvr_embedding, x.device, _EMBED_TAG[x.dtype], i.dtype == torch.int64, N, V, D, i.data_ptr(),
+              x.data_ptr(), x.stride(0) if V > 1 else D, scale, out.data_ptr(), _lib.address(order))
+    return out, order
 
 
-def _lookup_grad(g, ids, V, scale):
+def _lookup_grad(g, ids, V, scale, order=None):
     lib = _lib.load()
     D = g.shape[-1]
     i, g2 = _ids(ids), _plain(g)
@@ -48,16 +56,19 @@ def _lookup_grad(g, ids, V, scale):
     g2 = g2 if g2.stride(1) == 1 else g2.contiguous()
     tag, N = _EMBED_TAG[g.dtype], i.numel()
     gE = g2.new_empty(V, D)
-    ws_bytes = lib.swvr_embedding_bwd_workspace_size(tag, N, V, D)
-    ws = g2.new_empty(ws_bytes, dtype=torch.uint8)
+    ws, ws_bytes = None, 0
+    if N > _SORT_FREE:
+        ws_bytes = lib.swvr_embedding_bwd_workspace_size(tag, N, V, D)
+        ws = g2.new_empty(ws_bytes, dtype=torch.uint8)
+    a = _lib.address
     _lib.call(lib.swvr_embedding_bwd, g2.device, tag, i.dtype == torch.int64, N, V, D, i.data_ptr(), g2.data_ptr(),
-              g2.stride(0), scale, gE.data_ptr(), ws.data_ptr(), ws_bytes)
+              g2.stride(0), scale, a(order), gE.data_ptr(), a(ws), ws_bytes)
     return gE
 
 
 @torch.library.custom_op("swvr::embedding", mutates_args=())
 def _lookup_op(ids: torch.Tensor, E: torch.Tensor, scale: float) -> torch.Tensor:
-    return _lookup(ids, E, scale)
+    return _lookup(ids, E, scale)[0]
 
 
 @_lookup_op.register_fake
@@ -90,20 +101,23 @@ _lookup_op.register_autograd(_lookup_autograd, setup_context=_lookup_setup)
 
 
 class _Lookup(torch.autograd.Function):
-    """swvr::embedding / embedding_bwd as one node."""
+    """swvr::embedding / embedding_bwd as one node; the ids are sorted with the forward, whose launches cost the
+    host less than those from autograd's thread."""
 
     @staticmethod
     def forward(ctx, ids, E, scale):
-        ctx.save_for_backward(ids)
+        out, order = _lookup(ids, E, scale, True)
+        ctx.save_for_backward(ids, order)
         ctx.args = (E.shape[0], scale)
-        return _lookup(ids, E, scale)
+        return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
-        (ids,) = ctx.saved_tensors
-        grad = _lookup_grad if eager(g, ids) else _lookup_grad_op
-        return None, grad(g, ids, *ctx.args), None
+        ids, order = ctx.saved_tensors
+        if eager(g, ids):
+            return None, _lookup_grad(g, ids, *ctx.args, order), None
+        return None, _lookup_grad_op(g, ids, *ctx.args), None
 
 
 def embedding_lookup(ids, E, *, scale=1.0):
@@ -124,7 +138,7 @@ def embedding_lookup(ids, E, *, scale=1.0):
     if ids.device != E.device:
         raise ValueError(f"ids are on {ids.device} but E on {E.device}")
     if eager(ids, E):
-        return _Lookup.apply(ids, E, float(scale)) if _needs_grad(E) else _lookup(ids, E, scale)
+        return _Lookup.apply(ids, E, float(scale)) if _needs_grad(E) else _lookup(ids, E, scale)[0]
     if E.device.type == "cpu":
         _require_device(E)
     return _lookup_op(ids, E, float(scale))

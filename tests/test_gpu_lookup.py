@@ -71,7 +71,8 @@ def check(ids, E, g, scale=1.0):
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32, torch.float64])
 @pytest.mark.parametrize("N,V,D", [(1, 1, 1), (1, 1000, 64), (7, 3, 5), (64, 256, 8), (65, 257, 33), (300, 1000, 100),
-                                   (513, 511, 300), (1025, 70000, 16), (4096, 300, 130), (5000, 2049, 2050)])
+                                   (513, 511, 300), (1025, 70000, 16), (4096, 300, 130), (5000, 2049, 2050),
+                                   (1500, 200000, 40), (2048, 1000, 1030), (2049, 1000, 1030)])
 def test_types_and_sizes(dtype, N, V, D):
     E, ids, g = make(N, V, D, dtype, seed=N + D)
     check(ids, E, g, scale=1.0)
@@ -80,7 +81,7 @@ def test_types_and_sizes(dtype, N, V, D):
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("share", [0.3, 0.9, 1.0])
-@pytest.mark.parametrize("N,D", [(40, 24), (3000, 72), (20000, 64), (70001, 9)])
+@pytest.mark.parametrize("N,D", [(40, 24), (300, 520), (2048, 40), (2049, 40), (3000, 72), (20000, 64), (70001, 9)])
 def test_one_id_holds_most_tokens(dtype, share, N, D):
     """Segments over many runs, beginning and ending anywhere in one."""
     V = 1500
@@ -93,16 +94,21 @@ def test_one_id_holds_most_tokens(dtype, share, N, D):
 def test_several_ids_share_the_tokens():
     """Runs of equal ids of every length around the runs that are summed together."""
     lengths = [1, 7, 8, 9, 31, 32, 33, 63, 64, 65, 127, 500, 1023, 1024, 1025, 2100]
-    ids = torch.cat([torch.full((n,), 3 * i, device=DEV) for i, n in enumerate(lengths)])
-    ids = ids[torch.randperm(ids.numel(), device=DEV, generator=gen(2))]
-    g = torch.randn(ids.numel(), 40, device=DEV, generator=gen(3))
-    check(ids, torch.randn(50, 40, device=DEV), g)
+    for most in (130, 2100):              # in one launch, and in several
+        ids = torch.cat([torch.full((n,), 3 * i, device=DEV) for i, n in enumerate(lengths) if n <= most])
+        ids = ids[torch.randperm(ids.numel(), device=DEV, generator=gen(2))]
+        g = torch.randn(ids.numel(), 40, device=DEV, generator=gen(3))
+        check(ids, torch.randn(50, 40, device=DEV), g)
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float64])
 def test_padding_and_ids_outside_the_table(dtype):
-    E, ids, g = make(700, 300, 48, dtype)
-    check(torch.where(torch.rand(700, device=DEV) < 0.4, -1, ids), E, g)
+    check_padding(*make(700, 300, 48, dtype))
+    check_padding(*make(2700, 300, 48, dtype))
+
+
+def check_padding(E, ids, g):
+    check(torch.where(torch.rand(ids.numel(), device=DEV) < 0.4, -1, ids), E, g)
     check(torch.full_like(ids, -1), E, g)
     wild = ids.clone()
     wild[::7] = 300
@@ -156,6 +162,23 @@ def test_cotangents_of_every_stride():
     assert torch.equal(E2.grad.sum(), torch.tensor(33.0 * 24, device=DEV))
 
 
+def test_ids_changed_before_the_backward_are_refused():
+    E, ids, g = make(3000, 60, 8, torch.float32)
+    out = swvr_amd.embedding_lookup(ids, E.requires_grad_(True))
+    ids[0] += 1
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        torch.autograd.grad(out, E, g)
+
+
+def test_backward_twice_and_compiled_backward_give_the_same():
+    for n in (900, 2600):
+        E, ids, g = make(n, 700, 24, torch.float32)
+        out = swvr_amd.embedding_lookup(ids, E.requires_grad_(True))
+        first = torch.autograd.grad(out, E, g, retain_graph=True)[0]
+        assert torch.equal(torch.autograd.grad(out, E, g)[0], first)
+        assert torch.equal(torch.ops.swvr.embedding_bwd(g, ids, 700, 1.0), first)
+
+
 def test_gradient_against_differences():
     E, ids, _ = make(9, 6, 5, torch.float64)
     ids[2], ids[5] = -1, ids[0]
@@ -198,7 +221,11 @@ def test_another_stream():
 
 def test_captured_and_replayed():
     """Forward and backward in a graph, replayed with new ids and values between eager calls."""
-    E, ids, g = make(900, 500, 64, torch.bfloat16)
+    for n in (900, 2600):
+        captured(*make(n, 500, 64, torch.bfloat16))
+
+
+def captured(E, ids, g):
     E.requires_grad_(True)
 
     def step():
@@ -215,7 +242,7 @@ def test_captured_and_replayed():
     with torch.cuda.graph(graph):
         out, gE = step()
     for k in range(4):
-        ids.copy_(torch.randint(-1, 500, (900,), device=DEV, generator=gen(k)) if k != 2 else torch.full_like(ids, 7))
+        ids.copy_(torch.randint(-1, 500, ids.shape, device=DEV, generator=gen(k)) if k != 2 else torch.full_like(ids, 7))
         g.normal_(generator=gen(10 + k))
         graph.replay()
         torch.cuda.synchronize()

@@ -115,11 +115,11 @@ P = ctypes.c_void_p(16)
 
 
 def embedding(dtype=_lib.BF16, id64=1, N=4, V=8, D=4, ids=P, E=P, lde=4, out=P):
-    return _lib.load().swvr_embedding(dtype, id64, N, V, D, ids, E, lde, 1.0, out, None)
+    return _lib.load().swvr_embedding(dtype, id64, N, V, D, ids, E, lde, 1.0, out, None, None)
 
 
-def embedding_bwd(dtype=_lib.BF16, id64=1, N=4, V=8, D=4, ids=P, g=P, ldg=4, gE=P, ws=P, nbytes=1 << 20):
-    return _lib.load().swvr_embedding_bwd(dtype, id64, N, V, D, ids, g, ldg, 1.0, gE, ws, nbytes, None)
+def embedding_bwd(dtype=_lib.BF16, id64=1, N=4000, V=8, D=4, ids=P, g=P, ldg=4, gE=P, ws=P, nbytes=1 << 20):
+    return _lib.load().swvr_embedding_bwd(dtype, id64, N, V, D, ids, g, ldg, 1.0, None, gE, ws, nbytes, None)
 
 
 def sample(dtype=_lib.BF16, R=4, V=8, logits=P, ld=8, u=P, u64=0, tau=1.0, token=P, logprob=P, ws=P, nbytes=1 << 30):
