@@ -346,13 +346,19 @@ int swvr_embedding_bwd(int dtype, int id64, int64_t N, int64_t V, int64_t D, con
  * ([N] or one value), and writes gh [N,K], gW [V,K] and gb [V] (their dtype tags);
  * each may be NULL.  Only ids is read of the teacher's lists.  chunk as in swvr_bwd. */
 #define SWVR_MAX_TEACHER 1024
+/* Bytes of the scores [V][tokens] in fp32 that swvr_distill keeps at `scores` for
+ * swvr_distill_bwd, which then needs no product to form them again: for few tokens (those of
+ * the one-pass forward) and a W in the compute dtype, where they take at most twice W's bytes; 0
+ * elsewhere, and then `scores` must be NULL.  With NULL the backward recomputes them.  A call that
+ * keeps them sizes its workspace with weighted = 0. */
+size_t swvr_distill_scores_size(int dtype, int w_dtype, int64_t N, int64_t K, int64_t V, int64_t ldw);
 size_t swvr_distill_workspace_size(int dtype, int64_t N, int64_t K, int64_t V, int64_t T, int weighted);
 int swvr_distill(int dtype, int h_dtype, int w_dtype, int64_t N, int64_t K, int64_t V, int64_t T,
                  const void* h, int64_t ldh, const void* W, int64_t ldw, const void* bias, int bias_dtype,
                  float* bias_scaled, float logit_scale,
                  const void* ids, int id64, int64_t ldi, const void* teacher, int t_dtype, int64_t ldt,
                  float temperature, const float* weight, float z_loss_weight, int reduction,
-                 float* out, float* c, float* lse, float* p, float* q, float* coef,
+                 float* out, float* c, float* lse, float* p, float* q, float* coef, float* scores,
                  void* workspace, size_t workspace_bytes, void* stream);
 size_t swvr_distill_bwd_workspace_size(int dtype, int w_dtype, int64_t N, int64_t K, int64_t V, int64_t T,
                                        int64_t chunk, int need_gh);
@@ -361,7 +367,7 @@ int swvr_distill_bwd(int dtype, int h_dtype, int w_dtype, int64_t N, int64_t K, 
                      float logit_scale,
                      const void* ids, int id64, int64_t ldi, float temperature, float z_loss_weight, int reduction,
                      const float* g, const float* c, const float* lse, const float* p, const float* q,
-                     const float* coef, int64_t chunk, void* gh, int gh_dtype, void* gW, int gW_dtype,
+                     const float* coef, const float* scores, int64_t chunk, void* gh, int gh_dtype, void* gW, int gW_dtype,
                      void* gb, int gb_dtype,
                      void* workspace, size_t workspace_bytes, void* stream);
 

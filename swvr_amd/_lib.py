@@ -65,10 +65,11 @@ SIGNATURES = {
     "swvr_embedding_bwd": (_i, [_i, _i, _i64, _i64, _i64, _p, _p, _i64, ctypes.c_double, _p, _p, _p, _sz, _p]),
     "swvr_distill_workspace_size": (_sz, [_i, _i64, _i64, _i64, _i64, _i]),
     "swvr_distill": (_i, [_i, _i, _i, _i64, _i64, _i64, _i64, _p, _i64, _p, _i64, _p, _i, _p, _f, _p, _i, _i64, _p, _i, _i64,
-                          _f, _p, _f, _i, _p, _p, _p, _p, _p, _p, _p, _sz, _p]),
+                          _f, _p, _f, _i, _p, _p, _p, _p, _p, _p, _p, _p, _sz, _p]),
+    "swvr_distill_scores_size": (_sz, [_i, _i, _i64, _i64, _i64, _i64]),
     "swvr_distill_bwd_workspace_size": (_sz, [_i, _i, _i64, _i64, _i64, _i64, _i64, _i]),
     "swvr_distill_bwd": (_i, [_i, _i, _i, _i64, _i64, _i64, _i64, _p, _i64, _p, _i64, _p, _f, _p, _i, _i64, _f, _f, _i,
-                              _p, _p, _p, _p, _p, _p, _i64, _p, _i, _p, _i, _p, _i, _p, _sz, _p]),
+                              _p, _p, _p, _p, _p, _p, _p, _i64, _p, _i, _p, _i, _p, _i, _p, _sz, _p]),
     "swvr_sample": (_i, [_i, _i64, _i64, _p, _i64, _p, _i, ctypes.c_double, _p, _i64, _p, ctypes.c_double, _p,
                          ctypes.c_double, _p, _p, _p, _p, _sz, _p]),
     "swvr_sample_workspace_size": (_sz, [_i64, _i64]),

@@ -132,7 +132,8 @@ int check_storage(int dtype, int h_dtype, int w_dtype) {
 int fwd_common(int dtype, int h_dtype, int w_dtype, int64_t N, int64_t K, int64_t V, int64_t D, const void* h,
                int64_t ldh, const void* W, int64_t ldw, const void* E, int64_t lde, const float* bias,
                float logit_scale, float* O, float* lse, float* m_out, float* l_out, void* workspace,
-               size_t workspace_bytes, void* stream, bool active = false, const float* weight = nullptr) {
+               size_t workspace_bytes, void* stream, bool active = false, const float* weight = nullptr,
+               float* scores = nullptr) {
   g_err[0] = 0;
   int rc = check_common(dtype, N, K, V, D, h, ldh, W, ldw, E, lde);
   if (rc != SWVR_OK) return rc;
@@ -160,6 +161,7 @@ int fwd_common(int dtype, int h_dtype, int w_dtype, int64_t N, int64_t K, int64_
   p.D = (int)D;
   p.h_f32 = h_dtype != dtype;
   p.w_f32 = w_dtype != dtype;
+  p.scores = scores;
   hipError_t e = active ? fwd_launch_active(dtype, plan, p, weight, static_cast<char*>(workspace), O, lse,
                                             static_cast<hipStream_t>(stream))
                         : fwd_launch(dtype, plan, p, static_cast<char*>(workspace), O, lse, m_out, l_out,
@@ -175,7 +177,8 @@ int bwd_common(int dtype, int h_dtype, int w_dtype, int64_t N, int64_t K, int64_
                    void* workspace, size_t workspace_bytes, void* stream, const void* hq = nullptr,
                    int64_t K8 = 0, int64_t ldhq = 0, const float* h_scale = nullptr, const void* Wq = nullptr,
                    int64_t ldwq = 0, const float* w_scale = nullptr, const int* pt_id = nullptr,
-                   const float* pt_val = nullptr, int64_t n_pt = 0, int pt_T = 1) {
+                   const float* pt_val = nullptr, int64_t n_pt = 0, int pt_T = 1, const float* scores = nullptr,
+                   int64_t lds = 0) {
   g_err[0] = 0;
   int rc = check_common(dtype, N, K, V, D, h, ldh, W, ldw, E, lde);
   if (rc != SWVR_OK) return rc;
@@ -229,6 +232,8 @@ int bwd_common(int dtype, int h_dtype, int w_dtype, int64_t N, int64_t K, int64_
   p.pt_val = pt_val;
   p.n_pt = n_pt;
   p.pt_T = pt_T;
+  p.scores = scores;
+  p.lds = lds;
   hipError_t e = bwd_launch(dtype, plan, p, static_cast<hipStream_t>(stream));
   if (e != hipSuccess) return hip_fail(e, "backward launch");
   return SWVR_OK;
@@ -483,6 +488,12 @@ static int check_distill(int dtype, int64_t N, int64_t V, int64_t T, int id64, c
   return SWVR_OK;
 }
 
+size_t swvr_distill_scores_size(int dtype, int w_dtype, int64_t N, int64_t K, int64_t V, int64_t ldw) {
+  if (!is_dtype(dtype) || w_dtype != dtype || N <= 0 || K <= 0 || V <= 0 || ldw < K || N > INT32_MAX || V > INT32_MAX)
+    return 0;
+  return (size_t)swvr::fwd_kept_scores(dtype, N, K, V, ldw) * (size_t)V * sizeof(float);
+}
+
 size_t swvr_distill_workspace_size(int dtype, int64_t N, int64_t K, int64_t V, int64_t T, int weighted) {
   FwdPlan plan;
   if (N < 0 || V < 0 || T < 0 || !fwd_plan(dtype, N, K, V, 0, &plan, weighted != 0)) return 0;
@@ -493,7 +504,7 @@ int swvr_distill(int dtype, int h_dtype, int w_dtype, int64_t N, int64_t K, int6
                  int64_t ldh, const void* W, int64_t ldw, const void* bias, int bias_dtype, float* bias_scaled,
                  float logit_scale, const void* ids, int id64, int64_t ldi, const void* teacher, int t_dtype, int64_t ldt,
                  float temperature, const float* weight, float z_loss_weight, int reduction, float* out, float* c, float* lse, float* p,
-                 float* q, float* coef, void* workspace, size_t workspace_bytes, void* stream) {
+                 float* q, float* coef, float* scores, void* workspace, size_t workspace_bytes, void* stream) {
   int rc = check_distill(dtype, N, V, T, id64, ids, ldi, temperature, reduction);
   if (rc != SWVR_OK) return rc;
   if (!is_dtype(t_dtype)) return fail(SWVR_EDTYPE, "unsupported teacher dtype tag %d", t_dtype);
@@ -505,13 +516,18 @@ int swvr_distill(int dtype, int h_dtype, int w_dtype, int64_t N, int64_t K, int6
   if (reduction && !c) return fail(SWVR_EINVAL, "c must be non-null");
   if ((p == nullptr) != (q == nullptr) || (p == nullptr) != (coef == nullptr))
     return fail(SWVR_EINVAL, "p, q and coef must all be given or all NULL");
-  const size_t need = swvr_distill_workspace_size(dtype, N, K, V, T, weight != nullptr);
+  if (scores && N > 0 && swvr_distill_scores_size(dtype, w_dtype, N, K, V, ldw) == 0)
+    return fail(SWVR_EINVAL, "scores are not kept for N=%lld K=%lld V=%lld ldw=%lld", (long long)N, (long long)K,
+                (long long)V, (long long)ldw);
+  // a forward that keeps the scores computes every token's
+  const bool active = weight != nullptr && !scores;
+  const size_t need = swvr_distill_workspace_size(dtype, N, K, V, T, active);
   if (!workspace || workspace_bytes < need)
     return fail(SWVR_EWORKSPACE, "distillation workspace of %zu bytes needed, %zu given", need, workspace_bytes);
   const hipStream_t s = static_cast<hipStream_t>(stream);
   char* ws = static_cast<char*>(workspace);
   FwdPlan plan;
-  fwd_plan(dtype, N, K, V, 0, &plan, weight != nullptr);
+  fwd_plan(dtype, N, K, V, 0, &plan, active);
   const size_t fwd_bytes = plan.ws_bytes;
   float* z = reinterpret_cast<float*>(ws + up256(fwd_bytes));
   float* part = z + up256((size_t)N * T * 4) / 4;
@@ -522,7 +538,7 @@ int swvr_distill(int dtype, int h_dtype, int w_dtype, int64_t N, int64_t K, int6
   const float* const sb = bias ? bias_scaled : nullptr;
   // the log-sum-exps: a readout without columns
   rc = fwd_common(dtype, h_dtype, w_dtype, N, K, V, 0, h, ldh, W, ldw, W, 0, sb, scale, nullptr, lse, nullptr, nullptr,
-                  workspace, fwd_bytes, stream, weight != nullptr, weight);
+                  workspace, fwd_bytes, stream, active, weight, scores);
   if (rc != SWVR_OK) return rc;
   swvr::DistillParams d{};
   d.h = h;
@@ -570,14 +586,17 @@ int swvr_distill_bwd(int dtype, int h_dtype, int w_dtype, int64_t N, int64_t K, 
                      int64_t ldh, const void* W, int64_t ldw, const float* bias_scaled, float logit_scale,
                      const void* ids, int id64, int64_t ldi, float temperature, float z_loss_weight, int reduction, const float* g,
                      const float* c, const float* lse, const float* p, const float* q, const float* coef,
-                     int64_t chunk, void* gh, int gh_dtype, void* gW, int gW_dtype, void* gb, int gb_dtype,
-                     void* workspace, size_t workspace_bytes, void* stream) {
+                     const float* scores, int64_t chunk, void* gh, int gh_dtype, void* gW, int gW_dtype, void* gb,
+                     int gb_dtype, void* workspace, size_t workspace_bytes, void* stream) {
   int rc = check_distill(dtype, N, V, T, id64, ids, ldi, temperature, reduction);
   if (rc != SWVR_OK) return rc;
   if (chunk <= 0) return fail(SWVR_EINVAL, "chunk must be positive, got %lld", (long long)chunk);
   if (N > 0 && (!g || !lse || !p || !q || !coef || (reduction && !c)))
     return fail(SWVR_EINVAL, "g, c, lse, p, q and coef must be non-null");
   if (gb && !bias_scaled) return fail(SWVR_EINVAL, "gb requested without a bias");
+  if (scores && N > 0 && swvr_distill_scores_size(dtype, w_dtype, N, K, V, ldw) == 0)
+    return fail(SWVR_EINVAL, "scores are not kept for N=%lld K=%lld V=%lld ldw=%lld", (long long)N, (long long)K,
+                (long long)V, (long long)ldw);
   if (gb && !is_dtype(gb_dtype)) return fail(SWVR_EDTYPE, "unsupported gb dtype tag %d", gb_dtype);
   const size_t need = swvr_distill_bwd_workspace_size(dtype, w_dtype, N, K, V, T, chunk, gh != nullptr);
   if (!workspace || workspace_bytes < need)
@@ -627,7 +646,7 @@ int swvr_distill_bwd(int dtype, int h_dtype, int w_dtype, int64_t N, int64_t K, 
   rc = bwd_common(dtype, h_dtype, w_dtype, N, K, V, 0, h, ldh, W, ldw, W, 0, bias_scaled, logit_scale / temperature,
                   nullptr, lse, nullptr, nullptr, chunk, gh, gh_dtype, gW, gW_dtype, nullptr, 0, gb ? dense : nullptr, workspace,
                   up256(plan.ws_bytes), stream, nullptr, 0, 0, nullptr, nullptr, 0, nullptr, pt_id, pt_val, N * T,
-                  (int)T);
+                  (int)T, scores, scores ? swvr::fwd_kept_scores(dtype, N, K, V, ldw) : 0);
   if (rc != SWVR_OK) return rc;
   if (gb && V > 0) {
     if ((e = swvr::sort_ids(pt_id, 0, (int)(N * T), (int)V, order, sid, seg, s)) != hipSuccess ||

@@ -293,6 +293,40 @@ __device__ __forceinline__ void store_ds_block(const f32x16_t& ds, void* stage, 
   }
 }
 
+// dS of a chunk from the scores that the forward kept (D = 0: dS = P gLSE), and its column sums: a workgroup per 32
+// vocabulary rows, 8 threads per row, 4 consecutive tokens each, which are 4 consecutive positions of the stage.  Writes
+// the position blocks that hold active tokens, as the gradient GEMMs read them (rows past the chunk's as zeros).
+template <class T>
+__global__ __launch_bounds__(256) void bwd_kept_scores_kernel(const float* __restrict__ S, int64_t lds,
+                                                              const int* __restrict__ idx,
+                                                              const int* __restrict__ n_act,
+                                                              const float* __restrict__ lsed, int N_pad, int v0, int cv,
+                                                              int n_tb32, T* __restrict__ stage,
+                                                              float* __restrict__ gb) {
+  const int v = blockIdx.x * 32 + threadIdx.x / 8, j = threadIdx.x % 8, na = n_act[0];
+  const int tok0 = 8 * (j & 3) + 4 * (j >> 2);  // stage_tok(4 j)
+  const bool in = v < cv;
+  const float* const row = S + (int64_t)(in ? v0 + v : 0) * lds;
+  float db = 0.f;
+  for (int q0 = tok0; q0 - tok0 < na; q0 += 32) {
+    T ds[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int q = q0 + i;
+      const float x = in && q < na ? fast_exp(row[idx[q]] - lsed[q]) * -lsed[N_pad + q] : 0.f;
+      db += x;
+      ds[i] = from_float<T>(x);
+    }
+    struct alignas(4 * sizeof(T)) X {
+      T v[4];
+    } y = {{ds[0], ds[1], ds[2], ds[3]}};
+    if (stage) *reinterpret_cast<X*>(stage + stage_off(v, (q0 & ~31) + 4 * j, n_tb32)) = y;
+  }
+#pragma unroll
+  for (int o = 1; o < 8; o <<= 1) db += __shfl_xor(db, o);
+  if (gb && in && j == 0) gb[v0 + v] = db;
+}
+
 // The caller's elements of dS over the staged ones of a chunk: one thread per entry, those of other chunks and of
 // inactive tokens left out.  Position of token tok of a 32-token block: stage_tok's inverse.
 template <class T>
@@ -1694,6 +1728,7 @@ hipError_t bwd_run(const BwdPlan& plan, const BwdParams& p, hipStream_t stream) 
   auto wc_buf = [&](int c) { return Wc + (int64_t)(c & 1) * plan.C * p.K; };
   // e4m3 scores: e4m3 h over positions (bytes, read as K8 / 2 pairs) and the per-row multipliers
   const bool f8 = p.hq != nullptr;
+  const bool kept = p.scores != nullptr;  // the forward's scores: nothing of W, E or the bias is packed
   T* hqc = reinterpret_cast<T*>(ws + plan.off_hqc);
   float* multp = f8 ? reinterpret_cast<float*>(ws + plan.off_mult) : nullptr;
   const bool need_stage = p.gh || p.gW;
@@ -1701,7 +1736,7 @@ hipError_t bwd_run(const BwdPlan& plan, const BwdParams& p, hipStream_t stream) 
   const int dh_split = p.gW ? plan.dh_split_w : plan.dh_split_h;
   const bool gemm_de = pstage && p.gE;  // dE^T = gO^T P as tiles of the gradient GEMM launch
   // every chunk has a gradient GEMM launch: the W packing of the scores kernel rides on them
-  const bool fold_pack = !f8 && (need_stage || gemm_de);
+  const bool fold_pack = !f8 && !kept && (need_stage || gemm_de);
 
   {
     // delta, the active tokens, and the token-side operands over positions
@@ -1718,9 +1753,10 @@ hipError_t bwd_run(const BwdPlan& plan, const BwdParams& p, hipStream_t stream) 
     const int64_t nv = (int64_t)plan.V_pad * (plan.DP / 8);
     const T* E = static_cast<const T*>(p.E);
     timing_begin(kKindPack, stream);
-    pack_vocab_kernel<T><<<(unsigned)((nv + 255) / 256), 256, 0, stream>>>(E, p.lde, p.bias, p.V, p.D, plan.V_pad,
-                                                                           plan.DP, rows_vec16(E, p.lde), Ep, biasp,
-                                                                           p.h_scale, p.w_scale, p.scale, multp);
+    if (!kept)
+      pack_vocab_kernel<T><<<(unsigned)((nv + 255) / 256), 256, 0, stream>>>(E, p.lde, p.bias, p.V, p.D, plan.V_pad,
+                                                                             plan.DP, rows_vec16(E, p.lde), Ep, biasp,
+                                                                             p.h_scale, p.w_scale, p.scale, multp);
     if ((e = hipGetLastError()) != hipSuccess) return e;
     if (f8) {
       if (p.K > 0) {
@@ -1754,7 +1790,7 @@ hipError_t bwd_run(const BwdPlan& plan, const BwdParams& p, hipStream_t stream) 
       // packing also writes the row-major copy the dh product reads.
       const int64_t rows0 = p.V < plan.C ? p.V : plan.C;
       const int64_t pad0 = (rows0 + plan.BV - 1) / plan.BV * plan.BV;
-      if ((e = pack_src<T>(p.W, p.w_f32, p.ldw, (int)rows0, p.K, plan.hS, pad0, Wp, stream,
+      if (!kept && (e = pack_src<T>(p.W, p.w_f32, p.ldw, (int)rows0, p.K, plan.hS, pad0, Wp, stream,
                            fold_pack ? Wc : nullptr)) != hipSuccess)
         return e;
     }
@@ -1774,7 +1810,7 @@ hipError_t bwd_run(const BwdPlan& plan, const BwdParams& p, hipStream_t stream) 
     if ((int64_t)Gc * Cc > (int64_t)plan.G * plan.C) Gc = (int)((int64_t)plan.G * plan.C / Cc);
     if (Gc < plan.G) Gc = plan.G;  // a full chunk: the plan's G
     const int n_gpart_c = plan.n_gpart / plan.G * Gc;
-    if (!f8 && !fold_pack && c > 0) {
+    if (!f8 && !kept && !fold_pack && c > 0) {
       timing_begin(kKindPack, stream);
       e = pack_src<T>(static_cast<const char*>(p.W) + (int64_t)v0 * p.ldw * (p.w_f32 ? 4 : (int64_t)sizeof(T)),
                       p.w_f32, p.ldw, cv, p.K, plan.hS, Cc, Wp, stream, nullptr);
@@ -1812,7 +1848,15 @@ hipError_t bwd_run(const BwdPlan& plan, const BwdParams& p, hipStream_t stream) 
     sp.need_db = p.gb != nullptr;
     sp.n_act = n_act;
     sp.DP = plan.DP;
-    if ((e = dispatch_scores<T>(plan, sp, stream)) != hipSuccess) return e;
+    if (kept) {
+      timing_begin(kKindBwdScores, stream);
+      bwd_kept_scores_kernel<T><<<(unsigned)(Cc / 32), 256, 0, stream>>>(
+          p.scores, p.lds, idx, n_act, lsed, (int)plan.N_pad, v0, cv, sp.n_tb32, need_stage ? stage : nullptr, p.gb);
+      timing_end(kKindBwdScores, stream);
+      if ((e = hipGetLastError()) != hipSuccess) return e;
+    } else if ((e = dispatch_scores<T>(plan, sp, stream)) != hipSuccess) {
+      return e;
+    }
     if (p.pt_id && need_stage && p.n_pt > 0) {
       timing_begin(kKindDistill, stream);
       bwd_patch_kernel<T><<<(unsigned)((p.n_pt + 255) / 256), 256, 0, stream>>>(
@@ -1858,7 +1902,7 @@ hipError_t bwd_run(const BwdPlan& plan, const BwdParams& p, hipStream_t stream) 
       gp.n_act = n_act;
       // the reduction of the scores kernel's partials rides on this launch (the wide kernel's dE^T
       // is formed in it, so that reduction follows as a launch of its own)
-      fold_red = (p.gE || p.gb) && !gemm_de;
+      fold_red = (p.gE || p.gb) && !gemm_de && !kept;
       gp.n_red_v = (cv + GemmTile<T>::NT / 8 - 1) / (GemmTile<T>::NT / 8);
       gp.n_red = fold_red ? gp.n_red_v * (p.gE && p.D > 0 ? (p.D + kRedD - 1) / kRedD : 1) : 0;
       gp.part_db = part_db;
@@ -1890,7 +1934,7 @@ hipError_t bwd_run(const BwdPlan& plan, const BwdParams& p, hipStream_t stream) 
       }
       if ((e = dispatch_gemm<T>(plan, gp, stream)) != hipSuccess) return e;
     }
-    if ((p.gE || p.gb) && !fold_red) {
+    if ((p.gE || p.gb) && !fold_red && !kept) {
       timing_begin(kKindBwdReduce, stream);
       const dim3 grid((unsigned)((cv + kRedV - 1) / kRedV),
                       p.gE && p.D > 0 ? (unsigned)((p.D + kRedD - 1) / kRedD) : 1u);

@@ -65,23 +65,23 @@ __device__ __forceinline__ void load8(const S* row, float (&v)[8]) {
   for (int i = 0; i < 8; ++i) v[i] = (float)(T)x[i];
 }
 
-// z of kDotIds entries of a token per wave: h's 8 values of a lane serve them all.
-constexpr int kDotIds = 4;
-template <class T, class HS, class WS>
+// z of IDS entries of a token per wave: h's 8 values of a lane serve them all.  4 where waves are many; 1 with 4 steps
+// of its row in flight where they are few and each waits for its rows (8 tokens, T = 10, K = 4096: 24 -> 6 us).
+template <class T, class HS, class WS, int IDS, int STEPS>
 __global__ __launch_bounds__(256) void distill_dot_kernel(DistillParams p) {
-  const int groups = (p.T + kDotIds - 1) / kDotIds;
+  const int groups = (p.T + IDS - 1) / IDS;
   const int64_t gw = (int64_t)blockIdx.x * 4 + wave_id();
   if (gw >= (int64_t)p.N * groups) return;
-  const int n = (int)(gw / groups), k0 = (int)(gw % groups) * kDotIds;
+  const int n = (int)(gw / groups), k0 = (int)(gw % groups) * IDS;
   if (p.weight && p.weight[n] == 0.f) return;
   const int lane = lane_id();
   const HS* const h = static_cast<const HS*>(p.h) + (int64_t)n * p.ldh;
-  const WS* w[kDotIds];
-  bool in[kDotIds];
-  int id[kDotIds];
+  const WS* w[IDS];
+  bool in[IDS];
+  int id[IDS];
   bool any = false;
 #pragma unroll
-  for (int u = 0; u < kDotIds; ++u) {
+  for (int u = 0; u < IDS; ++u) {
     const int64_t x = k0 + u < p.T ? id_at(p, n, k0 + u) : -1;
     in[u] = x >= 0 && x < p.V;
     id[u] = in[u] ? (int)x : 0;
@@ -89,23 +89,30 @@ __global__ __launch_bounds__(256) void distill_dot_kernel(DistillParams p) {
     any |= in[u];
   }
   if (!any) return;
-  float acc[kDotIds];
+  float acc[IDS];
 #pragma unroll
-  for (int u = 0; u < kDotIds; ++u) acc[u] = 0.f;
-  for (int k = lane * 8; k < p.K; k += 512) {
-    float a[8];
-    load8<T, HS>(h + k, a);
+  for (int u = 0; u < IDS; ++u) acc[u] = 0.f;
+  for (int k = lane * 8; k < p.K; k += 512 * STEPS) {
+    float a[STEPS][8], b[STEPS][IDS][8];
 #pragma unroll
-    for (int u = 0; u < kDotIds; ++u) {
-      if (!in[u]) continue;
-      float b[8];
-      load8<T, WS>(w[u] + k, b);
+    for (int s = 0; s < STEPS; ++s) {
+      const int at = k + 512 * s < p.K ? k + 512 * s : k;  // (past the row: again, and not added)
+      load8<T, HS>(h + at, a[s]);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) acc[u] = fmaf(a[i], b[i], acc[u]);
+      for (int u = 0; u < IDS; ++u)
+        if (in[u]) load8<T, WS>(w[u] + at, b[s][u]);
     }
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s)
+      if (k + 512 * s < p.K)
+#pragma unroll
+        for (int u = 0; u < IDS; ++u)
+          if (in[u])
+#pragma unroll
+            for (int i = 0; i < 8; ++i) acc[u] = fmaf(a[s][i], b[s][u][i], acc[u]);
   }
 #pragma unroll
-  for (int u = 0; u < kDotIds; ++u) {
+  for (int u = 0; u < IDS; ++u) {
     const float s = wave_sum(acc[u]);
     if (lane == u && in[u]) p.z[(int64_t)n * p.T + k0 + u] = s * p.scale + (p.bias ? p.bias[id[u]] : 0.f);
   }
@@ -265,49 +272,70 @@ __global__ __launch_bounds__(256) void distill_prep_kernel(DistillGradParams p) 
   }
 }
 
-// gb[v] = (dense[v] - sum of t over the entries of v) / tau, a wave per id, in gb's dtype.
+// gb[v] = (dense[v] - sum of t over the entries of v) / tau in gb's dtype.  A thread per id, and for an id of more
+// than kBiasAlone entries a wave.  (A wave for every id, most of which have no entry: 38 us for V = 252561.)
+constexpr int kBiasAlone = 4;
 __global__ __launch_bounds__(256) void distill_bias_kernel(const int* __restrict__ order, const int* __restrict__ seg,
                                                            const float* __restrict__ t,
                                                            const float* __restrict__ dense, int V, float inv_tau,
                                                            void* __restrict__ gb, int gb_dtype) {
-  const int v = blockIdx.x * 4 + wave_id();
-  if (v >= V) return;
-  const int lane = lane_id(), i1 = seg[v + 1];
-  float s = 0.f;
-  for (int i = seg[v] + lane; i < i1; i += 256) {
-    float x[4];
+  __shared__ int s_long[256], s_n;
+  const int v = blockIdx.x * 256 + threadIdx.x, lane = lane_id();
+  if (threadIdx.x == 0) s_n = 0;
+  __syncthreads();
+  auto store = [&](int at, float sum) {
+    const float y = (dense[at] - sum) * inv_tau;
+    if (gb_dtype == kBF16)
+      static_cast<bf16_t*>(gb)[at] = (bf16_t)y;
+    else if (gb_dtype == kF16)
+      static_cast<f16_t*>(gb)[at] = (f16_t)y;
+    else
+      static_cast<float*>(gb)[at] = y;
+  };
+  if (v < V) {
+    const int i0 = seg[v], i1 = seg[v + 1];
+    if (i1 - i0 > kBiasAlone) {
+      s_long[atomicAdd(&s_n, 1)] = v;  // whose wave takes an id does not matter
+    } else {
+      float x[kBiasAlone];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) x[u] = i + 64 * u < i1 ? t[order[i + 64 * u]] : 0.f;
-    s += (x[0] + x[1]) + (x[2] + x[3]);
+      for (int u = 0; u < kBiasAlone; ++u) x[u] = i0 + u < i1 ? t[order[i0 + u]] : 0.f;
+      store(v, (x[0] + x[1]) + (x[2] + x[3]));
+    }
   }
-  s = wave_sum(s);
-  if (lane != 0) return;
-  const float y = (dense[v] - s) * inv_tau;
-  if (gb_dtype == kBF16)
-    static_cast<bf16_t*>(gb)[v] = (bf16_t)y;
-  else if (gb_dtype == kF16)
-    static_cast<f16_t*>(gb)[v] = (f16_t)y;
+  __syncthreads();
+  for (int j = wave_id(); j < s_n; j += 4) {
+    const int at = s_long[j], i1 = seg[at + 1];
+    float s = 0.f;
+    for (int i = seg[at] + lane; i < i1; i += 256) {
+      float x[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) x[u] = i + 64 * u < i1 ? t[order[i + 64 * u]] : 0.f;
+      s += (x[0] + x[1]) + (x[2] + x[3]);
+    }
+    s = wave_sum(s);
+    if (lane == 0) store(at, s);
+  }
+}
+
+template <class T, class HS, class WS>
+hipError_t dot_launch(const DistillParams& p, hipStream_t stream) {
+  constexpr int64_t kManyWaves = 4096;
+  const int64_t many = (int64_t)p.N * ((p.T + 3) / 4), few = (int64_t)p.N * p.T;
+  if (many >= kManyWaves)
+    distill_dot_kernel<T, HS, WS, 4, 1><<<(unsigned)((many + 3) / 4), 256, 0, stream>>>(p);
   else
-    static_cast<float*>(gb)[v] = y;
+    distill_dot_kernel<T, HS, WS, 1, 4><<<(unsigned)((few + 3) / 4), 256, 0, stream>>>(p);
+  return hipGetLastError();
 }
 
 template <class T>
 hipError_t dot_typed(const DistillParams& p, hipStream_t stream) {
-  const int64_t waves = (int64_t)p.N * ((p.T + kDotIds - 1) / kDotIds);
-  const unsigned blocks = (unsigned)((waves + 3) / 4);
   if constexpr (sizeof(T) == 2) {
-    if (p.h_f32 && p.w_f32)
-      distill_dot_kernel<T, float, float><<<blocks, 256, 0, stream>>>(p);
-    else if (p.h_f32)
-      distill_dot_kernel<T, float, T><<<blocks, 256, 0, stream>>>(p);
-    else if (p.w_f32)
-      distill_dot_kernel<T, T, float><<<blocks, 256, 0, stream>>>(p);
-    else
-      distill_dot_kernel<T, T, T><<<blocks, 256, 0, stream>>>(p);
-  } else {
-    distill_dot_kernel<T, T, T><<<blocks, 256, 0, stream>>>(p);
+    if (p.h_f32) return p.w_f32 ? dot_launch<T, float, float>(p, stream) : dot_launch<T, float, T>(p, stream);
+    if (p.w_f32) return dot_launch<T, T, float>(p, stream);
   }
-  return hipGetLastError();
+  return dot_launch<T, T, T>(p, stream);
 }
 
 }  // namespace
@@ -352,7 +380,7 @@ hipError_t distill_prep(const DistillGradParams& p, hipStream_t stream) {
 hipError_t distill_bias(const int* order, const int* seg, const float* t, const float* dense, int V, float inv_tau,
                         void* gb, int gb_dtype, hipStream_t stream) {
   timing_begin(kKindDistill, stream);
-  distill_bias_kernel<<<(unsigned)((V + 3) / 4), 256, 0, stream>>>(order, seg, t, dense, V, inv_tau, gb, gb_dtype);
+  distill_bias_kernel<<<(unsigned)((V + 255) / 256), 256, 0, stream>>>(order, seg, t, dense, V, inv_tau, gb, gb_dtype);
   timing_end(kKindDistill, stream);
   return hipGetLastError();
 }

@@ -1019,7 +1019,7 @@ void few_plan(int dtype, int64_t N, int64_t V, int64_t Dw, bool active, size_t o
   plan->few = takes_few(dtype, N);
   if (!plan->few) return;
   const bool two = dtype != kF32;
-  plan->few_DP = !two && Dw <= 32 ? 32 : Dw <= 64 ? 64 : Dw <= 128 ? 128 : 256;
+  plan->few_DP = Dw == 0 ? 0 : !two && Dw <= 32 ? 32 : Dw <= 64 ? 64 : Dw <= 128 ? 128 : 256;
   const int nb_max = plan->few_DP <= 128 ? 4 : 2;
   plan->few_NB = N <= 32 ? 1 : N <= 64 || nb_max == 2 ? 2 : 4;
   plan->few_tb = (int)((N + 32 * plan->few_NB - 1) / (32 * plan->few_NB));
@@ -1076,6 +1076,8 @@ FwdFewParams few_params(const FwdPlan& plan, const FwdParams& p, char* ws) {
   q.part_m = reinterpret_cast<float*>(ws + plan.few_m);
   q.part_l = reinterpret_cast<float*>(ws + plan.few_l);
   q.part_acc = reinterpret_cast<float*>(ws + plan.few_acc);
+  q.scores = p.scores;
+  q.lds = (int64_t)plan.few_tb * 32 * plan.few_NB;
   return q;
 }
 
@@ -1242,9 +1244,19 @@ bool fwd_plan(int dtype, int64_t N, int64_t K, int64_t V, int64_t D, FwdPlan* pl
   return true;
 }
 
+int64_t fwd_kept_scores(int dtype, int64_t N, int64_t K, int64_t V, int64_t ldw) {
+  FwdPlan plan;
+  if (N <= 0 || !fwd_plan(dtype, N, K, V, 0, &plan)) return 0;
+  FwdParams p{};
+  p.ldw = ldw;
+  const int64_t lds = (int64_t)plan.few_tb * 32 * plan.few_NB, esz = dtype == kF32 ? 4 : 2;
+  return plan.few && few_fits(plan, p, dtype) && lds * 4 <= 2 * K * esz ? lds : 0;
+}
+
 hipError_t fwd_launch(int dtype, const FwdPlan& plan, FwdParams p, char* ws, float* O, float* lse, float* m_out,
                       float* l_out, hipStream_t stream) {
   if (p.N == 0) return hipSuccess;
+  if (p.scores && !few_fits(plan, p, dtype)) return hipErrorInvalidValue;
   if (few_fits(plan, p, dtype)) return fwd_few(dtype, plan, p, nullptr, ws, O, lse, m_out, l_out, stream);
   p.n_tb = plan.n_tb;
   p.n_split = plan.n_split;

@@ -26,6 +26,8 @@
 //     The E^T operand is read from the row-major E tile with transposing LDS reads;
 //   * the waves' partial softmaxes are merged in LDS, so a workgroup writes one
 //     partial; fwd_combine_kernel merges those in a fixed order.
+// Without columns (D = 0: LSE alone, of a loss on the distribution itself) there are no E tile and no
+// acc, and the scores can be kept, [V][lds] in fp32, for a backward that then needs no product to form them.
 #include <type_traits>
 
 #include "common.hpp"
@@ -106,11 +108,12 @@ struct FewCfg {
   static constexpr bool HPART = HBYTES < NT * 16;  // h of a stage is less than one load per thread
   static constexpr int SB = TW::BYTES + HBYTES;
   static constexpr int L = TW::NI + NIH;            // loads a thread issues per stage (at least)
-  typedef FewETile<T, DP, NT> TE;
-  static constexpr int FIT = (kLdsBytes - TE::BYTES) / SB;
+  typedef FewETile<T, DP ? DP : 64, NT> TE;
+  static constexpr int EBYTES = DP ? TE::BYTES : 0;
+  static constexpr int FIT = (kLdsBytes - EBYTES) / SB;
   static constexpr int NS = FIT < 8 ? FIT : 8;
   static_assert(NS >= 2 && (NS - 2) * L < 64, "ring depth");
-  static constexpr int LDS = NS * SB + TE::BYTES;
+  static constexpr int LDS = NS * SB + EBYTES;
   // the merge of the waves' partials reuses the LDS: 4 x [DP][32] floats, then 4 x [32 NB] of two
   static_assert(kFewWV * (DP * 32 + 2 * 32 * NB) * 4 <= LDS, "merge fits");
 };
@@ -136,7 +139,7 @@ __global__ __launch_bounds__((FewCfg<T, WS, DP, FT, WT>::NT)) void fwd_few_kerne
   typedef typename C::TH TH;
   typedef typename C::TE TE;
   typedef typename Vec8<T>::type V8;
-  constexpr int BK = C::BK, HS = C::HS, NS = C::NS, SB = C::SB, L = C::L, DB = DP / 32;
+  constexpr int BK = C::BK, HS = C::HS, NS = C::NS, SB = C::SB, L = C::L, DB = DP ? DP / 32 : 1;
   constexpr int J = C::HK / 16;  // k16 steps per slice of h
   __shared__ __attribute__((aligned(1024))) char smem[C::LDS];
   char* const sE = smem + NS * SB;
@@ -234,7 +237,7 @@ __global__ __launch_bounds__((FewCfg<T, WS, DP, FT, WT>::NT)) void fwd_few_kerne
       slot = slot == NS - 1 ? 0 : slot + 1;
       // every wave has finished the stage before this one, whose slot the next load takes, and with
       // a tile's first stage the previous tile's epilogue, so its E tile can be replaced
-      if (kt == 0)
+      if (DP > 0 && kt == 0)
         TE::issue(static_cast<const T*>(p.E) + (int64_t)v0 * p.lde, p.lde * (int64_t)sizeof(T), v_end - v0, p.D, ldsE);
       issue_next();
       const char* st = smem + slot * SB;
@@ -257,7 +260,7 @@ __global__ __launch_bounds__((FewCfg<T, WS, DP, FT, WT>::NT)) void fwd_few_kerne
         }
     }
     // the E tile: covered by the stage waits after it unless the walk is short
-    if (nk < NS) {
+    if (DP > 0 && nk < NS) {
       wait_vmcnt<0>();
       stage_barrier();
     }
@@ -278,6 +281,16 @@ __global__ __launch_bounds__((FewCfg<T, WS, DP, FT, WT>::NT)) void fwd_few_kerne
         sacc[ft][r] = x;
         mx = fmaxf(mx, x);
       }
+      if constexpr (DP == 0) {
+        if (p.scores) {  // a register's 32 tokens of a row: whole lines
+          float* const s0 = p.scores + n0 + (wt * FT + ft) * 32 + (lane & 31);
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int v = v0 + 32 * wv + c_row(r, lane);
+            if (v < v_end) s0[(int64_t)v * p.lds] = sacc[ft][r];
+          }
+        }
+      }
       mx = wave_max32(mx);
       const float mnew = fmaxf(m[ft], mx);
       const float snew = TS ? tile_shift(mx, mnew) : mnew;
@@ -296,11 +309,13 @@ __global__ __launch_bounds__((FewCfg<T, WS, DP, FT, WT>::NT)) void fwd_few_kerne
       rs = wave_sum32(rs);
       l[ft] = TS ? shifted_sum(l[ft], m[ft], rs, shift, mnew) : l[ft] * alpha + rs;
       m[ft] = mnew;
+      if constexpr (DP > 0)
 #pragma unroll
-      for (int db = 0; db < DB; ++db)
+        for (int db = 0; db < DB; ++db)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) oacc[db][ft][r] *= alpha;
+          for (int r = 0; r < 16; ++r) oacc[db][ft][r] *= alpha;
     }
+    if constexpr (DP == 0) continue;
     // ---- acc^T[d][token] += E^T[d][v] P^T[v][token]
     const int ln = lane + opaque_zero();
 #pragma unroll
@@ -343,6 +358,7 @@ __global__ __launch_bounds__((FewCfg<T, WS, DP, FT, WT>::NT)) void fwd_few_kerne
       const float shift = M == kNegInf ? 0.f : M;
       if (wt == bt) {
         const float f = expf(sh[ft] - shift);  // exp(-inf) = 0: a wave of masked rows adds nothing
+        if constexpr (DP > 0)
 #pragma unroll
         for (int db = 0; db < DB; ++db)
 #pragma unroll
@@ -390,6 +406,7 @@ hipError_t dispatch_nb(const FwdFewParams& p, hipStream_t stream) {
 template <class T, class WS>
 hipError_t dispatch_dp(const FwdFewParams& p, hipStream_t stream) {
   switch (p.DP) {
+    case 0: return dispatch_nb<T, WS, 0>(p, stream);
     case 32:
       if constexpr (sizeof(T) == 4) return dispatch_nb<T, WS, 32>(p, stream);
       return hipErrorInvalidValue;

@@ -55,6 +55,7 @@ struct FwdParams {
   int h_f32, w_f32;    // h / W stored in fp32 (rounded to the compute dtype as they are packed)
   const float* h_scale;  // e4m3 forward: [1] dequantisation scale of h, else null
   const float* w_scale;  // e4m3 forward: [V] dequantisation scales of W's rows, else null
+  float* scores;         // D = 0 with few tokens: the scores, [V][fwd_kept_scores], are kept here; null: not
   // Active-token forward: [0] the count of active tokens, whose rows are packed
   // in position order (hp), [3] / [4] the token blocks and vocabulary splits
   // (fwd_active_grid_kernel), all on the device; null: every token, at its own row.
@@ -119,6 +120,10 @@ bool fwd_plan(int dtype, int64_t N, int64_t K, int64_t V, int64_t D, FwdPlan* pl
 // unnormalised acc in O) of the vocabulary rows given.
 hipError_t fwd_launch(int dtype, const FwdPlan& plan, FwdParams p, char* ws, float* O, float* lse, float* m_out,
                       float* l_out, hipStream_t stream);
+// Tokens per vocabulary row, with padding, of the scores that a forward without columns keeps (FwdParams::scores) for
+// a backward that then forms no scores, or 0 where it does not: it is the few-token kernel's, of a W stored in the
+// compute dtype, and the scores take at most twice W's bytes.
+int64_t fwd_kept_scores(int dtype, int64_t N, int64_t K, int64_t V, int64_t ldw);
 // The forward of the tokens with a non-zero weight (weight: fp32 [N]); O rows
 // and lse of the others are 0.  A zero-weight token whose h row holds an
 // infinity or a NaN stays active, and so does every token when W, E or the
@@ -139,7 +144,7 @@ struct FwdFewParams {
   const float* bias;   // [V] or null
   float scale;
   int N, K, V, D;
-  int DP, NB;          // padded D (32 fp32 only, 64, 128, 256), 32-token blocks per workgroup (1, 2, 4)
+  int DP, NB;          // padded D (0, 32 fp32 only, 64, 128, 256), 32-token blocks per workgroup (1, 2, 4)
   int n_tb, n_split;   // token blocks, vocabulary runs
   int n_wg;            // workgroups to launch (n_tb x n_split, or with n_act as many as may be needed)
   // active tokens only: hp holds their rows in position order, [3] / [4] of this device block the token
@@ -148,6 +153,8 @@ struct FwdFewParams {
   float* part_m;       // [n_split][N] (with n_act, rows of [3] x 32 NB positions)
   float* part_l;
   float* part_acc;     // [n_split][DP][N]
+  float* scores;       // DP = 0: [V][lds], or null
+  int64_t lds;
 };
 
 // Vocabulary runs of the few-token forward for n_tb token blocks over grp 32-row groups, when one
@@ -314,6 +321,9 @@ struct BwdParams {
   const float* pt_val;
   int64_t n_pt;
   int pt_T;
+  // with them: the scores that the forward kept, [V][lds] by token, or null (D = 0, W in the compute dtype)
+  const float* scores;
+  int64_t lds;
 };
 
 hipError_t bwd_launch(int dtype, const BwdPlan& plan, const BwdParams& p, hipStream_t stream);

@@ -1,4 +1,4 @@
-"""Distillation of the head from a teacher's top logits, without the [tokens, V] scores.
+"""Distillation of the head from a teacher's top logits, without a [tokens, V] matrix for many tokens.
 
 Where ``softmax_readout_mse`` trains the readout O against target vectors, ``softmax_distill`` trains the
 distribution itself against the part of a teacher's that is kept: its largest logits and their ids, the way
@@ -33,8 +33,9 @@ def _kept(kept, N, T, need_grad):
     return (at, lse, coef, coef + 4 * N, coef + 4 * (N + N * T)) if need_grad else (at, lse, None, None, None)
 
 
-def _forward(h, W, bias, teacher, ids, weight, tau, z, reduction, scale, cdt, need_grad):
-    """The loss, what ``_kept`` names, and the bias over tau in fp32 (empty without a bias)."""
+def _forward(h, W, bias, teacher, ids, weight, tau, z, reduction, scale, chunk, cdt, need_grad):
+    """The loss, what ``_kept`` names, the bias over tau in fp32 (empty without a bias), and the scores where the
+    library keeps them for the backward (few tokens, no chunk given; else empty)."""
     lib = _lib.load()
     N, K = h.shape
     V, T = W.shape[0], ids.shape[1]
@@ -47,15 +48,19 @@ def _forward(h, W, bias, teacher, ids, weight, tau, z, reduction, scale, cdt, ne
     out = hc.new_empty((N,) if reduction == 0 else (), dtype=torch.float32)
     kept = hc.new_empty(1 + N * (2 * T + 2) if need_grad else 1 + N, dtype=torch.float32)
     sb = hc.new_empty(V if b is not None else 0, dtype=torch.float32)
-    ws_bytes = lib.swvr_distill_workspace_size(tag, N, Kp, V, T, w is not None)
+    scores = None
+    if need_grad and chunk is None:
+        kept_bytes = lib.swvr_distill_scores_size(tag, w_tag, N, Kp, V, _lead_stride(Wc))
+        scores = hc.new_empty(kept_bytes // 4, dtype=torch.float32) if kept_bytes else None
+    ws_bytes = lib.swvr_distill_workspace_size(tag, N, Kp, V, T, w is not None and scores is None)
     ws = hc.new_empty(ws_bytes, dtype=torch.uint8)
     a = _lib.address
     c, lse, coef, p, q = _kept(kept, N, T, need_grad)
     _lib.call(lib.swvr_distill, h.device, tag, h_tag, w_tag, N, Kp, V, T, hc.data_ptr(), _lead_stride(hc),
               Wc.data_ptr(), _lead_stride(Wc), a(b), _lib.DTYPE_TAG[b.dtype] if b is not None else 0, sb.data_ptr(),
               scale, i.data_ptr(), i.dtype == torch.int64, i.stride(0), t.data_ptr(), _lib.DTYPE_TAG[t.dtype],
-              t.stride(0), tau, a(w), z, reduction, out.data_ptr(), c, lse, p, q, coef, ws.data_ptr(), ws_bytes)
-    return out, kept, sb
+              t.stride(0), tau, a(w), z, reduction, out.data_ptr(), c, lse, p, q, coef, a(scores), ws.data_ptr(), ws_bytes)
+    return out, kept, sb, scores
 
 
 def _bias(bias):
@@ -66,7 +71,7 @@ def _bias(bias):
     return (b if b.dtype in _lib.DTYPE_TAG else b.to(torch.float32)).contiguous()
 
 
-def _backward(g, h, W, bias, ids, kept, sb, tau, z, reduction, scale, chunk, cdt, need_h, need_W, need_b):
+def _backward(g, h, W, bias, ids, kept, sb, scores, tau, z, reduction, scale, chunk, cdt, need_h, need_W, need_b):
     lib = _lib.load()
     N, K = h.shape
     V, T = W.shape[0], ids.shape[1]
@@ -89,7 +94,8 @@ def _backward(g, h, W, bias, ids, kept, sb, tau, z, reduction, scale, chunk, cdt
     c, lse, coef, p, q = _kept(kept, N, T, True)
     _lib.call(lib.swvr_distill_bwd, dev, tag, h_tag, w_tag, N, Kp, V, T, hc.data_ptr(), _lead_stride(hc),
               Wc.data_ptr(), _lead_stride(Wc), sb.data_ptr() if bias is not None else None, scale, i.data_ptr(),
-              i.dtype == torch.int64, i.stride(0), tau, z, reduction, g32.data_ptr(), c, lse, p, q, coef, chunk, *of(gh),
+              i.dtype == torch.int64, i.stride(0), tau, z, reduction, g32.data_ptr(), c, lse, p, q, coef, _lib.address(scores),
+              chunk, *of(gh),
               *of(gW), *of(gb), ws.data_ptr(), ws_bytes)
     if gh is not None:
         gh = gh[:, :K] if Kp != K else gh
@@ -106,7 +112,7 @@ def _backward(g, h, W, bias, ids, kept, sb, tau, z, reduction, scale, chunk, cdt
 def _fwd_op(h: torch.Tensor, W: torch.Tensor, bias: Optional[torch.Tensor], teacher: torch.Tensor, ids: torch.Tensor,
             weight: Optional[torch.Tensor], tau: float, z: float, reduction: int, scale: float, chunk: int,
             cdt: torch.dtype, need_grad: bool) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    return _forward(h, W, bias, teacher, ids, weight, tau, z, reduction, scale, cdt, need_grad)
+    return _forward(h, W, bias, teacher, ids, weight, tau, z, reduction, scale, chunk, cdt, need_grad)[:3]
 
 
 @_fwd_op.register_fake
@@ -124,7 +130,7 @@ def _(h, W, bias, teacher, ids, weight, tau, z, reduction, scale, chunk, cdt, ne
 def _bwd_op(g: torch.Tensor, h: torch.Tensor, W: torch.Tensor, bias: Optional[torch.Tensor], ids: torch.Tensor,
             kept: torch.Tensor, sb: torch.Tensor, tau: float, z: float, reduction: int, scale: float, chunk: int,
             cdt: torch.dtype, need_h: bool, need_W: bool, need_b: bool) -> List[torch.Tensor]:
-    grads = _backward(g, h, W, bias, ids, kept, sb, tau, z, reduction, scale, chunk, cdt, need_h, need_W, need_b)
+    grads = _backward(g, h, W, bias, ids, kept, sb, None, tau, z, reduction, scale, chunk, cdt, need_h, need_W, need_b)
     # a custom op cannot return None: an empty tensor stands for "no gradient"
     return [x if x is not None else h.new_empty(0) for x in grads]
 
@@ -166,8 +172,8 @@ class _Distill(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, h, W, bias, teacher, ids, weight, tau, z, reduction, scale, chunk, cdt):
-        out, kept, sb = _forward(h, W, bias, teacher, ids, weight, tau, z, reduction, scale, cdt, True)
-        ctx.save_for_backward(h, W, bias, ids, kept, sb)
+        out, kept, sb, scores = _forward(h, W, bias, teacher, ids, weight, tau, z, reduction, scale, chunk, cdt, True)
+        ctx.save_for_backward(h, W, bias, ids, kept, sb, scores)
         ctx.args = (tau, z, reduction, scale, chunk, cdt)
         return out
 
@@ -179,7 +185,7 @@ class _Distill(torch.autograd.Function):
         if eager(g, *saved):
             grads = _backward(g, *saved, *ctx.args, *needs)
         else:
-            grads = _op_grads(g, saved, ctx.args, needs)
+            grads = _op_grads(g, saved[:-1], ctx.args, needs)
         return (*grads, *[None] * 9)
 
 
@@ -230,8 +236,10 @@ def softmax_distill(h, W, teacher_logits, teacher_ids, bias=None, *, temperature
     "mean" (the weighted sum over the sum of the weights of the tokens that have an entry; 0 without any),
     "sum" or "none" (the per-token terms).  The loss is fp32; there is no factor of ``temperature ** 2``.  The
     products run in autocast's dtype or the promotion of h's and W's (bf16, fp16 or fp32), and the backward
-    recomputes the scores ``chunk_size`` vocabulary rows at a time, as ``softmax_readout`` does.  Autograd
-    reaches h, W and bias; the teacher and the weight get none.
+    recomputes the scores ``chunk_size`` vocabulary rows at a time, as ``softmax_readout`` does.  An eager call
+    without a chunk keeps the scores of few tokens (up to 768, in fp32 any number) for it instead, where they take
+    at most twice W's bytes (K tokens in the 2-byte types, 2 K in fp32).  Autograd reaches h, W and bias; the
+    teacher and the weight get none.
     """
     _check(h, W, teacher_logits, teacher_ids, bias, weight, temperature, reduction)
     chunk = _chunk(chunk_size)
@@ -249,7 +257,7 @@ def softmax_distill(h, W, teacher_logits, teacher_ids, bias=None, *, temperature
         if need:
             out = _Distill.apply(h2, W, bias, t2, i2, w1, *args, chunk, cdt)
         else:
-            out = _forward(h2, W, bias, t2, i2, w1, *args, cdt, False)[0]
+            out = _forward(h2, W, bias, t2, i2, w1, *args, chunk, cdt, False)[0]
     else:
         if h.device.type == "cpu":
             _require_device(h)

@@ -128,14 +128,14 @@ def sample(dtype=_lib.BF16, R=4, V=8, logits=P, ld=8, u=P, u64=0, tau=1.0, token
 
 
 def distill_abi(dtype=_lib.BF16, N=4, K=16, V=8, T=2, h=P, ids=P, id64=1, teacher=P, t_dtype=_lib.F32, tau=1.0, red=2,
-                out=P, c=P, lse=P, p=P, q=P, coef=P, ws=P, nbytes=1 << 30):
+                out=P, c=P, lse=P, p=P, q=P, coef=P, scores=None, ws=P, nbytes=1 << 30):
     return _lib.load().swvr_distill(dtype, dtype, dtype, N, K, V, T, h, 16, P, 16, None, 0, None, 1.0, ids, id64, T, teacher,
-                                    t_dtype, T, tau, None, 0.0, red, out, c, lse, p, q, coef, ws, nbytes, None)
+                                    t_dtype, T, tau, None, 0.0, red, out, c, lse, p, q, coef, scores, ws, nbytes, None)
 
 
-def distill_bwd_abi(dtype=_lib.BF16, N=4, V=8, T=2, tau=1.0, chunk=8192, g=P, gb=None, ws=P, nbytes=1 << 30):
+def distill_bwd_abi(dtype=_lib.BF16, N=4, V=8, T=2, tau=1.0, chunk=8192, g=P, gb=None, scores=None, ws=P, nbytes=1 << 30):
     return _lib.load().swvr_distill_bwd(dtype, dtype, dtype, N, 16, V, T, P, 16, P, 16, None, 1.0, P, 1, T, tau, 0.0, 2,
-                                        g, P, P, P, P, P, chunk, P, dtype, P, dtype, gb, 2, ws, nbytes, None)
+                                        g, P, P, P, P, P, scores, chunk, P, dtype, P, dtype, gb, 2, ws, nbytes, None)
 
 
 @pytest.mark.parametrize("fn,kw,code", [
@@ -181,6 +181,8 @@ def distill_bwd_abi(dtype=_lib.BF16, N=4, V=8, T=2, tau=1.0, chunk=8192, g=P, gb
     (distill_abi, dict(K=12), _lib.EINVAL),
     (distill_abi, dict(h=ctypes.c_void_p(8)), _lib.EINVAL),
     (distill_abi, dict(nbytes=64), _lib.EWORKSPACE),
+    (distill_abi, dict(N=1000, V=4000, scores=P), _lib.EINVAL),       # more tokens than scores are kept of
+    (distill_bwd_abi, dict(N=1000, V=4000, scores=P), _lib.EINVAL),
     (distill_bwd_abi, dict(dtype=7), _lib.EDTYPE),
     (distill_bwd_abi, dict(chunk=0), _lib.EINVAL),
     (distill_bwd_abi, dict(g=None), _lib.EINVAL),
