@@ -122,7 +122,8 @@ hipError_t fwd_launch(int dtype, const FwdPlan& plan, FwdParams p, char* ws, flo
                       float* l_out, hipStream_t stream);
 // Tokens per vocabulary row, with padding, of the scores that a forward without columns keeps (FwdParams::scores) for
 // a backward that then forms no scores, or 0 where it does not: it is the few-token kernel's, of a W stored in the
-// compute dtype, and the scores take at most twice W's bytes.
+// compute dtype, and the scores take at most twice W's bytes and kKeptScoresMost.
+constexpr int64_t kKeptScoresMost = (int64_t)512 << 20;
 int64_t fwd_kept_scores(int dtype, int64_t N, int64_t K, int64_t V, int64_t ldw);
 // The forward of the tokens with a non-zero weight (weight: fp32 [N]); O rows
 // and lse of the others are 0.  A zero-weight token whose h row holds an

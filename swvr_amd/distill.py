@@ -238,8 +238,8 @@ def softmax_distill(h, W, teacher_logits, teacher_ids, bias=None, *, temperature
     products run in autocast's dtype or the promotion of h's and W's (bf16, fp16 or fp32), and the backward
     recomputes the scores ``chunk_size`` vocabulary rows at a time, as ``softmax_readout`` does.  An eager call
     without a chunk keeps the scores of few tokens (up to 768, in fp32 any number) for it instead, where they take
-    at most twice W's bytes (K tokens in the 2-byte types, 2 K in fp32).  Autograd reaches h, W and bias; the
-    teacher and the weight get none.
+    at most twice W's bytes (K tokens in the 2-byte types, 2 K in fp32) and 512 MB.  Autograd reaches h, W and
+    bias; the teacher and the weight get none.
     """
     _check(h, W, teacher_logits, teacher_ids, bias, weight, temperature, reduction)
     chunk = _chunk(chunk_size)

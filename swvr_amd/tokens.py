@@ -150,7 +150,8 @@ def _per_row(x, dtype, R):
     if x is None:
         return None
     x = _plain(x).reshape(R)
-    x = x if x.dtype == dtype else x.to(dtype)
+    if x.dtype != dtype:
+        x = (x.clamp(max=2 ** 31 - 1) if x.dtype == torch.int64 else x).to(dtype)
     return x if x.is_contiguous() else x.contiguous()
 
 
@@ -213,7 +214,7 @@ def sample_tokens(logits, u, *, temperature=1.0, top_k=None, top_p=None, min_p=N
     of nothing else gives token -1 and logprob -inf.
 
     Each setting is a number, or a tensor of u's shape with one per row (temperature, top_p and min_p are read
-    as fp32; a temperature below 0 or NaN counts as 0).  The same u, logits and settings give the same token on
+    as fp32; a temperature below 0 or NaN counts as 0, a min_p above 1 as 1).  The same u, logits and settings give the same token on
     every run and in any batch: the sums are exact.  No gradient.
     """
     if logits.dim() < 1 or logits.shape[-1] < 1:

@@ -191,6 +191,7 @@ def test_scores_are_kept_only_where_they_are_small():
     assert size(_lib.BF16, _lib.BF16, 513, 512, 32000, 512) == 0       # over twice W
     assert size(_lib.BF16, _lib.BF16, 769, 4096, 32000, 4096) == 0     # not the one-pass forward
     assert size(_lib.F32, _lib.F32, 2000, 1024, 32000, 1024) == 2048 * 32000 * 4
+    assert size(_lib.F32, _lib.F32, 2000, 1024, 66000, 1024) == 0      # over 512 MB
     assert size(_lib.BF16, _lib.F32, 64, 1024, 32000, 1024) == 0       # W rounded on the way
     assert size(_lib.BF16, _lib.BF16, 64, 1024, 32000, 1 << 24) == 0   # rows too far apart for that forward
     assert size(_lib.F64, _lib.F64, 64, 1024, 32000, 1024) == 0
@@ -393,6 +394,49 @@ def test_another_stream():
     assert torch.equal(loss, other) and all(torch.equal(a, c) for a, c in zip(grads, more))
 
 
+def test_two_streams_at_once():
+    """Two calls in flight on two streams, of the same tensors and of others, give what each gives alone."""
+    xs = [make(300, K, 4000, 6, torch.bfloat16, seed=K) for K in (64, 1024)]
+    want = [check(*x) for x in xs]
+    streams = [torch.cuda.Stream() for _ in xs]
+    for _ in range(3):
+        got = []
+        for s in streams:
+            s.wait_stream(torch.cuda.current_stream())
+        for s, (h, W, b, t, ids) in zip(streams, xs):
+            with torch.cuda.stream(s):
+                leaves = [x.detach().requires_grad_(True) for x in (h, W, b)]
+                loss = swvr_amd.softmax_distill(leaves[0], leaves[1], t, ids, leaves[2])
+                got.append((loss.detach(), torch.autograd.grad(loss, leaves)))
+        torch.cuda.synchronize()
+        for (loss, grads), (l0, g0) in zip(got, want):
+            assert torch.equal(loss, l0) and all(torch.equal(a, c) for a, c in zip(grads, g0))
+
+
+def test_double_backward_is_refused():
+    h, W, b, t, ids = make(20, 64, 90, 4, torch.float32)
+    h.requires_grad_(True)
+    loss = swvr_amd.softmax_distill(h, W, t, ids, b)
+    (gh,) = torch.autograd.grad(loss, h, create_graph=True)
+    with pytest.raises(RuntimeError):   # there is no graph to go back through
+        gh.sum().backward()
+
+
+def test_log_normalisers_of_a_readout_without_columns():
+    """An embedding of width 0: LSE alone, as with columns, and h's and W's gradients through it."""
+    for dtype, N in ((torch.bfloat16, 40), (torch.float32, 300), (torch.bfloat16, 900)):
+        h, W, b, _, _ = make(N, 64, 700, 1, dtype)
+        E = torch.randn(700, 16, device=DEV).to(dtype)
+        h.requires_grad_(True), W.requires_grad_(True)
+        _, lse0 = swvr_amd.softmax_readout(h, W, E[:, :0], b)
+        _, lse = swvr_amd.softmax_readout(h, W, E, b)
+        S = h.double() @ W.double().t() + b.double()
+        want = torch.logsumexp(S, dim=1)
+        assert rel_err(lse0, want) < 1e-6 and rel_err(lse, want) < 1e-6
+        g0, g = (torch.autograd.grad(x.sum(), (h, W)) for x in (lse0, lse))
+        assert all(rel_err(a, c) < 1e-2 for a, c in zip(g0, g))
+
+
 def test_compiled_whole():
     h, W, b, t, ids = make(200, 64, 900, 6, torch.bfloat16)
     want, want_g = check(h, W, b, t, ids, chunk_size=8192)
@@ -403,8 +447,9 @@ def test_compiled_whole():
         assert torch.equal(got, w)
 
 
-def test_captured_and_replayed():
-    h, W, b, t, ids = make(300, 64, 900, 6, torch.bfloat16)
+@pytest.mark.parametrize("K", [64, 1024])   # scores formed again, and kept
+def test_captured_and_replayed(K):
+    h, W, b, t, ids = make(300, K, 900, 6, torch.bfloat16)
     for x in (h, W, b):
         x.requires_grad_(True)
 

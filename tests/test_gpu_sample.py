@@ -143,6 +143,10 @@ def test_settings_of_each_row():
     for dtype in (torch.int32, torch.int16):
         token, _ = swvr_amd.sample_tokens(x, u, **{**kw, "top_k": kw["top_k"].clamp(-2, 5000).to(dtype)})
         assert torch.equal(token, want)
+    huge = torch.where(kw["top_k"] == 10 ** 6, 2 ** 32 + 1, kw["top_k"])   # 1, if it were cut to 32 bits
+    assert torch.equal(swvr_amd.sample_tokens(x, u, **{**kw, "top_k": huge})[0], want)
+    over = swvr_amd.sample_tokens(x, u, min_p=torch.full_like(u, 7.0))[0]
+    assert torch.equal(over, x.argmax(dim=1))
     # a row alone gives what it gives in the batch, whatever the layout
     for i in range(0, R, 5):
         one, _ = swvr_amd.sample_tokens(x[i], u[i], **{k: v[i] for k, v in kw.items()})
