@@ -799,6 +799,268 @@ __device__ __forceinline__ int distance_bin(uint32_t d) {
   return x < kBins ? (int)x : kBins - 1;
 }
 
+// LDS of a row's last workgroup.
+struct FinishShared {
+  u64 *list, *w, *sub, *sum, *out;  // [kList], [kList], [kSubsMost], [kRowWaves], [4]
+  int *n, *m;
+};
+
+// The token of row r from its list of n tokens (in LDS, after a barrier): with kTopKRow all that it keeps are in there,
+// with kTopPRow those of the bin in which its prefix ends, with kSumRow none; sub: the sums of sub-blocks
+// 2 threadIdx.x and the next (not with kTopKRow), crossing: as in Staged.
+template <class T>
+__device__ __forceinline__ void draw_row(const SampleParams& a, int64_t r, const RowSettings& s, const RowView<T>& v,
+                                         const Weigh& wt, RowKind kind, int n, int n_sub, u64 (&sub)[2],
+                                         const u64 (&crossing)[kCross], const FinishShared& sh) {
+  u64 *const s_list = sh.list, *const s_w = sh.w, *const s_sub = sh.sub, *const s_sum = sh.sum, *const s_out = sh.out;
+  int *const s_n = sh.n, *const s_m = sh.m;
+  constexpr int kPer = kList / kRowThreads;  // list entries of a thread
+  const int t0 = threadIdx.x * kPer, j0 = 2 * threadIdx.x;
+  auto draw = [&](u64 place, u64 total) {  // by one thread
+    const uint32_t key = key_at(place);
+    const double rel = key == wt.key_m ? 0.0 : ((double)logit_of(key) - wt.m) / s.tau;
+    a.token[r] = index_at(place);
+    a.logprob[r] = (float)(rel - log((double)total / a.one));
+  };
+  auto target_of = [&](u64 total) {
+    const double uz = s.u * (double)total;
+    return uz < (double)(total - 1) ? (u64)uz : total - 1;
+  };
+  if (kind == kTopKRow && n <= kFew) {
+    // few tokens, by one wave without barriers: each against all, for its place in the order and the weight before
+    // it, then for the kept weight before it by index
+    if (wave_id() != 0) return;
+    const int lane = lane_id();
+    u64 place[2], w[2], at[2] = {0, 0};
+    double rel[2];
+    int rank[2] = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      place[i] = lane + 64 * i < n ? s_list[lane + 64 * i] : 0;
+      rel[i] = place[i] != 0 ? wt.rel(key_at(place[i])) : 0;
+      s_w[lane + 64 * i] = w[i] = wt.fix(rel[i]);
+    }
+    if (lane < 4) s_list[n + lane] = s_w[kFew + lane] = 0;  // to a multiple of 4
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    for (int j = 0; j < n; j += 4)
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const u64 y = s_list[j + u], wy = s_w[j + u];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          rank[i] += y > place[i];
+          at[i] += y > place[i] ? wy : 0;
+        }
+      }
+    u64 z = 0, total = 0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) z += place[i] != 0 && rank[i] < s.k ? w[i] : 0;
+    z = wave_sum64(z);
+    const double pz = s.p < 1 ? s.p * (double)z : kPosInf, limit = pz > 0 ? pz : 0.5;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const bool keep = place[i] != 0 && rank[i] < s.k && (double)at[i] < limit && rel[i] >= s.min_p;
+      w[i] = keep ? w[i] : 0;
+      s_w[lane + 64 * i] = w[i];
+      total += w[i];
+      at[i] = 0;
+    }
+    total = wave_sum64(total);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    for (int j = 0; j < n; j += 4)
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const u64 y = s_list[j + u], wy = s_w[j + u];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) at[i] += (uint32_t)y > (uint32_t)place[i] ? wy : 0;
+      }
+    const u64 target = target_of(total);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (at[i] <= target && at[i] + w[i] > target) draw(place[i], total);
+    return;
+  }
+  u64 cut = 0;  // the last token of the prefix (0: every token)
+  for (int i = threadIdx.x; i < n_sub; i += kRowThreads) s_sub[i] = 0;
+  if (n > 0) {
+    // The cut: counts and weights of the list's tokens per bin of their distance below the largest key; with top-k the
+    // bin in which the k-th lies (where the list has more), and in it the cut and the weight up to it; then the bin in
+    // which the weight passes the limit of top-p.  A bin holds few tokens, each compared with all; one that holds over kFew (equal
+    // logits) has the whole list sorted instead.
+    const u64 before_list = kind == kTopPRow ? crossing[1] : 0;
+    u64* const bin_w = s_w;                                                     // [kBins]
+    uint32_t* const bin_n = reinterpret_cast<uint32_t*>(s_w + kBins);           // [kBins]
+    u64* const few = s_w + kBins + kBins / 2;                                   // [kFew] places, then weights
+    if (threadIdx.x == 0) *s_n = *s_m = 0;
+    for (int i = threadIdx.x; i < kBins + kBins / 2; i += kRowThreads) s_w[i] = 0;
+    __syncthreads();
+    u64 place[kPer], w[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int at = threadIdx.x + i * kRowThreads;
+      place[i] = at < n ? s_list[at] : 0;
+      const double rel = place[i] != 0 ? wt.rel(key_at(place[i])) : 0;
+      w[i] = wt.fix(rel);
+      if (place[i] != 0) {
+        const int bin = distance_bin(wt.key_m - key_at(place[i]));
+        atomicAdd(&bin_n[bin], 1u);
+        if (w[i]) atomicAdd(&bin_w[bin], w[i]);
+      }
+      if (!(rel >= s.min_p)) w[i] = 0;  // from here on: the weight it is drawn with
+    }
+    __syncthreads();
+    const u64 w0 = bin_w[j0], w1 = bin_w[j0 + 1];
+    const uint32_t n0 = bin_n[j0], n1 = bin_n[j0 + 1];
+    u64 all_w, all_n;
+    const u64 at_w = before_list + block_before64<kRowWaves>(w0 + w1, s_sum, &all_w);
+    const u64 at_n = block_before64<kRowWaves>(n0 + n1, s_sum, &all_n);
+    const u64 k = kind == kTopKRow && (u64)s.k < all_n ? (u64)s.k : all_n;
+    double limit = kPosInf;
+    if (kind == kTopPRow) limit = s.p * (double)crossing[2] > 0 ? s.p * (double)crossing[2] : 0.5;
+    // the tokens of a bin whose count or weight passes a limit, resolved by the first wave: s_out = the last token of
+    // the prefix and the weight up to it; false: too many
+    auto resolve = [&](bool mine0, bool mine1) -> bool {
+      if (mine0 || mine1) {
+        s_out[0] = mine0 ? j0 : j0 + 1;
+        s_out[1] = mine0 ? at_w : at_w + w0;
+        s_out[2] = mine0 ? at_n : at_n + n0;
+      }
+      __syncthreads();
+      const int bin = (int)s_out[0];
+      const u64 b_w = s_out[1], b_n = s_out[2];
+      const int m = (int)bin_n[bin];
+      if (m > kFew) return false;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i)
+        if (place[i] != 0 && distance_bin(wt.key_m - key_at(place[i])) == bin) few[atomicAdd(s_m, 1)] = place[i];
+      __syncthreads();
+      if (wave_id() == 0) {
+        const int lane = lane_id();
+        u64 x[2], y[2], at[2] = {b_w, b_w};
+        u64 rank[2] = {b_n, b_n};
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          x[i] = lane + 64 * i < m ? few[lane + 64 * i] : 0;
+          y[i] = x[i] != 0 ? wt.fix(wt.rel(key_at(x[i]))) : 0;
+          few[kFew + lane + 64 * i] = y[i];
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll 4
+        for (int j = 0; j < m; ++j) {
+          const u64 z = few[j], wz = few[kFew + j];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            rank[i] += z > x[i];
+            at[i] += z > x[i] ? wz : 0;
+          }
+        }
+        u64 last = ~0ull, sum = 0;  // the smallest place of the prefix
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const bool in = x[i] != 0 && rank[i] < k && (double)at[i] < limit;
+          last = in && x[i] < last ? x[i] : last;
+          sum += in ? y[i] : 0;
+        }
+        last = ~wave_max64(~last);
+        sum = wave_sum64(sum);
+        if (lane == 0) {
+          s_out[0] = last;
+          s_out[1] = b_w + sum;
+          *s_m = 0;
+        }
+      }
+      __syncthreads();
+      cut = s_out[0];
+      return true;
+    };
+    bool done = true;
+    if (kind == kTopKRow) {
+      u64 kept = all_w;
+      if (k < all_n) {
+        const bool in0 = at_n < k && at_n + n0 >= k, in1 = at_n + n0 < k && at_n + n0 + n1 >= k;
+        done = resolve(in0, in1);
+        kept = s_out[1];
+      }
+      if (done && s.p < 1) {
+        const double pz = s.p * (double)kept;
+        limit = pz > 0 ? pz : 0.5;
+        __syncthreads();
+        // the last bin that begins below the limit, of those up to the k-th's
+        const bool b0 = n0 > 0 && at_n < k && (double)at_w < limit;
+        const bool b1 = n1 > 0 && at_n + n0 < k && (double)(at_w + w0) < limit;
+        const bool e0 = b0 && ((double)(at_w + w0) >= limit || at_n + n0 >= k);
+        const bool e1 = b1 && ((double)(at_w + w0 + w1) >= limit || at_n + n0 + n1 >= k);
+        done = resolve(e0, e1 && !e0);
+      }
+    } else {
+      const bool b0 = (double)at_w < limit && (double)(at_w + w0) >= limit;
+      const bool b1 = (double)(at_w + w0) < limit && (double)(at_w + w0 + w1) >= limit;
+      done = resolve(b0, b1);
+    }
+    if (!done) {
+      __syncthreads();
+      const int n2 = pow2_at_least(n);
+      for (int i = n + threadIdx.x; i < n2; i += kRowThreads) s_list[i] = 0;
+      sort_descending(s_list, n2);
+      u64 sum = 0, x[kPer], all;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        const bool in = t0 + i < n && (u64)(t0 + i) < k;
+        sum += x[i] = in ? wt.fix(wt.rel(key_at(s_list[t0 + i]))) : 0;
+      }
+      u64 at = before_list + block_before64<kRowWaves>(sum, s_sum, &all);
+      if (kind == kTopKRow && s.p < 1) limit = s.p * (double)all > 0 ? s.p * (double)all : 0.5;
+      u64 prefix = 0;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        prefix += t0 + i < n && (u64)(t0 + i) < k && (double)at < limit;
+        at += x[i];
+      }
+      prefix = block_sum64<kRowWaves>(prefix, s_sum);
+      cut = s_list[prefix - 1];
+    }
+    // the prefix's tokens join the sub-blocks' sums (with top-k they are all there is)
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      if (place[i] >= cut && w[i]) atomicAdd(&s_sub[(index_at(place[i]) + v.lead) / kSub], w[i]);
+  }
+  // the sub-block that holds the token, then its place there
+  __syncthreads();
+  u64 total;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    if (kind == kTopKRow) sub[i] = 0;
+    if (j0 + i < n_sub) sub[i] += s_sub[j0 + i];
+  }
+  u64 at = block_before64<kRowWaves>(sub[0] + sub[1], s_sum, &total);
+  const u64 target = target_of(total);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    if (at <= target && at + sub[i] > target) {
+      s_out[0] = j0 + i;
+      s_out[1] = at;
+    }
+    at += sub[i];
+  }
+  __syncthreads();
+  const int64_t i0 = (int64_t)s_out[0] * kSub - v.lead + 2 * threadIdx.x;
+  at = s_out[1];
+  u64 place[2], w[2], all;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    place[i] = i0 + i >= 0 && i0 + i < v.V ? place_of(key_of((float)v.row[i0 + i]), i0 + i) : 0;
+    const double rel = wt.rel(key_at(place[i]));
+    w[i] = place[i] != 0 && place[i] >= cut && rel >= s.min_p ? wt.fix(rel) : 0;
+  }
+  at += block_before64<kRowWaves>(w[0] + w[1], s_sum, &all);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    if (at <= target && at + w[i] > target) draw(place[i], total);
+    at += w[i];
+  }
+}
+
 template <class T>
 __global__ __launch_bounds__(kRowThreads) void sample_finish_kernel(Staged p) {
   __shared__ u64 s_list[kList], s_w[kList], s_sub[kSubsMost], s_sum[kRowWaves], s_out[4];
@@ -829,18 +1091,6 @@ __global__ __launch_bounds__(kRowThreads) void sample_finish_kernel(Staged p) {
   const RowKind kind = kind_of(s, a.V);
   const RowView<T> v(a, r);
   const Weigh wt = weigh_of(a, s, key_at(first), s_powers);
-  constexpr int kPer = kList / kRowThreads;  // list entries of a thread
-  const int t0 = threadIdx.x * kPer;
-  auto draw = [&](u64 place, u64 total) {  // by one thread
-    const uint32_t key = key_at(place);
-    const double rel = key == wt.key_m ? 0.0 : ((double)logit_of(key) - wt.m) / s.tau;
-    a.token[r] = index_at(place);
-    a.logprob[r] = (float)(rel - log((double)total / a.one));
-  };
-  auto target_of = [&](u64 total) {
-    const double uz = s.u * (double)total;
-    return uz < (double)(total - 1) ? (u64)uz : total - 1;
-  };
 
   int n = 0;  // list entries
   if (kind == kTopKRow) {
@@ -916,61 +1166,6 @@ __global__ __launch_bounds__(kRowThreads) void sample_finish_kernel(Staged p) {
     }
     __syncthreads();
     n = s_n;
-    if (n <= kFew) {
-      // few tokens, by one wave without barriers: each against all, for its place in the order and the weight before
-      // it, then for the kept weight before it by index
-      if (wave_id() != 0) return;
-      const int lane = lane_id();
-      u64 place[2], w[2], at[2] = {0, 0};
-      double rel[2];
-      int rank[2] = {0, 0};
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        place[i] = lane + 64 * i < n ? s_list[lane + 64 * i] : 0;
-        rel[i] = place[i] != 0 ? wt.rel(key_at(place[i])) : 0;
-        s_w[lane + 64 * i] = w[i] = wt.fix(rel[i]);
-      }
-      if (lane < 4) s_list[n + lane] = s_w[kFew + lane] = 0;  // to a multiple of 4
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      for (int j = 0; j < n; j += 4)
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const u64 y = s_list[j + u], wy = s_w[j + u];
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            rank[i] += y > place[i];
-            at[i] += y > place[i] ? wy : 0;
-          }
-        }
-      u64 z = 0, total = 0;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) z += place[i] != 0 && rank[i] < s.k ? w[i] : 0;
-      z = wave_sum64(z);
-      const double pz = s.p < 1 ? s.p * (double)z : kPosInf, limit = pz > 0 ? pz : 0.5;
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const bool keep = place[i] != 0 && rank[i] < s.k && (double)at[i] < limit && rel[i] >= s.min_p;
-        w[i] = keep ? w[i] : 0;
-        s_w[lane + 64 * i] = w[i];
-        total += w[i];
-        at[i] = 0;
-      }
-      total = wave_sum64(total);
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      for (int j = 0; j < n; j += 4)
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const u64 y = s_list[j + u], wy = s_w[j + u];
-#pragma unroll
-          for (int i = 0; i < 2; ++i) at[i] += (uint32_t)y > (uint32_t)place[i] ? wy : 0;
-        }
-      const u64 target = target_of(total);
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-        if (at[i] <= target && at[i] + w[i] > target) draw(place[i], total);
-      return;
-    }
   } else if (kind == kTopPRow) {
     n = n_list;
     if ((int)threadIdx.x < n) s_list[threadIdx.x] = list0;
@@ -982,180 +1177,69 @@ __global__ __launch_bounds__(kRowThreads) void sample_finish_kernel(Staged p) {
     return;
   }
 
-  u64 cut = 0;  // the last token of the prefix (0: every token)
-  for (int i = threadIdx.x; i < p.n_sub; i += kRowThreads) s_sub[i] = 0;
-  if (n > 0) {
-    // The cut: counts and weights of the list's tokens per bin of their distance below the largest key; with top-k the
-    // bin in which the k-th lies, and in it the cut and the weight up to it; then the bin in which the weight passes
-    // the limit of top-p.  A bin holds few tokens, each compared with all; one that holds over kFew (equal
-    // logits) has the whole list sorted instead.
-    const u64 before_list = kind == kTopPRow ? crossing[1] : 0;
-    u64* const bin_w = s_w;                                                     // [kBins]
-    uint32_t* const bin_n = reinterpret_cast<uint32_t*>(s_w + kBins);           // [kBins]
-    u64* const few = s_w + kBins + kBins / 2;                                   // [kFew] places, then weights
-    if (threadIdx.x == 0) s_n = s_m = 0;
-    for (int i = threadIdx.x; i < kBins + kBins / 2; i += kRowThreads) s_w[i] = 0;
-    __syncthreads();
-    u64 place[kPer], w[kPer];
+  draw_row(a, r, s, v, wt, kind, n, p.n_sub, sub, crossing, FinishShared{s_list, s_w, s_sub, s_sum, s_out, &s_n, &s_m});
+}
+
+// ---------------------------------------------------------------- a short row
+// Up to kRowMost logits, in one launch: the row, read once, is the list.  A radix descent reads it up to 8 times from
+// L1, between barriers: 64 rows of 4096 with top-k and top-p took 35 us, so 18.  Without either there is no cut to find,
+// and the two passes of sample_row over the cached row are the shorter way (10 us; by the list 43).
+template <class T>
+__global__ __launch_bounds__(kRowThreads) void sample_short_kernel(SampleParams a) {
+  __shared__ u64 s_list[kList], s_w[kList], s_sub[4], s_sum[kRowWaves], s_out[4];
+  __shared__ double s_powers[kPowers];
+  __shared__ int s_n, s_m;
+  const int64_t r = blockIdx.x;
+  const RowView<T> v(a, r);
+  const int lead = v.lead % kLoad;
+  uint32_t key[2][kLoad];  // (a row that begins between two borders takes one load more than kRowMost / kTile)
+  int64_t i0[2];
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int at = threadIdx.x + i * kRowThreads;
-      place[i] = at < n ? s_list[at] : 0;
-      const double rel = place[i] != 0 ? wt.rel(key_at(place[i])) : 0;
-      w[i] = wt.fix(rel);
-      if (place[i] != 0) {
-        const int bin = distance_bin(wt.key_m - key_at(place[i]));
-        atomicAdd(&bin_n[bin], 1u);
-        if (w[i]) atomicAdd(&bin_w[bin], w[i]);
-      }
-      if (!(rel >= s.min_p)) w[i] = 0;  // from here on: the weight it is drawn with
+  for (int j = 0; j < 2; ++j) {
+    i0[j] = ((int64_t)j * kRowThreads + threadIdx.x) * kLoad - lead;
+    if (j == 0 || i0[j] < a.V)
+      load_keys(v.row, i0[j], v.V, key[j]);
+    else
+#pragma unroll
+      for (int u = 0; u < kLoad; ++u) key[j][u] = 0;
+  }
+  const RowSettings s = settings_of(a, r);
+  fill_powers(s_powers);
+  if (threadIdx.x == 0) s_n = s_m = 0;
+  u64 first = 0;
+  int c = 0;
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+#pragma unroll
+    for (int u = 0; u < kLoad; ++u) {
+      const u64 x = place_of(key[j][u], i0[j] + u);
+      first = x > first ? x : first;
+      c += x != 0;
     }
-    __syncthreads();
-    const u64 w0 = bin_w[j0], w1 = bin_w[j0 + 1];
-    const uint32_t n0 = bin_n[j0], n1 = bin_n[j0 + 1];
-    u64 all_w, all_n;
-    const u64 at_w = before_list + block_before64<kRowWaves>(w0 + w1, s_sum, &all_w);
-    const u64 at_n = block_before64<kRowWaves>(n0 + n1, s_sum, &all_n);
-    const u64 k = kind == kTopKRow && (u64)s.k < all_n ? (u64)s.k : all_n;
-    double limit = kPosInf;
-    if (kind == kTopPRow) limit = s.p * (double)crossing[2] > 0 ? s.p * (double)crossing[2] : 0.5;
-    // the tokens of a bin whose count or weight passes a limit, resolved by the first wave: s_out = the last token of
-    // the prefix and the weight up to it; false: too many
-    auto resolve = [&](bool mine0, bool mine1) -> bool {
-      if (mine0 || mine1) {
-        s_out[0] = mine0 ? j0 : j0 + 1;
-        s_out[1] = mine0 ? at_w : at_w + w0;
-        s_out[2] = mine0 ? at_n : at_n + n0;
-      }
-      __syncthreads();
-      const int bin = (int)s_out[0];
-      const u64 b_w = s_out[1], b_n = s_out[2];
-      const int m = (int)bin_n[bin];
-      if (m > kFew) return false;
-#pragma unroll
-      for (int i = 0; i < kPer; ++i)
-        if (place[i] != 0 && distance_bin(wt.key_m - key_at(place[i])) == bin) few[atomicAdd(&s_m, 1)] = place[i];
-      __syncthreads();
-      if (wave_id() == 0) {
-        const int lane = lane_id();
-        u64 x[2], y[2], at[2] = {b_w, b_w};
-        u64 rank[2] = {b_n, b_n};
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          x[i] = lane + 64 * i < m ? few[lane + 64 * i] : 0;
-          y[i] = x[i] != 0 ? wt.fix(wt.rel(key_at(x[i]))) : 0;
-          few[kFew + lane + 64 * i] = y[i];
-        }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  first = wave_max64(first);
+  if (lane_id() == 0) s_sum[wave_id()] = first;
+  __syncthreads();
 #pragma unroll 4
-        for (int j = 0; j < m; ++j) {
-          const u64 z = few[j], wz = few[kFew + j];
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            rank[i] += z > x[i];
-            at[i] += z > x[i] ? wz : 0;
-          }
-        }
-        u64 last = ~0ull, sum = 0;  // the smallest place of the prefix
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const bool in = x[i] != 0 && rank[i] < k && (double)at[i] < limit;
-          last = in && x[i] < last ? x[i] : last;
-          sum += in ? y[i] : 0;
-        }
-        last = ~wave_max64(~last);
-        sum = wave_sum64(sum);
-        if (lane == 0) {
-          s_out[0] = last;
-          s_out[1] = b_w + sum;
-          s_m = 0;
-        }
-      }
-      __syncthreads();
-      cut = s_out[0];
-      return true;
-    };
-    bool done = true;
-    if (kind == kTopKRow) {
-      const bool in0 = at_n < k && at_n + n0 >= k, in1 = at_n + n0 < k && at_n + n0 + n1 >= k;
-      done = resolve(in0, in1);
-      if (done && s.p < 1) {
-        const double pz = s.p * (double)s_out[1];
-        limit = pz > 0 ? pz : 0.5;
-        __syncthreads();
-        // the last bin that begins below the limit, of those up to the k-th's
-        const bool b0 = n0 > 0 && at_n < k && (double)at_w < limit;
-        const bool b1 = n1 > 0 && at_n + n0 < k && (double)(at_w + w0) < limit;
-        const bool e0 = b0 && ((double)(at_w + w0) >= limit || at_n + n0 >= k);
-        const bool e1 = b1 && ((double)(at_w + w0 + w1) >= limit || at_n + n0 + n1 >= k);
-        done = resolve(e0, e1 && !e0);
-      }
-    } else {
-      const bool b0 = (double)at_w < limit && (double)(at_w + w0) >= limit;
-      const bool b1 = (double)(at_w + w0) < limit && (double)(at_w + w0 + w1) >= limit;
-      done = resolve(b0, b1);
-    }
-    if (!done) {
-      __syncthreads();
-      const int n2 = pow2_at_least(n);
-      for (int i = n + threadIdx.x; i < n2; i += kRowThreads) s_list[i] = 0;
-      sort_descending(s_list, n2);
-      u64 sum = 0, x[kPer], all;
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        const bool in = t0 + i < n && (u64)(t0 + i) < k;
-        sum += x[i] = in ? wt.fix(wt.rel(key_at(s_list[t0 + i]))) : 0;
-      }
-      u64 at = before_list + block_before64<kRowWaves>(sum, s_sum, &all);
-      if (kind == kTopKRow && s.p < 1) limit = s.p * (double)all > 0 ? s.p * (double)all : 0.5;
-      u64 prefix = 0;
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        prefix += t0 + i < n && (u64)(t0 + i) < k && (double)at < limit;
-        at += x[i];
-      }
-      prefix = block_sum64<kRowWaves>(prefix, s_sum);
-      cut = s_list[prefix - 1];
-    }
-    // the prefix's tokens join the sub-blocks' sums (with top-k they are all there is)
-#pragma unroll
-    for (int i = 0; i < kPer; ++i)
-      if (place[i] >= cut && w[i]) atomicAdd(&s_sub[(index_at(place[i]) + v.lead) / kSub], w[i]);
+  for (int j = 0; j < kRowWaves; ++j) first = s_sum[j] > first ? s_sum[j] : first;
+  if (settled(a, r, s, first)) return;
+  const Weigh wt = weigh_of(a, s, key_at(first), s_powers);
+  if (s.k >= a.V && !(s.p < 1)) {
+    sample_row<T>(a, r, s, wt, RowShared{s_sum, s_out, s_w, reinterpret_cast<uint32_t*>(s_list)});
+    return;
   }
-  // the sub-block that holds the token, then its place there
+  int at = append(&s_n, c);
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+#pragma unroll
+    for (int u = 0; u < kLoad; ++u)
+      if (key[j][u] != 0) s_list[at++] = place_of(key[j][u], i0[j] + u);
   __syncthreads();
-  u64 total;
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    if (kind == kTopKRow) sub[i] = 0;
-    if (j0 + i < p.n_sub) sub[i] += s_sub[j0 + i];
-  }
-  u64 at = block_before64<kRowWaves>(sub[0] + sub[1], s_sum, &total);
-  const u64 target = target_of(total);
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    if (at <= target && at + sub[i] > target) {
-      s_out[0] = j0 + i;
-      s_out[1] = at;
-    }
-    at += sub[i];
-  }
+  const int n = s_n;
   __syncthreads();
-  const int64_t i0 = (int64_t)s_out[0] * kSub - v.lead + 2 * threadIdx.x;
-  at = s_out[1];
-  u64 place[2], w[2], all;
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    place[i] = i0 + i >= 0 && i0 + i < v.V ? place_of(key_of((float)v.row[i0 + i]), i0 + i) : 0;
-    const double rel = wt.rel(key_at(place[i]));
-    w[i] = place[i] != 0 && place[i] >= cut && rel >= s.min_p ? wt.fix(rel) : 0;
-  }
-  at += block_before64<kRowWaves>(w[0] + w[1], s_sum, &all);
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    if (at <= target && at + w[i] > target) draw(place[i], total);
-    at += w[i];
-  }
+  u64 sub[2] = {0, 0};
+  const u64 crossing[kCross] = {0, 0, 0};
+  draw_row(a, r, s, v, wt, kTopKRow, n, (int)((v.V + v.lead + kSub - 1) / kSub), sub, crossing,
+           FinishShared{s_list, s_w, s_sub, s_sum, s_out, &s_n, &s_m});
 }
 
 // Rows of one launch: their workspace (up to 85 KB each) stays under 180 MB.
@@ -1214,6 +1298,16 @@ hipError_t run_staged(const SampleParams& a, char* ws, hipStream_t stream) {
   return hipSuccess;
 }
 
+template <class T>
+hipError_t run(const SampleParams& a, char* ws, hipStream_t stream) {
+  if (is_staged(a.V)) return run_staged<T>(a, ws, stream);
+  if (a.V <= kRowMost)
+    sample_short_kernel<T><<<(unsigned)a.R, kRowThreads, 0, stream>>>(a);
+  else
+    sample_row_kernel<T><<<(unsigned)a.R, kRowThreads, 0, stream>>>(a);
+  return hipGetLastError();
+}
+
 }  // namespace
 
 size_t sample_workspace_bytes(int64_t R, int64_t V) { return is_staged(V) ? staged_sizes(R, V).all() : 0; }
@@ -1223,26 +1317,16 @@ hipError_t sample_launch(int dtype, SampleParams p, char* ws, hipStream_t stream
   int bits = 0;
   while (bits < 31 && ((int64_t)1 << bits) < p.V) ++bits;
   p.one = (double)((int64_t)1 << (bits < 12 ? 50 : 62 - bits));
-  const bool staged = is_staged(p.V);
   hipError_t e = hipSuccess;
   timing_begin(kKindSample, stream);
   switch (dtype) {
-    case kBF16:
-      if (staged) e = run_staged<bf16_t>(p, ws, stream);
-      else sample_row_kernel<bf16_t><<<(unsigned)p.R, kRowThreads, 0, stream>>>(p);
-      break;
-    case kF16:
-      if (staged) e = run_staged<f16_t>(p, ws, stream);
-      else sample_row_kernel<f16_t><<<(unsigned)p.R, kRowThreads, 0, stream>>>(p);
-      break;
-    case kF32:
-      if (staged) e = run_staged<float>(p, ws, stream);
-      else sample_row_kernel<float><<<(unsigned)p.R, kRowThreads, 0, stream>>>(p);
-      break;
+    case kBF16: e = run<bf16_t>(p, ws, stream); break;
+    case kF16: e = run<f16_t>(p, ws, stream); break;
+    case kF32: e = run<float>(p, ws, stream); break;
     default: return hipErrorInvalidValue;
   }
   timing_end(kKindSample, stream);
-  return e != hipSuccess ? e : hipGetLastError();
+  return e;
 }
 
 }  // namespace swvr

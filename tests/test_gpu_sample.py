@@ -98,6 +98,18 @@ def test_ties_at_every_cut(kw):
     check(x.bfloat16() * -1000, torch.rand(6, device=DEV, generator=gen(8)), **kw)
 
 
+@pytest.mark.parametrize("kw", [dict(), dict(top_k=50), dict(top_k=50, top_p=0.9), dict(top_k=150, top_p=0.9), dict(top_p=0.6),
+                                dict(top_k=4000, top_p=0.99, min_p=0.2), dict(top_p=0.95, min_p=0.3)], ids=str)
+@pytest.mark.parametrize("spread", [0.0, 0.01, 1.0, 60.0])
+@pytest.mark.parametrize("V,off", [(257, 0), (2049, 1), (4095, 2), (4096, 3), (4096, 7)])
+def test_short_rows_flat_to_peaked(kw, spread, V, off):
+    """Rows that fit one workgroup's list, up to a full one, beginning anywhere between two borders of loads."""
+    g = gen(V + off)
+    x = (spread * torch.randn(4, V + 9, device=DEV, generator=g)).bfloat16()
+    x[1] = x[1].sign()
+    check(x[:, off:off + V], torch.rand(4, device=DEV, generator=g), **kw)
+
+
 @pytest.mark.parametrize("kw", [dict(), dict(top_k=4), dict(top_p=0.8), dict(min_p=0.3), dict(temperature=0.0)], ids=str)
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 @pytest.mark.parametrize("V", [3001, 20011])   # a row in one launch, and in several
