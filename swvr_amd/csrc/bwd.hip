@@ -294,37 +294,71 @@ __device__ __forceinline__ void store_ds_block(const f32x16_t& ds, void* stage, 
 }
 
 // dS of a chunk from the scores that the forward kept (D = 0: dS = P gLSE), and its column sums: a workgroup per 32
-// vocabulary rows, 8 threads per row, 4 consecutive tokens each, which are 4 consecutive positions of the stage.  Writes
-// the position blocks that hold active tokens, as the gradient GEMMs read them (rows past the chunk's as zeros).
-template <class T>
-__global__ __launch_bounds__(256) void bwd_kept_scores_kernel(const float* __restrict__ S, int64_t lds,
+// vocabulary rows, 8 threads per row and part, 4 consecutive tokens each, which are 4 consecutive positions of the
+// stage.  Writes the position blocks that hold active tokens, as the gradient GEMMs read them (rows past the chunk's as
+// zeros).  Bound by memory: each score is read and its dS written once.  Active tokens lie scattered, so a score's
+// address waits for a load: U blocks' indices and then their scores go out before the first is used, and the P parts of
+// a workgroup take groups of U blocks in turn.  (U = 4, P = 2 for 1 and 1: 500 tokens of 32000 rows in bf16 39 -> 25 us,
+// 3.9 TB/s; 2000 in fp32 299 -> 138.  One block of tokens keeps 1 and 1.)
+template <class T, int U, int P>
+__global__ __launch_bounds__(256 * P) void bwd_kept_scores_kernel(const float* __restrict__ S, int64_t lds,
                                                               const int* __restrict__ idx,
                                                               const int* __restrict__ n_act,
                                                               const float* __restrict__ lsed, int N_pad, int v0, int cv,
                                                               int n_tb32, T* __restrict__ stage,
                                                               float* __restrict__ gb) {
-  const int v = blockIdx.x * 32 + threadIdx.x / 8, j = threadIdx.x % 8, na = n_act[0];
+  __shared__ float s_db[32];
+  const int part = threadIdx.x / 256, t = threadIdx.x % 256;
+  const int v = blockIdx.x * 32 + t / 8, j = t % 8, na = n_act[0];
   const int tok0 = 8 * (j & 3) + 4 * (j >> 2);  // stage_tok(4 j)
   const bool in = v < cv;
   const float* const row = S + (int64_t)(in ? v0 + v : 0) * lds;
   float db = 0.f;
-  for (int q0 = tok0; q0 - tok0 < na; q0 += 32) {
-    T ds[4];
+  for (int b0 = part * U; b0 * 32 < na; b0 += P * U) {
+    int4 at[U];
+    float4 lse[U], g[U];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int q = q0 + i;
-      const float x = in && q < na ? fast_exp(row[idx[q]] - lsed[q]) * -lsed[N_pad + q] : 0.f;
-      db += x;
-      ds[i] = from_float<T>(x);
+    for (int u = 0; u < U; ++u) {
+      // (N_pad is a multiple of 32; blocks past it read the last one's, and are left out below)
+      const int q = min((b0 + u) * 32, N_pad - 32) + tok0;
+      at[u] = *reinterpret_cast<const int4*>(idx + q);
+      lse[u] = *reinterpret_cast<const float4*>(lsed + q);
+      g[u] = *reinterpret_cast<const float4*>(lsed + N_pad + q);
     }
-    struct alignas(4 * sizeof(T)) X {
-      T v[4];
-    } y = {{ds[0], ds[1], ds[2], ds[3]}};
-    if (stage) *reinterpret_cast<X*>(stage + stage_off(v, (q0 & ~31) + 4 * j, n_tb32)) = y;
+    float x[U][4];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int q = (b0 + u) * 32 + tok0;
+      x[u][0] = row[q + 0 < na ? at[u].x : 0];
+      x[u][1] = row[q + 1 < na ? at[u].y : 0];
+      x[u][2] = row[q + 2 < na ? at[u].z : 0];
+      x[u][3] = row[q + 3 < na ? at[u].w : 0];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int q = (b0 + u) * 32 + tok0;
+      const float l[4] = {lse[u].x, lse[u].y, lse[u].z, lse[u].w}, c[4] = {g[u].x, g[u].y, g[u].z, g[u].w};
+      struct alignas(4 * sizeof(T)) X {
+        T v[4];
+      } y;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float ds = in && q + i < na ? fast_exp(x[u][i] - l[i]) * -c[i] : 0.f;
+        db += ds;
+        y.v[i] = from_float<T>(ds);
+      }
+      if (stage && (b0 + u) * 32 < na) *reinterpret_cast<X*>(stage + stage_off(v, (b0 + u) * 32 + 4 * j, n_tb32)) = y;
+    }
   }
+  if (!gb) return;
 #pragma unroll
   for (int o = 1; o < 8; o <<= 1) db += __shfl_xor(db, o);
-  if (gb && in && j == 0) gb[v0 + v] = db;
+  if constexpr (P == 2) {
+    if (part == 1 && j == 0) s_db[t / 8] = db;
+    __syncthreads();
+    db += s_db[t / 8];
+  }
+  if (part == 0 && in && j == 0) gb[v0 + v] = db;
 }
 
 // The caller's elements of dS over the staged ones of a chunk: one thread per entry, those of other chunks and of
@@ -1850,7 +1884,8 @@ hipError_t bwd_run(const BwdPlan& plan, const BwdParams& p, hipStream_t stream) 
     sp.DP = plan.DP;
     if (kept) {
       timing_begin(kKindBwdScores, stream);
-      bwd_kept_scores_kernel<T><<<(unsigned)(Cc / 32), 256, 0, stream>>>(
+      auto kernel = p.N <= 32 ? bwd_kept_scores_kernel<T, 1, 1> : bwd_kept_scores_kernel<T, 4, 2>;
+      kernel<<<(unsigned)(Cc / 32), p.N <= 32 ? 256 : 512, 0, stream>>>(
           p.scores, p.lds, idx, n_act, lsed, (int)plan.N_pad, v0, cv, sp.n_tb32, need_stage ? stage : nullptr, p.gb);
       timing_end(kKindBwdScores, stream);
       if ((e = hipGetLastError()) != hipSuccess) return e;
