@@ -1418,7 +1418,7 @@ struct PosRLoader {
 };
 
 // Single-tile pipelined reduction: acc += A[.., 0:k_total] B[.., 0:k_total]^T.
-template <class T, int BK, int FM, int FN, class TA, class TB>
+template <class T, int BK, int NS, int FM, int FN, class TA, class TB>
 __device__ __forceinline__ void gemm_loop(f32x16_t (&acc)[FM][FN], const TA& ta, const TB& tb, char* smem,
                                           int k_total, int a_row0, int b_row0) {
   constexpr int SB = TA::BYTES + TB::BYTES;
@@ -1432,13 +1432,13 @@ __device__ __forceinline__ void gemm_loop(f32x16_t (&acc)[FM][FN], const TA& ta,
     ta.issue(st, is_k * BK);
     tb.issue(st + TA::BYTES, is_k * BK);
     ++is_k;
-    is_slot = is_slot == kStages - 1 ? 0 : is_slot + 1;
+    is_slot = is_slot == NS - 1 ? 0 : is_slot + 1;
   };
 #pragma unroll
-  for (int s = 0; s < kStages - 1; ++s) issue_next();
+  for (int s = 0; s < NS - 1; ++s) issue_next();
   if (nk == 0) return;
-  Ring<kStages> ring{kStages - 1, nk};
-  ring.publish_next<L>();
+  Ring<NS> ring{NS - 1, nk};
+  ring.template publish_next<L>();
   tile_reduce<T, BK, L>(acc, ta, tb, smem, SB, ring, nk, a_row0, b_row0, issue_next);
 }
 
@@ -1453,9 +1453,13 @@ struct GemmTile {
   static constexpr int WM = 2;
   static constexpr int WN = wide ? 4 : 2;
   static constexpr int NT = 64 * WM * WN;
+  // The ring: NS stages of BK reduction elements.  fp32's matrix work takes 16 times as long, so one stage ahead is
+  // enough, and twice the elements per barrier leave the matrix cores busy 88% of the time for 80 with 4 stages of 16
+  // (2000 tokens, K = 1024, V = 32000: dW and dh 2.15 -> 2.02 ms, 130 TF/s).
+  static constexpr int BK = 32, NS = wide ? kStages : 2;
   // LDS: the operand ring, then (reused) the row-major epilogue staging of
   // half a tile in fp32 (rows padded by 8 floats: conflict-free writes)
-  static constexpr int RING_BYTES = kStages * 2 * GM * SliceK<T>::value * (int)sizeof(T);
+  static constexpr int RING_BYTES = NS * 2 * GM * BK * (int)sizeof(T);
   static constexpr int EPI_BYTES = GM / WM * (GN + 8) * 4;
   static constexpr int LDS_BYTES = RING_BYTES > EPI_BYTES ? RING_BYTES : EPI_BYTES;
 };
@@ -1468,7 +1472,7 @@ struct GemmTile {
 template <class T, bool DW>
 __device__ __forceinline__ void gemm_tile(const GemmParams& p, int t, char* smem, int run = 0) {
   typedef GemmTile<T> G;
-  constexpr int kBK = SliceK<T>::value;
+  constexpr int kBK = G::BK;
   constexpr int GM = G::GM, GN = G::GN, NT = G::NT;
   constexpr int FM = GM / (32 * G::WM), FN = GN / (32 * G::WN);
   const int w = wave_id();
@@ -1486,7 +1490,7 @@ __device__ __forceinline__ void gemm_tile(const GemmParams& p, int t, char* smem
     tb.setup(static_cast<const T*>(p.h) + nt * GN, p.ldh, p.K - nt * GN, p.N);
     // whole 32-position blocks of the active positions (padding positions
     // hold dS = 0 and zero rows of h)
-    gemm_loop<T, kBK, FM, FN>(acc, ta, tb, smem, (min(p.N, p.n_act[0]) + 31) & ~31, wm * (GM / G::WM),
+    gemm_loop<T, kBK, G::NS, FM, FN>(acc, ta, tb, smem, (min(p.N, p.n_act[0]) + 31) & ~31, wm * (GM / G::WM),
                               wn * (GN / G::WN));
   } else {
     const int k0 = min(p.cv, run * p.dh_rows), kn = min(p.cv - k0, p.dh_rows);
@@ -1497,7 +1501,7 @@ __device__ __forceinline__ void gemm_tile(const GemmParams& p, int t, char* smem
     RTile<T, GN, kBK, NT> tb;
     tb.setup(static_cast<const T*>(p.W) + (int64_t)(p.v0 - p.w_row0 + k0) * p.ldw + nt * GN, p.ldw, p.K - nt * GN,
              kn);
-    gemm_loop<T, kBK, FM, FN>(acc, ta, tb, smem, kn, wm * (GM / G::WM), wn * (GN / G::WN));
+    gemm_loop<T, kBK, G::NS, FM, FN>(acc, ta, tb, smem, kn, wm * (GM / G::WM), wn * (GN / G::WN));
   }
   const int rows = DW ? p.cv : p.N;
   const int row0 = mt * GM, col0 = nt * GN;
@@ -1527,7 +1531,7 @@ __device__ __forceinline__ void gemm_tile(const GemmParams& p, int t, char* smem
 template <class T>
 __device__ __forceinline__ void gemm_tile_de(const GemmParams& p, int t, char* smem) {
   typedef GemmTile<T> G;
-  constexpr int kBK = SliceK<T>::value;
+  constexpr int kBK = G::BK;
   constexpr int GM = G::GM, GN = G::GN, NT = G::NT;
   constexpr int FM = GM / (32 * G::WM), FN = GN / (32 * G::WN);
   const int w = wave_id();
@@ -1548,7 +1552,7 @@ __device__ __forceinline__ void gemm_tile_de(const GemmParams& p, int t, char* s
   StageKLoader<T, GN, kBK, NT> tb;
   tb.setup(p.pstage, nt * GN, p.cv - nt * GN, p.n_tb32);
   tb.base += (int64_t)(k0 >> 5) * 1024 * (int)sizeof(T);  // the run's first 32-position block
-  gemm_loop<T, kBK, FM, FN>(acc, ta, tb, smem, k1 - k0, wm * (GM / G::WM), wn * (GN / G::WN));
+  gemm_loop<T, kBK, G::NS, FM, FN>(acc, ta, tb, smem, k1 - k0, wm * (GM / G::WM), wn * (GN / G::WN));
   gemm_store<G>(acc, 1.f, p.part_dE + (int64_t)run * p.DP * p.C, nullptr, 0, p.DP, mt * GM, nt * GN, p.C, smem);
 }
 
@@ -1584,11 +1588,11 @@ __device__ __forceinline__ void gemm_pack_w(const GemmParams& p, int w, char* sm
 template <class T>
 __global__ __launch_bounds__(GemmTile<T>::NT) void bwd_gemm_kernel(GemmParams p) {
   typedef GemmTile<T> G;
-  constexpr int kBK = SliceK<T>::value;
+  constexpr int kBK = G::BK;
   constexpr int SB = KTile<T, G::GM, kBK, G::NT>::BYTES + RTile<T, G::GN, kBK, G::NT>::BYTES;
   static_assert(KTile<T, G::GM, kBK, G::NT>::BYTES == RTile<T, G::GM, kBK, G::NT>::BYTES,
                 "both A layouts stage the same bytes");
-  static_assert(kStages * SB <= G::LDS_BYTES, "ring fits");
+  static_assert(G::NS * SB <= G::LDS_BYTES, "ring fits");
   __shared__ __attribute__((aligned(1024))) char smem[G::LDS_BYTES];
   int b = blockIdx.x;
   {
