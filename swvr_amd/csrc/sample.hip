@@ -192,7 +192,9 @@ __device__ __forceinline__ RowSettings settings_of(const SampleParams& a, int64_
 // ---------------------------------------------------------------- a row by one workgroup
 // Passes over the row: the maximum; for top-k and top-p each, the cut by radix descent over the 32 key bits (11, 11
 // and 10 bits: a histogram of counts and weights, the bin where the count reaches k or the weight p Z_k), then the
-// place of the last kept one among equal logits; the kept sum; and the running sum up to the token.
+// place of the last kept one among equal logits; the kept sum; and the running sum up to the token.  For rows too
+// long for the launches below, for k above kTopK and for lists that overflow: up to 9 reads of the row by one CU, whose
+// latency bounds it (one row of 151936 in bf16 with top-k 5000 and top-p: WHOLE_FIG us, where top-k 50 takes ONE_FIG).
 template <class T>
 struct RowSampler {
   const T* row;
@@ -474,11 +476,13 @@ __global__ __launch_bounds__(kRowThreads) void sample_row_kernel(SampleParams a)
 //                        prefix of p Z ends; that bin's own tokens go to the row's list;
 //   sample_finish_kernel the token.  With top-k, the k-th largest of the groups' largest keys is a bound that at least
 //                        k tokens reach, and, the largest tokens lying scattered, few more: only the groups that
-//                        reach it are read again, and their tokens that do are sorted.  Without, the list is
-//                        sorted for the cut inside its bin, and the sub-block that holds the drawn token read again.
+//                        reach it are read again, and their tokens that do are the row's list.  The cut is found
+//                        in the list from counts and weights per bin (draw_row), then the sub-block that holds the
+//                        drawn token, which is read again.
 // So a row is read once with top-k, twice with min-p or nothing, three times with top-p, and its logits never sorted.
-// A list that would pass kList tokens, or kSegList from one workgroup (equal logits, a nearly flat row) leaves its row to sample_row, in the same
-// launch, as does a k above kTopK.  Every sum is one of whole numbers, so its order does not matter.
+// A list that would pass kList tokens, or kSegList from one workgroup (equal logits, a nearly flat row), leaves its
+// row to sample_row, in the same launch, as does a k above kTopK.  Every sum is one of whole numbers, so its order
+// does not matter.
 constexpr int kSub = 2048, kGroups = 4096, kList = 4096, kSegList = 2048, kTopK = 1024, kFew = 128;
 constexpr int64_t kRowMost = 4096, kStagedMost = ((int64_t)1 << 21) - 8;  // (groups of at most a wave's 512)
 constexpr int kSubsMost = (int)(((int64_t)1 << 21) / kSub);
@@ -583,6 +587,7 @@ __device__ __forceinline__ int bin_of(float l, const Weigh& w, float scale) {
   return l == w.m_f ? 0 : x < kBins - 1 ? (int)x : kBins - 1;
 }
 
+// Bound by memory: 512 rows of 151936 in bf16 (156 MB) in MAX_FIG us.
 template <class T>
 __global__ __launch_bounds__(256) void sample_max_kernel(Staged p) {
   const int64_t q = blockIdx.x / p.n_seg, r = p.r0 + q;
@@ -624,7 +629,8 @@ __global__ __launch_bounds__(256) void sample_max_kernel(Staged p) {
   if (lane_id() == 0) p.first[q * p.n_sub + b.sub] = first;
 }
 
-// (Workgroups of 16 waves add a quarter as many bins to the rows', and take longer: 47 us for 40.)
+// Bound by its arithmetic, some 25 fp64 and integer instructions a logit: HIST_FIG us for 512 rows of 151936 of which
+// half have top-p alone.  (Workgroups of 16 waves add a quarter as many bins to the rows', and take longer: 47 us for 40.)
 template <class T>
 __global__ __launch_bounds__(256) void sample_hist_kernel(Staged p) {
   __shared__ u64 s_hist[kBins];
@@ -656,6 +662,7 @@ __global__ __launch_bounds__(256) void sample_hist_kernel(Staged p) {
     if (s_hist[i]) atomicAdd(&p.hist[q * kBins + i], s_hist[i]);
 }
 
+// As the histogram, with its bins read by every workgroup (16 KB, from L2): SUMS_FIG us for those rows.
 template <class T>
 __global__ __launch_bounds__(256) void sample_sums_kernel(Staged p) {
   __shared__ u64 s_sum[4], s_cross[kCross], s_list[kSegList];
@@ -710,7 +717,7 @@ __global__ __launch_bounds__(256) void sample_sums_kernel(Staged p) {
       const double w = wt.rel(l);
       sum += bin < cross && w >= s.min_p ? wt.fix(w) : 0;
       hits |= (bin == cross && l > kNegInf) ? 1u << (j * kWaveLoad + u) : 0u;
-      // one element after another: left to it, the compiler keeps all 32 in flight, in 245 registers (60 + 20 -> 75 us)
+      // one element after another: left to it, the compiler keeps all 32 in flight, in 245 registers (75 us for 50)
       asm volatile("" : "+v"(hits), "+v"(sum));
     }
   }
@@ -1061,6 +1068,8 @@ __device__ __forceinline__ void draw_row(const SampleParams& a, int64_t r, const
   }
 }
 
+// One workgroup a row, bound by the latency of its steps, loads and barriers in turn: FIN1_FIG us for one row of 151936 with
+// top-k 50 and top-p, FIN512_FIG for 512 of mixed settings, two workgroups a CU.
 template <class T>
 __global__ __launch_bounds__(kRowThreads) void sample_finish_kernel(Staged p) {
   __shared__ u64 s_list[kList], s_w[kList], s_sub[kSubsMost], s_sum[kRowWaves], s_out[4];
@@ -1298,14 +1307,37 @@ hipError_t run_staged(const SampleParams& a, char* ws, hipStream_t stream) {
   return hipSuccess;
 }
 
+// The call without its first r0 rows.
+template <class T>
+SampleParams rows_from(SampleParams a, int64_t r0) {
+  auto from = [&](const float*& x) { x = x ? x + r0 : x; };
+  a.R -= r0;
+  a.logits = static_cast<const T*>(a.logits) + r0 * a.ld;
+  a.u = static_cast<const char*>(a.u) + r0 * (a.u64 ? 8 : 4);
+  from(a.tau_rows);
+  from(a.p_rows);
+  from(a.min_p_rows);
+  a.k_rows = a.k_rows ? a.k_rows + r0 : a.k_rows;
+  a.token += r0;
+  a.logprob += r0;
+  return a;
+}
+
 template <class T>
 hipError_t run(const SampleParams& a, char* ws, hipStream_t stream) {
   if (is_staged(a.V)) return run_staged<T>(a, ws, stream);
-  if (a.V <= kRowMost)
-    sample_short_kernel<T><<<(unsigned)a.R, kRowThreads, 0, stream>>>(a);
-  else
-    sample_row_kernel<T><<<(unsigned)a.R, kRowThreads, 0, stream>>>(a);
-  return hipGetLastError();
+  constexpr int64_t kMost = 1 << 21;  // rows: a grid has fewer than 2^32 threads
+  for (int64_t r0 = 0; r0 < a.R; r0 += kMost) {
+    const SampleParams p = rows_from<T>(a, r0);
+    const unsigned rows = (unsigned)(p.R < kMost ? p.R : kMost);
+    if (a.V <= kRowMost)
+      sample_short_kernel<T><<<rows, kRowThreads, 0, stream>>>(p);
+    else
+      sample_row_kernel<T><<<rows, kRowThreads, 0, stream>>>(p);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 }  // namespace

@@ -214,8 +214,8 @@ def sample_tokens(logits, u, *, temperature=1.0, top_k=None, top_p=None, min_p=N
     of nothing else gives token -1 and logprob -inf.
 
     Each setting is a number, or a tensor of u's shape with one per row (temperature, top_p and min_p are read
-    as fp32; a temperature below 0 or NaN counts as 0, a min_p above 1 as 1).  The same u, logits and settings give the same token on
-    every run and in any batch: the sums are exact.  No gradient.
+    as fp32; a temperature below 0 or NaN counts as 0, a min_p above 1 as 1).  The same u, logits and settings give
+    the same token on every run and in any batch: the sums are exact.  No gradient.
     """
     if logits.dim() < 1 or logits.shape[-1] < 1:
         raise ValueError(f"logits must be [..., V] with V >= 1, got {tuple(logits.shape)}")

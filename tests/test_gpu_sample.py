@@ -168,6 +168,26 @@ def test_settings_of_each_row():
     assert torch.equal(token.view(-1), want)
 
 
+@pytest.mark.parametrize("R,V", [(2 ** 21 + 7, 3), (2100, 4100)])   # more rows than one launch takes
+def test_many_rows(R, V):
+    g = gen(21)
+    x = 2 * torch.randn(R, V, device=DEV, generator=g).bfloat16()
+    u = torch.rand(R, device=DEV, generator=g)
+    kw = dict(temperature=torch.rand(R, device=DEV, generator=g), top_p=torch.rand(R, device=DEV, generator=g),
+              min_p=0.1 * torch.rand(R, device=DEV, generator=g), top_k=torch.randint(1, V, (R,), device=DEV, generator=g))
+    token, logprob = swvr_amd.sample_tokens(x, u, **kw)
+    assert int(token.min()) >= 0 and int(token.max()) < V and bool((logprob <= 0).all())
+    for rows in (slice(0, 5), slice(R // 2, R // 2 + 5), slice(R - 9, R)):
+        t, lp = check(x[rows], u[rows], **{k: v[rows] for k, v in kw.items()})
+        assert torch.equal(t, token[rows]) and torch.equal(lp, logprob[rows])
+
+
+@pytest.mark.parametrize("V", [1000, 9000])
+def test_many_draws_from_one_row(V):
+    x = torch.randn(V, device=DEV, generator=gen(22)).expand(7, V)
+    check(x, torch.rand(7, device=DEV, generator=gen(23)), top_p=0.9)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_views_off_every_alignment(dtype):
     big = (3 * torch.randn(6, 9000, device=DEV, generator=gen(12))).to(dtype)
