@@ -194,7 +194,7 @@ __device__ __forceinline__ RowSettings settings_of(const SampleParams& a, int64_
 // and 10 bits: a histogram of counts and weights, the bin where the count reaches k or the weight p Z_k), then the
 // place of the last kept one among equal logits; the kept sum; and the running sum up to the token.  For rows too
 // long for the launches below, for k above kTopK and for lists that overflow: up to 9 reads of the row by one CU, whose
-// latency bounds it (one row of 151936 in bf16 with top-k 5000 and top-p: WHOLE_FIG us, where top-k 50 takes ONE_FIG).
+// arithmetic and barriers bound it (a row of 151936 in bf16 with top-k 5000 and top-p: 420 us; top-k 50 takes 18).
 template <class T>
 struct RowSampler {
   const T* row;
@@ -587,7 +587,7 @@ __device__ __forceinline__ int bin_of(float l, const Weigh& w, float scale) {
   return l == w.m_f ? 0 : x < kBins - 1 ? (int)x : kBins - 1;
 }
 
-// Bound by memory: 512 rows of 151936 in bf16 (156 MB) in MAX_FIG us.
+// Bound by memory: 512 rows of 151936 in bf16 (156 MB) in 34 us, 4.6 TB/s.
 template <class T>
 __global__ __launch_bounds__(256) void sample_max_kernel(Staged p) {
   const int64_t q = blockIdx.x / p.n_seg, r = p.r0 + q;
@@ -629,8 +629,9 @@ __global__ __launch_bounds__(256) void sample_max_kernel(Staged p) {
   if (lane_id() == 0) p.first[q * p.n_sub + b.sub] = first;
 }
 
-// Bound by its arithmetic, some 25 fp64 and integer instructions a logit: HIST_FIG us for 512 rows of 151936 of which
-// half have top-p alone.  (Workgroups of 16 waves add a quarter as many bins to the rows', and take longer: 47 us for 40.)
+// Bound by its arithmetic, some 30 fp64 and integer instructions and an LDS add for each logit: 112 us for 512 rows of
+// 151936.  (Workgroups of 16 waves add a quarter as many bins to the rows', and take longer: 47 us for 40 on a third
+// as many rows.)
 template <class T>
 __global__ __launch_bounds__(256) void sample_hist_kernel(Staged p) {
   __shared__ u64 s_hist[kBins];
@@ -662,7 +663,7 @@ __global__ __launch_bounds__(256) void sample_hist_kernel(Staged p) {
     if (s_hist[i]) atomicAdd(&p.hist[q * kBins + i], s_hist[i]);
 }
 
-// As the histogram, with its bins read by every workgroup (16 KB, from L2): SUMS_FIG us for those rows.
+// As the histogram, with its bins read by every workgroup (16 KB, from L2): 121 us for those rows.
 template <class T>
 __global__ __launch_bounds__(256) void sample_sums_kernel(Staged p) {
   __shared__ u64 s_sum[4], s_cross[kCross], s_list[kSegList];
@@ -739,65 +740,6 @@ __global__ __launch_bounds__(256) void sample_sums_kernel(Staged p) {
     if (s_at + i < kList) p.list[q * kList + s_at + i] = s_list[i];
 }
 
-// s[0 .. n2), n2 a power of two up to kList, into descending order by kRowThreads threads: a bitonic network, of
-// which a thread holds 4 consecutive elements in registers.  Steps over 1 and 2 elements stay in the thread, those over
-// up to 128 in the wave (lane moves), and only wider ones go through LDS between barriers: 2048 elements, 66 steps,
-// took 18 us with all steps in LDS.
-__device__ __forceinline__ void order2(u64& a, u64& b, bool desc) {
-  const bool swap = (a < b) == desc && a != b;
-  const u64 x = a;
-  a = swap ? b : a;
-  b = swap ? x : b;
-}
-__device__ __forceinline__ void sort_descending(u64* s, int n2) {
-  const int i0 = threadIdx.x * 4;
-  const bool in = i0 < n2;
-  u64 x[4];
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < 4; ++i) x[i] = in && i0 + i < n2 ? s[i0 + i] : 0;
-#pragma unroll 1
-  for (int k = 2; k <= n2; k <<= 1) {
-#pragma unroll 1
-    for (int j = k >> 1; j >= 4; j >>= 1) {
-      const bool lower = (i0 & j) == 0, desc = (i0 & k) == 0;
-      u64 y[4];
-      if (j >= 256) {
-        __syncthreads();
-        if (in)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) s[i0 + i] = x[i];
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < 4; ++i) y[i] = in ? s[(i0 ^ j) + i] : 0;
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) y[i] = __shfl_xor(x[i], j / 4);
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = (x[i] > y[i]) == (lower == desc) ? x[i] : y[i];
-    }
-    if (k >= 4) {
-      const bool desc = (i0 & k) == 0;
-      order2(x[0], x[2], desc);
-      order2(x[1], x[3], desc);
-      order2(x[0], x[1], desc);
-      order2(x[2], x[3], desc);
-    } else {
-      order2(x[0], x[1], true);
-      order2(x[2], x[3], false);
-    }
-  }
-  __syncthreads();
-  if (in)
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (i0 + i < n2) s[i0 + i] = x[i];
-  __syncthreads();
-}
-
-__device__ __forceinline__ int pow2_at_least(int n) { return n <= 4 ? 4 : 1 << (32 - __clz(n - 1)); }
-
 // Bin of a key's distance d below the largest: 64 per octave of d (the upper bits of d as a float), so that the
 // largest keys, whatever they are, spread over many.
 constexpr uint32_t kOneBits = 127u << 6;  // 1.f's upper bits
@@ -808,7 +750,7 @@ __device__ __forceinline__ int distance_bin(uint32_t d) {
 
 // LDS of a row's last workgroup.
 struct FinishShared {
-  u64 *list, *w, *sub, *sum, *out;  // [kList], [kList], [kSubsMost], [kRowWaves], [4]
+  u64 *list, *w, *sub, *sum, *out;  // [kList], [kList], [kSubsMost], [kRowWaves], [6]
   int *n, *m;
 };
 
@@ -822,7 +764,7 @@ __device__ __forceinline__ void draw_row(const SampleParams& a, int64_t r, const
   u64 *const s_list = sh.list, *const s_w = sh.w, *const s_sub = sh.sub, *const s_sum = sh.sum, *const s_out = sh.out;
   int *const s_n = sh.n, *const s_m = sh.m;
   constexpr int kPer = kList / kRowThreads;  // list entries of a thread
-  const int t0 = threadIdx.x * kPer, j0 = 2 * threadIdx.x;
+  const int j0 = 2 * threadIdx.x;
   auto draw = [&](u64 place, u64 total) {  // by one thread
     const uint32_t key = key_at(place);
     const double rel = key == wt.key_m ? 0.0 : ((double)logit_of(key) - wt.m) / s.tau;
@@ -893,8 +835,7 @@ __device__ __forceinline__ void draw_row(const SampleParams& a, int64_t r, const
   if (n > 0) {
     // The cut: counts and weights of the list's tokens per bin of their distance below the largest key; with top-k the
     // bin in which the k-th lies (where the list has more), and in it the cut and the weight up to it; then the bin in
-    // which the weight passes the limit of top-p.  A bin holds few tokens, each compared with all; one that holds over kFew (equal
-    // logits) has the whole list sorted instead.
+    // which the weight passes the limit of top-p.  A bin holds few tokens, each compared with all, or is split again.
     const u64 before_list = kind == kTopPRow ? crossing[1] : 0;
     u64* const bin_w = s_w;                                                     // [kBins]
     uint32_t* const bin_n = reinterpret_cast<uint32_t*>(s_w + kBins);           // [kBins]
@@ -902,50 +843,114 @@ __device__ __forceinline__ void draw_row(const SampleParams& a, int64_t r, const
     if (threadIdx.x == 0) *s_n = *s_m = 0;
     for (int i = threadIdx.x; i < kBins + kBins / 2; i += kRowThreads) s_w[i] = 0;
     __syncthreads();
-    u64 place[kPer], w[kPer];
+    // (its tokens stay in LDS: the registers are needed below)
+    auto place = [&](int i) -> u64 {
+      const int at = threadIdx.x + i * kRowThreads;
+      return at < n ? s_list[at] : 0;
+    };
+    auto bin_of_place = [&](u64 x) { return distance_bin(wt.key_m - key_at(x)); };
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      const int at = threadIdx.x + i * kRowThreads;
-      place[i] = at < n ? s_list[at] : 0;
-      const double rel = place[i] != 0 ? wt.rel(key_at(place[i])) : 0;
-      w[i] = wt.fix(rel);
-      if (place[i] != 0) {
-        const int bin = distance_bin(wt.key_m - key_at(place[i]));
-        atomicAdd(&bin_n[bin], 1u);
-        if (w[i]) atomicAdd(&bin_w[bin], w[i]);
-      }
-      if (!(rel >= s.min_p)) w[i] = 0;  // from here on: the weight it is drawn with
+      const u64 x = place(i);
+      if (x == 0) continue;
+      const u64 w = wt.fix(wt.rel(key_at(x)));
+      atomicAdd(&bin_n[bin_of_place(x)], 1u);
+      if (w) atomicAdd(&bin_w[bin_of_place(x)], w);
     }
     __syncthreads();
     const u64 w0 = bin_w[j0], w1 = bin_w[j0 + 1];
     const uint32_t n0 = bin_n[j0], n1 = bin_n[j0 + 1];
     u64 all_w, all_n;
     const u64 at_w = before_list + block_before64<kRowWaves>(w0 + w1, s_sum, &all_w);
-    const u64 at_n = block_before64<kRowWaves>(n0 + n1, s_sum, &all_n);
-    const u64 k = kind == kTopKRow && (u64)s.k < all_n ? (u64)s.k : all_n;
+    const uint32_t at_n = (uint32_t)block_before64<kRowWaves>(n0 + n1, s_sum, &all_n);
+    const uint32_t k = kind == kTopKRow && s.k < (int64_t)all_n ? (uint32_t)s.k : (uint32_t)all_n;
     double limit = kPosInf;
-    if (kind == kTopPRow) limit = s.p * (double)crossing[2] > 0 ? s.p * (double)crossing[2] : 0.5;
-    // the tokens of a bin whose count or weight passes a limit, resolved by the first wave: s_out = the last token of
-    // the prefix and the weight up to it; false: too many
-    auto resolve = [&](bool mine0, bool mine1) -> bool {
-      if (mine0 || mine1) {
-        s_out[0] = mine0 ? j0 : j0 + 1;
-        s_out[1] = mine0 ? at_w : at_w + w0;
-        s_out[2] = mine0 ? at_n : at_n + n0;
+    // In a bin: the prefix ends in the last one that begins inside both limits.
+    auto ends = [&](uint32_t n_at, u64 w_at, uint32_t in_n, u64 in_w) {
+      return in_n > 0 && n_at < k && (double)w_at < limit && (n_at + in_n >= k || (double)(w_at + in_w) >= limit);
+    };
+    auto mark = [&](int bin, uint32_t n_at, u64 w_at, uint32_t in_n) {
+      s_out[0] = bin;
+      s_out[1] = w_at;
+      s_out[2] = n_at;
+      s_out[3] = in_n;
+    };
+    // the count's cut, then the weight's
+    u64 kept = all_w;
+#pragma unroll 1
+    for (int by_weight = k < all_n ? 0 : 1; by_weight < (kind == kTopPRow || s.p < 1 ? 2 : 1); ++by_weight) {
+      if (by_weight) {
+        const double pz = s.p * (double)(kind == kTopPRow ? crossing[2] : kept);
+        limit = pz > 0 ? pz : 0.5;
       }
+      if (ends(at_n, at_w, n0, w0)) mark(j0, at_n, at_w, n0);
+      else if (ends(at_n + n0, at_w + w0, n1, w1)) mark(j0 + 1, at_n + n0, at_w + w0, n1);
+      if (threadIdx.x == 0) s_out[4] = s_out[5] = 0;
       __syncthreads();
-      const int bin = (int)s_out[0];
-      const u64 b_w = s_out[1], b_n = s_out[2];
-      const int m = (int)bin_n[bin];
-      if (m > kFew) return false;
+      int m = (int)s_out[3];
+      u64 b_w = s_out[1];
+      uint32_t b_n = (uint32_t)s_out[2];
+      uint32_t here = 0;  // a bit for each of this thread's tokens that is in the bin
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        const u64 x = place(i);
+        here |= x != 0 && bin_of_place(x) == (int)s_out[0] ? 1u << i : 0u;
+      }
+      // Too many to compare (near or equal logits): bins over the range of their places, which narrows by 2^10 or
+      // more each time, so at most 6 times.  (Sorting the list instead: 48 rows of 128256 with top-p 60 us, so 53.)
+      while (m > kFew) {
+        u64 top = 0, low = 0;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+          const u64 x = place(i);
+          top = (here >> i & 1) && x > top ? x : top;
+          low = (here >> i & 1) && ~x > low ? ~x : low;
+        }
+        top = wave_max64(top);
+        low = wave_max64(low);
+        if (lane_id() == 0) {
+          atomicMax(&s_out[4], top);
+          atomicMax(&s_out[5], low);
+        }
+        for (int i = threadIdx.x; i < kBins + kBins / 2; i += kRowThreads) s_w[i] = 0;
+        __syncthreads();
+        top = s_out[4];
+        low = ~s_out[5];
+        const float scale = (float)(kBins - 1) / (float)(top - low);
+        auto bin_here = [&](u64 x) { return min(kBins - 1, (int)((float)(top - x) * scale)); };
+#pragma unroll
+        for (int i = 0; i < kPer; ++i)
+          if (here >> i & 1) {
+            const u64 x = place(i);
+            atomicAdd(&bin_n[bin_here(x)], 1u);
+            atomicAdd(&bin_w[bin_here(x)], wt.fix(wt.rel(key_at(x))));
+          }
+        __syncthreads();
+        const u64 x0 = bin_w[j0], x1 = bin_w[j0 + 1];
+        const uint32_t c0 = bin_n[j0], c1 = bin_n[j0 + 1];
+        u64 all;
+        const u64 x_at = b_w + block_before64<kRowWaves>(x0 + x1, s_sum, &all);
+        const uint32_t c_at = b_n + (uint32_t)block_before64<kRowWaves>(c0 + c1, s_sum, &all);
+        if (ends(c_at, x_at, c0, x0)) mark(j0, c_at, x_at, c0);
+        else if (ends(c_at + c0, x_at + x0, c1, x1)) mark(j0 + 1, c_at + c0, x_at + x0, c1);
+        if (threadIdx.x == 0) s_out[4] = s_out[5] = 0;
+        __syncthreads();
+        m = (int)s_out[3];
+        b_w = s_out[1];
+        b_n = (uint32_t)s_out[2];
+#pragma unroll
+        for (int i = 0; i < kPer; ++i)
+          if ((here >> i & 1) && bin_here(place(i)) != (int)s_out[0]) here &= ~(1u << i);
+      }
+      // each against all, by the first wave
 #pragma unroll
       for (int i = 0; i < kPer; ++i)
-        if (place[i] != 0 && distance_bin(wt.key_m - key_at(place[i])) == bin) few[atomicAdd(s_m, 1)] = place[i];
+        if (here >> i & 1) few[atomicAdd(s_m, 1)] = place(i);
       __syncthreads();
       if (wave_id() == 0) {
         const int lane = lane_id();
         u64 x[2], y[2], at[2] = {b_w, b_w};
-        u64 rank[2] = {b_n, b_n};
+        uint32_t rank[2] = {b_n, b_n};
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           x[i] = lane + 64 * i < m ? few[lane + 64 * i] : 0;
@@ -965,9 +970,9 @@ __device__ __forceinline__ void draw_row(const SampleParams& a, int64_t r, const
         u64 last = ~0ull, sum = 0;  // the smallest place of the prefix
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const bool in = x[i] != 0 && rank[i] < k && (double)at[i] < limit;
-          last = in && x[i] < last ? x[i] : last;
-          sum += in ? y[i] : 0;
+          const bool kept = x[i] != 0 && rank[i] < k && (double)at[i] < limit;
+          last = kept && x[i] < last ? x[i] : last;
+          sum += kept ? y[i] : 0;
         }
         last = ~wave_max64(~last);
         sum = wave_sum64(sum);
@@ -979,58 +984,18 @@ __device__ __forceinline__ void draw_row(const SampleParams& a, int64_t r, const
       }
       __syncthreads();
       cut = s_out[0];
-      return true;
-    };
-    bool done = true;
-    if (kind == kTopKRow) {
-      u64 kept = all_w;
-      if (k < all_n) {
-        const bool in0 = at_n < k && at_n + n0 >= k, in1 = at_n + n0 < k && at_n + n0 + n1 >= k;
-        done = resolve(in0, in1);
-        kept = s_out[1];
-      }
-      if (done && s.p < 1) {
-        const double pz = s.p * (double)kept;
-        limit = pz > 0 ? pz : 0.5;
-        __syncthreads();
-        // the last bin that begins below the limit, of those up to the k-th's
-        const bool b0 = n0 > 0 && at_n < k && (double)at_w < limit;
-        const bool b1 = n1 > 0 && at_n + n0 < k && (double)(at_w + w0) < limit;
-        const bool e0 = b0 && ((double)(at_w + w0) >= limit || at_n + n0 >= k);
-        const bool e1 = b1 && ((double)(at_w + w0 + w1) >= limit || at_n + n0 + n1 >= k);
-        done = resolve(e0, e1 && !e0);
-      }
-    } else {
-      const bool b0 = (double)at_w < limit && (double)(at_w + w0) >= limit;
-      const bool b1 = (double)(at_w + w0) < limit && (double)(at_w + w0 + w1) >= limit;
-      done = resolve(b0, b1);
-    }
-    if (!done) {
+      kept = s_out[1];
       __syncthreads();
-      const int n2 = pow2_at_least(n);
-      for (int i = n + threadIdx.x; i < n2; i += kRowThreads) s_list[i] = 0;
-      sort_descending(s_list, n2);
-      u64 sum = 0, x[kPer], all;
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        const bool in = t0 + i < n && (u64)(t0 + i) < k;
-        sum += x[i] = in ? wt.fix(wt.rel(key_at(s_list[t0 + i]))) : 0;
-      }
-      u64 at = before_list + block_before64<kRowWaves>(sum, s_sum, &all);
-      if (kind == kTopKRow && s.p < 1) limit = s.p * (double)all > 0 ? s.p * (double)all : 0.5;
-      u64 prefix = 0;
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        prefix += t0 + i < n && (u64)(t0 + i) < k && (double)at < limit;
-        at += x[i];
-      }
-      prefix = block_sum64<kRowWaves>(prefix, s_sum);
-      cut = s_list[prefix - 1];
     }
     // the prefix's tokens join the sub-blocks' sums (with top-k they are all there is)
 #pragma unroll
-    for (int i = 0; i < kPer; ++i)
-      if (place[i] >= cut && w[i]) atomicAdd(&s_sub[(index_at(place[i]) + v.lead) / kSub], w[i]);
+    for (int i = 0; i < kPer; ++i) {
+      const u64 x = place(i);
+      if (x == 0 || x < cut) continue;
+      const double rel = wt.rel(key_at(x));
+      const u64 w = rel >= s.min_p ? wt.fix(rel) : 0;
+      if (w) atomicAdd(&s_sub[(index_at(x) + v.lead) / kSub], w);
+    }
   }
   // the sub-block that holds the token, then its place there
   __syncthreads();
@@ -1068,11 +1033,11 @@ __device__ __forceinline__ void draw_row(const SampleParams& a, int64_t r, const
   }
 }
 
-// One workgroup a row, bound by the latency of its steps, loads and barriers in turn: FIN1_FIG us for one row of 151936 with
-// top-k 50 and top-p, FIN512_FIG for 512 of mixed settings, two workgroups a CU.
+// One workgroup a row, bound by the latency of its steps, loads and barriers in turn: 12 us for one row of 151936
+// with top-k 50 and top-p, 50 for 512 of them or of mixed settings, two workgroups a CU.
 template <class T>
 __global__ __launch_bounds__(kRowThreads) void sample_finish_kernel(Staged p) {
-  __shared__ u64 s_list[kList], s_w[kList], s_sub[kSubsMost], s_sum[kRowWaves], s_out[4];
+  __shared__ u64 s_list[kList], s_w[kList], s_sub[kSubsMost], s_sum[kRowWaves], s_out[6];
   __shared__ double s_powers[kPowers];
   __shared__ int s_n, s_m;
   const SampleParams& a = p.a;
@@ -1191,11 +1156,11 @@ __global__ __launch_bounds__(kRowThreads) void sample_finish_kernel(Staged p) {
 
 // ---------------------------------------------------------------- a short row
 // Up to kRowMost logits, in one launch: the row, read once, is the list.  A radix descent reads it up to 8 times from
-// L1, between barriers: 64 rows of 4096 with top-k and top-p took 35 us, so 18.  Without either there is no cut to find,
+// L1, between barriers: 64 rows of 4096 with top-k and top-p took 35 us, so 20.  Without either there is no cut to find,
 // and the two passes of sample_row over the cached row are the shorter way (10 us; by the list 43).
 template <class T>
 __global__ __launch_bounds__(kRowThreads) void sample_short_kernel(SampleParams a) {
-  __shared__ u64 s_list[kList], s_w[kList], s_sub[4], s_sum[kRowWaves], s_out[4];
+  __shared__ u64 s_list[kList], s_w[kList], s_sub[4], s_sum[kRowWaves], s_out[6];
   __shared__ double s_powers[kPowers];
   __shared__ int s_n, s_m;
   const int64_t r = blockIdx.x;
