@@ -11,6 +11,7 @@ flag included, so graphs and callers written against them keep working.  The
 flag chose between the reference's Triton and torch elementwise paths; here
 both are the same HIP kernels, so it is accepted and has no effect.
 """
+import functools
 from typing import List, Optional, Tuple
 
 import torch
@@ -336,6 +337,12 @@ _fwd_active_op.register_autograd(_autograd_backward_active, setup_context=_setup
 
 
 # ---------------------------------------------------------------- eager calls
+# (looked up once: through torch's modules the checks of a call and its backward take 2 us more)
+_is_compiling, _tracing_state = torch.compiler.is_compiling, torch._C._get_tracing_state
+_functorch_stack = torch._C._functorch.peek_interpreter_stack
+_dispatch_modes, _function_modes = torch._C._len_torch_dispatch_stack, torch._C._len_torch_function_stack
+
+
 def eager(*tensors):
     """Whether a call on these tensors (None allowed) may go to the library without the custom ops: plain
     GPU tensors, and nothing looking at the ops themselves (compilation, tracing, functorch transforms,
@@ -343,14 +350,25 @@ def eager(*tensors):
     host time per op and direction, of the 480 that a training step of 512 tokens in fp32 (N = 512,
     K = 256, V = 4096) took when its kernels take 160; without them, and with the loss in the readout's
     node (``readout_mse_eager``), it takes 270."""
-    if (torch.compiler.is_compiling() or torch._C._functorch.peek_interpreter_stack() is not None
-            or torch._C._len_torch_dispatch_stack() or torch._C._len_torch_function_stack()
-            or torch._C._get_tracing_state() is not None or forward_ad._current_level >= 0):
+    if (_is_compiling() or _functorch_stack() is not None or _dispatch_modes() or _function_modes()
+            or _tracing_state() is not None or forward_ad._current_level >= 0):
         return False
     for t in tensors:  # (a loop: 4 us less per call than a generator)
         if t is not None and not (t.is_cuda and type(t) in (torch.Tensor, torch.nn.Parameter)):
             return False
     return True
+
+
+def first_order(backward):
+    """``once_differentiable`` for the common case too: a backward without ``create_graph`` runs as it is (the
+    wrapper's own Python takes 5 us in autograd's thread)."""
+    checked = once_differentiable(backward)
+
+    @functools.wraps(backward)
+    def run(ctx, *grads):
+        return checked(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+    return run
 
 
 def _needs_grad(*tensors):

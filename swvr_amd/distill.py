@@ -9,11 +9,10 @@ swvr_distill, swvr_distill_bwd).
 from typing import List, Optional, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._ops import (DEFAULT_CHUNK, REDUCTIONS, _f32, _grad_buffer, _kpad, _lead_stride, _needs_grad, _operand, _plain,
-                   _require_device, _rows_staged, eager)
+                   _require_device, _rows_staged, eager, first_order)
 from .api import _chunk, _compute_dtype
 
 MAX_TEACHER = 1024
@@ -178,7 +177,7 @@ class _Distill(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
+    @first_order
     def backward(ctx, g):
         saved = ctx.saved_tensors
         needs = _needs(ctx, saved[2])

@@ -12,10 +12,9 @@ import math
 from typing import Optional, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._ops import _needs_grad, _plain, _require_device, eager
+from ._ops import _plain, _require_device, eager, first_order
 
 _EMBED_TAG = {**_lib.DTYPE_TAG, torch.float64: _lib.F64}
 _SORT_FREE = 2048  # tokens up to which the gradient needs neither order nor workspace (their sizes are 0)
@@ -112,7 +111,7 @@ class _Lookup(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
+    @first_order
     def backward(ctx, g):
         ids, order = ctx.saved_tensors
         if eager(g, ids):
@@ -138,7 +137,9 @@ def embedding_lookup(ids, E, *, scale=1.0):
     if ids.device != E.device:
         raise ValueError(f"ids are on {ids.device} but E on {E.device}")
     if eager(ids, E):
-        return _Lookup.apply(ids, E, float(scale)) if _needs_grad(E) else _lookup(ids, E, scale)[0]
+        if E.requires_grad and torch.is_grad_enabled():
+            return _Lookup.apply(ids, E, float(scale))
+        return _lookup(ids, E, scale)[0]
     if E.device.type == "cpu":
         _require_device(E)
     return _lookup_op(ids, E, float(scale))
