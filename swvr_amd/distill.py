@@ -58,7 +58,8 @@ def _forward(h, W, bias, teacher, ids, weight, tau, z, reduction, scale, chunk, 
     _lib.call(lib.swvr_distill, h.device, tag, h_tag, w_tag, N, Kp, V, T, hc.data_ptr(), _lead_stride(hc),
               Wc.data_ptr(), _lead_stride(Wc), a(b), _lib.DTYPE_TAG[b.dtype] if b is not None else 0, sb.data_ptr(),
               scale, i.data_ptr(), i.dtype == torch.int64, i.stride(0), t.data_ptr(), _lib.DTYPE_TAG[t.dtype],
-              t.stride(0), tau, a(w), z, reduction, out.data_ptr(), c, lse, p, q, coef, a(scores), ws.data_ptr(), ws_bytes)
+              t.stride(0), tau, a(w), z, reduction, out.data_ptr(), c, lse, p, q, coef, a(scores), ws.data_ptr(),
+              ws_bytes)
     return out, kept, sb, scores
 
 
@@ -93,9 +94,8 @@ def _backward(g, h, W, bias, ids, kept, sb, scores, tau, z, reduction, scale, ch
     c, lse, coef, p, q = _kept(kept, N, T, True)
     _lib.call(lib.swvr_distill_bwd, dev, tag, h_tag, w_tag, N, Kp, V, T, hc.data_ptr(), _lead_stride(hc),
               Wc.data_ptr(), _lead_stride(Wc), sb.data_ptr() if bias is not None else None, scale, i.data_ptr(),
-              i.dtype == torch.int64, i.stride(0), tau, z, reduction, g32.data_ptr(), c, lse, p, q, coef, _lib.address(scores),
-              chunk, *of(gh),
-              *of(gW), *of(gb), ws.data_ptr(), ws_bytes)
+              i.dtype == torch.int64, i.stride(0), tau, z, reduction, g32.data_ptr(), c, lse, p, q, coef,
+              _lib.address(scores), chunk, *of(gh), *of(gW), *of(gb), ws.data_ptr(), ws_bytes)
     if gh is not None:
         gh = gh[:, :K] if Kp != K else gh
         gh = gh.to(h.dtype) if gh.dtype != h.dtype else gh
@@ -238,7 +238,8 @@ def softmax_distill(h, W, teacher_logits, teacher_ids, bias=None, *, temperature
     recomputes the scores ``chunk_size`` vocabulary rows at a time, as ``softmax_readout`` does.  An eager call
     without a chunk keeps the scores of few tokens (up to 768, in fp32 any number) for it instead, where they take
     at most twice W's bytes (K tokens in the 2-byte types, 2 K in fp32) and 512 MB.  Autograd reaches h, W and
-    bias; the teacher and the weight get none.
+    bias; the teacher and the weight get none.  In fp16 the gradients, and the softmax's part of them, fall below the
+    type's range where many tokens share a mean: scale the loss, as fp16 training does.
     """
     _check(h, W, teacher_logits, teacher_ids, bias, weight, temperature, reduction)
     chunk = _chunk(chunk_size)

@@ -91,6 +91,16 @@ def test_one_id_holds_most_tokens(dtype, share, N, D):
         check(torch.where(hot, at, ids), E, g)
 
 
+@pytest.mark.parametrize("id_dtype", [torch.int64, torch.int32])
+@pytest.mark.parametrize("N", [9000, 100003])
+def test_few_ids_hold_half_the_tokens(id_dtype, N):
+    """Ids as text has them, the frequent ones first: one workgroup's ids hold more tokens than it keeps at a time."""
+    V = 30000
+    E, _, g = make(N, V, 12, torch.bfloat16, seed=N)
+    ids = (V ** torch.rand(N, device=DEV, generator=gen(4), dtype=torch.float64) - 1).to(id_dtype)
+    check(torch.where(torch.rand(N, device=DEV, generator=gen(5)) < 0.1, -1, ids), E, g)
+
+
 def test_several_ids_share_the_tokens():
     """Runs of equal ids of every length around the runs that are summed together."""
     lengths = [1, 7, 8, 9, 31, 32, 33, 63, 64, 65, 127, 500, 1023, 1024, 1025, 2100]

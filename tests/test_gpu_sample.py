@@ -182,6 +182,13 @@ def test_many_rows(R, V):
         assert torch.equal(t, token[rows]) and torch.equal(lp, logprob[rows])
 
 
+@pytest.mark.parametrize("kw", [dict(), dict(top_k=40, top_p=0.9), dict(top_p=0.7, min_p=0.01), dict(temperature=0.0)], ids=str)
+@pytest.mark.parametrize("V", [2 ** 21 - 8, 2 ** 21 + 5])   # the longest rows of the launches for many workgroups; longer
+def test_the_longest_rows(kw, V):
+    x = 3 * torch.randn(2, V, device=DEV, generator=gen(24))
+    check(x, torch.rand(2, device=DEV, generator=gen(25)), **kw)
+
+
 @pytest.mark.parametrize("V", [1000, 9000])
 def test_many_draws_from_one_row(V):
     x = torch.randn(V, device=DEV, generator=gen(22)).expand(7, V)
