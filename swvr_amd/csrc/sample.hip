@@ -483,7 +483,8 @@ __global__ __launch_bounds__(kRowThreads) void sample_row_kernel(SampleParams a)
 // A list that would pass kList tokens, or kSegList from one workgroup (equal logits, a nearly flat row), leaves its
 // row to sample_row, in the same launch, as does a k above kTopK.  Every sum is one of whole numbers, so its order
 // does not matter.
-constexpr int kSub = 2048, kGroups = 4096, kList = 4096, kSegList = 2048, kTopK = 1024, kFew = 128;
+constexpr int kSub = 2048, kGroups = 4096, kList = 4096, kSegList = 2048, kTopK = 1024, kFew = 128,
+              kDense = 512;
 constexpr int64_t kRowMost = 4096, kStagedMost = ((int64_t)1 << 21) - 8;  // (groups of at most a wave's 512)
 constexpr int kSubsMost = (int)(((int64_t)1 << 21) / kSub);
 constexpr int kWaveLoad = 8, kCross = 3;
@@ -663,10 +664,12 @@ __global__ __launch_bounds__(256) void sample_hist_kernel(Staged p) {
     if (s_hist[i]) atomicAdd(&p.hist[q * kBins + i], s_hist[i]);
 }
 
-// As the histogram, with its bins read by every workgroup (16 KB, from L2): 121 us for those rows.
+// As the histogram, with its bins read by every workgroup (16 KB, from L2), but few logits are in the prefix: they are
+// gathered in LDS and only they are weighed (121 us for those rows with all of them weighed, so 83).
 template <class T>
 __global__ __launch_bounds__(256) void sample_sums_kernel(Staged p) {
   __shared__ u64 s_sum[4], s_cross[kCross], s_list[kSegList];
+  __shared__ float s_dense[4][kDense];
   __shared__ double s_powers[kPowers];
   __shared__ int s_n, s_at;
   const int64_t q = blockIdx.x / p.n_seg, r = p.r0 + q;
@@ -704,24 +707,62 @@ __global__ __launch_bounds__(256) void sample_sums_kernel(Staged p) {
   __syncthreads();
   const Weigh wt = weigh_of(p.a, s, key_at(first), s_powers);
   const float scale = bin_scale(wt);
-  // the sum, and a bit for each token of the bin: those, few, are read again (kept apart, they hold no registers)
   u64 sum = 0;
-  uint32_t hits = 0;
+  uint32_t hits = 0, in = 0;  // a bit for each of this lane's tokens in the bin; in the prefix before it
+  int n_in = kDense + 1;
+  if (kind == kTopPRow) {
 #pragma unroll
-  for (int j = 0; j < kSteps; ++j) {
-    float x[kWaveLoad];
-    chunk_logits(v, b.first(j), b.c[j], x);
+    for (int j = 0; j < kSteps; ++j) {
+      float x[kWaveLoad];
+      chunk_logits(v, b.first(j), b.c[j], x);
 #pragma unroll
-    for (int u = 0; u < kWaveLoad; ++u) {
-      const float l = x[u];
-      const int bin = bin_of(l, wt, scale);
-      const double w = wt.rel(l);
-      sum += bin < cross && w >= s.min_p ? wt.fix(w) : 0;
-      hits |= (bin == cross && l > kNegInf) ? 1u << (j * kWaveLoad + u) : 0u;
-      // one element after another: left to it, the compiler keeps all 32 in flight, in 245 registers (75 us for 50)
-      asm volatile("" : "+v"(hits), "+v"(sum));
+      for (int u = 0; u < kWaveLoad; ++u) {
+        const int bin = bin_of(x[u], wt, scale);
+        in |= bin < cross ? 1u << (j * kWaveLoad + u) : 0u;
+        hits |= (bin == cross && x[u] > kNegInf) ? 1u << (j * kWaveLoad + u) : 0u;
+        asm volatile("" : "+v"(hits), "+v"(in));  // (for registers, as below: 105 us, so 83)
+      }
+    }
+    const int to = (int)wave_scan64((u64)__popc(in), Sum64());
+    n_in = __builtin_amdgcn_readlane(to, 63);
+    if (n_in <= kDense) {
+      // few of the sub-block: gathered, so that only they are weighed
+      float* const dense = s_dense[wave_id()];
+      int at = to - __popc(in);
+#pragma unroll
+      for (int j = 0; j < kSteps; ++j) {
+        float x[kWaveLoad];
+        chunk_logits(v, b.first(j), b.c[j], x);
+#pragma unroll
+        for (int u = 0; u < kWaveLoad; ++u)
+          if (in >> (j * kWaveLoad + u) & 1) {
+            dense[at] = x[u];
+            ++at;
+          }
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      for (int i = lane_id(); i < n_in; i += 64) {
+        const double w = wt.rel(dense[i]);
+        sum += w >= s.min_p ? wt.fix(w) : 0;
+      }
     }
   }
+  if (n_in > kDense) {
+    // (one element after another: left to it, the compiler keeps all 32 in flight, in 245 registers, 75 us for 50)
+#pragma unroll
+    for (int j = 0; j < kSteps; ++j) {
+      float x[kWaveLoad];
+      chunk_logits(v, b.first(j), b.c[j], x);
+#pragma unroll
+      for (int u = 0; u < kWaveLoad; ++u) {
+        const double w = wt.rel(x[u]);
+        const bool mine = kind != kTopPRow || (in >> (j * kWaveLoad + u) & 1);
+        sum += mine && w >= s.min_p ? wt.fix(w) : 0;
+        asm volatile("" : "+v"(sum));
+      }
+    }
+  }
+  // the bin's tokens, few, are read again (kept apart, they hold no registers)
   for (; hits != 0; hits &= hits - 1) {
     const int i = __ffs((int)hits) - 1;
     const int64_t at = b.first(i / kWaveLoad) + i % kWaveLoad;
