@@ -484,7 +484,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_row_kernel(SampleParams a)
 // row to sample_row, in the same launch, as does a k above kTopK.  Every sum is one of whole numbers, so its order
 // does not matter.
 constexpr int kSub = 2048, kGroups = 4096, kList = 4096, kSegList = 2048, kTopK = 1024, kFew = 128,
-              kDense = 512;
+              kDense = 512, kHistWaves = 8;
 constexpr int64_t kRowMost = 4096, kStagedMost = ((int64_t)1 << 21) - 8;  // (groups of at most a wave's 512)
 constexpr int kSubsMost = (int)(((int64_t)1 << 21) / kSub);
 constexpr int kWaveLoad = 8, kCross = 3;
@@ -499,7 +499,7 @@ struct Staged {
   int64_t r0;       // first row of this launch
   int n_sub;        // sub-blocks of a row
   int gshift;       // log2 of a group's logits
-  int n_seg;        // workgroups of 4 waves per row in the first three launches
+  int n_seg;        // workgroups of 4 waves per row (of the histogram, kHistWaves)
   u64* first;       // [rows][n_sub] place_of the sub-block's first token in order
   uint32_t* group;  // [rows][kGroups] largest keys
   u64* hist;        // [rows][kBins] weights
@@ -630,22 +630,23 @@ __global__ __launch_bounds__(256) void sample_max_kernel(Staged p) {
   if (lane_id() == 0) p.first[q * p.n_sub + b.sub] = first;
 }
 
-// Bound by its arithmetic, some 30 fp64 and integer instructions and an LDS add for each logit: 112 us for 512 rows of
-// 151936.  (Workgroups of 16 waves add a quarter as many bins to the rows', and take longer: 47 us for 40 on a third
-// as many rows.)
+// Bound by its arithmetic, some 30 fp64 and integer instructions and an LDS add for each logit: 102 us for 512 rows of
+// 151936.  (Of 4 waves, which add twice as many bins to the rows', 110; 16 leave fewer at work at its barriers: on a
+// third as many rows 47 us for the 40 of 4.)
 template <class T>
-__global__ __launch_bounds__(256) void sample_hist_kernel(Staged p) {
+__global__ __launch_bounds__(64 * kHistWaves) void sample_hist_kernel(Staged p) {
   __shared__ u64 s_hist[kBins];
   __shared__ double s_powers[kPowers];
-  const int64_t q = blockIdx.x / p.n_seg, r = p.r0 + q;
+  const int n_seg = (p.n_sub + kHistWaves - 1) / kHistWaves;
+  const int64_t q = blockIdx.x / n_seg, r = p.r0 + q;
   const RowSettings s = settings_of(p.a, r);
   if (kind_of(s, p.a.V) != kTopPRow) return;
   const RowView<T> v(p.a, r);
-  const SubBlock<T> b(p, v, (int)(blockIdx.x % p.n_seg), 4);
+  const SubBlock<T> b(p, v, (int)(blockIdx.x % n_seg), kHistWaves);
   const u64 first = row_first(p, q);
   if (first == 0) return;
   fill_powers(s_powers);
-  for (int i = threadIdx.x; i < kBins; i += 256) s_hist[i] = 0;
+  for (int i = threadIdx.x; i < kBins; i += 64 * kHistWaves) s_hist[i] = 0;
   __syncthreads();
   const Weigh wt = weigh_of(p.a, s, key_at(first), s_powers);
   const float scale = bin_scale(wt);
@@ -660,7 +661,7 @@ __global__ __launch_bounds__(256) void sample_hist_kernel(Staged p) {
     }
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < kBins; i += 256)
+  for (int i = threadIdx.x; i < kBins; i += 64 * kHistWaves)
     if (s_hist[i]) atomicAdd(&p.hist[q * kBins + i], s_hist[i]);
 }
 
@@ -1304,7 +1305,10 @@ hipError_t run_staged(const SampleParams& a, char* ws, hipStream_t stream) {
     const int64_t rows = a.R - p.r0 < kRowsMost ? a.R - p.r0 : kRowsMost;
     const unsigned blocks = (unsigned)(rows * p.n_seg);
     sample_max_kernel<T><<<blocks, 256, 0, stream>>>(p);
-    if (p.may_p) sample_hist_kernel<T><<<blocks, 256, 0, stream>>>(p);
+    if (p.may_p) {
+      const unsigned wide = (unsigned)(rows * ((p.n_sub + kHistWaves - 1) / kHistWaves));
+      sample_hist_kernel<T><<<wide, 64 * kHistWaves, 0, stream>>>(p);
+    }
     if (p.may_sum) sample_sums_kernel<T><<<blocks, 256, 0, stream>>>(p);
     sample_finish_kernel<T><<<(unsigned)rows, kRowThreads, 0, stream>>>(p);
     const hipError_t e = hipGetLastError();
