@@ -510,6 +510,8 @@ int swvr_distill(int dtype, int h_dtype, int w_dtype, int64_t N, int64_t K, int6
   if (!is_dtype(t_dtype)) return fail(SWVR_EDTYPE, "unsupported teacher dtype tag %d", t_dtype);
   if (bias && !is_dtype(bias_dtype)) return fail(SWVR_EDTYPE, "unsupported bias dtype tag %d", bias_dtype);
   if (bias && !bias_scaled) return fail(SWVR_EINVAL, "bias_scaled must be non-null with a bias");
+  if (bias && bias == bias_scaled && (bias_dtype != SWVR_F32 || temperature != 1.f))
+    return fail(SWVR_EINVAL, "bias_scaled may be an fp32 bias itself only at temperature 1");
   if (ldt < 0) return fail(SWVR_EINVAL, "ldt=%lld must not be negative", (long long)ldt);
   if (N > 0 && (!teacher || !lse)) return fail(SWVR_EINVAL, "teacher logits and lse must be non-null");
   if ((N > 0 || reduction) && !out) return fail(SWVR_EINVAL, "out must be non-null");
@@ -533,7 +535,7 @@ int swvr_distill(int dtype, int h_dtype, int w_dtype, int64_t N, int64_t K, int6
   float* part = z + up256((size_t)N * T * 4) / 4;
   const float inv_tau = 1.f / temperature, scale = logit_scale / temperature;
   hipError_t e = hipSuccess;
-  if (bias && (e = swvr::distill_scale(bias, bias_dtype, V, inv_tau, bias_scaled, s)) != hipSuccess)
+  if (bias && bias != bias_scaled && (e = swvr::distill_scale(bias, bias_dtype, V, inv_tau, bias_scaled, s)) != hipSuccess)
     return hip_fail(e, "bias launch");
   const float* const sb = bias ? bias_scaled : nullptr;
   // the log-sum-exps: a readout without columns

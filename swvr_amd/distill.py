@@ -32,9 +32,10 @@ def _kept(kept, N, T, need_grad):
     return (at, lse, coef, coef + 4 * N, coef + 4 * (N + N * T)) if need_grad else (at, lse, None, None, None)
 
 
-def _forward(h, W, bias, teacher, ids, weight, tau, z, reduction, scale, chunk, cdt, need_grad):
-    """The loss, what ``_kept`` names, the bias over tau in fp32 (empty without a bias), and the scores where the
-    library keeps them for the backward (few tokens, no chunk given; else empty)."""
+def _forward(h, W, bias, teacher, ids, weight, tau, z, reduction, scale, chunk, cdt, need_grad, alias=True):
+    """The loss, what ``_kept`` names, the bias over tau in fp32 (empty without a bias; with ``alias``, at tau = 1
+    an fp32 bias itself), and the scores where the library keeps them for the backward (few tokens, no chunk
+    given; else empty)."""
     lib = _lib.load()
     N, K = h.shape
     V, T = W.shape[0], ids.shape[1]
@@ -46,7 +47,10 @@ def _forward(h, W, bias, teacher, ids, weight, tau, z, reduction, scale, chunk, 
     tag = _lib.DTYPE_TAG[cdt]
     out = hc.new_empty((N,) if reduction == 0 else (), dtype=torch.float32)
     kept = hc.new_empty(1 + N * (2 * T + 2) if need_grad else 1 + N, dtype=torch.float32)
-    sb = hc.new_empty(V if b is not None else 0, dtype=torch.float32)
+    if alias and b is not None and tau == 1 and b.dtype == torch.float32:
+        sb = b
+    else:
+        sb = hc.new_empty(V if b is not None else 0, dtype=torch.float32)
     scores = None
     if need_grad and chunk is None:
         kept_bytes = lib.swvr_distill_scores_size(tag, w_tag, N, Kp, V, _lead_stride(Wc))
@@ -111,7 +115,8 @@ def _backward(g, h, W, bias, ids, kept, sb, scores, tau, z, reduction, scale, ch
 def _fwd_op(h: torch.Tensor, W: torch.Tensor, bias: Optional[torch.Tensor], teacher: torch.Tensor, ids: torch.Tensor,
             weight: Optional[torch.Tensor], tau: float, z: float, reduction: int, scale: float, chunk: int,
             cdt: torch.dtype, need_grad: bool) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    return _forward(h, W, bias, teacher, ids, weight, tau, z, reduction, scale, chunk, cdt, need_grad)[:3]
+    return _forward(h, W, bias, teacher, ids, weight, tau, z, reduction, scale, chunk, cdt, need_grad,
+                    alias=False)[:3]
 
 
 @_fwd_op.register_fake

@@ -413,6 +413,26 @@ def test_two_streams_at_once():
             assert torch.equal(loss, l0) and all(torch.equal(a, c) for a, c in zip(grads, g0))
 
 
+def test_parameters_changed_before_the_backward_are_refused():
+    for which in range(3):
+        h, W, b, t, ids = make(40, 64, 500, 4, torch.float32)
+        xs = [x.requires_grad_(True) for x in (h, W, b)]
+        loss = swvr_amd.softmax_distill(h, W, t, ids, b)
+        with torch.no_grad():
+            xs[which].add_(1)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+
+
+@pytest.mark.parametrize("tau", [1.0, 2.0])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_bias_that_is_a_view(dtype, tau):
+    """At temperature 1 a dense fp32 bias is read as it is; others are laid out and scaled first."""
+    h, W, b, t, ids = make(60, 64, 500, 4, torch.float32)
+    for view in (torch.stack([b, -b], dim=1).to(dtype)[:, 0], torch.cat([b, b]).to(dtype)[499:999], b[:1].to(dtype).expand(500)):
+        check(h, W, view, t, ids, tau=tau)
+
+
 def test_double_backward_is_refused():
     h, W, b, t, ids = make(20, 64, 90, 4, torch.float32)
     h.requires_grad_(True)

@@ -195,6 +195,14 @@ def test_abi_refusals(fn, kw, code):
     assert _lib.load().swvr_last_error()
 
 
+@pytest.mark.parametrize("bias_dtype,tau", [(_lib.BF16, 1.0), (_lib.F32, 2.0)])
+def test_abi_refuses_a_bias_as_its_own_scaled_copy(bias_dtype, tau):
+    lib = _lib.load()
+    assert lib.swvr_distill(_lib.BF16, _lib.BF16, _lib.BF16, 4, 16, 8, 2, P, 16, P, 16, P, bias_dtype, P, 1.0, P, 1, 2, P,
+                            _lib.F32, 2, tau, None, 0.0, 2, P, P, P, P, P, P, None, P, 1 << 30, None) == _lib.EINVAL
+    assert b"temperature 1" in lib.swvr_last_error()
+
+
 def test_abi_empty_calls_launch_nothing():
     assert embedding(N=0, ids=None, out=None) == _lib.OK
     assert embedding(D=0, lde=0, E=None, out=None) == _lib.OK
