@@ -1445,10 +1445,15 @@ __device__ __forceinline__ void gemm_loop(f32x16_t (&acc)[FM][FN], const TA& ta,
 // Tile of the gradient GEMMs: GM x GN per workgroup of WM x WN waves
 // (two waves per SIMD for bf16 / f16, so one wave's LDS and barrier waits
 // are covered by the other's matrix work).
-template <class T>
+// SMALL (fp32): a quarter of the tile, for launches of fewer than two tiles a CU and for reductions of few tokens, whose
+// tiles' prologues and stores weigh as much as their products.  512 tokens, K = 256: 192 tiles 42 us, so 26; 384 tiles
+// 57 and 46; 512 tiles 76 and 81; 500 tokens, K = 1024, 2512 tiles 523 and 575.  100 tokens, K = 512, 1256 tiles 99
+// and 79.
+constexpr int64_t kGemmFew = 512, kGemmFewTokens = 128;
+template <class T, bool SMALL = false>
 struct GemmTile {
   static constexpr bool wide = sizeof(T) == 2;
-  static constexpr int GM = wide ? 256 : 128;
+  static constexpr int GM = wide ? 256 : SMALL ? 64 : 128;
   static constexpr int GN = GM;
   static constexpr int WM = 2;
   static constexpr int WN = wide ? 4 : 2;
@@ -1469,9 +1474,8 @@ struct GemmTile {
 //   DW:  dW[v0+v][k]    = s sum_q stage[v][q] h[tok(q)][k]    (A: KTile layout, B: RTile layout)
 //   !DW: dh[tok(q)][k] += s sum_v stage[v][q] W[v0+v][k]      (A: RTile layout, B: RTile layout)
 // A dh tile covers run `run` of the chunk's vocabulary rows and adds to that run's accumulator.
-template <class T, bool DW>
+template <class T, class G, bool DW>
 __device__ __forceinline__ void gemm_tile(const GemmParams& p, int t, char* smem, int run = 0) {
-  typedef GemmTile<T> G;
   constexpr int kBK = G::BK;
   constexpr int GM = G::GM, GN = G::GN, NT = G::NT;
   constexpr int FM = GM / (32 * G::WM), FN = GN / (32 * G::WN);
@@ -1528,9 +1532,8 @@ __device__ __forceinline__ void gemm_tile(const GemmParams& p, int t, char* smem
 // split makes the dE^T work pieces of a tile, so a launch whose dW and dh tiles fill whole rounds
 // of the CUs is not left a round of a few whole dE^T tiles; the partials are summed in run order
 // by the reduction after the launch.
-template <class T>
+template <class T, class G>
 __device__ __forceinline__ void gemm_tile_de(const GemmParams& p, int t, char* smem) {
-  typedef GemmTile<T> G;
   constexpr int kBK = G::BK;
   constexpr int GM = G::GM, GN = G::GN, NT = G::NT;
   constexpr int FM = GM / (32 * G::WM), FN = GN / (32 * G::WN);
@@ -1585,9 +1588,9 @@ __device__ __forceinline__ void gemm_pack_w(const GemmParams& p, int w, char* sm
 // One launch covers the gradient products of a chunk: blocks [0, n_dw) are
 // dW tiles, then n_de dE^T tiles (wide scores kernel only), then dh tiles.
 // The dW and dE^T tiles (reductions over all active positions) are dealt first.
-template <class T>
-__global__ __launch_bounds__(GemmTile<T>::NT) void bwd_gemm_kernel(GemmParams p) {
-  typedef GemmTile<T> G;
+template <class T, bool SMALL>
+__global__ __launch_bounds__((GemmTile<T, SMALL>::NT)) void bwd_gemm_kernel(GemmParams p) {
+  typedef GemmTile<T, SMALL> G;
   constexpr int kBK = G::BK;
   constexpr int SB = KTile<T, G::GM, kBK, G::NT>::BYTES + RTile<T, G::GN, kBK, G::NT>::BYTES;
   static_assert(KTile<T, G::GM, kBK, G::NT>::BYTES == RTile<T, G::GM, kBK, G::NT>::BYTES,
@@ -1615,12 +1618,12 @@ __global__ __launch_bounds__(GemmTile<T>::NT) void bwd_gemm_kernel(GemmParams p)
   if (b < p.n_dw) {
     int r, c;
     grouped_tile(b, p.n_dw / p.n_n, p.n_n, &r, &c);
-    gemm_tile<T, true>(p, r * p.n_n + c, smem);
+    gemm_tile<T, G, true>(p, r * p.n_n + c, smem);
     return;
   }
   b -= p.n_dw;
   if (b < p.n_de) {
-    gemm_tile_de<T>(p, b, smem);
+    gemm_tile_de<T, G>(p, b, smem);
     return;
   }
   b -= p.n_de;
@@ -1637,7 +1640,7 @@ __global__ __launch_bounds__(GemmTile<T>::NT) void bwd_gemm_kernel(GemmParams p)
       }
       int r, c;
       grouped_order(t, n_t / p.n_n, p.n_n, &r, &c);
-      gemm_tile<T, false>(p, r * p.n_n + c, smem, run);
+      gemm_tile<T, G, false>(p, r * p.n_n + c, smem, run);
     }
   }
 }
@@ -1727,12 +1730,16 @@ hipError_t dispatch_scores(const BwdPlan& plan, const ScoresParams& sp, hipStrea
 }
 
 template <class T>
-hipError_t dispatch_gemm(const BwdPlan& plan, const GemmParams& gp, hipStream_t stream) {
+hipError_t dispatch_gemm(const BwdPlan& plan, bool small, const GemmParams& gp, hipStream_t stream) {
   const int blocks = gp.n_dw + gp.n_de + gp.n_dh + gp.n_red + gp.n_pack;
   if (blocks == 0) return hipSuccess;
   if (plan.GM != GemmTile<T>::GM || plan.GN != GemmTile<T>::GN) return hipErrorInvalidValue;
   timing_begin(kKindBwdGemm, stream);
-  bwd_gemm_kernel<T><<<blocks, GemmTile<T>::NT, 0, stream>>>(gp);
+  if constexpr (sizeof(T) == 4) {
+    static_assert(GemmTile<T, true>::NT == GemmTile<T>::NT, "one count of workgroups");
+    if (small) bwd_gemm_kernel<T, true><<<blocks, GemmTile<T>::NT, 0, stream>>>(gp);
+  }
+  if (!small) bwd_gemm_kernel<T, false><<<blocks, GemmTile<T>::NT, 0, stream>>>(gp);
   timing_end(kKindBwdGemm, stream);
   return hipGetLastError();
 }
@@ -1773,6 +1780,14 @@ hipError_t bwd_run(const BwdPlan& plan, const BwdParams& p, hipStream_t stream) 
   const bool reads_gOt = plan.kind == kScoresRing || f8;  // see ScoresTile::GT; the wide kernel forms no dE
   const int dh_split = p.gW ? plan.dh_split_w : plan.dh_split_h;
   const bool gemm_de = pstage && p.gE;  // dE^T = gO^T P as tiles of the gradient GEMM launch
+  // (the sums are the same in both)
+  auto tiles = [](int64_t m, int64_t n) {
+    return (m + GemmTile<T>::GM - 1) / GemmTile<T>::GM * ((n + GemmTile<T>::GN - 1) / GemmTile<T>::GN);
+  };
+  const bool small = sizeof(T) == 4 && (p.N <= kGemmFewTokens ||
+                                        (p.gW ? tiles(p.V < plan.C ? p.V : plan.C, p.K) : 0) +
+                                                (p.gh ? tiles(p.N, p.K) * dh_split : 0) < kGemmFew);
+  const int GM = small ? GemmTile<T, true>::GM : plan.GM, GN = small ? GemmTile<T, true>::GN : plan.GN;
   // every chunk has a gradient GEMM launch: the W packing of the scores kernel rides on them
   const bool fold_pack = !f8 && !kept && (need_stage || gemm_de);
 
@@ -1919,15 +1934,15 @@ hipError_t bwd_run(const BwdPlan& plan, const BwdParams& p, hipStream_t stream) 
       gp.K = p.K;
       gp.v0 = v0;
       gp.cv = cv;
-      gp.n_n = (p.K + plan.GN - 1) / plan.GN;
-      gp.n_dw = p.gW ? ((cv + plan.GM - 1) / plan.GM) * gp.n_n : 0;
+      gp.n_n = (p.K + GN - 1) / GN;
+      gp.n_dw = p.gW ? ((cv + GM - 1) / GM) * gp.n_n : 0;
       gp.dh_split = dh_split;
       gp.dh_rows = ((cv + dh_split - 1) / dh_split + 31) & ~31;
-      gp.n_dh_tiles = p.gh ? ((p.N + plan.GM - 1) / plan.GM) * gp.n_n : 0;
+      gp.n_dh_tiles = p.gh ? ((p.N + GM - 1) / GM) * gp.n_n : 0;
       gp.n_dh = gp.n_dh_tiles * dh_split;
-      gp.n_de_n = (cv + plan.GN - 1) / plan.GN;
+      gp.n_de_n = (cv + GN - 1) / GN;
       gp.de_split = de_split(plan.N_pad);
-      gp.n_de = gemm_de ? ((plan.DP + plan.GM - 1) / plan.GM) * gp.n_de_n * gp.de_split : 0;
+      gp.n_de = gemm_de ? ((plan.DP + GM - 1) / GM) * gp.n_de_n * gp.de_split : 0;
       gp.pstage = pstage;
       gp.gOp = gOp;
       gp.DP = plan.DP;
@@ -1971,7 +1986,7 @@ hipError_t bwd_run(const BwdPlan& plan, const BwdParams& p, hipStream_t stream) 
         const int iters = (gp.n_pack_tiles + H - 1) / H;
         gp.n_pack = iters < 1024 ? iters : 1024;
       }
-      if ((e = dispatch_gemm<T>(plan, gp, stream)) != hipSuccess) return e;
+      if ((e = dispatch_gemm<T>(plan, small, gp, stream)) != hipSuccess) return e;
     }
     if ((p.gE || p.gb) && !fold_red && !kept) {
       timing_begin(kKindBwdReduce, stream);
