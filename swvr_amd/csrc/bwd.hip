@@ -1588,15 +1588,13 @@ __device__ __forceinline__ void gemm_pack_w(const GemmParams& p, int w, char* sm
 // One launch covers the gradient products of a chunk: blocks [0, n_dw) are
 // dW tiles, then n_de dE^T tiles (wide scores kernel only), then dh tiles.
 // The dW and dE^T tiles (reductions over all active positions) are dealt first.
-template <class T, bool SMALL>
-__global__ __launch_bounds__((GemmTile<T, SMALL>::NT)) void bwd_gemm_kernel(GemmParams p) {
-  typedef GemmTile<T, SMALL> G;
+template <class T, class G>
+__device__ __forceinline__ void gemm_workgroup(const GemmParams& p, char* smem) {
   constexpr int kBK = G::BK;
   constexpr int SB = KTile<T, G::GM, kBK, G::NT>::BYTES + RTile<T, G::GN, kBK, G::NT>::BYTES;
   static_assert(KTile<T, G::GM, kBK, G::NT>::BYTES == RTile<T, G::GM, kBK, G::NT>::BYTES,
                 "both A layouts stage the same bytes");
   static_assert(G::NS * SB <= G::LDS_BYTES, "ring fits");
-  __shared__ __attribute__((aligned(1024))) char smem[G::LDS_BYTES];
   int b = blockIdx.x;
   {
     // the dE / db reduction's workgroups, then the next chunk's W packing, follow every GEMM
@@ -1643,6 +1641,17 @@ __global__ __launch_bounds__((GemmTile<T, SMALL>::NT)) void bwd_gemm_kernel(Gemm
       gemm_tile<T, G, false>(p, r * p.n_n + c, smem, run);
     }
   }
+}
+
+template <class T>
+__global__ __launch_bounds__(GemmTile<T>::NT) void bwd_gemm_kernel(GemmParams p) {
+  __shared__ __attribute__((aligned(1024))) char smem[GemmTile<T>::LDS_BYTES];
+  gemm_workgroup<T, GemmTile<T>>(p, smem);
+}
+
+__global__ __launch_bounds__((GemmTile<float, true>::NT)) void bwd_gemm_small_kernel(GemmParams p) {
+  __shared__ __attribute__((aligned(1024))) char smem[GemmTile<float, true>::LDS_BYTES];
+  gemm_workgroup<float, GemmTile<float, true>>(p, smem);
 }
 
 __global__ __launch_bounds__(256) void bwd_reduce_kernel(const float* __restrict__ part_dE,
@@ -1735,11 +1744,11 @@ hipError_t dispatch_gemm(const BwdPlan& plan, bool small, const GemmParams& gp, 
   if (blocks == 0) return hipSuccess;
   if (plan.GM != GemmTile<T>::GM || plan.GN != GemmTile<T>::GN) return hipErrorInvalidValue;
   timing_begin(kKindBwdGemm, stream);
-  if constexpr (sizeof(T) == 4) {
-    static_assert(GemmTile<T, true>::NT == GemmTile<T>::NT, "one count of workgroups");
-    if (small) bwd_gemm_kernel<T, true><<<blocks, GemmTile<T>::NT, 0, stream>>>(gp);
-  }
-  if (!small) bwd_gemm_kernel<T, false><<<blocks, GemmTile<T>::NT, 0, stream>>>(gp);
+  static_assert(GemmTile<float, true>::NT == GemmTile<float>::NT, "one count of the other workgroups");
+  if (small)
+    bwd_gemm_small_kernel<<<blocks, GemmTile<float, true>::NT, 0, stream>>>(gp);
+  else
+    bwd_gemm_kernel<T><<<blocks, GemmTile<T>::NT, 0, stream>>>(gp);
   timing_end(kKindBwdGemm, stream);
   return hipGetLastError();
 }
