@@ -1250,7 +1250,8 @@ int64_t fwd_kept_scores(int dtype, int64_t N, int64_t K, int64_t V, int64_t ldw)
   FwdParams p{};
   p.ldw = ldw;
   const int64_t lds = (int64_t)plan.few_tb * 32 * plan.few_NB, esz = dtype == kF32 ? 4 : 2;
-  return plan.few && few_fits(plan, p, dtype) && lds * 4 <= 2 * K * esz && lds * V * 4 <= kKeptScoresMost ? lds : 0;
+  const bool pays = lds * 4 <= 2 * K * esz || (dtype == kF32 && K >= kKeptScoresK);
+  return plan.few && few_fits(plan, p, dtype) && pays && lds * V * 4 <= kKeptScoresMost ? lds : 0;
 }
 
 hipError_t fwd_launch(int dtype, const FwdPlan& plan, FwdParams p, char* ws, float* O, float* lse, float* m_out,

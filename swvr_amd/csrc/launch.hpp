@@ -122,8 +122,10 @@ hipError_t fwd_launch(int dtype, const FwdPlan& plan, FwdParams p, char* ws, flo
                       float* l_out, hipStream_t stream);
 // Tokens per vocabulary row, with padding, of the scores that a forward without columns keeps (FwdParams::scores) for
 // a backward that then forms no scores, or 0 where it does not: it is the few-token kernel's, of a W stored in the
-// compute dtype, and the scores take at most twice W's bytes and kKeptScoresMost.
-constexpr int64_t kKeptScoresMost = (int64_t)512 << 20;
+// compute dtype, and the scores take at most twice W's bytes and kKeptScoresMost.  In fp32, whose products take 8 times
+// as long, K = kKeptScoresK is enough: 4582 tokens on V = 7190, forward and backward, K = 64 431 us without and 399
+// with them, 128 573 and 494, 512 1491 and 1090; 3000 on 30000, 64 690 and 695, 128 1052 and 947, 512 3474 and 2758.
+constexpr int64_t kKeptScoresMost = (int64_t)512 << 20, kKeptScoresK = 128;
 int64_t fwd_kept_scores(int dtype, int64_t N, int64_t K, int64_t V, int64_t ldw);
 // The forward of the tokens with a non-zero weight (weight: fp32 [N]); O rows
 // and lse of the others are 0.  A zero-weight token whose h row holds an

@@ -54,6 +54,10 @@ def _forward(h, W, bias, teacher, ids, weight, tau, z, reduction, scale, chunk, 
     scores = None
     if need_grad and chunk is None:
         kept_bytes = lib.swvr_distill_scores_size(tag, w_tag, N, Kp, V, _lead_stride(Wc))
+        # a forward that keeps them computes the tokens of weight zero too: not where that costs most (half of 3000
+        # dropped, K = 256, V = 30000: 1079 us without, 1168 with them)
+        if w is not None and kept_bytes > 2 * V * Kp * Wc.element_size():
+            kept_bytes = 0
         scores = hc.new_empty(kept_bytes // 4, dtype=torch.float32) if kept_bytes else None
     ws_bytes = lib.swvr_distill_workspace_size(tag, N, Kp, V, T, w is not None and scores is None)
     ws = hc.new_empty(ws_bytes, dtype=torch.uint8)
@@ -242,7 +246,8 @@ def softmax_distill(h, W, teacher_logits, teacher_ids, bias=None, *, temperature
     products run in autocast's dtype or the promotion of h's and W's (bf16, fp16 or fp32), and the backward
     recomputes the scores ``chunk_size`` vocabulary rows at a time, as ``softmax_readout`` does.  An eager call
     without a chunk keeps the scores of few tokens (up to 768, in fp32 any number) for it instead, where they take
-    at most twice W's bytes (K tokens in the 2-byte types, 2 K in fp32) and 512 MB.  Autograd reaches h, W and
+    at most 512 MB and twice W's bytes (K tokens in the 2-byte types, 2 K in fp32; in fp32 without a weight, any
+    number of tokens from K = 128 on).  Autograd reaches h, W and
     bias; the teacher and the weight get none.  In fp16 the gradients, and the softmax's part of them, fall below the
     type's range where many tokens share a mean: scale the loss, as fp16 training does.
     """

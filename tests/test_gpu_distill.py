@@ -183,6 +183,19 @@ def test_kept_scores(dtype, N, K, V, reduction):
     check(h, W, None, t, ids, reduction=reduction, g=g)
 
 
+@pytest.mark.parametrize("N,K,V", [(1500, 136, 700), (1500, 136, 9001)])
+@pytest.mark.parametrize("weighted", [False, True])
+def test_fp32_scores_of_many_tokens(N, K, V, weighted):
+    """fp32 keeps more of them where no weight may drop tokens; the same gradients either way."""
+    from swvr_amd import _lib
+    assert _lib.load().swvr_distill_scores_size(_lib.F32, _lib.F32, N, K, V, K) == 1536 * V * 4 > 2 * V * K * 4
+    h, W, b, t, ids = make(N, K, V, 5, torch.float32, seed=N)
+    ids[::9] = -1
+    weight = (torch.rand(N, device=DEV, generator=gen(1)) > 0.5).float() if weighted else None
+    check(h, W, b, t, ids, reduction="sum", weight=weight, tau=1.5)
+    check(h, W, b, t, ids, reduction="sum", weight=weight, chunk_size=512)
+
+
 def test_scores_are_kept_only_where_they_are_small():
     from swvr_amd import _lib
     size = lambda *a: _lib.load().swvr_distill_scores_size(*a)
