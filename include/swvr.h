@@ -350,8 +350,8 @@ int swvr_embedding_bwd(int dtype, int id64, int64_t N, int64_t V, int64_t D, con
 /* Bytes of the scores [V][tokens] in fp32 that swvr_distill keeps at `scores` for
  * swvr_distill_bwd, which then needs no product to form them again: for few tokens (those of
  * the one-pass forward) and a W in the compute dtype, where they take at most 512 MB and twice W's bytes
- * (fp32: or K is 128 or more); 0 elsewhere, and then `scores` must be NULL.  With NULL the backward recomputes them.  A call that
- * keeps them sizes its workspace with weighted = 0. */
+ * (fp32: or K is 128 or more); 0 elsewhere, and then `scores` must be NULL.  With NULL the backward
+ * recomputes them.  A call that keeps them sizes its workspace with weighted = 0. */
 size_t swvr_distill_scores_size(int dtype, int w_dtype, int64_t N, int64_t K, int64_t V, int64_t ldw);
 size_t swvr_distill_workspace_size(int dtype, int64_t N, int64_t K, int64_t V, int64_t T, int weighted);
 int swvr_distill(int dtype, int h_dtype, int w_dtype, int64_t N, int64_t K, int64_t V, int64_t T,

@@ -188,7 +188,8 @@ int bwd_common(int dtype, int h_dtype, int w_dtype, int64_t N, int64_t K, int64_
   if (gW && !is_dtype(gW_dtype)) return fail(SWVR_EDTYPE, "unsupported gW dtype tag %d", gW_dtype);
   if (gE && !is_dtype(gE_dtype)) return fail(SWVR_EDTYPE, "unsupported gE dtype tag %d", gE_dtype);
   if (gb && !bias) return fail(SWVR_EINVAL, "gb requested without a bias");
-  if (N > 0 && (!lse || (!glse && !pt_id) || (D > 0 && (!O || !gO)))) return fail(SWVR_EINVAL, "O, lse, gO and glse must be non-null");
+  if (N > 0 && (!lse || (!glse && !pt_id) || (D > 0 && (!O || !gO))))
+    return fail(SWVR_EINVAL, "O, lse, gO and glse must be non-null");
   BwdPlan plan;
   if (!bwd_plan(dtype, N, K, V, D, chunk, gh != nullptr, &plan, w_dtype != dtype, hq ? K8 : 0))
     return fail(SWVR_EDTYPE, "no backward kernel for dtype %d, D=%lld", dtype, (long long)D);
@@ -503,8 +504,8 @@ size_t swvr_distill_workspace_size(int dtype, int64_t N, int64_t K, int64_t V, i
 int swvr_distill(int dtype, int h_dtype, int w_dtype, int64_t N, int64_t K, int64_t V, int64_t T, const void* h,
                  int64_t ldh, const void* W, int64_t ldw, const void* bias, int bias_dtype, float* bias_scaled,
                  float logit_scale, const void* ids, int id64, int64_t ldi, const void* teacher, int t_dtype, int64_t ldt,
-                 float temperature, const float* weight, float z_loss_weight, int reduction, float* out, float* c, float* lse, float* p,
-                 float* q, float* coef, float* scores, void* workspace, size_t workspace_bytes, void* stream) {
+                 float temperature, const float* weight, float z_loss_weight, int reduction, float* out, float* c,
+                 float* lse, float* p, float* q, float* coef, float* scores, void* workspace, size_t workspace_bytes, void* stream) {
   int rc = check_distill(dtype, N, V, T, id64, ids, ldi, temperature, reduction);
   if (rc != SWVR_OK) return rc;
   if (!is_dtype(t_dtype)) return fail(SWVR_EDTYPE, "unsupported teacher dtype tag %d", t_dtype);

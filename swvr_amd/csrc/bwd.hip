@@ -1804,7 +1804,8 @@ hipError_t bwd_run(const BwdPlan& plan, const BwdParams& p, hipStream_t stream) 
     // delta, the active tokens, and the token-side operands over positions
     timing_begin(kKindBwdDelta, stream);
     if (!p.pt_id)
-      bwd_delta_kernel<T><<<(unsigned)(((int64_t)p.N * kDeltaLanes + 255) / 256), 256, 0, stream>>>(p.O, p.gO, p.glse, p.N, p.D, delta, flag);
+      bwd_delta_kernel<T><<<(unsigned)(((int64_t)p.N * kDeltaLanes + 255) / 256), 256, 0, stream>>>(
+          p.O, p.gO, p.glse, p.N, p.D, delta, flag);
     if ((e = compact_tokens(flag, p.N, idx, inv, n_act, stream)) != hipSuccess) return e;
     const int64_t n = (int64_t)plan.N_pad * plan.DP;
     bwd_pack_kernel<T><<<(int)((n + 255) / 256), 256, 0, stream>>>(p.gO, p.lse, delta, idx, n_act, p.D,
