@@ -240,9 +240,9 @@ __global__ __launch_bounds__(256) void distill_prep_kernel(DistillGradParams p) 
     p.delta[n] = -cn;
     p.flag[n] = cn != 0.f;  // NaN != 0
   }
-  // ids as the matrix has them, -1 outside it
+  // ids as the matrix has them, -1 outside it; a dropped token has none, whatever its p holds
   auto id_of = [&](int k) -> int {
-    if (k >= p.T || w == 0.f) return -1;
+    if (k >= p.T || gn == 0.f) return -1;
     const int64_t i = (int64_t)n * p.ldi + k;
     const int64_t id = p.id64 ? static_cast<const int64_t*>(p.ids)[i] : (int64_t)static_cast<const int*>(p.ids)[i];
     return id >= 0 && id < p.V ? (int)id : -1;

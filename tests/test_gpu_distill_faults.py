@@ -1,0 +1,60 @@
+"""softmax_distill where its inputs are at fault: ids outside the vocabulary and NaN must show in the loss and in every
+gradient that their token reaches, and in nothing else."""
+import math
+
+import pytest
+import torch
+
+import swvr_amd
+from swvr_amd import _lib
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+DTYPES = [torch.bfloat16, torch.float16, torch.float32]
+N, K, V, T, BAD = 40, 512, 300, 5, 7
+
+
+def make(dtype, seed=0):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    r = lambda *s, sc=1.0: (sc * torch.randn(*s, device=DEV, generator=g)).to(dtype)
+    ids = torch.randint(0, V, (N, T), device=DEV, generator=g)
+    return r(N, K), r(V, K, sc=2 * K ** -0.5), r(V, sc=0.5), torch.randn(N, T, device=DEV, generator=g), ids
+
+
+def step(h, W, b, t, ids, reduction, g=None, **kw):
+    """(loss, gh, gW, gb) of one call."""
+    xs = [x.detach().requires_grad_(True) for x in (h, W, b)]
+    loss = swvr_amd.softmax_distill(xs[0], xs[1], t, ids, xs[2], reduction=reduction, **kw)
+    return (loss.detach(), *torch.autograd.grad(loss, xs, torch.ones_like(loss) if g is None else g))
+
+
+def spoil(how, t, ids):
+    t, ids = t.clone(), ids.clone()
+    if how == "id":
+        ids[BAD, 2] = V
+    elif how == "id past 32 bits":
+        ids[BAD, 2] = 2 ** 32 + 5          # 5, if it were cut
+    elif how == "improbable id":           # e^-300 is 0 in fp32
+        t[BAD, 2], ids[BAD, 2] = t[BAD].max() - 300, V
+    else:
+        t[BAD, 2] = math.nan
+    return t, ids
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("chunk", [None, 128])
+def test_a_token_at_fault_that_nothing_asks_for(dtype, chunk):
+    """Its term left out of what is differentiated, or its weight zero: the gradients of the others."""
+    h, W, b, t, ids = make(dtype)
+    t2, ids2 = spoil("id", t, ids)
+    t2[BAD, 0] = math.nan
+    keep = torch.ones(N, device=DEV)
+    keep[BAD] = 0
+    want = step(h, W, b, t, ids, "none", g=keep, chunk_size=chunk)
+    got = step(h, W, b, t2, ids2, "none", g=keep, chunk_size=chunk)
+    assert got[0][BAD].isnan()
+    for a, c in zip(got[1:], want[1:]):
+        assert torch.equal(a, c) and torch.isfinite(a).all()
+    for a, c in zip(step(h, W, b, t2, ids2, "mean", weight=keep, chunk_size=chunk),
+                    step(h, W, b, t, ids, "mean", weight=keep, chunk_size=chunk)):
+        assert torch.equal(a, c) and torch.isfinite(a).all()
