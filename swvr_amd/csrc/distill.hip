@@ -18,7 +18,8 @@
 //                         its elements, so the difference is rounded once, not its two terms;
 //   distill_bias_kernel   takes the sums of g_n p off gb, over the entries sorted by id (sort_ids).
 // An entry with a negative id or a logit of -inf is absent; a token without entries, or of weight zero, has
-// loss 0, no share in c and no gradient.  An id of V or more makes its token's loss NaN.
+// loss 0, no share in c and no gradient.  An id of V or more makes its token's loss NaN, and so are the gradients of
+// a token whose divergence is NaN for any reason: coef carries it to them, so that a check of them finds it.
 #include <cfloat>
 
 #include "common.hpp"
@@ -154,6 +155,7 @@ __global__ __launch_bounds__(256) void distill_loss_kernel(DistillParams p, floa
     }
     m = wave_max(m);
     if (w == 0.f || __ballot(has) == 0) w = 0.f;
+    float coef = w;
     if (w != 0.f) {
       auto mass = [&](float t) { return t != kNegInf ? expf(t - m) : 0.f; };
       float sum = mass(mine.t);
@@ -163,7 +165,8 @@ __global__ __launch_bounds__(256) void distill_loss_kernel(DistillParams p, floa
       auto term = [&](const Entry& e, int k, float z) {
         const float logq = e.id >= p.V ? __builtin_nanf("") : e.id >= 0 ? z - lse : kNegInf;
         const float logp = e.t - lp, pk = e.t != kNegInf ? expf(logp) : 0.f;
-        if (pk != 0.f) kl += pk * (logp - logq);  // NaN != 0
+        // (NaN != 0; an id outside the vocabulary shows whatever its probability rounds to)
+        if (pk != 0.f || (e.t != kNegInf && e.id >= p.V)) kl += pk * (logp - logq);
         if (p.p) {
           p.p[(int64_t)n * p.T + k] = pk;
           p.q[(int64_t)n * p.T + k] = e.id >= p.V ? 0.f : expf(logq);
@@ -175,13 +178,14 @@ __global__ __launch_bounds__(256) void distill_loss_kernel(DistillParams p, floa
         term(e, k, e.id >= 0 && e.id < p.V ? p.z[(int64_t)n * p.T + k] : 0.f);
       }
       tok = wave_sum(kl);
+      if (tok != tok) coef = tok;  // the gradients that the token reaches are NaN too
       if (p.zw != 0.f) tok += p.zw * (lse * lse);
       tok *= w;
     } else if (p.p) {
       for (int k = lane; k < p.T; k += 64) p.p[(int64_t)n * p.T + k] = p.q[(int64_t)n * p.T + k] = 0.f;
     }
     if (lane == 0) {
-      if (p.coef) p.coef[n] = w;
+      if (p.coef) p.coef[n] = coef;
       if (p.reduce == 0) p.out[n] = tok;
     }
   }
@@ -231,8 +235,9 @@ __global__ __launch_bounds__(256) void distill_prep_kernel(DistillGradParams p) 
   const int n = blockIdx.x * 4 + wave_id();
   if (n >= p.N) return;
   const int lane = lane_id();
-  const float w = p.coef[n];
-  const float gn = w == 0.f ? 0.f : p.g[p.reduce == 0 ? n : 0] * w * (p.reduce == 0 ? 1.f : p.c[0]);
+  const float w = p.coef[n], g = w == 0.f ? 0.f : p.g[p.reduce == 0 ? n : 0];
+  // a cotangent of zero drops the token, as a weight of zero does, whatever it holds
+  const float gn = g == 0.f ? 0.f : g * w * (p.reduce == 0 ? 1.f : p.c[0]);
   float cn = p.zw != 0.f && w != 0.f ? gn * (1.f + 2.f * p.zw * p.lse[n]) : gn;
   // the backward leaves out tokens of gLSE = 0: one whose two terms cancel stays
   if (cn == 0.f && gn != 0.f) cn = FLT_MIN;

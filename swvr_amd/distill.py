@@ -238,7 +238,8 @@ def softmax_distill(h, W, teacher_logits, teacher_ids, bias=None, *, temperature
     (``teacher_logits`` and integer ``teacher_ids``, both ``[..., T]``), each token contributes
     ``sum_k p_k (log p_k - S[id_k] + LSE)``, plus ``z_loss_weight * LSE^2``.  One entry per token is cross entropy.
     An entry with a negative id or a logit of -inf is absent; ids may repeat.  A token without entries
-    contributes nothing, and an id of V or more makes its token's term NaN.
+    contributes nothing.  An id of V or more makes its token's term NaN, and with it the gradients that the token
+    reaches: its row of h's, all of W's and bias's.
 
     ``weight`` (``[...]``) multiplies each term; a zero drops the token, whatever its inputs hold.  ``reduction``:
     "mean" (the weighted sum over the sum of the weights of the tokens that have an entry; 0 without any),

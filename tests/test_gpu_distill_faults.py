@@ -42,6 +42,25 @@ def spoil(how, t, ids):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("how", ["id", "id past 32 bits", "improbable id", "nan"])
+@pytest.mark.parametrize("reduction", ["none", "sum", "mean"])
+@pytest.mark.parametrize("chunk", [None, 128])   # scores kept, and formed again in three chunks
+def test_a_token_at_fault_shows_in_its_gradients(dtype, how, reduction, chunk):
+    tag = _lib.DTYPE_TAG[dtype]
+    assert _lib.load().swvr_distill_scores_size(tag, tag, N, K, V, K) > 0
+    h, W, b, t, ids = make(dtype)
+    good = step(h, W, b, t, ids, reduction, chunk_size=chunk)
+    loss, gh, gW, gb = step(h, W, b, *spoil(how, t, ids), reduction, chunk_size=chunk)
+    rest = torch.arange(N, device=DEV) != BAD
+    if reduction == "none":
+        assert loss[BAD].isnan() and torch.equal(loss[rest], good[0][rest])
+    else:
+        assert loss.isnan()
+    assert gh[BAD].isnan().all() and torch.equal(gh[rest], good[1][rest])
+    assert gW.isnan().all() and gb.isnan().all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("chunk", [None, 128])
 def test_a_token_at_fault_that_nothing_asks_for(dtype, chunk):
     """Its term left out of what is differentiated, or its weight zero: the gradients of the others."""
