@@ -136,7 +136,7 @@ __global__ __launch_bounds__(256) void distill_loss_kernel(DistillParams p, floa
     auto entry = [&](int k) {
       Entry e;
       e.id = id_at(p, n, k);
-      const float t = load_as(p.teacher, (int64_t)n * p.ldt + k, p.t_dtype) * p.inv_tau;
+      const float t = load_as(p.teacher, (int64_t)n * p.ldt + k, p.t_dtype);
       e.t = e.id < 0 ? kNegInf : t;
       return e;
     };
@@ -157,14 +157,17 @@ __global__ __launch_bounds__(256) void distill_loss_kernel(DistillParams p, floa
     if (w == 0.f || __ballot(has) == 0) w = 0.f;
     float coef = w;
     if (w != 0.f) {
-      auto mass = [&](float t) { return t != kNegInf ? expf(t - m) : 0.f; };
+      // (the distance from the largest before the division: a logit of the type's lowest value stays one at any
+      // temperature, where the quotient would be -inf, an absent entry's)
+      auto below = [&](float t) { return (t - m) * p.inv_tau; };
+      auto mass = [&](float t) { return t != kNegInf ? expf(below(t)) : 0.f; };
       float sum = mass(mine.t);
       for (int k = lane + 64; k < p.T; k += 64) sum += mass(entry(k).t);
-      const float lp = m + logf(wave_sum(sum));
+      const float lp = logf(wave_sum(sum));
       float kl = 0.f;
       auto term = [&](const Entry& e, int k, float z) {
         const float logq = e.id >= p.V ? __builtin_nanf("") : e.id >= 0 ? z - lse : kNegInf;
-        const float logp = e.t - lp, pk = e.t != kNegInf ? expf(logp) : 0.f;
+        const float logp = below(e.t) - lp, pk = e.t != kNegInf ? expf(logp) : 0.f;
         // (NaN != 0; an id outside the vocabulary shows whatever its probability rounds to)
         if (pk != 0.f || (e.t != kNegInf && e.id >= p.V)) kl += pk * (logp - logq);
         if (p.p) {

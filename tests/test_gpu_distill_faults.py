@@ -1,5 +1,6 @@
 """softmax_distill where its inputs are at fault: ids outside the vocabulary and NaN must show in the loss and in every
-gradient that their token reaches, and in nothing else."""
+gradient that their token reaches, and in nothing else; and at the ends of its inputs' ranges, where nothing may be
+lost."""
 import math
 
 import pytest
@@ -7,6 +8,8 @@ import torch
 
 import swvr_amd
 from swvr_amd import _lib
+
+from .test_gpu_distill import close, formula
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -77,3 +80,36 @@ def test_a_token_at_fault_that_nothing_asks_for(dtype, chunk):
     for a, c in zip(step(h, W, b, t2, ids2, "mean", weight=keep, chunk_size=chunk),
                     step(h, W, b, t, ids, "mean", weight=keep, chunk_size=chunk)):
         assert torch.equal(a, c) and torch.isfinite(a).all()
+
+
+@pytest.mark.parametrize("t_dtype", DTYPES)
+@pytest.mark.parametrize("tau", [1.0, 0.5, 0.01])
+@pytest.mark.parametrize("many", [1, 20])       # lists within a wave's 64 entries, and longer ones
+def test_teachers_of_lowest_and_highest_values(t_dtype, tau, many):
+    """Finite logits, however low, are entries: a list of nothing else is uniform at every temperature."""
+    h, W, b, _, ids = make(torch.float32)
+    ids = ids.repeat(1, many)
+    low, top = torch.finfo(t_dtype).min, torch.finfo(t_dtype).max
+    t = torch.zeros(N, T * many, device=DEV, dtype=t_dtype)
+    t[::8] = low
+    t[1::8] = low
+    t[1::8, 3] = 0
+    t[2::8] = top
+    t[3::8, 0], t[3::8, 1:] = top, low
+    t[4::8, ::2], t[4::8, 1::2] = low, -math.inf
+    t[5::8, ::2], t[5::8, 1::2] = -math.inf, top
+    t[6::8] = -math.inf
+    # the softmax's probabilities underflow at low temperatures: those below fp32's smallest normal number, 2^-126, may
+    # come as 0, so an element of dS is off by that much more (its cotangent is 1 or less, its LSE term 0), and a
+    # gradient by the sum of it times what the element is multiplied by
+    f = 2.0 ** -126 / tau
+    floor = dict(h=f * W.double().abs().sum(dim=0), W=f * h.double().abs().sum(dim=0), b=f * N)
+    for reduction in ("none", "mean"):
+        loss, *grads = step(h, W, b, t, ids, reduction, temperature=tau)
+        want, want_g, tol = formula(h, W, b, t, ids, tau=tau, reduction=reduction)
+        close(loss, want, tol["loss"])
+        for name, got in zip("hWb", grads):
+            close(got, want_g[name], tol[name] + floor[name])
+        if reduction == "none":
+            assert (loss[6::8] == 0).all() and (loss[::8] != 0).all()
+        assert (grads[0][6::8] == 0).all() and (grads[0][::8] != 0).any(dim=1).all()
