@@ -336,7 +336,8 @@ int swvr_embedding_bwd(int dtype, int id64, int64_t N, int64_t V, int64_t D, con
  * ids [N,T] (row stride ldi; int64 with id64 = 1, else int32), teacher [N,T] (row
  * stride ldt, t_dtype).  An entry with a negative id or a teacher logit of -inf is
  * absent; a token without entries, or of weight 0, has term 0.  An id of V or
- * more makes its token's term NaN.  Where a token's kl is NaN, coef is, and its cotangent is not zero, its row
+ * more makes its token's term NaN.  temperature is positive, and it and its
+ * reciprocal are at most 3e38.  Where a token's kl is NaN, coef is, and its cotangent is not zero, its row
  * of gh and all of gW and gb are NaN.  Ids may repeat within a token.  weight: fp32
  * [N] or NULL (1).  T is 1 to SWVR_MAX_TEACHER.  h, W as in swvr_fwd_mixed; bias [V] in
  * its own dtype or NULL, and with it bias_scaled [V], which gets bias / temperature.

@@ -482,8 +482,8 @@ static int check_distill(int dtype, int64_t N, int64_t V, int64_t T, int id64, c
   if (id64 != 0 && id64 != 1) return fail(SWVR_EINVAL, "teacher ids are int32 (0) or int64 (1), got %d", id64);
   if (ldi < 0) return fail(SWVR_EINVAL, "ldi=%lld must not be negative", (long long)ldi);
   if (N > 0 && !ids) return fail(SWVR_EINVAL, "teacher ids must be non-null");
-  if (!(temperature > 0.f) || temperature > 3e38f)
-    return fail(SWVR_EINVAL, "temperature must be positive and finite, got %g", (double)temperature);
+  if (!(temperature > 0.f) || temperature > 3e38f || 1.f / temperature > 3e38f)
+    return fail(SWVR_EINVAL, "temperature must be positive, and it and its reciprocal finite, got %g", (double)temperature);
   if (reduction < SWVR_REDUCE_NONE || reduction > SWVR_REDUCE_MEAN)
     return fail(SWVR_EINVAL, "unknown reduction %d", reduction);
   return SWVR_OK;

@@ -222,8 +222,8 @@ def _check(h, W, teacher, ids, bias, weight, temperature, reduction):
     for name, x in (("teacher_logits", teacher), ("weight", weight)):
         if x is not None and x.requires_grad:
             raise ValueError(f"{name} gets no gradient: detach it")
-    if not 0 < temperature < 3e38:
-        raise ValueError(f"temperature must be positive and finite, got {temperature}")
+    if not 4e-39 < temperature < 3e38:  # (its reciprocal is held in fp32 too)
+        raise ValueError(f"temperature must be between 4e-39 and 3e38, got {temperature}")
     if reduction not in REDUCTIONS:
         raise ValueError(f"unknown reduction {reduction!r}")
 
