@@ -152,7 +152,8 @@ def _per_row(x, dtype, R):
         return None
     x = _plain(x).reshape(R)
     if x.dtype != dtype:
-        x = (x.clamp(max=2 ** 31 - 1) if x.dtype == torch.int64 else x).to(dtype)
+        # (top_k: any k of 0 or less is all, and so is one past V, which is below 2^31)
+        x = (x.to(torch.int64).clamp(0, 2 ** 31 - 1) if dtype == torch.int32 else x).to(dtype)
     return x if x.is_contiguous() else x.contiguous()
 
 

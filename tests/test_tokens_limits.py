@@ -5,6 +5,7 @@ import torch
 
 import swvr_amd
 from swvr_amd import _lib
+from swvr_amd.tokens import _per_row
 
 from .test_tokens_host import distill, distill_abi, distill_bwd_abi
 
@@ -25,3 +26,16 @@ def test_temperatures_in_range(tau):
         distill(temperature=tau)
     for fn in (distill_abi, distill_bwd_abi):
         assert fn(tau=tau, nbytes=64) == _lib.EWORKSPACE
+
+
+def test_top_k_of_any_integer_type_keeps_its_meaning():
+    """As the kernels get it, in 32 bits: 0 or less is all, and so is 2^31 - 1, the most that V can be."""
+    most = 2 ** 31 - 1
+    wide = torch.tensor([-2 ** 63, -2 ** 32 + 5, -2 ** 31 - 1, -1, 0, 7, most, 2 ** 31, 2 ** 32 + 5, 2 ** 63 - 1])
+    got = _per_row(wide, torch.int32, 10)
+    assert got.dtype == torch.int32 and got.tolist() == [0, 0, 0, 0, 0, 7, most, most, most, most]
+    assert _per_row(torch.tensor([-5, 0, 200, 32767]).short(), torch.int32, 4).tolist() == [0, 0, 200, 32767]
+    assert _per_row(torch.tensor([255, 3], dtype=torch.uint8), torch.int32, 2).tolist() == [255, 3]
+    for dtype, x in ((torch.uint32, 2 ** 32 - 1), (torch.uint64, 2 ** 32 + 5), (torch.uint64, 2 ** 64 - 1)):
+        got = _per_row(torch.tensor([x, 9], dtype=dtype), torch.int32, 2).tolist()
+        assert got[0] in (0, most) and got[1] == 9, (dtype, x, got)   # all of them, either way
