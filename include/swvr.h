@@ -312,12 +312,13 @@ int swvr_mse_loss_noalloc(int64_t N, int64_t D, const float* O, const float* lse
  * The gradient gE [V,D] (dense, every row written):
  *   gE[v] = scale * sum over n with ids[n] = v of g[n]    g [N,D], row stride ldg >= 0
  * summed in fp32 (fp64) in an order that the ids alone fix, so it is the same on
- * every run.  D and the strides are unrestricted; pointers are aligned to
- * their elements.  N and V are below 2^31.
+ * every run.  The strides are unrestricted; pointers are aligned to
+ * their elements.  N is below 2^31, V and D are at most SWVR_EMBED_MAX.
  * The order comes from sorting the ids, which the lookup can do ahead of the
  * gradient: with sorted (swvr_embedding_sorted_size bytes; 0 for few tokens, whose
  * gradient sorts by itself) it writes the order there, and the gradient of the same
  * ids takes it.  sorted NULL: not written, and the gradient sorts in its workspace. */
+#define SWVR_EMBED_MAX (1 << 30)
 int swvr_embedding(int dtype, int id64, int64_t N, int64_t V, int64_t D, const void* ids,
                    const void* E, int64_t lde, double scale, void* out, int* sorted, void* stream);
 size_t swvr_embedding_sorted_size(int64_t N, int64_t V);

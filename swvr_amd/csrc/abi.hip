@@ -400,12 +400,18 @@ int swvr_bwd(int dtype, int64_t N, int64_t K, int64_t V, int64_t D, const void* 
 }
 
 // ---------------------------------------------------------------- embedding lookup
+// The kernels step over columns and rows of the table in 32 bits, past the last by up to a workgroup's.
+static bool embed_sizes(int64_t N, int64_t V, int64_t D) {
+  return N >= 0 && V >= 0 && D >= 0 && N <= INT32_MAX && V <= SWVR_EMBED_MAX && D <= SWVR_EMBED_MAX;
+}
+
 static int check_embed(int dtype, int id64, int64_t N, int64_t V, int64_t D, const void* ids) {
   g_err[0] = 0;
   if (!is_dtype(dtype) && dtype != SWVR_F64) return fail(SWVR_EDTYPE, "unsupported dtype tag %d", dtype);
   if (id64 != 0 && id64 != 1) return fail(SWVR_EINVAL, "ids are int32 (0) or int64 (1), got %d", id64);
-  if (N < 0 || V < 0 || D < 0 || N > INT32_MAX || V > INT32_MAX - 1 || D > INT32_MAX)
-    return fail(SWVR_EINVAL, "bad sizes N=%lld V=%lld D=%lld", (long long)N, (long long)V, (long long)D);
+  if (!embed_sizes(N, V, D))
+    return fail(SWVR_EINVAL, "bad sizes N=%lld V=%lld D=%lld (N below 2^31, V and D at most 2^30)", (long long)N,
+                (long long)V, (long long)D);
   if (N > 0 && !ids) return fail(SWVR_EINVAL, "ids must be non-null");
   return SWVR_OK;
 }
@@ -434,12 +440,12 @@ int swvr_embedding(int dtype, int id64, int64_t N, int64_t V, int64_t D, const v
 }
 
 size_t swvr_embedding_sorted_size(int64_t N, int64_t V) {
-  if (N < 0 || V < 0 || N > INT32_MAX || V > INT32_MAX - 1) return 0;
+  if (!embed_sizes(N, V, 0)) return 0;
   return swvr::embed_sorted_ints(N, V) * sizeof(int);
 }
 
 size_t swvr_embedding_bwd_workspace_size(int dtype, int64_t N, int64_t V, int64_t D) {
-  if ((!is_dtype(dtype) && dtype != SWVR_F64) || N < 0 || V < 0 || D < 0 || N > INT32_MAX || V > INT32_MAX - 1) return 0;
+  if ((!is_dtype(dtype) && dtype != SWVR_F64) || !embed_sizes(N, V, D)) return 0;
   return swvr::embed_grad_workspace_bytes(dtype, N, V, D);
 }
 

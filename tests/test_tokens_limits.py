@@ -7,7 +7,7 @@ import swvr_amd
 from swvr_amd import _lib
 from swvr_amd.tokens import _per_row
 
-from .test_tokens_host import distill, distill_abi, distill_bwd_abi
+from .test_tokens_host import distill, distill_abi, distill_bwd_abi, embedding, embedding_bwd
 
 
 @pytest.mark.parametrize("tau", [1e-45, 1e-39, 3e-39, 3.2e38])
@@ -39,3 +39,30 @@ def test_top_k_of_any_integer_type_keeps_its_meaning():
     for dtype, x in ((torch.uint32, 2 ** 32 - 1), (torch.uint64, 2 ** 32 + 5), (torch.uint64, 2 ** 64 - 1)):
         got = _per_row(torch.tensor([x, 9], dtype=dtype), torch.int32, 2).tolist()
         assert got[0] in (0, most) and got[1] == 9, (dtype, x, got)   # all of them, either way
+
+
+MOST = 2 ** 30
+
+
+@pytest.mark.parametrize("size", [MOST + 1, 2 ** 31 - 256, 2 ** 31 - 2, 2 ** 31 - 1])
+def test_tables_past_the_kernels_32_bit_steps(size):
+    """Odd widths next to 2^31 would step past it in 32 bits, and the rows' borders too: both are refused."""
+    lib = _lib.load()
+    for fn in (embedding, embedding_bwd):
+        for kw in (dict(D=size, lde=size) if fn is embedding else dict(D=size, ldg=size), dict(V=size)):
+            assert fn(**kw) == _lib.EINVAL and b"bad sizes" in lib.swvr_last_error(), kw
+    assert lib.swvr_embedding_sorted_size(5000, size) == 0
+    for args in ((_lib.BF16, 5000, size, 4), (_lib.BF16, 5000, 4, size)):
+        assert lib.swvr_embedding_bwd_workspace_size(*args) == 0
+
+
+def test_the_largest_tables():
+    """(past the check of the sizes: refused for what is missing)"""
+    lib = _lib.load()
+    assert embedding(V=MOST, E=None) == _lib.EINVAL and b"non-null" in lib.swvr_last_error()
+    assert embedding(D=MOST, lde=MOST, E=None) == _lib.EINVAL and b"non-null" in lib.swvr_last_error()
+    for kw in (dict(V=MOST), dict(D=MOST, ldg=MOST)):
+        assert embedding_bwd(nbytes=16, **kw) == _lib.EWORKSPACE
+    # order, ids and segments; a part in fp32 at each of two ends of 32 (N = 4000: 16) tokens' runs
+    assert lib.swvr_embedding_sorted_size(4000, MOST) == 4 * (2 * 4000 + MOST + 1)
+    assert lib.swvr_embedding_bwd_workspace_size(_lib.BF16, 4000, 4, MOST) >= 250 * 2 * MOST * 4
