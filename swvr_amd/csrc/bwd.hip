@@ -642,7 +642,7 @@ __global__ __launch_bounds__((ScoresTile<T, DP>::NT)) void bwd_scores_kernel(Sco
 //   into an LDS region of its own, and gO and gO^T (16 KB each) share one side
 //   stage, so three slots stay free through the epilogue and the ring carries
 //   the next block's first slices without a pause.
-// The bias sits in registers, LSE / delta in a double-buffered LDS strip.
+// The bias sits in registers, LSE / delta in LDS strips of two (DP = 32: three) blocks.
 template <class T, int DP>
 struct ScoresRingTile {
   static constexpr int BM = 256, BV = 256, WT = 2, WV = 4, NT = 64 * WT * WV, NS = 4;
@@ -670,15 +670,19 @@ __global__ __launch_bounds__(512) void bwd_scores_ring_kernel(ScoresParams p) {
   constexpr bool PIN_E = DP == 32 && !F8;
   static_assert(!PIN_E || (TG::BYTES + TGT::BYTES == SB && TG::NI + TGT::NI == L), "gO | gO^T fill one stage");
   constexpr int N_SIDE = PIN_E ? 1 : 3;  // side stages per token block
+  // LSE / delta strips.  The ring runs NS - 1 = 3 stages ahead of the epilogue where its slots are free (PIN_E); a
+  // block of one K-slice (K <= 32) is two stages, so the strip of the block after next is loaded while this one's is read
+  constexpr int N_LD = PIN_E ? 3 : 2;
+  static_assert(!PIN_E || N_LD * (1 + N_SIDE) > N_SIDE + NS - 1, "no strip is replaced while it is read");
 
   __shared__ __attribute__((aligned(1024)))
-  char smem[NS * SB + 2 * 2 * BM * 4 + (F8 ? BV * 8 : 0) + (PIN_E ? TE::BYTES : 0)];
-  float* const sLD = reinterpret_cast<float*>(smem + NS * SB);  // [2 buffers][LSE BM | delta BM]
+  char smem[NS * SB + N_LD * 2 * BM * 4 + (F8 ? BV * 8 : 0) + (PIN_E ? TE::BYTES : 0)];
+  float* const sLD = reinterpret_cast<float*>(smem + NS * SB);  // [N_LD][LSE BM | delta BM]
   // F8: (bias, score factor) of the tile's rows, read in the epilogue (two fewer registers per
   // row block than holding both); the bf16 kernel holds the bias in registers
-  float2* const sBM = reinterpret_cast<float2*>(smem + NS * SB + 2 * 2 * BM * 4);
+  float2* const sBM = reinterpret_cast<float2*>(smem + NS * SB + N_LD * 2 * BM * 4);
   // PIN_E: the workgroup's E tile
-  char* const sEpin = smem + NS * SB + 2 * 2 * BM * 4;
+  char* const sEpin = smem + NS * SB + N_LD * 2 * BM * 4;
 
   const int lane = lane_id(), w = wave_id();
   const int wt = w / C::WV, wv = w % C::WV;
@@ -733,12 +737,12 @@ __global__ __launch_bounds__(512) void bwd_scores_ring_kernel(ScoresParams p) {
     if (is_sub < nk) {
       if (is_sub == 0) {
         ta.rebase(n0);
-        // LSE and delta of the block into strip (block & 1), ahead of its slices
+        // LSE and delta of the block into its strip, ahead of its slices
         // (offsets recomputed per block, see opaque_zero)
         const int c = (int)threadIdx.x + opaque_zero();
         if (c < BM / 2) {
           const uint32_t off = c < BM / 4 ? (uint32_t)(n0 + 4 * c) * 4 : (uint32_t)(p.N_pad + n0 + 4 * (c - BM / 4)) * 4;
-          dma_batch1(make_rsrc(p.lsed), off, ldsL + (is_blk & 1) * (2 * BM * 4) + w * 1024);
+          dma_batch1(make_rsrc(p.lsed), off, ldsL + (uint32_t)is_blk % N_LD * (2 * BM * 4) + w * 1024);
         }
       }
       ta.issue(st, is_sub * kBK);
@@ -859,7 +863,7 @@ __global__ __launch_bounds__(512) void bwd_scores_ring_kernel(ScoresParams p) {
         const int lr = ln & 31;
         const int vl = wv * WVR + fv * 32 + lr;  // tile-local row of this lane
         const char* sGte = smem + slot_gt * SB + (PIN_E ? TG::BYTES : 0);
-        const float* sLe = sLD + (blk & 1) * (2 * BM);
+        const float* sLe = sLD + (uint32_t)blk % N_LD * (2 * BM);
         const float* sDe = sLe + BM;
         const int tr0 = wt * WTR + ft * 32;  // first token of the block
         float dbs = 0.f;
