@@ -69,9 +69,9 @@ __device__ __forceinline__ void load8(const S* row, float (&v)[8]) {
 // z of IDS entries of a token per wave: h's 8 values of a lane serve them all.  4 where waves are many; 1 with 4 steps
 // of its row in flight where they are few and each waits for its rows (8 tokens, T = 10, K = 4096: 24 -> 6 us).
 template <class T, class HS, class WS, int IDS, int STEPS>
-__global__ __launch_bounds__(256) void distill_dot_kernel(DistillParams p) {
+__global__ __launch_bounds__(256) void distill_dot_kernel(DistillParams p, int64_t b0) {
   const int groups = (p.T + IDS - 1) / IDS;
-  const int64_t gw = (int64_t)blockIdx.x * 4 + wave_id();
+  const int64_t gw = (b0 + blockIdx.x) * 4 + wave_id();
   if (gw >= (int64_t)p.N * groups) return;
   const int n = (int)(gw / groups), k0 = (int)(gw % groups) * IDS;
   if (p.weight && p.weight[n] == 0.f) return;
@@ -330,11 +330,12 @@ template <class T, class HS, class WS>
 hipError_t dot_launch(const DistillParams& p, hipStream_t stream) {
   constexpr int64_t kManyWaves = 4096;
   const int64_t many = (int64_t)p.N * ((p.T + 3) / 4), few = (int64_t)p.N * p.T;
-  if (many >= kManyWaves)
-    distill_dot_kernel<T, HS, WS, 4, 1><<<(unsigned)((many + 3) / 4), 256, 0, stream>>>(p);
-  else
-    distill_dot_kernel<T, HS, WS, 1, 4><<<(unsigned)((few + 3) / 4), 256, 0, stream>>>(p);
-  return hipGetLastError();
+  return launch_in_parts(((many >= kManyWaves ? many : few) + 3) / 4, 256, [&](int64_t b0, unsigned n) {
+    if (many >= kManyWaves)
+      distill_dot_kernel<T, HS, WS, 4, 1><<<n, 256, 0, stream>>>(p, b0);
+    else
+      distill_dot_kernel<T, HS, WS, 1, 4><<<n, 256, 0, stream>>>(p, b0);
+  });
 }
 
 template <class T>

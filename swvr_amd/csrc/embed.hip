@@ -44,10 +44,10 @@ __device__ __forceinline__ int64_t load_id(const void* ids, int id64, int64_t i)
 template <class T, int VB>
 __global__ __launch_bounds__(256) void embed_lookup_kernel(const void* __restrict__ ids, int id64, int64_t N, int V,
                                                            const T* __restrict__ E, int64_t lde, int D, int lpr,
-                                                           double scale, T* __restrict__ out) {
+                                                           double scale, T* __restrict__ out, int64_t b0) {
   typedef Vec<T, VB> X;
   typedef typename SumType<T>::type A;
-  const int64_t n = (int64_t)blockIdx.x * (256 / lpr) + threadIdx.x / lpr;
+  const int64_t n = (b0 + blockIdx.x) * (256 / lpr) + threadIdx.x / lpr;
   if (n >= N) return;
   const int64_t id = load_id(ids, id64, n);
   const int cpr = D / X::n;
@@ -260,13 +260,13 @@ struct EmbedGradKernelParams {
 constexpr int kZeroRows = 16;
 
 template <class T, int VB>
-__global__ __launch_bounds__(256) void embed_sum_kernel(EmbedGradKernelParams p) {
+__global__ __launch_bounds__(256) void embed_sum_kernel(EmbedGradKernelParams p, int b0) {
   typedef Vec<T, VB> X;
   typedef typename SumType<T>::type A;
-  const int cpr = p.D / X::n;
+  const int cpr = p.D / X::n, block = b0 + (int)blockIdx.x;
   T* const gE = static_cast<T*>(p.gE);
-  if ((int)blockIdx.x >= p.n_sum) {
-    const int v0 = (((int)blockIdx.x - p.n_sum) * 4 + wave_id()) * kZeroRows;
+  if (block >= p.n_sum) {
+    const int v0 = ((block - p.n_sum) * 4 + wave_id()) * kZeroRows;
     const int lane = lane_id();
     // the rows' borders once, one lane each
     const int b = v0 + lane <= p.V && lane <= kZeroRows ? p.seg[v0 + lane] : 0;
@@ -286,8 +286,8 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(EmbedGradKernelParams p)
     return;
   }
   const int rpb = 256 / p.lpr;
-  const int64_t run = (int64_t)((int)blockIdx.x / p.n_ct) * rpb + threadIdx.x / p.lpr;
-  const int c = ((int)blockIdx.x % p.n_ct) * p.lpr + threadIdx.x % p.lpr;
+  const int64_t run = (int64_t)(block / p.n_ct) * rpb + threadIdx.x / p.lpr;
+  const int c = (block % p.n_ct) * p.lpr + threadIdx.x % p.lpr;
   const int M = p.seg[p.V];
   const int64_t p0 = run * p.run;
   if (p0 >= M || c >= cpr) return;
@@ -344,16 +344,16 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(EmbedGradKernelParams p)
 // (an id that fills a large share of the tokens), a quarter of its parts each.
 constexpr int kJoinAlone = 16, kJoinCols = 256;
 template <class T>
-__global__ __launch_bounds__(256) void embed_join_kernel(EmbedGradKernelParams p, int n_ct) {
+__global__ __launch_bounds__(256) void embed_join_kernel(EmbedGradKernelParams p, int n_ct, int b0) {
   typedef typename SumType<T>::type A;
   struct alignas(16) A4 {
     A v[4];
   };
   __shared__ int s_last[4];
   __shared__ A4 s_sum[4][64];
-  const int lane = lane_id(), w = wave_id();
-  const int64_t j0 = (int64_t)((int)blockIdx.x / n_ct) * 4;
-  const int d = ((int)blockIdx.x % n_ct) * kJoinCols + 4 * lane;
+  const int lane = lane_id(), w = wave_id(), block = b0 + (int)blockIdx.x;
+  const int64_t j0 = (int64_t)(block / n_ct) * 4;
+  const int d = (block % n_ct) * kJoinCols + 4 * lane;
   const int M = p.seg[p.V];
   const A* const part = static_cast<const A*>(p.part);
   // the sum of the parts of runs a .. b of the segment that begins in run j (parts are dpad wide, a multiple of 8)
@@ -615,10 +615,12 @@ hipError_t embed_lookup_launch(const EmbedParams& p, hipStream_t stream) {
     constexpr int VB = decltype(w)::value;
     const int lpr = lanes_per_row(p.D / (VB / (int)sizeof(T))), rpb = 256 / lpr;
     timing_begin(kKindEmbed, stream);
-    embed_lookup_kernel<T, VB><<<(unsigned)((p.N + rpb - 1) / rpb), 256, 0, stream>>>(
-        p.ids, p.id64, p.N, p.V, static_cast<const T*>(p.E), p.lde, p.D, lpr, p.scale, static_cast<T*>(p.out));
+    const hipError_t e = launch_in_parts((p.N + rpb - 1) / rpb, 256, [&](int64_t b0, unsigned n) {
+      embed_lookup_kernel<T, VB><<<n, 256, 0, stream>>>(p.ids, p.id64, p.N, p.V, static_cast<const T*>(p.E), p.lde, p.D,
+                                                        lpr, p.scale, static_cast<T*>(p.out), b0);
+    });
     timing_end(kKindEmbed, stream);
-    return hipGetLastError();
+    return e;
   });
 }
 
@@ -719,23 +721,27 @@ hipError_t embed_grad_launch(const EmbedParams& p, const int* sorted, char* ws, 
     if (sums + zeros > INT32_MAX) return hipErrorInvalidValue;
     k.n_sum = (int)sums;
     timing_begin(kKindEmbed, stream);
-    embed_sum_kernel<T, VB><<<(unsigned)(sums + zeros), 256, 0, stream>>>(k);
+    const hipError_t launched = launch_in_parts(sums + zeros, 256, [&](int64_t b0, unsigned n) {
+      embed_sum_kernel<T, VB><<<n, 256, 0, stream>>>(k, (int)b0);
+    });
     timing_end(kKindEmbed, stream);
-    return hipGetLastError();
+    return launched;
   });
   if (e != hipSuccess || runs < 2) return e;
   const int n_ct = (p.D + kJoinCols - 1) / kJoinCols;
   const int64_t blocks = (runs + 3) / 4 * n_ct;
   if (blocks > INT32_MAX) return hipErrorInvalidValue;
   timing_begin(kKindEmbed, stream);
-  switch (p.dtype) {
-    case kBF16: embed_join_kernel<bf16_t><<<(unsigned)blocks, 256, 0, stream>>>(k, n_ct); break;
-    case kF16: embed_join_kernel<f16_t><<<(unsigned)blocks, 256, 0, stream>>>(k, n_ct); break;
-    case kF32: embed_join_kernel<float><<<(unsigned)blocks, 256, 0, stream>>>(k, n_ct); break;
-    default: embed_join_kernel<double><<<(unsigned)blocks, 256, 0, stream>>>(k, n_ct); break;
-  }
+  e = launch_in_parts(blocks, 256, [&](int64_t b0, unsigned n) {
+    switch (p.dtype) {
+      case kBF16: embed_join_kernel<bf16_t><<<n, 256, 0, stream>>>(k, n_ct, (int)b0); break;
+      case kF16: embed_join_kernel<f16_t><<<n, 256, 0, stream>>>(k, n_ct, (int)b0); break;
+      case kF32: embed_join_kernel<float><<<n, 256, 0, stream>>>(k, n_ct, (int)b0); break;
+      default: embed_join_kernel<double><<<n, 256, 0, stream>>>(k, n_ct, (int)b0); break;
+    }
+  });
   timing_end(kKindEmbed, stream);
-  return hipGetLastError();
+  return e;
 }
 
 }  // namespace swvr

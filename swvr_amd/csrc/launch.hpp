@@ -397,6 +397,19 @@ void f64_plan(int64_t N, int64_t V, int64_t D, int64_t chunk, int64_t* C, size_t
 hipError_t f64_fwd(const F64Params& p, hipStream_t stream);
 hipError_t f64_bwd(const F64Params& p, hipStream_t stream);
 
+// launch(b0, n) for the workgroups b0 .. b0 + n - 1 of `blocks`, in launches of fewer than the 2^32 threads that a grid
+// holds.
+template <class F>
+hipError_t launch_in_parts(int64_t blocks, int threads, F&& launch) {
+  const int64_t most = ((int64_t)1 << 31) / threads;
+  for (int64_t b0 = 0; b0 < blocks; b0 += most) {
+    launch(b0, (unsigned)(blocks - b0 < most ? blocks - b0 : most));
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
+}
+
 // ---------------------------------------------------------------- embedding lookup
 struct EmbedParams {
   int dtype;           // of E, out, g and gE: 0 bf16, 1 f16, 2 f32, 4 f64

@@ -66,3 +66,9 @@ def test_the_largest_tables():
     # order, ids and segments; a part in fp32 at each of two ends of 32 (N = 4000: 16) tokens' runs
     assert lib.swvr_embedding_sorted_size(4000, MOST) == 4 * (2 * 4000 + MOST + 1)
     assert lib.swvr_embedding_bwd_workspace_size(_lib.BF16, 4000, 4, MOST) >= 250 * 2 * MOST * 4
+
+
+def test_more_tokens_than_a_grid_of_waves():
+    for fn in (distill_abi, distill_bwd_abi):
+        assert fn(N=2 ** 26, T=1) == _lib.EINVAL and b"bad sizes" in _lib.load().swvr_last_error()
+        assert fn(N=2 ** 26 - 1, T=1, nbytes=64) == _lib.EWORKSPACE
