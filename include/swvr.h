@@ -340,7 +340,8 @@ int swvr_embedding_bwd(int dtype, int id64, int64_t N, int64_t V, int64_t D, con
  * more makes its token's term NaN.  temperature is positive, and it and its
  * reciprocal are at most 3e38.  Where a token's kl is NaN, coef is, and its cotangent is not zero, its row
  * of gh and all of gW and gb are NaN.  Ids may repeat within a token.  weight: fp32
- * [N] or NULL (1).  T is 1 to SWVR_MAX_TEACHER, N below 2^26 and N T below 2^31.  h, W as in swvr_fwd_mixed; bias [V] in
+ * [N] or NULL (1).  T is 1 to SWVR_MAX_TEACHER, N below 2^26, N T below
+ * 2^31 and V at most SWVR_EMBED_MAX.  h, W as in swvr_fwd_mixed; bias [V] in
  * its own dtype or NULL, and with it bias_scaled [V], which gets bias / temperature.
  * (bias_scaled == bias is right for an fp32 bias at temperature 1, and nothing is written.)
  * lse [N] is written, c [1] too (not for NONE).  For the gradient: p and q

@@ -484,9 +484,9 @@ static int check_distill(int dtype, int64_t N, int64_t V, int64_t T, int id64, c
   if (!is_dtype(dtype)) return fail(SWVR_EDTYPE, "unsupported operand dtype tag %d", dtype);
   // (a wave for each token: a grid's threads)
   constexpr int64_t kTokensMost = ((int64_t)1 << 26) - 1;
-  if (N < 0 || V < 0 || T < 1 || T > SWVR_MAX_TEACHER || N > kTokensMost || V > INT32_MAX - 1 || N * T > INT32_MAX)
-    return fail(SWVR_EINVAL, "bad sizes N=%lld V=%lld T=%lld (T 1 to %d, N below 2^26, N T below 2^31)", (long long)N,
-                (long long)V, (long long)T, SWVR_MAX_TEACHER);
+  if (N < 0 || V < 0 || T < 1 || T > SWVR_MAX_TEACHER || N > kTokensMost || V > SWVR_EMBED_MAX || N * T > INT32_MAX)
+    return fail(SWVR_EINVAL, "bad sizes N=%lld V=%lld T=%lld (T 1 to %d, N below 2^26, N T below 2^31, V at most 2^30)",
+                (long long)N, (long long)V, (long long)T, SWVR_MAX_TEACHER);
   if (id64 != 0 && id64 != 1) return fail(SWVR_EINVAL, "teacher ids are int32 (0) or int64 (1), got %d", id64);
   if (ldi < 0) return fail(SWVR_EINVAL, "ldi=%lld must not be negative", (long long)ldi);
   if (N > 0 && !ids) return fail(SWVR_EINVAL, "teacher ids must be non-null");
@@ -498,7 +498,7 @@ static int check_distill(int dtype, int64_t N, int64_t V, int64_t T, int id64, c
 }
 
 size_t swvr_distill_scores_size(int dtype, int w_dtype, int64_t N, int64_t K, int64_t V, int64_t ldw) {
-  if (!is_dtype(dtype) || w_dtype != dtype || N <= 0 || K <= 0 || V <= 0 || ldw < K || N > INT32_MAX || V > INT32_MAX)
+  if (!is_dtype(dtype) || w_dtype != dtype || N <= 0 || K <= 0 || V <= 0 || ldw < K || N > INT32_MAX || V > SWVR_EMBED_MAX)
     return 0;
   return (size_t)swvr::fwd_kept_scores(dtype, N, K, V, ldw) * (size_t)V * sizeof(float);
 }

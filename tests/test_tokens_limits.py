@@ -72,3 +72,11 @@ def test_more_tokens_than_a_grid_of_waves():
     for fn in (distill_abi, distill_bwd_abi):
         assert fn(N=2 ** 26, T=1) == _lib.EINVAL and b"bad sizes" in _lib.load().swvr_last_error()
         assert fn(N=2 ** 26 - 1, T=1, nbytes=64) == _lib.EWORKSPACE
+
+
+@pytest.mark.parametrize("V", [MOST + 1, 2 ** 31 - 200, 2 ** 31 - 2])
+def test_vocabularies_past_the_kernels_32_bit_steps(V):
+    for fn in (distill_abi, distill_bwd_abi):
+        assert fn(V=V) == _lib.EINVAL and b"bad sizes" in _lib.load().swvr_last_error()
+        assert fn(V=MOST, nbytes=64) == _lib.EWORKSPACE
+    assert _lib.load().swvr_distill_scores_size(_lib.BF16, _lib.BF16, 1, 2048, V, 2048) == 0
