@@ -4,6 +4,7 @@
 #include <stdio.h>
 #include <string.h>
 
+#include <algorithm>
 #include <cstddef>
 #include <mutex>
 #include <vector>
@@ -129,6 +130,11 @@ int check_storage(int dtype, int h_dtype, int w_dtype) {
   return SWVR_OK;
 }
 
+// A launch of 2^32 threads or more runs the remainder alone, without an error: such sizes are refused.
+int check_threads(int64_t most) {
+  return most + 1024 < ((int64_t)1 << 32) ? SWVR_OK : fail(SWVR_EINVAL, "sizes need a launch of 2^32 threads or more");
+}
+
 int fwd_common(int dtype, int h_dtype, int w_dtype, int64_t N, int64_t K, int64_t V, int64_t D, const void* h,
                int64_t ldh, const void* W, int64_t ldw, const void* E, int64_t lde, const float* bias,
                float logit_scale, float* O, float* lse, float* m_out, float* l_out, void* workspace,
@@ -144,6 +150,9 @@ int fwd_common(int dtype, int h_dtype, int w_dtype, int64_t N, int64_t K, int64_
   if (!fwd_plan(dtype, N, K, V, D, &plan, active))
     return fail(SWVR_EDTYPE, "no forward kernel for dtype %d, D=%lld", dtype, (long long)D);
   if (N == 0) return SWVR_OK;
+  // the merge's 4 columns of a token in a pass of DS, the flags' wave a token
+  if ((rc = check_threads(std::max(N * ((std::min<int64_t>(D, plan.DS) + 3) / 4), active ? 64 * N : 0))) != SWVR_OK)
+    return rc;
   if (!workspace || workspace_bytes < plan.ws_bytes)
     return fail(SWVR_EWORKSPACE, "forward workspace of %zu bytes needed, %zu given", plan.ws_bytes, workspace_bytes);
   FwdParams p{};
@@ -193,6 +202,10 @@ int bwd_common(int dtype, int h_dtype, int w_dtype, int64_t N, int64_t K, int64_
   BwdPlan plan;
   if (!bwd_plan(dtype, N, K, V, D, chunk, gh != nullptr, &plan, w_dtype != dtype, hq ? K8 : 0))
     return fail(SWVR_EDTYPE, "no backward kernel for dtype %d, D=%lld", dtype, (long long)D);
+  // gO's packing, E's, delta's 16 lanes a token, gh's 4 columns
+  if ((rc = check_threads(std::max({plan.N_pad * plan.DP, (int64_t)plan.V_pad * (plan.DP / 8), 16 * N,
+                                    gh ? N * (K / 4) : 0}))) != SWVR_OK)
+    return rc;
   if (N > 0 && (!workspace || workspace_bytes < plan.ws_bytes))
     return fail(SWVR_EWORKSPACE, "backward workspace of %zu bytes needed, %zu given", plan.ws_bytes, workspace_bytes);
   BwdParams p{};
@@ -822,6 +835,7 @@ int swvr_fwd_f64(int64_t N, int64_t K, int64_t V, int64_t D, const double* h, in
   if (rc != SWVR_OK) return rc;
   if (N == 0) return SWVR_OK;
   if (!lse || (D > 0 && !O)) return fail(SWVR_EINVAL, "O and lse must be non-null");
+  if ((rc = check_threads(std::max(256 * N, N * D))) != SWVR_OK) return rc;  // a workgroup a token, its columns
   const size_t need = swvr_fwd_f64_workspace_size(N, V, D, chunk);
   if (!workspace || workspace_bytes < need)
     return fail(SWVR_EWORKSPACE, "fp64 forward workspace of %zu bytes needed, %zu given", need, workspace_bytes);
@@ -866,6 +880,7 @@ int swvr_bwd_f64(int64_t N, int64_t K, int64_t V, int64_t D, const double* h, in
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (N > 0 && (!lse || !glse || (D > 0 && (!O || !gO))))
     return fail(SWVR_EINVAL, "O, lse, gO and glse must be non-null");
+  if ((rc = check_threads(N * std::min(chunk, V))) != SWVR_OK) return rc;  // a chunk's scores
   const size_t need = swvr_bwd_f64_workspace_size(N, V, D, chunk);
   if (N > 0 && (!workspace || workspace_bytes < need))
     return fail(SWVR_EWORKSPACE, "fp64 backward workspace of %zu bytes needed, %zu given", need, workspace_bytes);
@@ -955,6 +970,7 @@ int swvr_mse_loss(int64_t N, int64_t D, const float* O, const float* lse, const 
   g_err[0] = 0;
   if (N < 0 || D < 1) return fail(SWVR_EINVAL, "bad sizes N=%lld D=%lld", (long long)N, (long long)D);
   if (N > INT32_MAX || D > INT32_MAX || N * D > ((int64_t)1 << 40)) return fail(SWVR_EINVAL, "sizes too large");
+  if (const int rc = check_threads(16 * N); rc != SWVR_OK) return rc;  // 16 lanes a token
   if (!is_dtype(target_dtype)) return fail(SWVR_EDTYPE, "unsupported target dtype tag %d", target_dtype);
   if (reduction < SWVR_REDUCE_NONE || reduction > SWVR_REDUCE_MEAN)
     return fail(SWVR_EINVAL, "unknown reduction %d", reduction);
