@@ -139,13 +139,16 @@ def _bwd_op(g: torch.Tensor, h: torch.Tensor, W: torch.Tensor, bias: Optional[to
             kept: torch.Tensor, sb: torch.Tensor, tau: float, z: float, reduction: int, scale: float, chunk: int,
             cdt: torch.dtype, need_h: bool, need_W: bool, need_b: bool) -> List[torch.Tensor]:
     grads = _backward(g, h, W, bias, ids, kept, sb, None, tau, z, reduction, scale, chunk, cdt, need_h, need_W, need_b)
-    # a custom op cannot return None: an empty tensor stands for "no gradient"
-    return [x if x is not None else h.new_empty(0) for x in grads]
+    # a custom op cannot return None: an empty tensor stands for "no gradient" (and dense ones, as traced: h's with
+    # padded rows is a view)
+    return [x.contiguous() if x is not None else h.new_empty(0) for x in grads]
 
 
 @_bwd_op.register_fake
 def _(g, h, W, bias, ids, kept, sb, tau, z, reduction, scale, chunk, cdt, need_h, need_W, need_b):
-    return [torch.empty_like(x) if need else h.new_empty(0) for need, x in ((need_h, h), (need_W, W), (need_b, bias))]
+    # (dense whatever the parameter's layout)
+    return [torch.empty(x.shape, dtype=x.dtype, device=x.device) if need else h.new_empty(0)
+            for need, x in ((need_h, h), (need_W, W), (need_b, bias))]
 
 
 def _setup_context(ctx, inputs, output):
