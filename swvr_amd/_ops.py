@@ -281,14 +281,16 @@ def _bwd_op(gO: torch.Tensor, glse: torch.Tensor, h: torch.Tensor, W: torch.Tens
             need_b: bool) -> List[torch.Tensor]:
     grads = _backward(gO, glse, h, W, E, bias, O, lse, logit_scale, chunk, cdt,
                       need_h, need_W, need_E, need_b)
-    # a custom op cannot return None: an empty tensor stands for "no gradient"
-    return [g if g is not None else h.new_empty(0) for g in grads]
+    # a custom op cannot return None: an empty tensor stands for "no gradient" (and dense ones, as traced: h's with
+    # padded rows is a view)
+    return [g.contiguous() if g is not None else h.new_empty(0) for g in grads]
 
 
 @_bwd_op.register_fake
 def _(gO, glse, h, W, E, bias, O, lse, logit_scale, chunk, cdt, use_triton, need_h, need_W, need_E, need_b):
     like = [(need_h, h), (need_W, W), (need_E, E), (need_b, bias)]
-    return [torch.empty_like(x) if need else h.new_empty(0) for need, x in like]
+    # dense whatever the parameter's layout (x.new_empty is given x's by inductor)
+    return [torch.empty(x.shape, dtype=x.dtype, device=x.device) if need else h.new_empty(0) for need, x in like]
 
 
 def _setup_context(ctx, inputs, output):
