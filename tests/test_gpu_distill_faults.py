@@ -113,3 +113,30 @@ def test_teachers_of_lowest_and_highest_values(t_dtype, tau, many):
         if reduction == "none":
             assert (loss[6::8] == 0).all() and (loss[::8] != 0).all()
         assert (grads[0][6::8] == 0).all() and (grads[0][::8] != 0).any(dim=1).all()
+
+
+@pytest.mark.parametrize("dtype,K", [(torch.bfloat16, 1024), (torch.float16, 1024), (torch.float32, 256)])
+@pytest.mark.parametrize("reduction", ["none", "mean"])
+@pytest.mark.parametrize("chunk", [None, 128])
+def test_dropped_tokens_may_hold_anything_where_scores_are_kept(dtype, K, reduction, chunk):
+    """A forward that keeps the scores computes the dropped tokens' too; token 0, whose scores padding reads, among them."""
+    n, tag = 70, _lib.DTYPE_TAG[dtype]
+    assert _lib.load().swvr_distill_scores_size(tag, tag, n, K, V, K) > 0
+    g = torch.Generator(device=DEV).manual_seed(K)
+    h = torch.randn(n, K, device=DEV, generator=g).to(dtype)
+    W = (2 * K ** -0.5 * torch.randn(V, K, device=DEV, generator=g)).to(dtype)
+    b = torch.randn(V, device=DEV, generator=g).to(dtype)
+    t, ids = torch.randn(n, T, device=DEV, generator=g), torch.randint(0, V, (n, T), device=DEV, generator=g)
+    weight = torch.ones(n, device=DEV)
+    weight[::4] = 0
+    want = step(h, W, b, t, ids, reduction, weight=weight, chunk_size=chunk)
+    h2, t2, ids2 = h.clone(), t.clone(), ids.clone()
+    h2[::8], h2[4::8] = math.nan, math.inf
+    t2[::4], ids2[::4] = math.nan, 10 ** 9
+    for a, c in zip(step(h2, W, b, t2, ids2, reduction, weight=weight, chunk_size=chunk), want):
+        assert torch.equal(a, c) and torch.isfinite(a).all()
+    # dropped by having no entries
+    ids3 = ids2.clone()
+    ids3[::4] = -1
+    for a, c in zip(step(h2, W, b, t2, ids3, reduction, chunk_size=chunk), want):
+        assert torch.equal(a, c)
