@@ -361,6 +361,15 @@ def eager(*tensors):
     return True
 
 
+def no_tangents(*tensors):
+    """Refuse tensors (None allowed) that carry a forward-mode tangent: the custom ops have no rule for it, and without
+    an input that requires a gradient they would drop it in silence."""
+    if forward_ad._current_level >= 0 and not _is_compiling():
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError("swvr_amd: forward-mode derivatives are not supported")
+
+
 def first_order(backward):
     """``once_differentiable`` for the common case too: a backward without ``create_graph`` runs as it is (the
     wrapper's own Python takes 5 us in autograd's thread)."""
@@ -468,6 +477,7 @@ def softmax_readout_op(h2, W, E, bias, logit_scale, chunk, cdt):
     None: the library's choice on an eager call; the ops, whose sizes may be symbols, take 8192."""
     if eager(h2, W, E, bias):
         return _readout_eager(h2, W, E, bias, None, logit_scale, chunk, cdt)
+    no_tangents(h2, W, E, bias)
     chunk = chunk or DEFAULT_CHUNK
     if h2.device.type not in ("cuda", "cpu"):  # meta / fake tracing: no autocast state
         return _fwd_op(h2, W, E, bias, float(logit_scale), int(chunk), cdt, True)
@@ -480,6 +490,7 @@ def softmax_readout_active_op(h2, W, E, bias, weight, logit_scale, chunk, cdt):
     of 0 instead of their readout (``swvr_fwd_active``); ``weight`` is [N], no gradient."""
     if eager(h2, W, E, bias, weight):
         return _readout_eager(h2, W, E, bias, weight, logit_scale, chunk, cdt)
+    no_tangents(h2, W, E, bias)
     chunk = chunk or DEFAULT_CHUNK
     if h2.device.type not in ("cuda", "cpu"):
         return _fwd_active_op(h2, W, E, bias, weight, float(logit_scale), int(chunk), cdt)

@@ -12,7 +12,7 @@ import torch
 
 from . import _lib
 from ._ops import (DEFAULT_CHUNK, REDUCTIONS, _f32, _grad_buffer, _kpad, _lead_stride, _needs_grad, _operand, _plain,
-                   _require_device, _rows_staged, eager, first_order)
+                   _require_device, _rows_staged, eager, first_order, no_tangents)
 from .api import _chunk, _compute_dtype
 
 MAX_TEACHER = 1024
@@ -273,6 +273,7 @@ def softmax_distill(h, W, teacher_logits, teacher_ids, bias=None, *, temperature
         else:
             out = _forward(h2, W, bias, t2, i2, w1, *args, chunk, cdt, False)[0]
     else:
+        no_tangents(h, W, teacher_logits, bias, weight)
         if h.device.type == "cpu":
             _require_device(h)
         if h.device.type == "cuda":

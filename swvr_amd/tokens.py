@@ -14,7 +14,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from ._ops import _plain, _require_device, eager, first_order
+from ._ops import _plain, _require_device, eager, first_order, no_tangents
 
 _EMBED_TAG = {**_lib.DTYPE_TAG, torch.float64: _lib.F64}
 _SORT_FREE = 2048  # tokens up to which the gradient needs neither order nor workspace (their sizes are 0)
@@ -140,6 +140,7 @@ def embedding_lookup(ids, E, *, scale=1.0):
         if E.requires_grad and torch.is_grad_enabled():
             return _Lookup.apply(ids, E, float(scale))
         return _lookup(ids, E, scale)[0]
+    no_tangents(E)
     if E.device.type == "cpu":
         _require_device(E)
     return _lookup_op(ids, E, float(scale))

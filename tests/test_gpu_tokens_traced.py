@@ -75,3 +75,39 @@ def test_lookup_and_sample_compiled_on_any_layout():
     torch._dynamo.reset()
     got = torch.compile(lambda a, c: swvr_amd.sample_tokens(a * 1, c * 1, top_p=0.9), fullgraph=True)(x, u)
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_transforms_are_right_or_refused():
+    """Forward mode finds no rule on the ops, and a tangent is never dropped in silence; vmap calls them item by item."""
+    import torch.autograd.forward_ad as fwd
+    h, W, b, t, ids = make(20, 64, 90, 4, torch.float32)
+    E, at = torch.randn(90, 8, device=DEV), torch.randint(0, 90, (5,), device=DEV)
+    target, u = torch.randn(20, 8, device=DEV), torch.full((90,), 0.5, device=DEV)
+    weight = torch.ones(20, device=DEV)
+    calls = [(lambda x: swvr_amd.softmax_distill(x, W, t, ids, b), h),
+             (lambda x: swvr_amd.softmax_distill(x, W, t, ids, b, reduction="none"), h),
+             (lambda x: swvr_amd.embedding_lookup(at, x), E),
+             (lambda x: swvr_amd.softmax_readout(x, W, E, b)[0], h),
+             (lambda x: swvr_amd.softmax_readout_mse(x, W, E, target, b), h),
+             (lambda x: swvr_amd.softmax_readout_mse(x, W, E, target, b, weight=weight), h)]
+    errors = (RuntimeError, NotImplementedError)
+    for call, x in calls:
+        with fwd.dual_level():
+            for y in (x, x.detach().requires_grad_(True)):
+                with pytest.raises(errors):
+                    call(fwd.make_dual(y, torch.ones_like(y)))
+            call(x)                                        # (a level without a tangent is no matter)
+        with pytest.raises(errors):
+            torch.func.jvp(call, (x,), (torch.ones_like(x),))
+        both = torch.func.vmap(call)(torch.stack([x, x * 2]))
+        for got, y in zip(both, (x, x * 2)):
+            want = call(y)
+            assert torch.allclose(got, want, rtol=1e-5, atol=1e-6)
+    # sampling has no derivative
+    sample = lambda x: swvr_amd.sample_tokens(x, u)
+    with fwd.dual_level():
+        token, logprob = sample(fwd.make_dual(E, torch.ones_like(E)))
+        assert fwd.unpack_dual(logprob).tangent is None
+    assert torch.equal(token, sample(E)[0])
+    tokens, _ = torch.func.vmap(sample)(torch.stack([E, -E]))
+    assert torch.equal(tokens[0], token) and torch.equal(tokens[1], sample(-E)[0])
