@@ -306,14 +306,14 @@ int swvr_mse_loss_noalloc(int64_t N, int64_t D, const float* O, const float* lse
 /* Embedding lookup, the readout of single tokens (no reference counterpart):
  *   out[n] = scale * E[ids[n]]        ids [N] (int64 with id64 = 1, else int32),
  *                                     E [V,D] (row stride lde), out [N,D]
- * in E's dtype (SWVR_BF16, SWVR_F16, SWVR_F32 or SWVR_F64): the product in fp32
- * (fp64), rounded once.  A negative id gives a row of zeros, an id of V or more
+ * in E's dtype (SWVR_BF16, SWVR_F16, SWVR_F32 or SWVR_F64): the product and scale in
+ * fp32 (fp64), rounded to it.  A negative id gives a row of zeros, an id of V or more
  * a row of NaN; neither is read through.
  * The gradient gE [V,D] (dense, every row written):
  *   gE[v] = scale * sum over n with ids[n] = v of g[n]    g [N,D], row stride ldg >= 0
  * summed in fp32 (fp64) in an order that the ids alone fix, so it is the same on
- * every run.  The strides are unrestricted; pointers are aligned to
- * their elements.  N is below 2^31, V and D are at most SWVR_EMBED_MAX.
+ * every run.  lde >= D; pointers are aligned to their elements.  N is below 2^31, V and
+ * D are at most SWVR_EMBED_MAX.
  * The order comes from sorting the ids, which the lookup can do ahead of the
  * gradient: with sorted (swvr_embedding_sorted_size bytes; 0 for few tokens, whose
  * gradient sorts by itself) it writes the order there, and the gradient of the same
@@ -337,13 +337,13 @@ int swvr_embedding_bwd(int dtype, int id64, int64_t N, int64_t V, int64_t D, con
  * ids [N,T] (row stride ldi; int64 with id64 = 1, else int32), teacher [N,T] (row
  * stride ldt, t_dtype).  An entry with a negative id or a teacher logit of -inf is
  * absent; a token without entries, or of weight 0, has term 0.  An id of V or
- * more makes its token's term NaN.  temperature is positive, and it and its
- * reciprocal are at most 3e38.  Where a token's kl is NaN, coef is, and its cotangent is not zero, its row
- * of gh and all of gW and gb are NaN.  Ids may repeat within a token.  weight: fp32
- * [N] or NULL (1).  T is 1 to SWVR_MAX_TEACHER, N below 2^26, N T below
- * 2^31 and V at most SWVR_EMBED_MAX.  h, W as in swvr_fwd_mixed; bias [V] in
- * its own dtype or NULL, and with it bias_scaled [V], which gets bias / temperature.
- * (bias_scaled == bias is right for an fp32 bias at temperature 1, and nothing is written.)
+ * more makes its token's term NaN.  Where a token's kl is NaN, its coef is, and unless its
+ * cotangent is zero its row of gh and all of gW and gb are NaN.  Ids may repeat within a
+ * token.  temperature is positive, and it and its reciprocal are at most 3e38.  weight: fp32
+ * [N] or NULL (1).  T is 1 to SWVR_MAX_TEACHER, N below 2^26, N T below 2^31 and V at most
+ * SWVR_EMBED_MAX.  h, W as in swvr_fwd_mixed; bias [V] in its own dtype or NULL, and with it
+ * bias_scaled [V], which gets bias / temperature.  (bias_scaled == bias is right for an fp32
+ * bias at temperature 1, and nothing is written.)
  * lse [N] is written, c [1] too (not for NONE).  For the gradient: p and q
  * ([N,T], the teacher's and the student's probabilities at the ids) and coef [N]
  * are written (all NULL: no gradient).

@@ -9,7 +9,8 @@
 //   gh = s / tau dS W,   gW = s / tau dS^T h,   gb = colsum(dS) / tau.
 //
 // LSE and the dense part of the gradients are the readout's forward and backward (with no embedding: D = 0,
-// gO = 0, gLSE = c_n), so the [N, V] scores are never in memory.  What is here is the sparse part:
+// gO = 0, gLSE = c_n), so the [N, V] scores are not in memory but where few tokens' are kept from the forward for the
+// backward (fwd_kept_scores).  What is here is the sparse part:
 //   distill_dot_kernel    z at the teacher's ids: dot products of h's row with gathered rows of W in fp32
 //                         (2 N T K flops; bound by the gather, N T rows of W);
 //   distill_loss_kernel   p, the loss's terms and softmax(z) at the ids (one wave per token);
@@ -66,8 +67,10 @@ __device__ __forceinline__ void load8(const S* row, float (&v)[8]) {
   for (int i = 0; i < 8; ++i) v[i] = (float)(T)x[i];
 }
 
-// z of IDS entries of a token per wave: h's 8 values of a lane serve them all.  4 where waves are many; 1 with 4 steps
-// of its row in flight where they are few and each waits for its rows (8 tokens, T = 10, K = 4096: 24 -> 6 us).
+// z of IDS entries of a token per wave: h's 8 values of a lane serve them all.  4 where that leaves kManyWaves waves
+// (with the whole forward, bf16: 4096 tokens, T = 64, K = 256 111 -> 79 us, K = 4096 436 -> 345; 512 tokens, T = 32,
+// K = 4096 83 -> 77); 1 with 4 steps of its row in flight where they are few and each waits for its rows (8 tokens,
+// T = 10, K = 4096: 24 -> 6 us; 500, T = 16, K = 4096, with the forward 74.7 -> 71.8).
 template <class T, class HS, class WS, int IDS, int STEPS>
 __global__ __launch_bounds__(256) void distill_dot_kernel(DistillParams p, int64_t b0) {
   const int groups = (p.T + IDS - 1) / IDS;

@@ -580,8 +580,9 @@ __device__ __forceinline__ u64 row_first(const Staged& p, int64_t q) {
   return wave_max64(first);
 }
 
-// Bin of a key: its distance below the largest in units of 46 log2-steps of weight / kBins (past that, weights are 0),
-// in fp32: no smaller for a smaller logit.
+// Bin of a key: its distance below the largest in units of 46 log2-steps of weight / kBins, in fp32: no smaller for a
+// smaller logit.  The last bin takes everything farther away too: weights of 0, but in rows of up to 65536 logits, whose
+// weights have 46 to 49 bits.
 __device__ __forceinline__ float bin_scale(const Weigh& w) { return (float)(w.to_log2 * (kBins / 46.0)); }
 __device__ __forceinline__ int bin_of(float l, const Weigh& w, float scale) {
   const float x = (w.m_f - l) * scale;

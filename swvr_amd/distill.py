@@ -249,11 +249,11 @@ def softmax_distill(h, W, teacher_logits, teacher_ids, bias=None, *, temperature
     "sum" or "none" (the per-token terms).  The loss is fp32; there is no factor of ``temperature ** 2``.  The
     products run in autocast's dtype or the promotion of h's and W's (bf16, fp16 or fp32), and the backward
     recomputes the scores ``chunk_size`` vocabulary rows at a time, as ``softmax_readout`` does.  An eager call
-    without a chunk keeps the scores of few tokens (up to 768, in fp32 any number) for it instead, where they take
-    at most 512 MB and twice W's bytes (K tokens in the 2-byte types, 2 K in fp32; in fp32 without a weight, any
-    number of tokens from K = 128 on).  Autograd reaches h, W and
-    bias; the teacher and the weight get none.  In fp16 the gradients, and the softmax's part of them, fall below the
-    type's range where many tokens share a mean: scale the loss, as fp16 training does.
+    without a chunk, and with W in the products' dtype (fp32 parameters under autocast are not), keeps the scores of
+    few tokens (up to 768, in fp32 any number) for it instead, where they take at most 512 MB and twice W's bytes (K
+    tokens in the 2-byte types, 2 K in fp32; in fp32 without a weight, any number of tokens from K = 128 on).
+    Autograd reaches h, W and bias; the teacher and the weight get none.  In fp16 the gradients, and the softmax's
+    part of them, fall below the type's range where many tokens share a mean: scale the loss, as fp16 training does.
     """
     _check(h, W, teacher_logits, teacher_ids, bias, weight, temperature, reduction)
     chunk = _chunk(chunk_size)

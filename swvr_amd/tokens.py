@@ -122,11 +122,12 @@ class _Lookup(torch.autograd.Function):
 def embedding_lookup(ids, E, *, scale=1.0):
     """Rows of the embedding table: ``scale * E[ids]``, shape ``ids.shape + (D,)``, in E's dtype.
 
-    ids: integers of any shape; E: ``[V, D]`` (each up to 2^30) in bf16, fp16, fp32 or fp64.  The product is rounded once.  A
-    negative id is padding: a row of zeros, and no share in the gradient.  Nothing can be raised for an id
-    of V or more without waiting for the GPU: its row is NaN.  E's gradient is dense, each row the sum of
-    its tokens' cotangents in fp32 (fp64 for fp64), in an order that depends on the ids alone, so it is the
-    same on every run.
+    ids: integers of any shape; E: ``[V, D]`` (each up to 2^30) in bf16, fp16, fp32 or fp64.  The product is
+    formed in fp32, with scale in fp32 (fp64 for fp64), and rounded to E's dtype.  A negative id is padding: a row
+    of zeros, and no share in the gradient.  Nothing can be raised for an id of V or more without waiting for the
+    GPU: its row is NaN, and no row of the gradient is its.  E's gradient is dense, each row the sum of its
+    tokens' cotangents in fp32 (fp64 for fp64), in an order that depends on the ids alone, so it is the same on
+    every run.
     """
     if E.dim() != 2:
         raise ValueError(f"E must be 2-D, got {tuple(E.shape)}")
