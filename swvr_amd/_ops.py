@@ -577,6 +577,7 @@ _mse_op.register_autograd(_mse_autograd_backward, setup_context=_mse_setup_conte
 def mse_loss_op(O2, lse, target2, weight, z_loss_weight, reduction):
     """Fused loss over ``O2`` [N, D] and ``lse`` [N] (swvr/api.py:53-66); ``reduction`` is
     "none", "sum" or "mean".  Returns the loss ([N] for "none", else a scalar)."""
+    no_tangents(O2, lse, target2, weight)
     need_grad = torch.is_grad_enabled() and (O2.requires_grad or lse.requires_grad)
     out, _, _, _ = _mse_op(O2, lse, target2, weight, float(z_loss_weight), REDUCTIONS[reduction], need_grad)
     return out

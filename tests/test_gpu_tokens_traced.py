@@ -103,6 +103,8 @@ def test_transforms_are_right_or_refused():
         for got, y in zip(both, (x, x * 2)):
             want = call(y)
             assert torch.allclose(got, want, rtol=1e-5, atol=1e-6)
+    with fwd.dual_level(), pytest.raises(errors):          # the loss's target
+        swvr_amd.softmax_readout_mse(h, W, E, fwd.make_dual(target, torch.ones_like(target)), b)
     # sampling has no derivative
     sample = lambda x: swvr_amd.sample_tokens(x, u)
     with fwd.dual_level():
