@@ -395,6 +395,56 @@ int swvr_sample(int dtype, int64_t R, int64_t V, const void* logits, int64_t ld,
                 double top_p, const float* top_p_rows, double min_p, const float* min_p_rows,
                 int64_t* token, float* logprob, void* workspace, size_t workspace_bytes, void* stream);
 
+/* The head in 8-bit integers, no reference counterpart.  Rows x [R,K] are held as
+ *   scale[r] = max(max_k |x[r,k]|, 1e-30) * fl(1/127)   (fp32)
+ *   q[r,k]   = x[r,k] / scale[r] to the nearest whole number, halves to even, by the exact quotient
+ * in an image of swvr_int8_size bytes, whose layout is the library's own (16-byte aligned; K at most
+ * 2^17, R at most 2^30).  A row with an infinity or a NaN has scale NaN and q 0.
+ *   swvr_int8_quantize   image and scales of x in bf16, fp16 or fp32 (row stride ld);
+ *   swvr_int8_pack       the image of integers q [R,K] (row stride ldq) quantised elsewhere;
+ *   swvr_int8_unpack     out [R,K] = scale q in fp32;
+ *   swvr_int8_logits     out[n,v] = logit_scale sh[n] sw[v] sum_k qh[n,k] qw[v,k] + bias[v]
+ *                        [N,V] in out_dtype, h [N,K] quantised so within the call (into the workspace),
+ *                        the sum exact in 32-bit integers, the rest in fp32; bias [V] in bias_dtype or
+ *                        NULL.  N up to 2^24. */
+size_t swvr_int8_size(int64_t R, int64_t K);
+int swvr_int8_quantize(int dtype, int64_t R, int64_t K, const void* x, int64_t ld, void* image, float* scale,
+                       void* stream);
+int swvr_int8_pack(int64_t R, int64_t K, const void* q, int64_t ldq, void* image, void* stream);
+int swvr_int8_unpack(int64_t R, int64_t K, const void* image, const float* scale, float* out, void* stream);
+size_t swvr_int8_logits_workspace_size(int64_t N, int64_t K);
+int swvr_int8_logits(int dtype, int out_dtype, int64_t N, int64_t K, int64_t V, const void* h, int64_t ldh,
+                     const void* w_image, const float* w_scale, const void* bias, int bias_dtype, float logit_scale,
+                     void* out, void* workspace, size_t workspace_bytes, void* stream);
+
+/* A step of beam search over logits [B*W,V] (row stride ld >= 0) of B sequences with W beams each, no reference
+ * counterpart.  scores [B,W] (fp64 with s64 = 1, else fp32) are the beams' sums so far.  Beam w's candidates are
+ * its tokens v with sum = scores[b,w] + logit[v] - logsumexp(logits), or where finished[b,w] (one byte; NULL:
+ * nowhere) is not 0 the one token end_id with sum = scores[b,w].  They are ranked by sum / length^length_penalty,
+ * in fp64: length = lengths[b,w] (int64; NULL: 1 for all), plus 1 for a beam that is not finished, and at least 1.
+ * The k best go out in order (equal ones by beam, then logit, then token): token and parent (the beam) [B,k] int64,
+ * score [B,k] the sum in the type of scores.  NaN and -inf logits are no candidates; a beam with a +inf logit, with
+ * nothing else or with a score that is not finite has none.  Where fewer than k are left: token and parent -1,
+ * score -inf.  W and k up to SWVR_MAX_BEAMS, V up to 2^21, length_penalty 0 to 16. */
+#define SWVR_MAX_BEAMS 256
+size_t swvr_select_beams_workspace_size(int64_t B, int64_t W, int64_t V, int64_t k);
+int swvr_select_beams(int dtype, int64_t B, int64_t W, int64_t V, int64_t k, const void* logits, int64_t ld,
+                      const void* scores, int s64, const uint8_t* finished, int64_t end_id, const int64_t* lengths,
+                      double length_penalty, int64_t* token, int64_t* parent, void* score, void* workspace,
+                      size_t workspace_bytes, void* stream);
+
+/* States by beam: for n states of one geometry dst[i][b,j,...] = src[i][b, parents[b,j], ...], no reference
+ * counterpart.  src and dst are host arrays of n device pointers.  A state is [B, beams, n2, n1] runs of `run`
+ * bytes; element (b, w, x2, x1) begins b strides[0] + w strides[1] + x2 strides[2] + x1 strides[3] bytes into
+ * it (src_strides, dst_strides: host arrays of 4).  parents [B,k] are int64 (id64 = 1) or int32; one outside
+ * 0 .. W - 1 gives zeros.  With dst NULL the states are reordered in place: k = W, at most
+ * SWVR_MAX_BEAMS_IN_PLACE, beams that keep their parent are not touched, and no byte may belong to two
+ * elements or states.  A beam of more than one run is below 2^32 bytes. */
+#define SWVR_MAX_BEAMS_IN_PLACE 64
+int swvr_reorder_beams(int64_t n, const void* const* src, void* const* dst, int64_t B, int64_t W, int64_t k,
+                       const void* parents, int id64, int64_t run, int64_t n1, int64_t n2,
+                       const int64_t* src_strides, const int64_t* dst_strides, void* stream);
+
 /* Matrix-core throughput probe (measurement only; no reference counterpart):
  * `workgroups` workgroups of 8 waves, each wave `iters` steps of a 4 x 2 grid
  * of 32x32x16 bf16 MFMAs (2^18 flops per wave-step) on operands from

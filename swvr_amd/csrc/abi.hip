@@ -64,7 +64,8 @@ const char* kKindNames[kNumKinds] = {"fwd_tile_kernel",   "fwd_combine_kernel", 
                                      "fill_zero_kernel",  "operand_packing",    "bwd_expand_kernel",
                                      "mse_loss",          "quantize_e4m3",      "readout_f64",
                                      "probe_mfma",        "embedding",          "sort_ids",
-                                     "distill",           "sample_tokens"};
+                                     "distill",           "sample_tokens",      "int8_logits",
+                                     "select_beams",      "reorder_beams"};
 
 bool is_dtype(int d) { return d == SWVR_BF16 || d == SWVR_F16 || d == SWVR_F32; }
 
@@ -724,6 +725,213 @@ int swvr_sample(int dtype, int64_t R, int64_t V, const void* logits, int64_t ld,
   p.logprob = logprob;
   hipError_t e = swvr::sample_launch(dtype, p, static_cast<char*>(workspace), static_cast<hipStream_t>(stream));
   if (e != hipSuccess) return hip_fail(e, "sampling launch");
+  return SWVR_OK;
+}
+
+// ---------------------------------------------------------------- 8-bit integers
+static int check_int8(int64_t R, int64_t K) {
+  g_err[0] = 0;
+  if (R < 0 || R > SWVR_EMBED_MAX || K < 1 || K > ((int64_t)1 << 17))
+    return fail(SWVR_EINVAL, "bad sizes of %lld rows of K=%lld (rows at most 2^30, K 1 to 2^17)", (long long)R, (long long)K);
+  return SWVR_OK;
+}
+
+size_t swvr_int8_size(int64_t R, int64_t K) {
+  if (check_int8(R, K) != SWVR_OK) return 0;
+  return (size_t)swvr::int8_image_bytes(R, K);
+}
+
+int swvr_int8_quantize(int dtype, int64_t R, int64_t K, const void* x, int64_t ld, void* image, float* scale,
+                       void* stream) {
+  const int rc = check_int8(R, K);
+  if (rc != SWVR_OK) return rc;
+  if (!is_dtype(dtype)) return fail(SWVR_EDTYPE, "unsupported dtype tag %d", dtype);
+  if (ld < 0) return fail(SWVR_EINVAL, "ld=%lld must not be negative", (long long)ld);
+  if (R == 0) return SWVR_OK;
+  if (!x || !image || !scale || !aligned16(image))
+    return fail(SWVR_EINVAL, "x, image (16-byte aligned) and scale must be non-null");
+  if (reinterpret_cast<uintptr_t>(x) % (dtype == SWVR_F32 ? 4 : 2))
+    return fail(SWVR_EINVAL, "x must be aligned to its elements");
+  const hipError_t e = swvr::int8_quantize(dtype, x, ld, R, K, image, scale, 1, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "int8 quantisation launch");
+  return SWVR_OK;
+}
+
+int swvr_int8_pack(int64_t R, int64_t K, const void* q, int64_t ldq, void* image, void* stream) {
+  const int rc = check_int8(R, K);
+  if (rc != SWVR_OK) return rc;
+  if (ldq < 0) return fail(SWVR_EINVAL, "ldq=%lld must not be negative", (long long)ldq);
+  if (R == 0) return SWVR_OK;
+  if (!q || !image || !aligned16(image)) return fail(SWVR_EINVAL, "q and image (16-byte aligned) must be non-null");
+  const hipError_t e = swvr::int8_pack(q, ldq, R, K, image, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "int8 packing launch");
+  return SWVR_OK;
+}
+
+int swvr_int8_unpack(int64_t R, int64_t K, const void* image, const float* scale, float* out, void* stream) {
+  const int rc = check_int8(R, K);
+  if (rc != SWVR_OK) return rc;
+  if (R == 0) return SWVR_OK;
+  if (!image || !scale || !out || !aligned16(image) || !aligned16(out))
+    return fail(SWVR_EINVAL, "image, out (16-byte aligned) and scale must be non-null");
+  const hipError_t e = swvr::int8_unpack(image, scale, R, K, out, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "int8 unpacking launch");
+  return SWVR_OK;
+}
+
+static size_t int8_scales_bytes(int64_t N) { return up256((size_t)N * sizeof(float)); }
+
+size_t swvr_int8_logits_workspace_size(int64_t N, int64_t K) {
+  if (check_int8(N, K) != SWVR_OK) return 0;
+  return int8_scales_bytes(N) + (size_t)swvr::int8_image_bytes(N, K);
+}
+
+int swvr_int8_logits(int dtype, int out_dtype, int64_t N, int64_t K, int64_t V, const void* h, int64_t ldh,
+                     const void* w_image, const float* w_scale, const void* bias, int bias_dtype, float logit_scale,
+                     void* out, void* workspace, size_t workspace_bytes, void* stream) {
+  int rc = check_int8(N, K);
+  if (rc == SWVR_OK) rc = check_int8(V, K);
+  if (rc != SWVR_OK) return rc;
+  // (tiles of 256 x 256 by 512 threads each: a grid's threads)
+  if (N > ((int64_t)1 << 24) || ((N + 255) / 256) * ((V + 255) / 256) >= ((int64_t)1 << 23))
+    return fail(SWVR_EINVAL, "bad sizes N=%lld V=%lld (N at most 2^24, tiles of 256 x 256 below 2^23)", (long long)N, (long long)V);
+  if (!is_dtype(dtype) || !is_dtype(out_dtype) || (bias && !is_dtype(bias_dtype)))
+    return fail(SWVR_EDTYPE, "unsupported dtype tags %d, %d, %d", dtype, out_dtype, bias_dtype);
+  if (ldh < 0) return fail(SWVR_EINVAL, "ldh=%lld must not be negative", (long long)ldh);
+  if (N == 0 || V == 0) return SWVR_OK;
+  if (!h || !w_image || !w_scale || !out || !aligned16(w_image))
+    return fail(SWVR_EINVAL, "h, the image (16-byte aligned), its scales and out must be non-null");
+  const size_t need = swvr_int8_logits_workspace_size(N, K);
+  if (workspace_bytes < need || !workspace || !aligned16(workspace))
+    return fail(SWVR_EWORKSPACE, "int8 workspace of %zu bytes (16-byte aligned) needed, %zu given", need, workspace_bytes);
+  swvr::Int8Params p{};
+  float* scales = static_cast<float*>(workspace);
+  char* image = static_cast<char*>(workspace) + int8_scales_bytes(N);
+  p.h = image;
+  p.h_scale = scales;
+  p.w = static_cast<const char*>(w_image);
+  p.w_scale = w_scale;
+  p.bias = bias;
+  p.b_dtype = bias_dtype;
+  p.scale = logit_scale;
+  p.N = (int)N;
+  p.V = (int)V;
+  p.S = (int)swvr::int8_slices(K);
+  p.out = out;
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  // (tokens past N are left as they are: their products are not written)
+  hipError_t e = swvr::int8_quantize(dtype, h, ldh, N, K, image, scales, 0, s);
+  if (e == hipSuccess) e = swvr::int8_logits(out_dtype, p, s);
+  if (e != hipSuccess) return hip_fail(e, "int8 logits launch");
+  return SWVR_OK;
+}
+
+// ---------------------------------------------------------------- beams
+static int check_beams(int64_t B, int64_t W, int64_t V, int64_t k) {
+  g_err[0] = 0;
+  if (B < 0 || W < 1 || W > SWVR_MAX_BEAMS || k < 1 || k > SWVR_MAX_BEAMS || V < 1 || V > swvr::kBeamVocabMost)
+    return fail(SWVR_EINVAL, "bad sizes B=%lld W=%lld V=%lld k=%lld (W and k 1 to %d, V 1 to 2^21)", (long long)B,
+                (long long)W, (long long)V, (long long)k, SWVR_MAX_BEAMS);
+  // (a workgroup of 256 threads for 8192 logits)
+  if (B > ((int64_t)1 << 23) || B * W * ((V + 8191) / 8192) >= ((int64_t)1 << 24))
+    return fail(SWVR_EINVAL, "bad sizes B=%lld W=%lld V=%lld: a grid has fewer than 2^32 threads", (long long)B,
+                (long long)W, (long long)V);
+  return SWVR_OK;
+}
+
+size_t swvr_select_beams_workspace_size(int64_t B, int64_t W, int64_t V, int64_t k) {
+  if (check_beams(B, W, V, k) != SWVR_OK) return 0;
+  return swvr::beams_workspace_bytes(B, (int)W, V, (int)k);
+}
+
+int swvr_select_beams(int dtype, int64_t B, int64_t W, int64_t V, int64_t k, const void* logits, int64_t ld,
+                      const void* scores, int s64, const uint8_t* finished, int64_t end_id, const int64_t* lengths,
+                      double length_penalty, int64_t* token, int64_t* parent, void* score, void* workspace,
+                      size_t workspace_bytes, void* stream) {
+  const int rc = check_beams(B, W, V, k);
+  if (rc != SWVR_OK) return rc;
+  if (!is_dtype(dtype)) return fail(SWVR_EDTYPE, "unsupported logits dtype tag %d", dtype);
+  if (ld < 0) return fail(SWVR_EINVAL, "ld=%lld must not be negative", (long long)ld);
+  if (s64 != 0 && s64 != 1) return fail(SWVR_EINVAL, "scores are fp32 (0) or fp64 (1), got %d", s64);
+  if (finished && (end_id < 0 || end_id >= V))
+    return fail(SWVR_EINVAL, "end_id=%lld must be a token of 0 to V - 1", (long long)end_id);
+  if (!(length_penalty >= 0 && length_penalty <= 16))
+    return fail(SWVR_EINVAL, "length_penalty must be between 0 and 16, got %g", length_penalty);
+  if (B == 0) return SWVR_OK;
+  if (!logits || !scores || !token || !parent || !score)
+    return fail(SWVR_EINVAL, "logits, scores, token, parent and score must be non-null");
+  if (reinterpret_cast<uintptr_t>(logits) % (dtype == SWVR_F32 ? 4 : 2))
+    return fail(SWVR_EINVAL, "logits must be aligned to their elements");
+  const size_t need = swvr::beams_workspace_bytes(B, (int)W, V, (int)k);
+  if (workspace_bytes < need || !workspace || reinterpret_cast<uintptr_t>(workspace) % 8)
+    return fail(SWVR_EWORKSPACE, "selection workspace of %zu bytes (8-byte aligned) needed, %zu given", need, workspace_bytes);
+  swvr::BeamParams p{};
+  p.B = B;
+  p.W = (int)W;
+  p.V = V;
+  p.k = (int)k;
+  p.logits = logits;
+  p.ld = ld;
+  p.scores = scores;
+  p.s64 = s64;
+  p.finished = finished;
+  p.end_id = end_id;
+  p.lengths = lengths;
+  p.alpha = length_penalty;
+  p.token = token;
+  p.parent = parent;
+  p.score = score;
+  const hipError_t e = swvr::beams_launch(dtype, p, static_cast<char*>(workspace), static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "beam selection launch");
+  return SWVR_OK;
+}
+
+int swvr_reorder_beams(int64_t n, const void* const* src, void* const* dst, int64_t B, int64_t W, int64_t k,
+                       const void* parents, int id64, int64_t run, int64_t n1, int64_t n2, const int64_t* src_strides,
+                       const int64_t* dst_strides, void* stream) {
+  g_err[0] = 0;
+  constexpr int64_t kMost = (int64_t)1 << 40;
+  if (n < 0 || B < 0 || W < 1 || k < 1 || W > SWVR_MAX_BEAMS || k > SWVR_MAX_BEAMS || run < 0 || n1 < 0 || n2 < 0 ||
+      n > kMost || B > kMost || (double)run * (double)n1 * (double)n2 * (double)B > (double)kMost)
+    return fail(SWVR_EINVAL, "bad sizes n=%lld B=%lld W=%lld k=%lld of %lld x %lld runs of %lld bytes (W and k 1 to %d)",
+                (long long)n, (long long)B, (long long)W, (long long)k, (long long)n2, (long long)n1, (long long)run,
+                SWVR_MAX_BEAMS);
+  if (n1 * n2 > 1 && run * n1 * n2 >= ((int64_t)1 << 32))
+    return fail(SWVR_EINVAL, "states in pieces must have less than 4 GB a beam, got %lld x %lld of %lld bytes", (long long)n2,
+                (long long)n1, (long long)run);
+  if (id64 != 0 && id64 != 1) return fail(SWVR_EINVAL, "parents are int32 (0) or int64 (1), got %d", id64);
+  if (!dst && (k != W || W > SWVR_MAX_BEAMS_IN_PLACE))
+    return fail(SWVR_EINVAL, "in place as many beams come as go, at most %d; got W=%lld k=%lld", SWVR_MAX_BEAMS_IN_PLACE,
+                (long long)W, (long long)k);
+  if (n == 0 || B == 0 || run == 0 || n1 == 0 || n2 == 0) return SWVR_OK;
+  if (!src || !parents || !src_strides || (dst && !dst_strides))
+    return fail(SWVR_EINVAL, "src, parents and the strides must be non-null");
+  for (int64_t i = 0; i < n; ++i)
+    if (!src[i] || (dst && !dst[i])) return fail(SWVR_EINVAL, "state %lld must be non-null", (long long)i);
+  const int64_t* ds = dst ? dst_strides : src_strides;
+  for (int i = 0; i < 4; ++i)
+    if (src_strides[i] < 0 || ds[i] < 0) return fail(SWVR_EINVAL, "strides must not be negative");
+  for (int64_t i0 = 0; i0 < n; i0 += swvr::kReorderStates) {
+    swvr::ReorderParams p{};
+    p.n = (int)std::min<int64_t>(n - i0, swvr::kReorderStates);
+    for (int i = 0; i < p.n; ++i) {
+      p.src[i] = static_cast<const char*>(src[i0 + i]);
+      p.dst[i] = dst ? static_cast<char*>(dst[i0 + i]) : static_cast<char*>(const_cast<void*>(src[i0 + i]));
+    }
+    p.B = B;
+    p.W = (int)W;
+    p.k = (int)k;
+    p.parents = parents;
+    p.id64 = id64;
+    p.in_place = !dst;
+    p.run = run;
+    p.n1 = n1;
+    p.n2 = n2;
+    p.src_b = src_strides[0], p.src_w = src_strides[1], p.src_2 = src_strides[2], p.src_1 = src_strides[3];
+    p.dst_b = ds[0], p.dst_w = ds[1], p.dst_2 = ds[2], p.dst_1 = ds[3];
+    const hipError_t e = swvr::reorder_launch(p, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return hip_fail(e, "reordering launch");
+  }
   return SWVR_OK;
 }
 

@@ -29,6 +29,8 @@ typedef __attribute__((__vector_size__(8 * sizeof(__bf16)))) __bf16 bf16x8_t;
 typedef __attribute__((__vector_size__(8 * sizeof(_Float16)))) _Float16 f16x8_t;
 typedef __attribute__((__vector_size__(8 * sizeof(float)))) float f32x8_t;
 typedef __attribute__((__vector_size__(16 * sizeof(float)))) float f32x16_t;
+typedef int i32x4_t __attribute__((ext_vector_type(4)));
+typedef int i32x16_t __attribute__((ext_vector_type(16)));
 
 enum { kBF16 = 0, kF16 = 1, kF32 = 2, kFP8 = 3, kF64 = 4 };  // kFP8: h, W in OCP e4m3; E in bf16
 
@@ -36,6 +38,7 @@ template <class T> struct Vec8;
 template <> struct Vec8<bf16_t> { typedef bf16x8_t type; };
 template <> struct Vec8<f16_t> { typedef f16x8_t type; };
 template <> struct Vec8<float> { typedef f32x8_t type; };
+template <> struct Vec8<int8_t> { typedef i32x4_t type; };  // 8-bit integers: 16 values per lane, a k32 step
 
 constexpr float kNegInf = -__builtin_huge_valf();
 constexpr float kPosInf = __builtin_huge_valf();
@@ -58,6 +61,10 @@ __device__ __forceinline__ void mfma_k16(f32x16_t& c, f16x8_t a, f16x8_t b) {
 __device__ __forceinline__ void mfma_k16(f32x16_t& c, f32x8_t a, f32x8_t b) {
 #pragma unroll
   for (int t = 0; t < 8; ++t) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[t], b[t], c, 0, 0, 0);
+}
+
+__device__ __forceinline__ void mfma_k16(i32x16_t& c, i32x4_t a, i32x4_t b) {
+  c = __builtin_amdgcn_mfma_i32_32x32x32_i8(a, b, c, 0, 0, 0);
 }
 
 __device__ __forceinline__ f32x16_t zero16() {
@@ -670,8 +677,8 @@ __device__ __forceinline__ void load_step(StepOps<T, FM, FN>& o, const OA& ao, c
   for (int fn = 0; fn < FN; ++fn) o.b[fn] = bo.read(sB, j, fn);
 }
 
-template <class T, int FM, int FN>
-__device__ __forceinline__ void mma_step(f32x16_t (&acc)[FM][FN], const StepOps<T, FM, FN>& o) {
+template <class T, int FM, int FN, class Acc>
+__device__ __forceinline__ void mma_step(Acc (&acc)[FM][FN], const StepOps<T, FM, FN>& o) {
 #pragma unroll
   for (int fm = 0; fm < FM; ++fm)
 #pragma unroll
@@ -684,8 +691,8 @@ __device__ __forceinline__ void mma_step(f32x16_t (&acc)[FM][FN], const StepOps<
 // that uses its predecessor, so only one A operand is double-buffered at a
 // time (register budget) while every read still has at least the rest of the
 // step's MFMAs to land.
-template <class T, int FM, int FN, class OA, class OB>
-__device__ __forceinline__ void mma_load_step(f32x16_t (&acc)[FM][FN], const StepOps<T, FM, FN>& cur,
+template <class T, int FM, int FN, class OA, class OB, class Acc>
+__device__ __forceinline__ void mma_load_step(Acc (&acc)[FM][FN], const StepOps<T, FM, FN>& cur,
                                               StepOps<T, FM, FN>& nxt, const OA& ao, const OB& bo, const char* sA,
                                               const char* sB, int j) {
 #pragma unroll
@@ -727,8 +734,8 @@ struct Ring {
 // current one used (free once the current stage is published), or nothing
 // when the walk has no more.  On return the ring points at the tile's last
 // stage; the caller publishes the next tile's first stage.
-template <class T, int BK, int L, int FM, int FN, class TA, class TB, class R, class F>
-__device__ __forceinline__ void tile_reduce(f32x16_t (&acc)[FM][FN], const TA& ta, const TB& tb, const char* smem,
+template <class T, int BK, int L, int FM, int FN, class Acc, class TA, class TB, class R, class F>
+__device__ __forceinline__ void tile_reduce(Acc (&acc)[FM][FN], const TA& ta, const TB& tb, const char* smem,
                                             int sb, R& ring, int nk, int a_row0, int b_row0, F&& issue_next) {
   constexpr int J = BK / 16;
   OpOffsets<typename TA::Layout, FM, J> ao;
@@ -817,7 +824,6 @@ __device__ __forceinline__ void tile_reduce_multi(f32x16_t (&acc)[FM][FN], const
 }
 
 typedef int i32x8_t __attribute__((ext_vector_type(8)));
-typedef int i32x4_t __attribute__((ext_vector_type(4)));
 
 // 32 bytes of e4m3 operand from two 16-byte reads.
 __device__ __forceinline__ i32x8_t cat16(bf16x8_t lo, bf16x8_t hi) {

@@ -25,6 +25,9 @@ enum KernelKind {
   kKindSortIds,
   kKindDistill,
   kKindSample,
+  kKindInt8,
+  kKindBeams,
+  kKindReorder,
   kNumKinds
 };
 
@@ -512,6 +515,74 @@ struct SampleParams {
 };
 size_t sample_workspace_bytes(int64_t R, int64_t V);
 hipError_t sample_launch(int dtype, SampleParams p, char* ws, hipStream_t stream);
+
+// ---------------------------------------------------------------- 8-bit integers
+// Rows held in integers as the matrix cores take them: for 32 rows and 64 reduction values 2 KB, the 16-byte
+// chunks of values 16c .. 16c + 15 of the 32 rows one after another, c = 0 .. 3.  [rows / 32][K / 64][2048], rows
+// padded to 256 and K to 64, both with zeros.
+constexpr int64_t kInt8Rows = 256, kInt8K = 64, kInt8Block = 2048;
+inline int64_t int8_slices(int64_t K) { return (K + kInt8K - 1) / kInt8K; }
+inline int64_t int8_image_bytes(int64_t R, int64_t K) {
+  return (R + kInt8Rows - 1) / kInt8Rows * (kInt8Rows / 32) * int8_slices(K) * kInt8Block;
+}
+// x [R][ld] -> image and scales [R]; with pad the padding rows are written too.
+hipError_t int8_quantize(int dtype, const void* x, int64_t ld, int64_t R, int64_t K, void* image, float* scale, int pad,
+                         hipStream_t stream);
+hipError_t int8_pack(const void* q, int64_t ld, int64_t R, int64_t K, void* image, hipStream_t stream);
+hipError_t int8_unpack(const void* image, const float* scale, int64_t R, int64_t K, float* out, hipStream_t stream);
+struct Int8Params {
+  const char* h;          // image of N rows
+  const float* h_scale;   // [N]
+  const char* w;          // image of V rows
+  const float* w_scale;   // [V]
+  const void* bias;       // [V], b_dtype, or null
+  int b_dtype;
+  float scale;
+  int N, V, S;            // S: slices of 64 reduction values
+  void* out;              // [N][V]
+  int n_vt, n_tb;         // tiles
+};
+hipError_t int8_logits(int out_dtype, Int8Params p, hipStream_t stream);
+
+// ---------------------------------------------------------------- beams
+struct BeamParams {
+  int64_t B;               // sequences
+  int W;                   // beams
+  int64_t V;
+  int k;
+  const void* logits;      // [B W][ld]
+  int64_t ld;
+  const void* scores;      // [B][W] fp64 (s64) or fp32
+  int s64;
+  const uint8_t* finished; // [B][W] or null
+  int64_t end_id;
+  const int64_t* lengths;  // [B][W] or null
+  double alpha;
+  int64_t* token;          // [B][k]
+  int64_t* parent;         // [B][k]
+  void* score;             // [B][k], as scores
+};
+constexpr int kBeamsMost = 256;             // beams, and candidates kept
+constexpr int64_t kBeamVocabMost = (int64_t)1 << 21;
+size_t beams_workspace_bytes(int64_t B, int W, int64_t V, int k);
+hipError_t beams_launch(int dtype, const BeamParams& p, char* ws, hipStream_t stream);
+
+// States by beam: state i of sequence b and beam w at src[i] + b src_b + w src_w, n1 x n2 runs of `run` bytes at
+// strides src_1, src_2; all strides in bytes.
+constexpr int kReorderStates = 64, kReorderInPlace = 64;
+struct ReorderParams {
+  const char* src[kReorderStates];
+  char* dst[kReorderStates];
+  int n;                   // states
+  int64_t B;
+  int W, k;
+  const void* parents;     // [B][k] int64 (id64) or int32
+  int id64;
+  int in_place;            // src is dst, and W is k
+  int64_t run, n1, n2;
+  int64_t src_b, src_w, src_1, src_2, dst_b, dst_w, dst_1, dst_2;
+};
+hipError_t reorder_launch(const ReorderParams& p, hipStream_t stream);
 
 // Matrix-core throughput probe (probe.hip): workgroups of 8 waves, iters k16 steps of
 // 8 MFMAs per wave; out receives workgroups * 512 floats.
