@@ -863,8 +863,8 @@ int swvr_select_beams(int dtype, int64_t B, int64_t W, int64_t V, int64_t k, con
   if (reinterpret_cast<uintptr_t>(logits) % (dtype == SWVR_F32 ? 4 : 2))
     return fail(SWVR_EINVAL, "logits must be aligned to their elements");
   const size_t need = swvr::beams_workspace_bytes(B, (int)W, V, (int)k);
-  if (workspace_bytes < need || !workspace || reinterpret_cast<uintptr_t>(workspace) % 8)
-    return fail(SWVR_EWORKSPACE, "selection workspace of %zu bytes (8-byte aligned) needed, %zu given", need, workspace_bytes);
+  if (workspace_bytes < need || !workspace || !aligned16(workspace))
+    return fail(SWVR_EWORKSPACE, "selection workspace of %zu bytes (16-byte aligned) needed, %zu given", need, workspace_bytes);
   swvr::BeamParams p{};
   p.B = B;
   p.W = (int)W;

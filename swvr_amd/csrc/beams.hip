@@ -8,12 +8,13 @@
 // 1.1e-12 of itself and an lse by less, where fp32's 1e-7 would swap a pair in one of a few thousand steps.  What is
 // summed in which order depends on V alone: the same beams have the same sums wherever they stand.
 //
-// Three launches:
-//   beam_scan_kernel   reads the logits once: per sub-block of kSub (a wave) the maximum and the sum of exponentials
-//                      relative to it, per group of 64 or 512 consecutive logits its maximum;
+// Launches:
+//   beam_scan_kernel   reads the logits once: per group of 128 its maximum, per sub-block of 2048 (a wave) its own and
+//                      the sum of exponentials relative to it;
 //   beam_row_kernel    per beam the lse, and its own k best: they lie in the k groups of the largest maxima (equal ones
 //                      by index), which alone are read again;
-//   beam_merge_kernel  per sequence the best of its beams' lists.
+//   beam_merge_kernel  per sequence the best of its beams' lists;
+// the last two in one, a workgroup per sequence (beam_pick_kernel), for up to 16 beams and 64 candidates.
 #include <algorithm>
 
 #include "common.hpp"
@@ -24,16 +25,15 @@ namespace swvr {
 
 namespace {
 
-constexpr int kSub = 2048, kLane = 8, kSteps = kSub / (64 * kLane);
-constexpr int kScanWaves = 4, kGroupsMost = 4096, kListMost = 4096;
-constexpr int64_t kSmallGroups = (int64_t)kGroupsMost * 64;  // V up to which groups have 64 logits
+constexpr int kGroup = 128, kLane = 8, kStep = 64 * kLane, kSteps = 4, kSub = kSteps * kStep, kSubGroups = kSub / kGroup;
+constexpr int kScanWaves = 4, kGroupsMost = (int)(kBeamVocabMost / kGroup), kListMost = 4096;
 
 struct BeamWork {
   BeamParams a;
-  int n_sub, n_seg, gshift, n_group;
+  int n_sub, n_seg, n_group;
+  float* group;      // [rows][n_group] maxima, n_group = kSubGroups n_sub
   float* sub_max;    // [rows][n_sub]
   double* sub_sum;   // [rows][n_sub]
-  float* group;      // [rows][n_group]
   double* rank;      // [rows][k]
   double* sum;       // [rows][k]
   int* token;        // [rows][k]
@@ -63,20 +63,21 @@ __device__ __forceinline__ double exp_rel(float x, double m) {
   p = fma(p, f, 0.2402265069581299);
   p = fma(p, f, 0.6931471805459335);
   p = fma(p, f, 1.0);
-  return __longlong_as_double(__double_as_longlong(p) + ((long long)(int)__double_as_longlong(y) << 52));
+  // (on the high word alone: a 64-bit shift and addition are two instructions for one)
+  return __hiloint2double(__double2hiint(p) + (__double2loint(y) << 20), __double2loint(p));
 }
 
 template <int CTRL>
 __device__ __forceinline__ float dpp_max(float x) {
   return fmaxf(x, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, true)));
 }
-// Maximum over groups of 8 lanes (quad_perm 1 0 3 2, 2 3 0 1, row_half_mirror), and over the wave.
+// Maximum over groups of 8 lanes (quad_perm 1 0 3 2, 2 3 0 1, row_half_mirror), and over the wave (x8: max8's).
 __device__ __forceinline__ float max8(float x) {
   x = dpp_max<0xB1>(x);
   x = dpp_max<0x4E>(x);
   return dpp_max<0x141>(x);
 }
-__device__ __forceinline__ float max64(float x8) {  // x8: max8's
+__device__ __forceinline__ float max64(float x8) {
   x8 = dpp_max<0x140>(x8);  // row_mirror
   float m = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x8), 0));
   m = fmaxf(m, __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x8), 16)));
@@ -84,11 +85,23 @@ __device__ __forceinline__ float max64(float x8) {  // x8: max8's
   return fmaxf(m, __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x8), 48)));
 }
 
-// kLane consecutive logits from any element on (rows begin anywhere where V is odd).
+// kLane consecutive logits from any element on (rows begin anywhere where V is odd), -inf past the row's end.
 template <class T>
-struct __attribute__((packed, aligned(sizeof(T)))) LaneLogits {
-  T v[kLane];
-};
+using Logits = typename Vec8<T>::type;
+static_assert(kLane == 8, "a vector of 8 a lane");
+template <class T>
+__device__ __forceinline__ Logits<T> whole_logits(const T* x) {
+  typedef Logits<T> __attribute__((aligned(sizeof(T)))) Unaligned;
+  return *reinterpret_cast<const Unaligned*>(x);
+}
+template <class T>
+__device__ __forceinline__ Logits<T> load_logits(const T* x, int64_t i, int64_t V) {
+  if (i + kLane <= V) return whole_logits(x + i);
+  Logits<T> c;
+#pragma unroll
+  for (int u = 0; u < kLane; ++u) c[u] = i + u < V ? x[i + u] : (T)kNegInf;
+  return c;
+}
 
 template <class T>
 __global__ __launch_bounds__(64 * kScanWaves) void beam_scan_kernel(BeamWork p) {
@@ -98,35 +111,26 @@ __global__ __launch_bounds__(64 * kScanWaves) void beam_scan_kernel(BeamWork p) 
   if ((p.a.finished && p.a.finished[row]) || !alive(score_of(p.a, row))) return;
   const T* const x = static_cast<const T*>(p.a.logits) + row * p.a.ld;
   const int64_t i0 = (int64_t)sub * kSub + lane_id() * kLane, V = p.a.V;
-  float l[kSteps][kLane];
-  LaneLogits<T> c[kSteps];
+  Logits<T> c[kSteps];
+  if ((int64_t)(sub + 1) * kSub <= V) {  // (the whole wave's: all loads go out before the first is waited for)
 #pragma unroll
-  for (int j = 0; j < kSteps; ++j)
-    if (i0 + j * 64 * kLane + kLane <= V) c[j] = *reinterpret_cast<const LaneLogits<T>*>(x + i0 + j * 64 * kLane);
-  float m = kNegInf;
+    for (int j = 0; j < kSteps; ++j) c[j] = whole_logits(x + i0 + j * kStep);
+  } else {
+#pragma unroll
+    for (int j = 0; j < kSteps; ++j) c[j] = load_logits(x, i0 + j * kStep, V);
+  }
+  float m = kNegInf, mine = kNegInf;  // mine: of the group of 16 lanes in step lane % 16
+  float l[kSteps][kLane];
 #pragma unroll
   for (int j = 0; j < kSteps; ++j) {
-    const int64_t i = i0 + j * 64 * kLane;
-    if (i + kLane <= V) {
 #pragma unroll
-      for (int u = 0; u < kLane; ++u) l[j][u] = (float)c[j].v[u];
-    } else {
-#pragma unroll
-      for (int u = 0; u < kLane; ++u) l[j][u] = i + u < V ? (float)x[i + u] : kNegInf;
-    }
+    for (int u = 0; u < kLane; ++u) l[j][u] = (float)c[j][u];
     float k = kNegInf;
 #pragma unroll
     for (int u = 0; u < kLane; ++u) k = fmaxf(k, l[j][u]);  // (NaN: the other)
-    k = max8(k);
-    const int64_t g = (i0 - lane_id() * kLane + j * 64 * kLane) >> 6;  // first group of 64 of this step
-    if (p.gshift == 6) {
-      if ((lane_id() & 7) == 0 && g + lane_id() / 8 < p.n_group) p.group[row * p.n_group + g + lane_id() / 8] = k;
-      m = fmaxf(m, k);
-    } else {
-      const float k64 = max64(k);
-      if (lane_id() == 0 && (g >> 3) < p.n_group) p.group[row * p.n_group + (g >> 3)] = k64;
-      m = fmaxf(m, k64);
-    }
+    k = dpp_max<0x140>(max8(k));  // (row_mirror)
+    mine = (lane_id() & 15) == j ? k : mine;
+    m = fmaxf(m, k);
   }
   m = max64(m);
   const double by = m > kNegInf && m < kPosInf ? (double)m : 0.0;
@@ -137,34 +141,40 @@ __global__ __launch_bounds__(64 * kScanWaves) void beam_scan_kernel(BeamWork p) 
     for (int u = 0; u < kLane; ++u) sum += exp_rel(l[j][u], by);
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+  static_assert(kGroup == 16 * kLane, "a group is 16 lanes' logits of a step");
+  if ((lane_id() & 15) < kSteps)
+    p.group[row * p.n_group + sub * kSubGroups + (lane_id() & 15) * 4 + lane_id() / 16] = mine;
   if (lane_id() == 0) {
     p.sub_max[row * p.n_sub + sub] = m;
     p.sub_sum[row * p.n_sub + sub] = sum;
   }
 }
 
-// How many of s[0 .. n - 1] (n padded with zeros to a multiple of 4) are larger than x.
+// How many of s[0 .. n - 1] (n padded with zeros to a multiple of kPad) are larger than x.
+constexpr int kPad = 8;
 __device__ __forceinline__ int above(const u64* s, int n, u64 x) {
   int c = 0;
-  for (int i = 0; i < n; i += 4) {
+#pragma unroll 1
+  for (int i = 0; i < n; i += kPad) {
 #pragma unroll
-    for (int u = 0; u < 4; ++u) c += s[i + u] > x;
+    for (int u = 0; u < kPad; ++u) c += s[i + u] > x;
   }
   return c;
 }
 
 constexpr int kRowThreads = 256;
 
-// lengths of 0 count as 1
-__device__ __forceinline__ double divisor(const BeamParams& a, int64_t row, int more) {
-  if (!a.lengths || a.alpha == 0) return 1.0;
-  const int64_t n = a.lengths[row] + more;
-  return pow((double)(n > 1 ? n : 1), a.alpha);
+// What a candidate's sum is divided by (lengths of 0 count as 1).
+__device__ __forceinline__ int64_t length_of(const BeamParams& a, int64_t row, int more) { return a.lengths[row] + more; }
+__device__ __forceinline__ double divisor(const BeamParams& a, int64_t length) {
+  return pow((double)(length > 1 ? length : 1), a.alpha);
 }
+__device__ __forceinline__ bool divides(const BeamParams& a) { return a.lengths && a.alpha != 0; }
 
 template <class T>
 __global__ __launch_bounds__(kRowThreads) void beam_row_kernel(BeamWork p) {
-  __shared__ u64 s_best[kRowThreads], s_list[kListMost + 4];
+  __shared__ __attribute__((aligned(16))) u64 s_best[kRowThreads], s_list[kListMost + kPad];
+  __shared__ u64 s_order[kBeamsMost];
   __shared__ int s_group[kBeamsMost];
   __shared__ double s_sum[kRowThreads / 64];
   __shared__ float s_max[kRowThreads / 64];
@@ -182,7 +192,7 @@ __global__ __launch_bounds__(kRowThreads) void beam_row_kernel(BeamWork p) {
   }
   if (p.a.finished && p.a.finished[row]) {
     if (t == 0) {
-      rank[0] = score / divisor(p.a, row, 0);
+      rank[0] = divides(p.a) ? score / divisor(p.a, length_of(p.a, row, 0)) : score;
       sums[0] = score;
       tokens[0] = (int)p.a.end_id;
       p.count[row] = 1;
@@ -190,11 +200,11 @@ __global__ __launch_bounds__(kRowThreads) void beam_row_kernel(BeamWork p) {
     return;
   }
   // ---- lse, in an order of V alone
+  const float* const group = p.group + row * p.n_group;
   float m = kNegInf;
   for (int i = t; i < p.n_sub; i += kRowThreads) m = fmaxf(m, p.sub_max[row * p.n_sub + i]);
   m = max64(max8(m));
   if (lane_id() == 0) s_max[wave_id()] = m;
-  if (t == 0) s_n = 0;
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < kRowThreads / 64; ++i) m = fmaxf(m, s_max[i]);
@@ -210,102 +220,80 @@ __global__ __launch_bounds__(kRowThreads) void beam_row_kernel(BeamWork p) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
   if (lane_id() == 0) s_sum[wave_id()] = sum;
-  // ---- a bound that k groups reach: the k-th of the threads' best
-  constexpr int kPer = kGroupsMost / kRowThreads;
-  u64 mine[kPer], best = 0;
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const int g = i * kRowThreads + t;
-    mine[i] = g < p.n_group ? place_of(key_of(p.group[row * p.n_group + g]), g) : 0;
-    best = mine[i] > best ? mine[i] : best;
-  }
-  s_best[t] = best;
-  if (t == 0) s_bound = 1;
-  __syncthreads();
-  const double rest = log(s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3]);  // lse - m
-  if (best && above(s_best, kRowThreads, best) == k - 1) s_bound = best;
-  __syncthreads();
-  u64 bound = s_bound;
-#pragma unroll
-  for (int i = 0; i < kPer; ++i)
-    if (mine[i] >= bound) s_list[atomicAdd(&s_n, 1)] = mine[i];
-  __syncthreads();
-  const int n1 = s_n;
-  if (t < 4) s_list[n1 + t] = 0;
-  __syncthreads();
-  for (int i = t; i < n1; i += kRowThreads) {
-    const u64 x = s_list[i];
-    const int r = above(s_list, n1, x);
-    if (r < k) s_group[r] = (int)index_at(x);
-  }
-  // ---- the same among the logits of the k first groups
-  const int groups = n1 < k ? n1 : k, logits = groups << p.gshift;
-  const T* const x = static_cast<const T*>(p.a.logits) + row * p.a.ld;
-  auto place = [&](int i) -> u64 {
-    const int64_t v = ((int64_t)s_group[i >> p.gshift] << p.gshift) + (i & ((1 << p.gshift) - 1));
-    return v < p.a.V ? place_of(key_of((float)x[v]), v) : 0;
-  };
-  __syncthreads();
-  best = 0;
-  for (int i = t; i < logits; i += kRowThreads) {
-    const u64 y = place(i);
-    best = y > best ? y : best;
-  }
-  s_best[t] = best;
-  if (t == 0) {
-    s_bound = 1;
-    s_n = 0;
-  }
-  __syncthreads();
-  if (best && above(s_best, kRowThreads, best) == k - 1) s_bound = best;
-  __syncthreads();
-  bound = s_bound;
-  for (int i = t; i < logits; i += kRowThreads) {
-    const u64 y = place(i);
-    if (y >= bound) {
+  // The k first of n entries place(i), in order, to s_list; how many.  A bound that k of them reach (the k-th of the
+  // threads' best), the few that reach it, and of these the places; where they are too many for the list (many large
+  // ones with few threads) a round of maxima for each.
+  auto first = [&](int n, auto&& place) -> int {
+    u64 best = 0;
+    for (int i = t; i < n; i += kRowThreads) {
+      const u64 x = place(i);
+      best = x > best ? x : best;
+    }
+    __syncthreads();
+    s_best[t] = best;
+    if (t == 0) {
+      s_bound = 1;
+      s_n = 0;
+    }
+    __syncthreads();
+    if (best && above(s_best, kRowThreads, best) == k - 1) s_bound = best;
+    __syncthreads();
+    for (int i = t; i < n; i += kRowThreads) {
+      const u64 x = place(i);
+      if (x < s_bound) continue;
       const int at = atomicAdd(&s_n, 1);
-      if (at < kListMost) s_list[at] = y;
+      if (at < kListMost) s_list[at] = x;
     }
-  }
-  __syncthreads();
-  int n2 = s_n;
-  if (n2 > kListMost) {
-    // (many large logits with few threads: one round of maxima for each token)
-    u64 last = ~0ull;
-    n2 = 0;
-    for (int r = 0; r < k; ++r) {
-      best = 0;
-      for (int i = t; i < logits; i += kRowThreads) {
-        const u64 y = place(i);
-        best = y < last && y > best ? y : best;
-      }
-      best = wave_max64(best);
-      __syncthreads();
-      if (lane_id() == 0) s_best[wave_id()] = best;
-      __syncthreads();
+    __syncthreads();
+    int found = s_n;
+    if (found > kListMost) {
+      u64 last = ~0ull;
+      for (found = 0; found < k; ++found) {
+        best = 0;
+        for (int i = t; i < n; i += kRowThreads) {
+          const u64 x = place(i);
+          best = x < last && x > best ? x : best;
+        }
+        best = wave_max64(best);
+        __syncthreads();
+        if (lane_id() == 0) s_best[wave_id()] = best;
+        __syncthreads();
 #pragma unroll
-      for (int i = 0; i < kRowThreads / 64; ++i) best = s_best[i] > best ? s_best[i] : best;
-      if (best == 0) break;
-      if (t == 0) s_list[r] = best;
-      last = best;
-      n2 = r + 1;
+        for (int i = 0; i < kRowThreads / 64; ++i) best = s_best[i] > best ? s_best[i] : best;
+        if (best == 0) break;
+        if (t == 0) s_list[found] = best;
+        last = best;
+      }
     }
-  }
-  __syncthreads();
-  if (t < 4) s_list[n2 + t] = 0;
-  __syncthreads();
-  const double by = divisor(p.a, row, 1);
-  for (int i = t; i < n2; i += kRowThreads) {
-    const u64 y = s_list[i];
-    const int r = above(s_list, n2, y);
-    if (r < k) {
-      const double s = score + (((double)logit_of(key_at(y)) - (double)m) - rest);
-      rank[r] = s / by;
-      sums[r] = s;
-      tokens[r] = (int)index_at(y);
+    __syncthreads();
+    if (t < kPad) s_list[found + t] = 0;
+    __syncthreads();
+    for (int i = t; i < found; i += kRowThreads) {
+      const u64 x = s_list[i];
+      const int r = above(s_list, found, x);
+      if (r < k) s_order[r] = x;
     }
+    __syncthreads();
+    return found < k ? found : k;
+  };
+  const int groups = first(p.n_group, [&](int i) { return place_of(key_of(group[i]), i); });
+  if (t < groups) s_group[t] = (int)index_at(s_order[t]);
+  __syncthreads();
+  const T* const x = static_cast<const T*>(p.a.logits) + row * p.a.ld;
+  const int n2 = first(groups * kGroup, [&](int i) -> u64 {
+    const int v = s_group[i / kGroup] * kGroup + i % kGroup;
+    return v < p.a.V ? place_of(key_of((float)x[v]), v) : 0;
+  });
+  const double rest = log(s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3]);  // lse - m
+  const double by = divides(p.a) ? divisor(p.a, length_of(p.a, row, 1)) : 1.0;
+  if (t < n2) {
+    const u64 y = s_order[t];
+    const double s = score + (((double)logit_of(key_at(y)) - (double)m) - rest);
+    rank[t] = s / by;
+    sums[t] = s;
+    tokens[t] = (int)index_at(y);
   }
-  if (t == 0) p.count[row] = n2 < k ? n2 : k;
+  if (t == 0) p.count[row] = n2;
 }
 
 // One wave per sequence: a lane holds the first candidate left of its beams (lane, lane + 64, ...); k times the best of
@@ -367,22 +355,284 @@ __global__ __launch_bounds__(64) void beam_merge_kernel(BeamWork p) {
   }
 }
 
+// ---- both in one launch: a workgroup per sequence, a wave per beam (or two beams)
+// Bound by the latency of what follows upon each other: what the scan left, the few groups' logits, and one barrier
+// before the merge.  Loops stay loops, with as little as can be: unrolled to hold all maxima in registers this took 15 us
+// for 4 beams of 151936, most of it to fetch its own instructions.
+constexpr int kPickBeams = 16, kPickWaves = 8, kPickMost = 64, kPickList = 256;
+
+__device__ __forceinline__ void wave_fence() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
+
+struct AddF64 {
+  __device__ __forceinline__ u64 operator()(u64 a, u64 b) const {
+    return (u64)__double_as_longlong(__longlong_as_double((long long)a) + __longlong_as_double((long long)b));
+  }
+};
+
+// A list of a wave in LDS: the places of values that are at least `least` go to its end, but for -inf.  (Past kPickList
+// they are counted, not kept.)
+struct WaveList {
+  u64* at;
+  int n;
+  __device__ __forceinline__ void add(float x, int i, float least) {
+    const bool in = x >= least && x > kNegInf;
+    const uint64_t hit = __ballot(in);
+    if (hit == 0) return;
+    const int to = n + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(hit >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)hit, 0));
+    if (in && to < kPickList) at[to] = (u64)__float_as_uint(x) << 32 | (uint32_t)i;  // (in_order makes places of them)
+    n += __popcll(hit);
+  }
+  __device__ __forceinline__ static u64 raw(u64 place) {
+    return (u64)__float_as_uint(logit_of(key_at(place))) << 32 | (uint32_t)index_at(place);
+  }
+  // The k first of all, in rounds of maxima: best(x) is this lane's first entry after x.  For lists that overflow
+  // (many large ones with few lanes, equal ones).
+  template <class F>
+  __device__ __forceinline__ void by_rounds(int k, F&& best) {
+    u64 last = ~0ull;
+#pragma unroll 1
+    for (n = 0; n < k; ++n) {
+      last = wave_max64(best(last));
+      if (last == 0) break;
+      if (lane_id() == 0) at[n] = raw(last);
+    }
+  }
+  // f(entry, its place) for the k first.
+  template <class F>
+  __device__ __forceinline__ void in_order(int k, F&& f) {
+    wave_fence();
+#pragma unroll 1
+    for (int i = lane_id(); i < n; i += 64)
+      at[i] = place_of(key_of(__uint_as_float((uint32_t)(at[i] >> 32))), (uint32_t)at[i]);
+    if (lane_id() < kPad) at[n + lane_id()] = 0;
+    wave_fence();
+#pragma unroll 1
+    for (int i = lane_id(); i < n; i += 64) {
+      const u64 x = at[i];
+      const int r = above(at, n, x);
+      if (r < k) f(x, r);
+    }
+    wave_fence();
+  }
+};
+
+// A value that k of the lanes' x or more reach: the k-th largest among the maxima of 4 lanes (up to 8), 2 (up to 16) or
+// one; -inf where there are fewer.  s: 64 words of LDS.
+__device__ __forceinline__ float reached_by(float x, int k, float* s) {
+  int cells = 64, cell = lane_id();
+  if (k <= 16) x = dpp_max<0xB1>(x), cells = 32, cell >>= 1;
+  if (k <= 8) x = dpp_max<0x4E>(x), cells = 16, cell >>= 1;
+  s[cell] = x;
+  wave_fence();
+  int larger = 0;
+  const float4* const q = reinterpret_cast<const float4*>(s);
+#pragma unroll 1
+  for (int i = 0; i < cells / 4; i += 4)
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const float4 y = q[i + u];
+      larger += (y.x > x) + (y.y > x) + (y.z > x) + (y.w > x);
+    }
+  wave_fence();
+  // the smallest of those that fewer than k exceed
+  return -max64(max8(larger < k ? -x : kNegInf));
+}
+
+template <class T>
+__global__ __launch_bounds__(64 * kPickWaves) void beam_pick_kernel(BeamWork p) {
+  __shared__ __attribute__((aligned(16))) u64 s_lists[kPickWaves][kPickList + kPad];
+  __shared__ u64 s_chosen[kPickWaves][kPickMost];
+  // candidate i of beam w at w k + i
+  __shared__ double s_rank[kPickBeams * kPickMost], s_sum[kPickBeams * kPickMost];
+  __shared__ int64_t s_length[kPickBeams];
+  __shared__ int s_token[kPickBeams * kPickMost], s_before[kPickBeams * kPickMost], s_count[kPickBeams];
+  const int b = (int)blockIdx.x;
+  const int lane = lane_id(), k = p.a.k, W = p.a.W;
+  u64* const chosen = s_chosen[wave_id()];
+  // beam w's candidates to s_sum, s_token, best first; how many
+  auto choose = [&](int w) -> int {
+    // (sizes that the compiler takes for new ones: it keeps what follows from them across beams, in more registers than
+    // there are)
+    int n_group = p.n_group, n_sub = p.n_sub, k = p.a.k, lane = lane_id();
+    asm volatile("" : "+s"(n_group), "+s"(n_sub), "+s"(k), "+v"(lane));
+    const int64_t row = (int64_t)b * W + w;
+    const float* const group = p.group + row * n_group;
+    const double* const sub_sum = p.sub_sum + row * n_sub;
+    const float* const sub_max = p.sub_max + row * n_sub;
+    // All that is needed of a row of up to 262144 goes out at once (a round trip takes 1000 cycles and more); what is
+    // further on is read where it is used.
+    constexpr int kHeld = 32;
+    float g[kHeld];
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j) {
+      if (j % 16 == 0 && j * 64 >= n_group) break;
+      g[j] = group[min(j * 64 + lane, n_group - 1)];
+    }
+    const float max0 = sub_max[min(lane, n_sub - 1)], max1 = sub_max[min(lane + 64, n_sub - 1)];
+    const double sum0 = sub_sum[min(lane, n_sub - 1)], sum1 = sub_sum[min(lane + 64, n_sub - 1)];
+    const double score = score_of(p.a, row);
+    const bool done = p.a.finished && p.a.finished[row];
+    if (divides(p.a) && lane == 0) s_length[w] = length_of(p.a, row, done ? 0 : 1);
+    if (!alive(score)) return 0;
+    if (done) {
+      if (lane == 0) {
+        s_sum[w * k] = score;
+        s_token[w * k] = (int)p.a.end_id;
+      }
+      return 1;
+    }
+    float top = kNegInf;
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j) {
+      if (j % 16 == 0 && j * 64 >= n_group) break;
+      g[j] = j * 64 + lane < n_group ? g[j] : kNegInf;
+      top = fmaxf(top, g[j]);
+    }
+#pragma unroll 1
+    for (int i = kHeld * 64 + lane; i < n_group; i += 64) top = fmaxf(top, group[i]);
+    const float m = max64(max8(top));
+    if (!(m > kNegInf && m < kPosInf)) return 0;  // nothing to choose (at +inf: no sum is a number)
+    // ---- the k first groups: a bound that k of them reach (the k-th of the lanes' best), the few that reach it, in order
+    WaveList list{s_lists[wave_id()], 0};
+    float least = reached_by(top, k, reinterpret_cast<float*>(list.at));
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j) {
+      if (j % 16 == 0 && j * 64 >= n_group) break;
+      list.add(g[j], j * 64 + lane, least);
+    }
+#pragma unroll 1
+    for (int i = kHeld * 64; i < n_group; i += 64)
+      list.add(i + lane < n_group ? group[min(i + lane, n_group - 1)] : kNegInf, i + lane, least);
+    if (list.n > kPickList)
+      list.by_rounds(k, [&](u64 last) {
+        u64 y = 0;
+#pragma unroll 1
+        for (int i = lane; i < n_group; i += 64) {
+          const u64 x = place_of(key_of(group[i]), i);
+          y = x < last && x > y ? x : y;
+        }
+        return y;
+      });
+    list.in_order(k, [&](u64 x, int r) { chosen[r] = x; });
+    // ---- the k first of their logits: none below the k-th group's largest
+    const int groups = list.n < k ? list.n : k;
+    least = groups == k ? logit_of(key_at(chosen[k - 1])) : kNegInf;
+    const T* const x = static_cast<const T*>(p.a.logits) + row * p.a.ld;
+    const int V = (int)p.a.V;
+    // A lane's two of a group; at the row's end its last two are read, of which those from the lane's first on count.
+    typedef T Pair __attribute__((ext_vector_type(2), aligned(sizeof(T))));
+    static_assert(kGroup == 128, "two logits a lane");
+    list.n = 0;
+    constexpr int kAhead = 8;
+#pragma unroll 1
+    for (int s0 = 0; s0 < groups; s0 += kAhead) {
+      Pair c[kAhead];
+      int at[kAhead];
+#pragma unroll
+      for (int s = 0; s < kAhead; ++s) {
+        at[s] = (int)index_at(chosen[min(s0 + s, groups - 1)]) * kGroup + lane * 2;
+        c[s] = *reinterpret_cast<const Pair*>(x + min(at[s], V - 2));
+      }
+#pragma unroll
+      for (int s = 0; s < kAhead; ++s) {
+        if (s0 + s >= groups) break;
+        const int from = min(at[s], V - 2);
+        list.add(from == at[s] ? (float)c[s][0] : kNegInf, from, least);
+        list.add(from + 1 >= at[s] ? (float)c[s][1] : kNegInf, from + 1, least);
+      }
+    }
+    if (list.n > kPickList)
+      list.by_rounds(k, [&](u64 last) {
+        u64 y = 0;
+#pragma unroll 1
+        for (int s = 0; s < groups; ++s)
+#pragma unroll 1
+          for (int u = lane; u < kGroup; u += 64) {
+            const int i = (int)index_at(chosen[s]) * kGroup + u;
+            const u64 z = i < V ? place_of(key_of((float)x[i]), i) : 0;
+            y = z < last && z > y ? z : y;
+          }
+        return y;
+      });
+    // ---- lse - m, in an order of V alone
+    double sum = 0;
+#pragma unroll 1
+    for (int i = lane; i < n_sub; i += 64) {
+      const float mi = i == lane ? max0 : i == lane + 64 ? max1 : sub_max[i];
+      const double si = i == lane ? sum0 : i == lane + 64 ? sum1 : sub_sum[i];
+      if (mi > kNegInf) sum += si * exp((double)mi - (double)m);
+    }
+    sum = __longlong_as_double((long long)last_lane64(wave_scan64((u64)__double_as_longlong(sum), AddF64())));
+    const double rest = log(sum);
+    list.in_order(k, [&](u64 z, int r) {
+      const double y = score + (((double)logit_of(key_at(z)) - (double)m) - rest);
+      s_sum[w * k + r] = y;
+      s_token[w * k + r] = (int)index_at(z);
+    });
+    return list.n < k ? list.n : k;
+  };
+#pragma unroll 1
+  for (int w = wave_id(); w < W; w += kPickWaves) {
+    const int n = choose(w);
+    if (lane == 0) s_count[w] = n;
+    wave_fence();  // (the lists are the next beam's)
+  }
+#pragma unroll 1
+  for (int w = wave_id(); w < W; w += kPickWaves) {
+    const double by = divides(p.a) ? divisor(p.a, s_length[w]) : 1.0;
+    if (lane >= k) continue;
+    s_rank[w * k + lane] = lane < s_count[w] ? s_sum[w * k + lane] / by : -__builtin_huge_val();  // (none: after all that are)
+    s_before[w * k + lane] = 0;
+  }
+  __syncthreads();
+  // ---- how many come before each candidate of the wave's beam: 2^n lanes each, every one with its share of the others
+  auto put = [&](int64_t at, int64_t token, int64_t parent, double score) {
+    p.a.token[at] = token;
+    p.a.parent[at] = parent;
+    if (p.a.s64) static_cast<double*>(p.a.score)[at] = score;
+    else static_cast<float*>(p.a.score)[at] = (float)score;
+  };
+  int width = 1;
+  while (width < k) width *= 2;
+  const int i = lane & (width - 1), share = lane / width, shares = 64 / width, all = W * k;
+#pragma unroll 1
+  for (int w = wave_id(); w < W; w += kPickWaves) {
+    const int me = w * k + i, n = s_count[w];
+    const double mine = i < n ? s_rank[me] : 0;
+    int before = 0;
+#pragma unroll 4
+    for (int e = share; e < all; e += shares) {
+      const double x = s_rank[e];
+      before += x > mine || (x == mine && e < me);
+    }
+    if (i < n) atomicAdd(&s_before[me], before);
+    wave_fence();
+    if (lane < n) {
+      const int to = s_before[w * k + lane];
+      if (to < k) put((int64_t)b * k + to, s_token[w * k + lane], w, s_sum[w * k + lane]);
+    }
+  }
+  if (wave_id() == 0) {
+    const int found = (int)wave_sum64(lane < W ? s_count[lane] : 0);
+    if (lane >= found && lane < k) put((int64_t)b * k + lane, -1, -1, -__builtin_huge_val());
+  }
+}
+
 int64_t up8(int64_t x) { return (x + 7) / 8 * 8; }
 
 struct BeamSizes {
-  int n_sub, gshift, n_group;
-  int64_t sub_max, sub_sum, group, rank, sum, token, count;
-  int64_t all() const { return sub_max + sub_sum + group + rank + sum + token + count; }
+  int n_sub, n_group;
+  int64_t group, sub_max, sub_sum, rank, sum, token, count;
+  int64_t all() const { return group + sub_max + sub_sum + rank + sum + token + count; }
 };
 BeamSizes beam_sizes(int64_t rows, int64_t V, int k) {
   BeamSizes z;
   z.n_sub = (int)((V + kSub - 1) / kSub);
-  z.gshift = V <= kSmallGroups ? 6 : 9;
-  z.n_group = (int)((V + (1 << z.gshift) - 1) >> z.gshift);
+  z.n_group = z.n_sub * kSubGroups;
+  z.group = rows * z.n_group * 4;
+  z.sub_max = up8(rows * z.n_sub * 4);
   z.sub_sum = rows * z.n_sub * 8;
   z.rank = z.sum = rows * k * 8;
-  z.sub_max = up8(rows * z.n_sub * 4);
-  z.group = up8(rows * z.n_group * 4);
   z.token = up8(rows * k * 4);
   z.count = up8(rows * 4);
   return z;
@@ -392,8 +642,12 @@ template <class T>
 hipError_t run(BeamWork p, hipStream_t stream) {
   const int64_t rows = p.a.B * p.a.W;
   beam_scan_kernel<T><<<(unsigned)(rows * p.n_seg), 64 * kScanWaves, 0, stream>>>(p);
-  beam_row_kernel<T><<<(unsigned)rows, kRowThreads, 0, stream>>>(p);
-  beam_merge_kernel<<<(unsigned)p.a.B, 64, 0, stream>>>(p);
+  if (p.a.W <= kPickBeams && p.a.k <= kPickMost && p.a.V >= 2) {
+    beam_pick_kernel<T><<<(unsigned)p.a.B, 64 * std::min(p.a.W, kPickWaves), 0, stream>>>(p);
+  } else {
+    beam_row_kernel<T><<<(unsigned)rows, kRowThreads, 0, stream>>>(p);
+    beam_merge_kernel<<<(unsigned)p.a.B, 64, 0, stream>>>(p);
+  }
   return hipGetLastError();
 }
 
@@ -465,15 +719,14 @@ hipError_t beams_launch(int dtype, const BeamParams& a, char* ws, hipStream_t st
   p.a = a;
   p.n_sub = z.n_sub;
   p.n_seg = (z.n_sub + kScanWaves - 1) / kScanWaves;
-  p.gshift = z.gshift;
   p.n_group = z.n_group;
-  p.sub_sum = reinterpret_cast<double*>(ws);
+  p.group = reinterpret_cast<float*>(ws);
+  p.sub_sum = reinterpret_cast<double*>(ws += z.group);
   p.rank = reinterpret_cast<double*>(ws += z.sub_sum);
   p.sum = reinterpret_cast<double*>(ws += z.rank);
-  p.sub_max = reinterpret_cast<float*>(ws += z.sum);
-  p.group = reinterpret_cast<float*>(ws += z.sub_max);
-  p.token = reinterpret_cast<int*>(ws += z.group);
+  p.token = reinterpret_cast<int*>(ws += z.sum);
   p.count = reinterpret_cast<int*>(ws += z.token);
+  p.sub_max = reinterpret_cast<float*>(ws += z.count);
   hipError_t e;
   timing_begin(kKindBeams, stream);
   switch (dtype) {

@@ -211,7 +211,7 @@ def logits(dtype=_lib.BF16, out_dtype=_lib.BF16, N=4, K=16, V=9, h=A, ldh=16, im
     (select, dict(scores=None), _lib.EINVAL),
     (select, dict(parent=None), _lib.EINVAL),
     (select, dict(ws=None), _lib.EWORKSPACE),
-    (select, dict(ws=ctypes.c_void_p(4100)), _lib.EWORKSPACE),
+    (select, dict(ws=ctypes.c_void_p(4104)), _lib.EWORKSPACE),
     (select, dict(nbytes=16), _lib.EWORKSPACE),
     (reorder, dict(n=-1), _lib.EINVAL),
     (reorder, dict(B=-1), _lib.EINVAL),
@@ -286,5 +286,5 @@ def test_sizes():
     assert lib.swvr_int8_size(300, 100) == 16 * 2 * 2048 and lib.swvr_int8_size(0, 5) == 0 and lib.swvr_int8_size(5, 0) == 0
     assert lib.swvr_int8_logits_workspace_size(300, 100) == 1280 + 16 * 2 * 2048
     assert lib.swvr_select_beams_workspace_size(2, 257, 9, 1) == 0
-    # of 6 rows of 5000 logits: 3 sub-blocks, 79 groups, 4 candidates
-    assert lib.swvr_select_beams_workspace_size(2, 3, 5000, 4) == 6 * 3 * 8 + 2 * 6 * 4 * 8 + 72 + 6 * 79 * 4 + 96 + 24
+    # of 6 rows of 5000 logits: 3 sub-blocks of 16 groups, 4 candidates
+    assert lib.swvr_select_beams_workspace_size(2, 3, 5000, 4) == 6 * 3 * (8 + 4 + 16 * 4) + 6 * 4 * 2 * 8 + 6 * 4 * 4 + 6 * 4
