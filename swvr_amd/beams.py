@@ -13,6 +13,7 @@ candidates in the next step.  The kernels run on the current stream (C ABI: swvr
 """
 import ctypes
 import functools
+import math
 from typing import List, Optional, Tuple
 
 import torch
@@ -32,23 +33,24 @@ def _dense(x, dtype):
     return x if x.is_contiguous() else x.contiguous()
 
 
+@functools.lru_cache(maxsize=256)
+def _workspace(B, W, V, k):
+    return _lib.load().swvr_select_beams_workspace_size(B, W, V, k)
+
+
 def _select(logits, scores, k, finished, end_id, lengths, alpha):
-    x, V, W = _plain(logits), logits.shape[-1], logits.shape[-2]
+    x, (*lead, W, V) = _plain(logits), logits.shape
     x = x if x.dim() == 2 else x.reshape(-1, V)
     x = x if x.stride(1) == 1 and x.stride(0) >= 0 else x.contiguous()
     s = _dense(scores, scores.dtype if scores.dtype == torch.float64 else torch.float32)
     finished, lengths = _dense(finished, torch.bool), _dense(lengths, torch.int64)
-    B = 1
-    for n in scores.shape[:-1]:
-        B *= n
-    shape = (*scores.shape[:-1], k)
-    token, parent, out = (x.new_empty(shape, dtype=d) for d in (torch.int64, torch.int64, s.dtype))
-    a, lib = _lib.address, _lib.load()
-    ws_bytes = lib.swvr_select_beams_workspace_size(B, W, V, k)
-    ws = x.new_empty(ws_bytes, dtype=torch.uint8)
-    _lib.call(lib.swvr_select_beams, x.device, _lib.DTYPE_TAG[x.dtype], B, W, V, k, x.data_ptr(),
-              x.stride(0) if x.shape[0] > 1 else V, s.data_ptr(), s.dtype == torch.float64, a(finished), end_id, a(lengths),
-              alpha, token.data_ptr(), parent.data_ptr(), out.data_ptr(), ws.data_ptr(), ws_bytes)
+    B, shape, ld = math.prod(lead), (*lead, k), x.stride(0) if x.shape[0] > 1 else V
+    token, parent = x.new_empty(shape, dtype=torch.int64), x.new_empty(shape, dtype=torch.int64)
+    out, ws_bytes = s.new_empty(shape), _workspace(B, W, V, k)
+    ws, a = x.new_empty(ws_bytes, dtype=torch.uint8), _lib.address
+    _lib.call(_lib.load().swvr_select_beams, x.device, _lib.DTYPE_TAG[x.dtype], B, W, V, k, x.data_ptr(), ld, s.data_ptr(),
+              s.dtype == torch.float64, a(finished), end_id, a(lengths), alpha, token.data_ptr(), parent.data_ptr(),
+              out.data_ptr(), ws.data_ptr(), ws_bytes)
     return token, parent, out
 
 
@@ -84,15 +86,14 @@ def select_beams(logits, scores, k=None, *, finished=None, end_id=None, lengths=
     candidates.  Where fewer than k are left, token and parent are -1 and the score -inf.  W and k are at most 256, V
     at most 2^21.  No gradient; the same result on every run.
     """
-    if logits.dim() < 2 or not 1 <= logits.shape[-1] <= MAX_V or not 1 <= logits.shape[-2] <= MAX_BEAMS:
-        raise ValueError(f"logits must be [..., W, V] with 1 <= W <= {MAX_BEAMS} and 1 <= V <= 2^21, got {tuple(logits.shape)}")
+    shape = logits.shape
+    if len(shape) < 2 or not 1 <= shape[-1] <= MAX_V or not 1 <= shape[-2] <= MAX_BEAMS:
+        raise ValueError(f"logits must be [..., W, V] with 1 <= W <= {MAX_BEAMS} and 1 <= V <= 2^21, got {tuple(shape)}")
     if logits.dtype not in _lib.DTYPE_TAG:
         raise NotImplementedError(f"swvr_amd: logits dtype {logits.dtype} is not supported (bf16, fp16, fp32)")
-    if scores.shape != logits.shape[:-1]:
-        raise ValueError(f"scores must have shape {tuple(logits.shape[:-1])}, got {tuple(scores.shape)}")
     if not scores.dtype.is_floating_point:
         raise ValueError(f"scores must be floating point, got {scores.dtype}")
-    k = logits.shape[-2] if k is None else int(k)
+    k = shape[-2] if k is None else int(k)
     if not 1 <= k <= MAX_BEAMS:
         raise ValueError(f"k must be between 1 and {MAX_BEAMS}, got {k}")
     if not 0 <= length_penalty <= 16:
@@ -102,32 +103,33 @@ def select_beams(logits, scores, k=None, *, finished=None, end_id=None, lengths=
     for name, x in (("scores", scores), ("finished", finished), ("lengths", lengths)):
         if x is None:
             continue
-        if x.shape != scores.shape:
-            raise ValueError(f"{name} must have shape {tuple(scores.shape)}, got {tuple(x.shape)}")
+        if x.shape != shape[:-1]:
+            raise ValueError(f"{name} must have shape {tuple(shape[:-1])}, got {tuple(x.shape)}")
         if x.device != logits.device:
             raise ValueError(f"{name} is on {x.device} but logits on {logits.device}")
+    end = 0
     if finished is not None:
         if finished.dtype != torch.bool:
             raise ValueError(f"finished must be bool, got {finished.dtype}")
-        if end_id is None or not 0 <= end_id < logits.shape[-1]:
+        if end_id is None or not 0 <= end_id < shape[-1]:
             raise ValueError(f"finished needs end_id, a token of 0 to V - 1, got {end_id}")
+        end = int(end_id)
     if lengths is not None and (lengths.dtype.is_floating_point or lengths.dtype.is_complex or lengths.dtype == torch.bool):
         raise ValueError(f"lengths must be integers, got {lengths.dtype}")
-    end = int(end_id) if finished is not None else 0
-    no_tangents(logits, scores)
-    args = (logits.detach(), scores.detach(), k, finished, end, lengths, float(length_penalty))
     if eager(logits, scores, finished, lengths):
-        return _select(*args)
+        return _select(logits, scores, k, finished, end, lengths, float(length_penalty))
+    no_tangents(logits, scores)
     if logits.device.type == "cpu":
         _require_device(logits)
-    return _select_op(*args)
+    return _select_op(logits.detach(), scores.detach(), k, finished, end, lengths, float(length_penalty))
 
 
 # ---------------------------------------------------------------- states
 @functools.lru_cache(maxsize=1024)
 def _geometry(shape, strides, itemsize, nb):
     """Of a state [lead..., W, rest...] with nb leading dimensions: (run, n1, n2, strides, dst strides per beam of a
-    dense copy's (n2, n1)), bytes; None where more dimensions are left after merging than the kernel walks."""
+    dense copy's (n2, n1)), bytes; None where the kernel cannot walk them: more dimensions left after merging, or pieces
+    that make 4 GB a beam."""
     def merged(dims):
         out = []
         for n, s in dims:
@@ -148,6 +150,8 @@ def _geometry(shape, strides, itemsize, nb):
         return None
     rest = [(1, 0)] * (2 - len(rest)) + rest
     (n2, s2), (n1, s1) = rest
+    if n1 * n2 > 1 and run * n1 * n2 * itemsize >= 2 ** 32:   # (the library's limit of a beam in pieces)
+        return None
     step = tuple(s * itemsize for s in (lead[0][1] if lead else 0, strides[nb] if shape[nb] > 1 else 0, s2, s1))
     return run * itemsize, n1, n2, step, (run * n1 * itemsize if n2 > 1 else 0, run * itemsize if n1 > 1 else 0)
 
@@ -172,30 +176,37 @@ def _reorder(states, parents, inplace):
     B = 1
     for n in ids.shape[:-1]:
         B *= n
-    groups, out, seen = {}, [], set()
+    groups, out, seen, last = {}, [], set(), None
     for x in states:
-        if not inplace:
-            x = _plain(x.resolve_conj() if x.is_conj() else x)
-        shape, strides = x.shape, x.stride()
         if inplace:
             if x.is_neg() or x.is_conj() or x._is_zerotensor():
                 raise ValueError("a lazily negated, conjugated or memoryless state cannot be reordered in place")
-            if _overlaps(shape, strides):
-                raise ValueError(f"a state with shared elements (strides {strides}) cannot be reordered in place")
-            if x.numel() and x.data_ptr() in seen:
+            at = x.data_ptr()
+            if at in seen and x.numel():
                 raise ValueError("the same state twice cannot be reordered in place")
-            seen.add(x.data_ptr())
-        g = _geometry(shape, strides, x.element_size(), nb) if x.numel() else ()
-        if g is None:
-            if inplace:
-                raise ValueError(f"a state of shape {tuple(shape)} with strides {strides} has too many separate dimensions to "
-                                 "be reordered in place")
+            seen.add(at)
+        else:
+            x = _plain(x.resolve_conj() if x.is_conj() else x)
+        layout = (x.shape, x.stride(), x.element_size())
+        if layout != last:   # (the caches of all layers have one)
+            last, (shape, strides, _) = layout, layout
+            if inplace and _overlaps(shape, strides):
+                raise ValueError(f"a state with shared elements (strides {strides}) cannot be reordered in place")
+            g = _geometry(*layout, nb) if x.numel() else ()
+            if g is None and inplace:
+                raise ValueError(f"a state of shape {tuple(shape)} with strides {strides} has too many separate dimensions (or "
+                                 "pieces, of a beam of 4 GB) to be reordered in place")
+            new = (*shape[:nb], k, *shape[nb + 1:])
+            dense = g is None
+            if dense:
+                g = _geometry(shape, x.contiguous().stride(), x.element_size(), nb)
+            if g:
+                src, dst = groups.setdefault(g, ([], []))
+        if dense:
             x = x.contiguous()
-            g = _geometry(x.shape, x.stride(), x.element_size(), nb)
-        y = x if inplace else torch.empty((*shape[:nb], k, *shape[nb + 1:]), dtype=x.dtype, device=x.device)
+        y = x if inplace else torch.empty(new, dtype=x.dtype, device=x.device)
         out.append(y)
         if g:
-            src, dst = groups.setdefault(g, ([], []))
             src.append(x)
             dst.append(y)
     lib = _lib.load()
@@ -242,8 +253,8 @@ def reorder_beams(states, parents, *, inplace=False):
 
     Gives new tensors (of the structure of ``states``), or with ``inplace`` the states themselves, reordered where they
     are: beams that keep their place are then neither read nor written.  In place k must be W, at most 64; leading
-    dimensions have to be one in memory, the ones after the beams at most three after merging, and no element may be
-    part of a state twice or of two states.  No gradient: where one would be recorded the call is refused.
+    dimensions have to be one in memory, the ones after the beams at most three after merging (one, where a beam has 4
+    GB), and no element may be part of a state twice or of two states.  No gradient: where one would be recorded the call is refused.
     """
     alone = isinstance(states, torch.Tensor)
     xs = [states] if alone else list(states)
@@ -257,22 +268,22 @@ def reorder_beams(states, parents, *, inplace=False):
         raise ValueError(f"states and parents must have 1 to {MAX_BEAMS} beams, got {W} and {k}")
     if inplace and (k != W or W > MAX_IN_PLACE):
         raise ValueError(f"in place as many beams come as go, at most {MAX_IN_PLACE}: got {W} and {k}")
-    grad, lead, device = torch.is_grad_enabled(), parents.shape[:-1], parents.device
+    grad, lead, device, shape = torch.is_grad_enabled(), parents.shape[:-1], parents.device, None
     for x in xs:
-        if x.dim() <= nb or x.shape[nb] != W or x.shape[:nb] != lead:
-            raise ValueError(f"states must be [{', '.join(map(str, (*lead, W)))}, ...], got {tuple(x.shape)}")
+        if x.shape != shape:
+            shape = x.shape
+            if len(shape) <= nb or shape[nb] != W or shape[:nb] != lead:
+                raise ValueError(f"states must be [{', '.join(map(str, (*lead, W)))}, ...], got {tuple(shape)}")
         if x.device != device:
             raise ValueError(f"a state is on {x.device} but parents on {device}")
         if grad and x.requires_grad:
             raise ValueError("reorder_beams has no gradient: call it under torch.no_grad() or on detached tensors")
-    no_tangents(*xs)
     if eager(parents, *xs):
         out = _reorder(xs, parents, inplace)
         if inplace:
-            for x in xs:
-                if not x.is_inference():
-                    torch.autograd.graph.increment_version(x)
+            torch.autograd.graph.increment_version([x for x in xs if not x.is_inference()])
     else:
+        no_tangents(*xs)
         if device.type == "cpu":
             _require_device(parents)
         if inplace:

@@ -141,6 +141,9 @@ def test_geometry_of_states():
     assert g(x[:, :, :, :7, :5]) == (10, 7, 4, (1920, 640, 160, 16), (70, 10))
     assert g(x[..., ::2]) == (2, 160, 1, (1920, 640, 0, 4), (0, 2))
     assert g(x[:, :, ::2, ::3, ::2]) is None
+    big = torch.zeros(2, 3, 2 ** 16, 2 ** 16, device="meta", dtype=torch.uint8)   # 4 GB a beam: in one piece alone
+    assert g(big) == (2 ** 32, 1, 1, (3 * 2 ** 32, 2 ** 32, 0, 0), (0, 0)) and g(big[..., 1:]) is not None
+    assert g(torch.zeros(2, 3, 2 ** 17, 2 ** 16, device="meta", dtype=torch.uint8)[..., 1:]) is None
     y = torch.zeros(2, 3, 4, 8)
     assert g(y, 2) == (32, 1, 1, (128, 32, 0, 0), (0, 0))
     assert g(y[:, :2], 2) is None           # leading dimensions apart
