@@ -399,7 +399,7 @@ int swvr_sample(int dtype, int64_t R, int64_t V, const void* logits, int64_t ld,
  *   scale[r] = max(max_k |x[r,k]|, 1e-30) * fl(1/127)   (fp32)
  *   q[r,k]   = x[r,k] / scale[r] to the nearest whole number, halves to even, by the exact quotient
  * in an image of swvr_int8_size bytes, whose layout is the library's own (16-byte aligned; K at most
- * 2^17, R at most 2^30).  A row with an infinity or a NaN has scale NaN and q 0.
+ * 2^17, R at most 2^25).  A row with an infinity or a NaN has scale NaN and q 0.
  *   swvr_int8_quantize   image and scales of x in bf16, fp16 or fp32 (row stride ld);
  *   swvr_int8_pack       the image of integers q [R,K] (row stride ldq) quantised elsewhere;
  *   swvr_int8_unpack     out [R,K] = scale q in fp32;

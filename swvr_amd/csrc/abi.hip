@@ -731,8 +731,9 @@ int swvr_sample(int dtype, int64_t R, int64_t V, const void* logits, int64_t ld,
 // ---------------------------------------------------------------- 8-bit integers
 static int check_int8(int64_t R, int64_t K) {
   g_err[0] = 0;
-  if (R < 0 || R > SWVR_EMBED_MAX || K < 1 || K > ((int64_t)1 << 17))
-    return fail(SWVR_EINVAL, "bad sizes of %lld rows of K=%lld (rows at most 2^30, K 1 to 2^17)", (long long)R, (long long)K);
+  // (a wave for each row: a grid's threads)
+  if (R < 0 || R > ((int64_t)1 << 25) || K < 1 || K > ((int64_t)1 << 17))
+    return fail(SWVR_EINVAL, "bad sizes of %lld rows of K=%lld (rows at most 2^25, K 1 to 2^17)", (long long)R, (long long)K);
   return SWVR_OK;
 }
 
@@ -771,6 +772,8 @@ int swvr_int8_pack(int64_t R, int64_t K, const void* q, int64_t ldq, void* image
 int swvr_int8_unpack(int64_t R, int64_t K, const void* image, const float* scale, float* out, void* stream) {
   const int rc = check_int8(R, K);
   if (rc != SWVR_OK) return rc;
+  if (((R + 31) / 32) * ((K + 255) / 256) >= ((int64_t)1 << 24))
+    return fail(SWVR_EINVAL, "%lld rows of K=%lld: a grid has fewer than 2^32 threads", (long long)R, (long long)K);
   if (R == 0) return SWVR_OK;
   if (!image || !scale || !out || !aligned16(image) || !aligned16(out))
     return fail(SWVR_EINVAL, "image, out (16-byte aligned) and scale must be non-null");
@@ -792,9 +795,9 @@ int swvr_int8_logits(int dtype, int out_dtype, int64_t N, int64_t K, int64_t V, 
   int rc = check_int8(N, K);
   if (rc == SWVR_OK) rc = check_int8(V, K);
   if (rc != SWVR_OK) return rc;
-  // (tiles of 256 x 256 by 512 threads each: a grid's threads)
-  if (N > ((int64_t)1 << 24) || ((N + 255) / 256) * ((V + 255) / 256) >= ((int64_t)1 << 23))
-    return fail(SWVR_EINVAL, "bad sizes N=%lld V=%lld (N at most 2^24, tiles of 256 x 256 below 2^23)", (long long)N, (long long)V);
+  // (512 threads for 256 x 128 logits: a grid's threads)
+  if (N > ((int64_t)1 << 24) || ((N + 127) / 128) * ((V + 255) / 256) >= ((int64_t)1 << 23))
+    return fail(SWVR_EINVAL, "bad sizes N=%lld V=%lld (N at most 2^24, tiles of 128 x 256 below 2^23)", (long long)N, (long long)V);
   if (!is_dtype(dtype) || !is_dtype(out_dtype) || (bias && !is_dtype(bias_dtype)))
     return fail(SWVR_EDTYPE, "unsupported dtype tags %d, %d, %d", dtype, out_dtype, bias_dtype);
   if (ldh < 0) return fail(SWVR_EINVAL, "ldh=%lld must not be negative", (long long)ldh);

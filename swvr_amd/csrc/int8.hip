@@ -47,25 +47,33 @@ namespace {
 // ---------------------------------------------------------------- quantisation
 constexpr float kTinyAmax = 1e-30f;
 
-// 16 consecutive values of a row from k on, 0 past K; vec: 16-byte aligned rows.
+// 16 consecutive values of a row from k on, 0 past K, as they are stored: loads of several go out before the first is
+// used.  Rows begin at any element (K odd).
 template <class Src>
-__device__ __forceinline__ void load16(const Src* row, int k, int K, bool vec, float (&v)[16]) {
-  if (vec && k + 16 <= K) {
-    constexpr int CE = 16 / (int)sizeof(Src);
-    struct alignas(16) X {
-      Src v[CE];
-    };
+struct Sixteen {
+  typedef Src V __attribute__((ext_vector_type(8)));
+  V v[2];
+  __device__ __forceinline__ void load(const Src* row, int k, int K) {
+    typedef V __attribute__((aligned(sizeof(Src)))) Unaligned;
+    if (k + 16 <= K) {
 #pragma unroll
-    for (int j = 0; j < 16 / CE; ++j) {
-      const X x = *reinterpret_cast<const X*>(row + k + j * CE);
+      for (int h = 0; h < 2; ++h) v[h] = *reinterpret_cast<const Unaligned*>(row + k + 8 * h);
+    } else {
 #pragma unroll
-      for (int i = 0; i < CE; ++i) v[j * CE + i] = (float)x.v[i];
+      for (int i = 0; i < 16; ++i) v[i / 8][i % 8] = k + i < K ? row[k + i] : (Src)0.f;
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = k + i < K ? (float)row[k + i] : 0.f;
   }
-}
+  __device__ __forceinline__ float operator[](int i) const { return (float)v[i / 8][i % 8]; }
+  // the larger of m and all magnitudes, by their bits: an infinity or a NaN is larger than any number
+  __device__ __forceinline__ uint32_t magnitude(uint32_t m) const {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const uint32_t b = __float_as_uint((*this)[i]) & 0x7fffffffu;
+      m = b > m ? b : m;
+    }
+    return m;
+  }
+};
 
 // x / s to the nearest whole number, halves to even, as the exact quotient has it: the product with 1 / s may fall
 // on the other side of a border, which the remainder x - q s shows (exact in one fma: where it is near s / 2 it is a
@@ -78,28 +86,37 @@ __device__ __forceinline__ int quantize(float x, float s, float inv, float half)
   return a > half || (a == half && (n & 1)) ? n + up : n;
 }
 
-// TPR threads a row: 8 for many rows, whose 16-byte chunks then go out as 128-byte runs; a workgroup for few.
-template <class Src, int TPR>
-__global__ __launch_bounds__(256) void int8_quantize_kernel(const Src* __restrict__ x, int64_t ld, int64_t R, int K, int S,
-                                                            int vec, char* __restrict__ image, float* __restrict__ scale) {
+// TPR threads a row, a wave for many rows and a workgroup for few, each with NC pieces of 16 values in registers, so
+// that rows of up to 16 NC TPR values are read once (longer ones twice).  A piece goes out as one 16-byte chunk of the
+// image; the workgroup's rows are neighbours in it, 8 of them 128 bytes in a row.  (8 threads a row, whose chunks go out
+// together but who read their rows twice: 151936 x 2560 in bf16 415 us.)
+constexpr int kManyRows = 8;
+template <class Src, int TPR, int NC>
+__global__ __launch_bounds__(TPR == 64 ? 64 * kManyRows : TPR) void int8_quantize_kernel(
+    const Src* __restrict__ x, int64_t ld, int64_t R, int K, int S, char* __restrict__ image, float* __restrict__ scale) {
   __shared__ uint32_t s_max[4];
-  const int64_t r = (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
-  const int j = threadIdx.x % TPR;
+  const int64_t r = TPR == 64 ? (int64_t)blockIdx.x * kManyRows + wave_id() : (int64_t)blockIdx.x;
+  const int j = TPR == 64 ? lane_id() : (int)threadIdx.x;
   const Src* row = x + r * ld;
-  // the largest magnitude by its bits: an infinity or a NaN is larger than any number
+  Sixteen<Src> v[NC];
   uint32_t m = 0;
-  if (r < R)
-    for (int k = j * 16; k < K; k += TPR * 16) {
-      float v[16];
-      load16(row, k, K, vec != 0, v);
+  if (r < R) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const uint32_t b = __float_as_uint(v[i]) & 0x7fffffffu;
-        m = b > m ? b : m;
-      }
+    for (int c = 0; c < NC; ++c) {
+      const int k = (c * TPR + j) * 16;
+      if (c * TPR * 16 < K) v[c].load(row, k < K ? k : K, K);
     }
 #pragma unroll
-  for (int o = 1; o < (TPR < 64 ? TPR : 64); o <<= 1) {
+    for (int c = 0; c < NC; ++c)
+      if (c * TPR * 16 < K) m = v[c].magnitude(m);
+    for (int k = (NC * TPR + j) * 16; k < K; k += TPR * 16) {
+      Sixteen<Src> y;
+      y.load(row, k, K);
+      m = y.magnitude(m);
+    }
+  }
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
     const uint32_t y = __shfl_xor(m, o);
     m = y > m ? y : m;
   }
@@ -112,16 +129,25 @@ __global__ __launch_bounds__(256) void int8_quantize_kernel(const Src* __restric
   const bool fine = m < 0x7f800000u;
   const float s = fmaxf(__uint_as_float(m), kTinyAmax) * (1.f / 127.f), inv = 1.f / s, half = 0.5f * s;
   if (j == 0 && r < R) scale[r] = fine ? s : __uint_as_float(0x7fc00000u);
+  const bool any = r < R && fine;
   char* out = image + (r >> 5) * S * kInt8Block + (r & 31) * 16;
-  for (int k = j * 16; k < S * 64; k += TPR * 16) {
+  auto put = [&](const Sixteen<Src>& y, int k) {
     uint32_t w[4] = {0, 0, 0, 0};
-    if (r < R && fine && k < K) {
-      float v[16];
-      load16(row, k, K, vec != 0, v);
+    if (any && k < K) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) w[i / 4] |= (uint32_t)(quantize(v[i], s, inv, half) & 255) << (8 * (i % 4));
+      for (int i = 0; i < 16; ++i) w[i / 4] |= (uint32_t)(quantize(y[i], s, inv, half) & 255) << (8 * (i % 4));
     }
     *reinterpret_cast<uint4*>(out + (int64_t)(k >> 4) * 512) = make_uint4(w[0], w[1], w[2], w[3]);
+  };
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    const int k = (c * TPR + j) * 16;
+    if (k < S * 64) put(v[c], k);
+  }
+  for (int k = (NC * TPR + j) * 16; k < S * 64; k += TPR * 16) {
+    Sixteen<Src> y;
+    if (any) y.load(row, k < K ? k : K, K);
+    put(y, k);
   }
 }
 
@@ -145,26 +171,42 @@ __global__ __launch_bounds__(256) void int8_pack_kernel(const int8_t* __restrict
   }
 }
 
-// The values that an image stands for, in fp32 [R][K], 8 threads a row.
+// The values that an image stands for, in fp32 [R][K]: 32 rows x kUnpackK values through LDS, so that the image comes
+// in and rows go out in long pieces (16 bytes a lane; a chunk's 512 bytes padded to 528: no bank conflicts).
+constexpr int kUnpackK = 256;
 __global__ __launch_bounds__(256) void int8_unpack_kernel(const char* __restrict__ image, const float* __restrict__ scale,
-                                                          int64_t R, int K, int S, float* __restrict__ out) {
-  const int64_t r = (int64_t)blockIdx.x * 32 + threadIdx.x / 8;
-  if (r >= R) return;
-  const char* in = image + (r >> 5) * S * kInt8Block + (r & 31) * 16;
-  const float s = scale[r];
-  float* row = out + r * K;
-  for (int k = (threadIdx.x % 8) * 16; k < K; k += 128) {
-    const uint4 w = *reinterpret_cast<const uint4*>(in + (int64_t)(k >> 4) * 512);
-    int8_t b[16];
-    __builtin_memcpy(b, &w, 16);
-    if (K % 4 == 0 && k + 16 <= K) {
+                                                          int64_t R, int K, int S, int pieces, float* __restrict__ out) {
+  constexpr int kPitch = 528;
+  __shared__ __attribute__((aligned(16))) char s_q[kUnpackK / 16 * kPitch];
+  const int64_t r0 = blockIdx.x / pieces * 32;
+  const int k0 = blockIdx.x % pieces * kUnpackK;
+  const char* in = image + (r0 >> 5) * S * kInt8Block + (int64_t)(k0 >> 4) * 512;
 #pragma unroll
-      for (int i = 0; i < 16; i += 4)
-        *reinterpret_cast<float4*>(row + k + i) = make_float4(b[i] * s, b[i + 1] * s, b[i + 2] * s, b[i + 3] * s);
+  for (int i = 0; i < kUnpackK / 16 * 32 / 256; ++i) {
+    const int c = i * 256 + threadIdx.x;  // chunk c / 32 of row c % 32
+    if (k0 + (c / 32) * 16 < S * 64)
+      *reinterpret_cast<uint4*>(s_q + (c / 32) * kPitch + (c % 32) * 16) = *reinterpret_cast<const uint4*>(in + c * 16);
+  }
+  __syncthreads();
+  const int k = k0 + lane_id() * 4;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int row = wave_id() * 8 + i;
+    if (r0 + row >= R || k >= K) continue;
+    const int w = *reinterpret_cast<const int*>(s_q + (lane_id() / 4) * kPitch + row * 16 + (lane_id() % 4) * 4);
+    const float s = scale[r0 + row];
+    typedef float F4 __attribute__((ext_vector_type(4)));
+    typedef F4 __attribute__((aligned(4))) Unaligned;
+    F4 y;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) y[u] = (float)(w << (24 - 8 * u) >> 24) * s;
+    float* to = out + (r0 + row) * K + k;
+    if (k + 4 <= K) {
+      *reinterpret_cast<Unaligned*>(to) = y;
     } else {
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (k + i < K) row[k + i] = b[i] * s;
+      for (int u = 0; u < 4; ++u)
+        if (k + u < K) to[u] = y[u];
     }
   }
 }
@@ -178,8 +220,8 @@ __device__ __forceinline__ float bias_at(const Int8Params& p, int v) {
 }
 __device__ __forceinline__ float wscale_at(const Int8Params& p, int v) { return v < p.V ? p.w_scale[v] : 0.f; }
 
-// Up to 32 NB tokens: bound by reading W's integers once.  A workgroup takes 32 G of W's rows, its four waves a
-// quarter of the reduction each, operands straight from memory; the quarters are added in LDS.
+// Up to 32 NB tokens on few rows: a workgroup takes 32 G of W's rows, its four waves a quarter of the reduction each,
+// operands straight from memory; the quarters are added in LDS.
 template <class Out, int NB, int G, int U>
 __global__ __launch_bounds__(256) void int8_few_kernel(Int8Params p) {
   constexpr int kRegs = G * NB * 16, kPitch = 65;
@@ -253,12 +295,13 @@ struct __attribute__((packed, aligned(sizeof(Out)))) OutChunk {
   Out v[16 / sizeof(Out)];
 };
 
-// A wave's 32 FM vocabulary rows (from v0) x 32 FN tokens (from n0), through `room` (LDS of this wave, 8704 bytes): a
-// lane holds 4 rows of a token, and goes out with 16 bytes of a token's 256.
+// A wave's 32 FM vocabulary rows (from v0) x 32 FN tokens (from n0), through `room` (LDS of this wave, up to 8704 bytes):
+// a lane holds 4 rows of a token, and goes out with 16 bytes of a token's 256 (fewer with fewer rows).
 template <class Out, int FM, int FN>
 __device__ __forceinline__ void store_tile(const Int8Params& p, const i32x16_t (&acc)[FM][FN], char* room,
                                            const float* scale, const float* bias, int v0, int n0) {
-  constexpr int E = (int)sizeof(Out), FP = 8 / E, kPitch = 256 + 16;  // FP: blocks of 32 rows in 256 bytes
+  constexpr int E = (int)sizeof(Out), FP = FM < 8 / E ? FM : 8 / E;  // FP: blocks of 32 rows in a piece
+  constexpr int kBytes = FP * 32 * E, kPitch = kBytes + 16, kLanes = kBytes / 16;
   static_assert(FM % FP == 0, "whole pieces");
   struct alignas(4 * E) Four {
     Out v[4];
@@ -285,8 +328,8 @@ __device__ __forceinline__ void store_tile(const Int8Params& p, const i32x16_t (
         }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int t = i * 4 + lane / 16, at = (lane % 16) * 16;
+      for (int i = 0; i < kLanes / 2; ++i) {
+        const int t = i * (64 / kLanes) + lane / kLanes, at = (lane % kLanes) * 16;
         const int v = v0 + f0 * 32 + at / E;
         const OutChunk<Out> y = *reinterpret_cast<const OutChunk<Out>*>(__builtin_assume_aligned(room + t * kPitch + at, 16));
         if (nb + t >= p.N) continue;
@@ -304,28 +347,27 @@ __device__ __forceinline__ void store_tile(const Int8Params& p, const i32x16_t (
   }
 }
 
-// Many tokens: 256 x 256 tiles of 8 waves, the readout's reduction loop (tile_reduce) on integer operands.
-constexpr int kBV = 256, kBM = 256, kTileThreads = 512;
-template <class Out>
-__global__ __launch_bounds__(kTileThreads) void int8_tile_kernel(Int8Params p) {
-  constexpr int NS = 4, FM = 4, FN = 2;
-  typedef I8Tile<kBV, kTileThreads> TA;
-  typedef I8Tile<kBM, kTileThreads> TB;
+// Many tokens: BV x BM tiles of WV x WT waves, the readout's reduction loop (tile_reduce) on integer operands.
+template <class Out, int BV, int BM, int WV, int WT, int NS>
+__global__ __launch_bounds__(64 * WV * WT) void int8_tile_kernel(Int8Params p) {
+  constexpr int NT = 64 * WV * WT, FM = BV / WV / 32, FN = BM / WT / 32;
+  typedef I8Tile<BV, NT> TA;
+  typedef I8Tile<BM, NT> TB;
   constexpr int SB = TA::BYTES + TB::BYTES, L = TA::NI + TB::NI;
   __shared__ __attribute__((aligned(1024))) char smem[NS * SB];
-  __shared__ __attribute__((aligned(16))) float s_scale[kBV], s_bias[kBV];
-  const int w = wave_id(), wv = w >> 2, wt = w & 3;
+  __shared__ __attribute__((aligned(16))) float s_scale[BV], s_bias[BV];
+  const int w = wave_id(), wv = w / WT, wt = w % WT;
   int vt, tb;
   grouped_tile(blockIdx.x, p.n_vt, p.n_tb, &vt, &tb);
-  if (threadIdx.x < kBV) {
-    s_scale[threadIdx.x] = wscale_at(p, vt * kBV + (int)threadIdx.x);
-    s_bias[threadIdx.x] = bias_at(p, vt * kBV + (int)threadIdx.x);
+  for (int i = threadIdx.x; i < BV; i += NT) {
+    s_scale[i] = wscale_at(p, vt * BV + i);
+    s_bias[i] = bias_at(p, vt * BV + i);
   }
   const uint32_t lds0 = lds_addr(smem);
   TA ta;
-  ta.setup(p.w, vt * kBV, p.S);
+  ta.setup(p.w, vt * BV, p.S);
   TB th;
-  th.setup(p.h, tb * kBM, p.S);
+  th.setup(p.h, tb * BM, p.S);
   int is = 0, is_slot = 0;
   auto issue_next = [&]() {
     if (is >= p.S) return;
@@ -346,36 +388,63 @@ __global__ __launch_bounds__(kTileThreads) void int8_tile_kernel(Int8Params p) {
       for (int r = 0; r < 16; ++r) acc[fm][fn][r] = 0;
   Ring<NS> ring{NS - 1, p.S};
   ring.template publish_next<L>();
-  tile_reduce<int8_t, 32, L>(acc, ta, th, smem, SB, ring, p.S, wv * 128, wt * 64, issue_next);  // (two steps a slice)
+  tile_reduce<int8_t, 32, L>(acc, ta, th, smem, SB, ring, p.S, wv * (BV / WV), wt * (BM / WT), issue_next);  // (two steps a slice)
   stage_barrier();  // every wave has read its last operands: the ring holds the epilogue's rows
-  store_tile<Out, FM, FN>(p, acc, smem + w * (NS * SB / 8), s_scale + wv * 128, s_bias + wv * 128, vt * kBV + wv * 128,
-                          tb * kBM + wt * 64);
+  store_tile<Out, FM, FN>(p, acc, smem + w * (NS * SB / (WV * WT)), s_scale + wv * (BV / WV), s_bias + wv * (BV / WV),
+                          vt * BV + wv * (BV / WV), tb * BM + wt * (BM / WT));
 }
 
 template <class Src>
-hipError_t quantize_typed(const Src* x, int64_t ld, int64_t R, int64_t K, char* image, float* scale, int pad,
+hipError_t quantize_typed(const Src* x, int64_t ld, int64_t R, int64_t K64, char* image, float* scale, int pad,
                           hipStream_t stream) {
-  const int S = (int)int8_slices(K);
-  const int vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && (ld * (int64_t)sizeof(Src)) % 16 == 0;
+  const int K = (int)K64, S = (int)int8_slices(K);
   const int64_t rows = pad ? (R + kInt8Rows - 1) / kInt8Rows * kInt8Rows : R;
-  if (R < 8192)
-    int8_quantize_kernel<Src, 256><<<(unsigned)rows, 256, 0, stream>>>(x, ld, R, (int)K, S, vec, image, scale);
+  const unsigned many = (unsigned)((rows + kManyRows - 1) / kManyRows);
+  // (a wave a row from 2048 rows on, 8 waves for each CU: 512 rows of 4096 in bf16 ...)
+  if (rows < 2048)
+    int8_quantize_kernel<Src, 256, 2><<<(unsigned)rows, 256, 0, stream>>>(x, ld, R, K, S, image, scale);
+  else if (K <= 1024)
+    int8_quantize_kernel<Src, 64, 1><<<many, 64 * kManyRows, 0, stream>>>(x, ld, R, K, S, image, scale);
+  else if (K <= 4096)
+    int8_quantize_kernel<Src, 64, 4><<<many, 64 * kManyRows, 0, stream>>>(x, ld, R, K, S, image, scale);
   else
-    int8_quantize_kernel<Src, 8><<<(unsigned)((rows + 31) / 32), 256, 0, stream>>>(x, ld, R, (int)K, S, vec, image, scale);
+    int8_quantize_kernel<Src, 64, 8><<<many, 64 * kManyRows, 0, stream>>>(x, ld, R, K, S, image, scale);
   return hipGetLastError();
 }
 
+template <class Out, int BV, int BM, int WV, int WT, int NS>
+void tile_launch(Int8Params p, hipStream_t stream) {
+  p.n_vt = (p.V + BV - 1) / BV;
+  p.n_tb = (p.N + BM - 1) / BM;
+  int8_tile_kernel<Out, BV, BM, WV, WT, NS><<<(unsigned)(p.n_vt * p.n_tb), 64 * WV * WT, 0, stream>>>(p);
+}
+
+// Tiles that fill the card: about one for each of its 256 CUs.
+constexpr int64_t kFull = 240;
+
+// Up to 64 tokens reading W bounds a call, at 5.6 TB/s; tiles of 128 x 64 through LDS reach that wherever there is one for
+// each CU, and with fewer rows the kernel without LDS, whose workgroups are smaller: (K = 4096, V = 16000, 1 token: 11.1
+// us, tiles 16.0; K = 2560, V = 151936, 48 tokens: 99 us, tiles 81.)  With more tokens the largest tile that fills the
+// card (200 tokens, K = 4096: 256 x 256 on V = 128256 142 us and 256 x 128 153; on V = 32000 52 and 37; 128 x 128 on V =
+// 16000 24, 256 x 128 28), and of 256 x 256 and 256 x 128 the one with the fewer padded tokens.
 template <class Out>
 hipError_t logits_typed(Int8Params p, hipStream_t stream) {
-  if (p.N <= 32) {
+  auto tiles = [&](int bv, int bm) { return (int64_t)((p.V + bv - 1) / bv) * ((p.N + bm - 1) / bm); };
+  auto padded = [&](int bm) { return (int64_t)((p.N + bm - 1) / bm * bm); };
+  if (p.N <= 32 && tiles(128, 32) < kFull)
     int8_few_kernel<Out, 1, 1, 4><<<(unsigned)((p.V + 31) / 32), 256, 0, stream>>>(p);
-  } else if (p.N <= 64) {
+  else if (p.N > 32 && p.N <= 64 && tiles(64, 64) < kFull)
     int8_few_kernel<Out, 2, 1, 2><<<(unsigned)((p.V + 31) / 32), 256, 0, stream>>>(p);
-  } else {
-    p.n_vt = (p.V + kBV - 1) / kBV;
-    p.n_tb = (p.N + kBM - 1) / kBM;
-    int8_tile_kernel<Out><<<(unsigned)(p.n_vt * p.n_tb), kTileThreads, 0, stream>>>(p);
-  }
+  else if (p.N <= 64)
+    tile_launch<Out, 128, 64, 2, 2, 4>(p, stream);
+  else if (p.N > 128 && tiles(256, 256) >= kFull && padded(256) <= 1.05 * padded(128))
+    tile_launch<Out, 256, 256, 2, 4, 3>(p, stream);
+  else if (p.N > 128 && tiles(256, 128) >= kFull)
+    tile_launch<Out, 256, 128, 4, 2, 3>(p, stream);
+  else if (tiles(128, 128) >= kFull)
+    tile_launch<Out, 128, 128, 2, 4, 4>(p, stream);
+  else
+    tile_launch<Out, 64, 128, 2, 2, 4>(p, stream);
   return hipGetLastError();
 }
 
@@ -410,8 +479,9 @@ hipError_t int8_pack(const void* q, int64_t ld, int64_t R, int64_t K, void* imag
 hipError_t int8_unpack(const void* image, const float* scale, int64_t R, int64_t K, float* out, hipStream_t stream) {
   if (R == 0 || K == 0) return hipSuccess;
   timing_begin(kKindQuant, stream);
-  int8_unpack_kernel<<<(unsigned)((R + 31) / 32), 256, 0, stream>>>(static_cast<const char*>(image), scale, R, (int)K,
-                                                                    (int)int8_slices(K), out);
+  const int pieces = (int)((K + kUnpackK - 1) / kUnpackK);
+  int8_unpack_kernel<<<(unsigned)((R + 31) / 32 * pieces), 256, 0, stream>>>(static_cast<const char*>(image), scale, R, (int)K,
+                                                                             (int)int8_slices(K), pieces, out);
   timing_end(kKindQuant, stream);
   return hipGetLastError();
 }

@@ -19,7 +19,7 @@ import torch
 from . import _lib
 from ._ops import _plain, _require_device, eager, no_tangents
 
-K_MAX, ROWS_MAX = 2 ** 17, 2 ** 30
+K_MAX, ROWS_MAX = 2 ** 17, 2 ** 25
 
 
 class Int8Rows(NamedTuple):
@@ -131,7 +131,7 @@ def _sizes(name, x):
     if x.dim() != 2:
         raise ValueError(f"{name} must be 2-D, got {tuple(x.shape)}")
     if not 1 <= x.shape[1] <= K_MAX or x.shape[0] > ROWS_MAX:
-        raise ValueError(f"{name} must have 1 to 2^17 columns and at most 2^30 rows, got {tuple(x.shape)}")
+        raise ValueError(f"{name} must have 1 to 2^17 columns and at most 2^25 rows, got {tuple(x.shape)}")
 
 
 def _no_gradient(what, *tensors):

@@ -64,6 +64,7 @@ H = torch.zeros(4, 16)
     lambda: int8.quantize_rows(torch.zeros(9)),
     lambda: int8.quantize_rows(torch.zeros(9, 0)),
     lambda: int8.quantize_rows(torch.zeros(2, 2 ** 17 + 1, **META)),
+    lambda: int8.quantize_rows(torch.zeros(2 ** 25 + 1, 2, **META)),
     lambda: int8.pack_rows(torch.zeros(9, 16), torch.zeros(9)),
     lambda: int8.pack_rows(torch.zeros(9, 16, dtype=torch.int8), torch.zeros(8)),
     lambda: int8.pack_rows(torch.zeros(9, 16, dtype=torch.int8), torch.zeros(9, dtype=torch.int32)),
@@ -237,7 +238,7 @@ def logits(dtype=_lib.BF16, out_dtype=_lib.BF16, N=4, K=16, V=9, h=A, ldh=16, im
     (reorder, dict(steps=(24, -8, 0, 0)), _lib.EINVAL),
     (quantize, dict(dtype=_lib.F64), _lib.EDTYPE),
     (quantize, dict(R=-1), _lib.EINVAL),
-    (quantize, dict(R=2 ** 30 + 1), _lib.EINVAL),
+    (quantize, dict(R=2 ** 25 + 1), _lib.EINVAL),
     (quantize, dict(K=0), _lib.EINVAL),
     (quantize, dict(K=2 ** 17 + 1), _lib.EINVAL),
     (quantize, dict(ld=-1), _lib.EINVAL),
@@ -249,6 +250,7 @@ def logits(dtype=_lib.BF16, out_dtype=_lib.BF16, N=4, K=16, V=9, h=A, ldh=16, im
     (pack, dict(ld=-1), _lib.EINVAL),
     (pack, dict(q=None), _lib.EINVAL),
     (unpack, dict(R=-1), _lib.EINVAL),
+    (unpack, dict(R=2 ** 25, K=4097), _lib.EINVAL),
     (unpack, dict(scale=None), _lib.EINVAL),
     (unpack, dict(out=ctypes.c_void_p(4100)), _lib.EINVAL),
     (logits, dict(dtype=_lib.F64), _lib.EDTYPE),
