@@ -64,14 +64,37 @@ struct Sixteen {
     }
   }
   __device__ __forceinline__ float operator[](int i) const { return (float)v[i / 8][i % 8]; }
-  // the larger of m and all magnitudes, by their bits: an infinity or a NaN is larger than any number
-  __device__ __forceinline__ uint32_t magnitude(uint32_t m) const {
+};
+
+// The largest magnitude of a row by its bits, so that an infinity or a NaN is larger than any number; 2-byte types two
+// at a time.
+template <class Src>
+struct Magnitude {
+  typedef uint16_t U2 __attribute__((ext_vector_type(2)));
+  uint32_t m = 0;
+  __device__ __forceinline__ void add(const Sixteen<Src>& y) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const uint32_t b = __float_as_uint((*this)[i]) & 0x7fffffffu;
-      m = b > m ? b : m;
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < 2 * (int)sizeof(Src); ++i) {
+        uint32_t w;
+        __builtin_memcpy(&w, reinterpret_cast<const char*>(&y.v[h]) + 4 * i, 4);
+        if constexpr (sizeof(Src) == 2) {
+          m = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(U2, m), __builtin_bit_cast(U2, w & 0x7fff7fffu)));
+        } else {
+          const uint32_t b = w & 0x7fffffffu;
+          m = b > m ? b : m;
+        }
+      }
+  }
+  // as the bits of an fp32
+  __device__ __forceinline__ uint32_t bits() const {
+    if constexpr (sizeof(Src) == 4) {
+      return m;
+    } else {
+      const uint16_t a = (uint16_t)m, b = (uint16_t)(m >> 16);
+      return __float_as_uint((float)__builtin_bit_cast(Src, a > b ? a : b)) & 0x7fffffffu;
     }
-    return m;
   }
 };
 
@@ -85,6 +108,35 @@ __device__ __forceinline__ int quantize(float x, float s, float inv, float half)
   const float a = fabsf(d);
   return a > half || (a == half && (n & 1)) ? n + up : n;
 }
+// 16 of them as bytes.  The sum with 1.5 2^23 is rounded to a whole number, whose low byte is the value; only a lane
+// with a remainder of half a step or more needs a second look.
+template <class Src>
+__device__ __forceinline__ uint4 quantize16(const Sixteen<Src>& x, float s, float inv, float half) {
+  constexpr float kRound = 12582912.f;
+  uint32_t w[4];
+  float far = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t b[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const float y = fmaf(x[4 * i + u], inv, kRound);
+      far = fmaxf(far, fabsf(fmaf(kRound - y, s, x[4 * i + u])));
+      b[u] = __float_as_uint(y);
+    }
+    const uint32_t lo = __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400), hi = __builtin_amdgcn_perm(b[3], b[2], 0x0c0c0400);
+    w[i] = __builtin_amdgcn_perm(hi, lo, 0x05040100);
+  }
+  if (far >= half) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      w[i] = 0;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) w[i] |= (uint32_t)(quantize(x[4 * i + u], s, inv, half) & 255) << (8 * u);
+    }
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
 
 // TPR threads a row, a wave for many rows and a workgroup for few, each with NC pieces of 16 values in registers, so
 // that rows of up to 16 NC TPR values are read once (longer ones twice).  A piece goes out as one 16-byte chunk of the
@@ -95,11 +147,11 @@ template <class Src, int TPR, int NC>
 __global__ __launch_bounds__(TPR == 64 ? 64 * kManyRows : TPR) void int8_quantize_kernel(
     const Src* __restrict__ x, int64_t ld, int64_t R, int K, int S, char* __restrict__ image, float* __restrict__ scale) {
   __shared__ uint32_t s_max[4];
-  const int64_t r = TPR == 64 ? (int64_t)blockIdx.x * kManyRows + wave_id() : (int64_t)blockIdx.x;
+  const int64_t r = TPR == 64 ? (int64_t)xcd_swizzle(blockIdx.x, gridDim.x) * kManyRows + wave_id() : (int64_t)blockIdx.x;
   const int j = TPR == 64 ? lane_id() : (int)threadIdx.x;
   const Src* row = x + r * ld;
   Sixteen<Src> v[NC];
-  uint32_t m = 0;
+  Magnitude<Src> most;
   if (r < R) {
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
@@ -108,13 +160,14 @@ __global__ __launch_bounds__(TPR == 64 ? 64 * kManyRows : TPR) void int8_quantiz
     }
 #pragma unroll
     for (int c = 0; c < NC; ++c)
-      if (c * TPR * 16 < K) m = v[c].magnitude(m);
+      if (c * TPR * 16 < K) most.add(v[c]);
     for (int k = (NC * TPR + j) * 16; k < K; k += TPR * 16) {
       Sixteen<Src> y;
       y.load(row, k, K);
-      m = y.magnitude(m);
+      most.add(y);
     }
   }
+  uint32_t m = most.bits();
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
     const uint32_t y = __shfl_xor(m, o);
@@ -131,23 +184,36 @@ __global__ __launch_bounds__(TPR == 64 ? 64 * kManyRows : TPR) void int8_quantiz
   if (j == 0 && r < R) scale[r] = fine ? s : __uint_as_float(0x7fc00000u);
   const bool any = r < R && fine;
   char* out = image + (r >> 5) * S * kInt8Block + (r & 31) * 16;
-  auto put = [&](const Sixteen<Src>& y, int k) {
-    uint32_t w[4] = {0, 0, 0, 0};
-    if (any && k < K) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) w[i / 4] |= (uint32_t)(quantize(y[i], s, inv, half) & 255) << (8 * (i % 4));
-    }
-    *reinterpret_cast<uint4*>(out + (int64_t)(k >> 4) * 512) = make_uint4(w[0], w[1], w[2], w[3]);
+  auto chunk = [&](const Sixteen<Src>& y, int k) {
+    return any && k < K ? quantize16(y, s, inv, half) : make_uint4(0, 0, 0, 0);
   };
+  if constexpr (TPR == 64) {
+    // the 8 rows' chunks of 16 values meet in LDS (row w's of chunk c in place w ^ c % 8 of 8: no bank conflicts), and
+    // 8 lanes write their 128 bytes
+    __shared__ uint4 s_out[NC * 64 * kManyRows];
 #pragma unroll
-  for (int c = 0; c < NC; ++c) {
-    const int k = (c * TPR + j) * 16;
-    if (k < S * 64) put(v[c], k);
+    for (int c = 0; c < NC; ++c) {
+      const int i = c * 64 + j;
+      if (i * 16 < S * 64) s_out[i * kManyRows + (wave_id() ^ (i % kManyRows))] = chunk(v[c], i * 16);
+    }
+    __syncthreads();
+    char* const to = image + (r >> 5) * S * kInt8Block + (r - wave_id() & 31) * 16;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const int q = c * 64 * kManyRows + (int)threadIdx.x, i = q / kManyRows, w = q % kManyRows;
+      if (i * 16 < S * 64) *reinterpret_cast<uint4*>(to + (int64_t)i * 512 + w * 16) = s_out[i * kManyRows + (w ^ (i % kManyRows))];
+    }
+  } else {
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const int k = (c * TPR + j) * 16;
+      if (k < S * 64) *reinterpret_cast<uint4*>(out + (int64_t)(k >> 4) * 512) = chunk(v[c], k);
+    }
   }
   for (int k = (NC * TPR + j) * 16; k < S * 64; k += TPR * 16) {
     Sixteen<Src> y;
     if (any) y.load(row, k < K ? k : K, K);
-    put(y, k);
+    *reinterpret_cast<uint4*>(out + (int64_t)(k >> 4) * 512) = chunk(y, k);
   }
 }
 
