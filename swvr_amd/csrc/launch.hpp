@@ -541,6 +541,7 @@ struct Int8Params {
   int N, V, S;            // S: slices of 64 reduction values
   void* out;              // [N][V]
   int n_vt, n_tb;         // tiles
+  int lines;              // whether out's rows are whole 128-byte lines
 };
 hipError_t int8_logits(int out_dtype, Int8Params p, hipStream_t stream);
 
