@@ -361,14 +361,15 @@ struct __attribute__((packed, aligned(sizeof(Out)))) OutChunk {
   Out v[16 / sizeof(Out)];
 };
 
-// A wave's 32 FM vocabulary rows (from v0) x 32 FN tokens (from n0), through `room` (LDS of this wave, up to 8704 bytes):
-// a lane holds 4 rows of a token, and goes out with 16 bytes of a token's 256 (fewer with fewer rows).
-template <class Out, int FM, int FN>
+// A wave's 32 FM vocabulary rows (from v0) x 32 FN tokens (from n0), through `room` (ROOM bytes of LDS, this wave's): a
+// lane holds 4 rows of a token, and goes out with 16 bytes of a token's 256 (128 with fewer rows or less room).
+template <class Out, int FM, int FN, int ROOM>
 __device__ __forceinline__ void store_tile(const Int8Params& p, const i32x16_t (&acc)[FM][FN], char* room,
                                            const float* scale, const float* bias, int v0, int n0) {
-  constexpr int E = (int)sizeof(Out), FP = FM < 8 / E ? FM : 8 / E;  // FP: blocks of 32 rows in a piece
+  constexpr int E = (int)sizeof(Out), kFit = ROOM >= 32 * (256 + 16) ? 8 / E : 4 / E;
+  constexpr int FP = FM < kFit ? FM : kFit;  // blocks of 32 rows in a piece
   constexpr int kBytes = FP * 32 * E, kPitch = kBytes + 16, kLanes = kBytes / 16;
-  static_assert(FM % FP == 0, "whole pieces");
+  static_assert(FM % FP == 0 && 32 * kPitch <= ROOM, "whole pieces, which fit");
   struct alignas(4 * E) Four {
     Out v[4];
   };
@@ -459,7 +460,8 @@ __global__ __launch_bounds__(64 * WV * WT) void int8_tile_kernel(Int8Params p) {
   ring.template publish_next<L>();
   tile_reduce<int8_t, 32, L>(acc, ta, th, smem, SB, ring, p.S, wv * (BV / WV), wt * (BM / WT), issue_next);  // (two steps a slice)
   stage_barrier();  // every wave has read its last operands: the ring holds the epilogue's rows
-  store_tile<Out, FM, FN>(p, acc, smem + w * (NS * SB / (WV * WT)), s_scale + wv * (BV / WV), s_bias + wv * (BV / WV),
+  constexpr int kRoom = NS * SB / (WV * WT);
+  store_tile<Out, FM, FN, kRoom>(p, acc, smem + w * kRoom, s_scale + wv * (BV / WV), s_bias + wv * (BV / WV),
                           vt * BV + wv * (BV / WV), tb * BM + wt * (BM / WT));
 }
 

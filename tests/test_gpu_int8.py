@@ -148,6 +148,19 @@ def test_logits(N, V, K, dtype):
     check_logits(h, w, bias, logit_scale=0.3, dtype=torch.float32)
 
 
+# a size for each tile, with rows that share lines and rows of whole ones
+@pytest.mark.parametrize("V", [0, 1])
+@pytest.mark.parametrize("N,rows", [(3, 5000), (40, 9000), (5, 31104), (40, 16128), (100, 31104), (300, 21120), (300, 31104),
+                                    (500, 31104), (200, 3000)])
+def test_logits_of_every_tile(N, rows, V):
+    V = rows - 103 * V
+    h = torch.randn(N, 72, device=DEV, generator=gen(N)).to(torch.bfloat16)
+    w = int8.quantize_rows(torch.randn(V, 72, device=DEV, generator=gen(V)))
+    bias = torch.randn(V, device=DEV, generator=gen(V + 1))
+    for dtype in (torch.bfloat16, torch.float32):
+        check_logits(h, w, bias, dtype=dtype)
+
+
 @pytest.mark.parametrize("out", TYPES)
 @pytest.mark.parametrize("kind", TYPES + [torch.float64])
 def test_types_of_the_bias_and_the_logits(kind, out):
