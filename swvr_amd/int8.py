@@ -54,12 +54,13 @@ def _quantize(x):
     return q, scale
 
 
-def _pack(x):
+def _pack(x, scale):
     x = _rows(x)
     R, K = x.shape
-    q = x.new_empty(_image_shape(R, K))
+    q, kept = x.new_empty(_image_shape(R, K)), x.new_empty(R, dtype=torch.float32)
+    kept.copy_(scale)
     _lib.call(_lib.load().swvr_int8_pack, x.device, R, K, x.data_ptr(), _ld(x), q.data_ptr())
-    return q
+    return q, kept
 
 
 def _unpack(q, scale, R, K):
@@ -97,13 +98,13 @@ def _(x):
 
 
 @torch.library.custom_op("swvr::int8_pack", mutates_args=())
-def _pack_op(x: torch.Tensor) -> torch.Tensor:
-    return _pack(x)
+def _pack_op(x: torch.Tensor, scale: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    return _pack(x, scale)
 
 
 @_pack_op.register_fake
-def _(x):
-    return x.new_empty(_image_shape(*x.shape))
+def _(x, scale):
+    return x.new_empty(_image_shape(*x.shape)), x.new_empty(x.shape[0], dtype=torch.float32)
 
 
 @torch.library.custom_op("swvr::int8_unpack", mutates_args=())
@@ -159,7 +160,7 @@ def quantize_rows(x):
 
 
 def pack_rows(q, scale):
-    """``Int8Rows`` from integers ``q`` [R, K] (int8, as a file holds them) and their scales [R]."""
+    """``Int8Rows`` from integers ``q`` [R, K] (int8, as a file holds them) and their scales [R]; both are copied."""
     _sizes("q", q)
     if q.dtype != torch.int8:
         raise ValueError(f"q must be int8, got {q.dtype}")
@@ -168,12 +169,14 @@ def pack_rows(q, scale):
     if scale.device != q.device:
         raise ValueError(f"scale is on {scale.device} but q on {q.device}")
     no_tangents(scale)
-    kept = _plain(scale.detach()).to(torch.float32, copy=True, memory_format=torch.contiguous_format)  # not the caller's
+    scale = scale.detach()
     if eager(q, scale):
-        return Int8Rows(_pack(q), kept, (q.shape[0], q.shape[1]))
-    if q.device.type == "cpu":
-        _require_device(q)
-    return Int8Rows(_pack_op(q), kept, (q.shape[0], q.shape[1]))
+        q8, kept = _pack(q, scale)
+    else:
+        if q.device.type == "cpu":
+            _require_device(q)
+        q8, kept = _pack_op(q, scale)
+    return Int8Rows(q8, kept, (q.shape[0], q.shape[1]))
 
 
 def _checked(w):

@@ -161,6 +161,21 @@ def test_logits_of_every_tile(N, rows, V):
         check_logits(h, w, bias, dtype=dtype)
 
 
+def test_more_values_than_32_bits_count():
+    x = torch.randn(1000, 8192, device=DEV, generator=gen(40)).to(torch.bfloat16).repeat(300, 1)     # 2.5e9
+    x[-1] *= 3
+    w = int8.quantize_rows(x)
+    last = int8.quantize_rows(x[-300:].clone())
+    assert torch.equal(w.scale[-300:], last.scale)
+    back = int8.dequantize(w)
+    assert torch.equal(back[-300:], int8.dequantize(last)) and torch.equal(back[:1000], back[1000:2000])
+    del x, back
+    h = torch.randn(9000, 8192, device=DEV, generator=gen(41)).to(torch.bfloat16)                    # 2.7e9 logits
+    out = int8.head_logits(h, w)
+    for rows in (slice(0, 3), slice(8990, 9000)):
+        assert torch.equal(out[rows], int8.head_logits(h[rows], w))
+
+
 @pytest.mark.parametrize("out", TYPES)
 @pytest.mark.parametrize("kind", TYPES + [torch.float64])
 def test_types_of_the_bias_and_the_logits(kind, out):
@@ -279,7 +294,8 @@ def test_as_traced_and_compiled():
     for x in (W, W.t().contiguous().t()):
         torch.library.opcheck(torch.ops.swvr.int8_quantize.default, (x,), test_utils=utils)
     q = torch.randint(-9, 9, (77, 100), device=DEV, dtype=torch.int8)
-    torch.library.opcheck(torch.ops.swvr.int8_pack.default, (q,), test_utils=utils)
+    for scale in (w.scale, w.scale.double(), torch.stack([w.scale, w.scale], dim=1)[:, 0]):
+        torch.library.opcheck(torch.ops.swvr.int8_pack.default, (q, scale), test_utils=utils)
     torch.library.opcheck(torch.ops.swvr.int8_unpack.default, (w.q, w.scale, 77, 100), test_utils=utils)
     for x in (h, h.transpose(0, 1)):
         torch.library.opcheck(torch.ops.swvr.int8_logits.default, (x, w.q, w.scale, bias, 77, 0.5, torch.float32), test_utils=utils)
@@ -287,6 +303,9 @@ def test_as_traced_and_compiled():
     torch._dynamo.reset()
     got = torch.compile(lambda a, b: int8.head_logits(a * 2, w, b, dtype=torch.float32), fullgraph=True)(h, bias)
     assert torch.equal(got, want)
+    torch._dynamo.reset()
+    packed = torch.compile(lambda a, b: int8.dequantize(int8.pack_rows(a, b)), fullgraph=True)(q, w.scale)
+    assert torch.equal(packed, q.float() * w.scale[:, None])
     torch._dynamo.reset()
     back = torch.compile(lambda a: int8.dequantize(int8.quantize_rows(a * 1)), fullgraph=True)(W)
     assert torch.equal(back, int8.dequantize(w))
