@@ -176,14 +176,14 @@ def _reorder(states, parents, inplace):
     B = 1
     for n in ids.shape[:-1]:
         B *= n
-    groups, out, seen, last = {}, [], set(), None
+    groups, out, seen, last = {}, [], {parents.data_ptr()}, None
     for x in states:
         if inplace:
             if x.is_neg() or x.is_conj() or x._is_zerotensor():
                 raise ValueError("a lazily negated, conjugated or memoryless state cannot be reordered in place")
             at = x.data_ptr()
             if at in seen and x.numel():
-                raise ValueError("the same state twice cannot be reordered in place")
+                raise ValueError("the same state twice, or the parents, cannot be reordered in place")
             seen.add(at)
         else:
             x = _plain(x.resolve_conj() if x.is_conj() else x)
@@ -254,7 +254,7 @@ def reorder_beams(states, parents, *, inplace=False):
     Gives new tensors (of the structure of ``states``), or with ``inplace`` the states themselves, reordered where they
     are: beams that keep their place are then neither read nor written.  In place k must be W, at most 64; leading
     dimensions have to be one in memory, the ones after the beams at most three after merging (one, where a beam has 4
-    GB), and no element may be part of a state twice or of two states.  No gradient: where one would be recorded the call is refused.
+    GB), and no element may be part of a state twice, of two states or of the parents.  No gradient: where one would be recorded the call is refused.
     """
     alone = isinstance(states, torch.Tensor)
     xs = [states] if alone else list(states)

@@ -14,7 +14,7 @@
 //   beam_row_kernel    per beam the lse, and its own k best: they lie in the k groups of the largest maxima (equal ones
 //                      by index), which alone are read again;
 //   beam_merge_kernel  per sequence the best of its beams' lists;
-// the last two in one, a workgroup per sequence (beam_pick_kernel), for up to 16 beams and 64 candidates.
+// the last two in one, a workgroup per sequence (beam_pick_kernel), for up to 16 beams and 32 candidates.
 #include <algorithm>
 
 #include "common.hpp"
@@ -150,6 +150,8 @@ __global__ __launch_bounds__(64 * kScanWaves) void beam_scan_kernel(BeamWork p) 
   }
 }
 
+__device__ __forceinline__ void wave_fence() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
+
 // How many of s[0 .. n - 1] (n padded with zeros to a multiple of kPad) are larger than x.
 constexpr int kPad = 8;
 __device__ __forceinline__ int above(const u64* s, int n, u64 x) {
@@ -224,11 +226,20 @@ __global__ __launch_bounds__(kRowThreads) void beam_row_kernel(BeamWork p) {
   // threads' best), the few that reach it, and of these the places; where they are too many for the list (many large
   // ones with few threads) a round of maxima for each.
   auto first = [&](int n, auto&& place) -> int {
+    // f(place) for this thread's entries, several of them read before the first is used
+    auto each = [&](auto&& f) {
+      constexpr int kAhead = 8;
+#pragma unroll 1
+      for (int i0 = t; i0 < n; i0 += kAhead * kRowThreads) {
+        u64 x[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) x[u] = i0 + u * kRowThreads < n ? place(i0 + u * kRowThreads) : 0;
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) f(x[u]);
+      }
+    };
     u64 best = 0;
-    for (int i = t; i < n; i += kRowThreads) {
-      const u64 x = place(i);
-      best = x > best ? x : best;
-    }
+    each([&](u64 x) { best = x > best ? x : best; });
     __syncthreads();
     s_best[t] = best;
     if (t == 0) {
@@ -238,22 +249,19 @@ __global__ __launch_bounds__(kRowThreads) void beam_row_kernel(BeamWork p) {
     __syncthreads();
     if (best && above(s_best, kRowThreads, best) == k - 1) s_bound = best;
     __syncthreads();
-    for (int i = t; i < n; i += kRowThreads) {
-      const u64 x = place(i);
-      if (x < s_bound) continue;
+    const u64 bound = s_bound;
+    each([&](u64 x) {
+      if (x < bound) return;
       const int at = atomicAdd(&s_n, 1);
       if (at < kListMost) s_list[at] = x;
-    }
+    });
     __syncthreads();
     int found = s_n;
     if (found > kListMost) {
       u64 last = ~0ull;
       for (found = 0; found < k; ++found) {
         best = 0;
-        for (int i = t; i < n; i += kRowThreads) {
-          const u64 x = place(i);
-          best = x < last && x > best ? x : best;
-        }
+        each([&](u64 x) { best = x < last && x > best ? x : best; });
         best = wave_max64(best);
         __syncthreads();
         if (lane_id() == 0) s_best[wave_id()] = best;
@@ -296,72 +304,78 @@ __global__ __launch_bounds__(kRowThreads) void beam_row_kernel(BeamWork p) {
   if (t == 0) p.count[row] = n2;
 }
 
-// One wave per sequence: a lane holds the first candidate left of its beams (lane, lane + 64, ...); k times the best of
-// all goes out, and its beam's next comes up.
+// One wave per sequence: a lane holds the first candidate left of its beam (of PER neighbouring ones); k times the best
+// of all is noted, and its beam's next comes up, from LDS as far as it holds them.  What was noted goes out at the end.
+template <int PER>
 __global__ __launch_bounds__(64) void beam_merge_kernel(BeamWork p) {
+  constexpr int kHeld = 4096;
+  __shared__ double s_rank[kHeld];
+  __shared__ int s_from[kBeamsMost];  // beam << 8 | place in its list
   const int64_t b = blockIdx.x;
-  const int W = p.a.W, k = p.a.k, lane = threadIdx.x;
-  constexpr int kPer = kBeamsMost / 64;
-  int at[kPer], n[kPer];
-  double head[kPer];
+  const int W = p.a.W, k = p.a.k, lane = threadIdx.x, held = min(k, kHeld / W);
+  for (int i = lane; i < W * held; i += 64) {
+    const int w = i / held, at = i % held;
+    if (at < p.count[b * W + w]) s_rank[i] = p.rank[(b * W + w) * k + at];
+  }
+  wave_fence();
+  auto key = [&](int w, int at) {  // larger for a larger rank; not 0
+    const double x = at < held ? s_rank[w * held + at] : p.rank[(b * W + w) * k + at];
+    const u64 y = (u64)__double_as_longlong(x + 0.0);
+    return y >> 63 ? ~y : y | (u64)1 << 63;
+  };
+  int at[PER], n[PER];
+  u64 head[PER];
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const int w = i * 64 + lane;
+  for (int i = 0; i < PER; ++i) {
+    const int w = lane * PER + i;
     at[i] = 0;
     n[i] = w < W ? p.count[b * W + w] : 0;
-    head[i] = n[i] > 0 ? p.rank[(b * W + w) * k] : 0;
+    head[i] = n[i] > 0 ? key(w, 0) : 0;
   }
-  for (int r = 0; r < k; ++r) {
-    // this lane's best beam (-1: none), then the wave's
-    int w = -1;
-    double x = 0;
+  int found = 0;
+#pragma unroll 1
+  for (; found < k; ++found) {
+    u64 best = head[0];
 #pragma unroll
-    for (int i = 0; i < kPer; ++i)
-      if (at[i] < n[i] && (w < 0 || head[i] > x)) {
-        w = i * 64 + lane;
-        x = head[i];
-      }
+    for (int i = 1; i < PER; ++i) best = head[i] > best ? head[i] : best;
+    const u64 top = wave_max64(best);
+    if (top == 0) break;
+    if (lane == __builtin_ctzll(__ballot(best == top))) {
+      bool open = true;  // the first of this lane's that has it
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const double y = __shfl_xor(x, o);
-      const int v = __shfl_xor(w, o);
-      if (v >= 0 && (w < 0 || y > x || (y == x && v < w))) {
-        x = y;
-        w = v;
-      }
-    }
-    const int64_t out = b * k + r;
-    if (w < 0) {
-      if (lane == 0) {
-        p.a.token[out] = -1;
-        p.a.parent[out] = -1;
-        if (p.a.s64) static_cast<double*>(p.a.score)[out] = -__builtin_huge_val();
-        else static_cast<float*>(p.a.score)[out] = kNegInf;
-      }
-      continue;
-    }
-    if (lane == (w & 63)) {
-#pragma unroll
-      for (int i = 0; i < kPer; ++i)
-        if (i == w >> 6) {
-          const int64_t from = (b * W + w) * k + at[i];
-          p.a.token[out] = p.token[from];
-          p.a.parent[out] = w;
-          if (p.a.s64) static_cast<double*>(p.a.score)[out] = p.sum[from];
-          else static_cast<float*>(p.a.score)[out] = (float)p.sum[from];
-          if (++at[i] < n[i]) head[i] = p.rank[from + 1];
+      for (int i = 0; i < PER; ++i)
+        if (open && head[i] == top) {
+          open = false;
+          const int w = lane * PER + i;
+          s_from[found] = w << 8 | at[i];
+          head[i] = ++at[i] < n[i] ? key(w, at[i]) : 0;
         }
     }
   }
+  wave_fence();
+  for (int r = lane; r < k; r += 64) {
+    const int64_t to = b * k + r;
+    const int w = r < found ? s_from[r] >> 8 : -1;
+    const int64_t from = r < found ? (b * W + w) * k + (s_from[r] & 255) : 0;
+    const double score = r < found ? p.sum[from] : -__builtin_huge_val();
+    p.a.token[to] = r < found ? p.token[from] : -1;
+    p.a.parent[to] = w;
+    if (p.a.s64) static_cast<double*>(p.a.score)[to] = score;
+    else static_cast<float*>(p.a.score)[to] = (float)score;
+  }
 }
 
-// ---- both in one launch: a workgroup per sequence, a wave per beam (or two beams)
+// ---- both in one launch: a workgroup per sequence, a wave per beam
 // Bound by the latency of what follows upon each other: what the scan left, the few groups' logits, and one barrier
 // before the merge.  Loops stay loops, with as little as can be: unrolled to hold all maxima in registers this took 15 us
 // for 4 beams of 151936, most of it to fetch its own instructions.
-constexpr int kPickBeams = 16, kPickWaves = 8, kPickMost = 64, kPickList = 256;
+constexpr int kPickBeams = 16, kPickMost = 32, kPickList = 256;
 
-__device__ __forceinline__ void wave_fence() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
+// base + i as a scalar base and a 32-bit offset (not an address in two registers for each load in flight).
+template <class T>
+__device__ __forceinline__ const T* at_offset(const T* base, int i) {
+  return reinterpret_cast<const T*>(reinterpret_cast<const char*>(base) + (uint32_t)i * (uint32_t)sizeof(T));
+}
 
 struct AddF64 {
   __device__ __forceinline__ u64 operator()(u64 a, u64 b) const {
@@ -439,9 +453,9 @@ __device__ __forceinline__ float reached_by(float x, int k, float* s) {
 }
 
 template <class T>
-__global__ __launch_bounds__(64 * kPickWaves) void beam_pick_kernel(BeamWork p) {
-  __shared__ __attribute__((aligned(16))) u64 s_lists[kPickWaves][kPickList + kPad];
-  __shared__ u64 s_chosen[kPickWaves][kPickMost];
+__global__ __launch_bounds__(64 * kPickBeams) void beam_pick_kernel(BeamWork p) {
+  __shared__ __attribute__((aligned(16))) u64 s_lists[kPickBeams][kPickList + kPad];
+  __shared__ u64 s_chosen[kPickBeams][kPickMost];
   // candidate i of beam w at w k + i
   __shared__ double s_rank[kPickBeams * kPickMost], s_sum[kPickBeams * kPickMost];
   __shared__ int64_t s_length[kPickBeams];
@@ -449,12 +463,9 @@ __global__ __launch_bounds__(64 * kPickWaves) void beam_pick_kernel(BeamWork p) 
   const int b = (int)blockIdx.x;
   const int lane = lane_id(), k = p.a.k, W = p.a.W;
   u64* const chosen = s_chosen[wave_id()];
-  // beam w's candidates to s_sum, s_token, best first; how many
-  auto choose = [&](int w) -> int {
-    // (sizes that the compiler takes for new ones: it keeps what follows from them across beams, in more registers than
-    // there are)
-    int n_group = p.n_group, n_sub = p.n_sub, k = p.a.k, lane = lane_id();
-    asm volatile("" : "+s"(n_group), "+s"(n_sub), "+s"(k), "+v"(lane));
+  const int w = wave_id(), n_group = p.n_group, n_sub = p.n_sub;
+  // the beam's candidates to s_sum, s_token, best first; how many
+  auto choose = [&]() -> int {
     const int64_t row = (int64_t)b * W + w;
     const float* const group = p.group + row * n_group;
     const double* const sub_sum = p.sub_sum + row * n_sub;
@@ -466,7 +477,7 @@ __global__ __launch_bounds__(64 * kPickWaves) void beam_pick_kernel(BeamWork p) 
 #pragma unroll
     for (int j = 0; j < kHeld; ++j) {
       if (j % 16 == 0 && j * 64 >= n_group) break;
-      g[j] = group[min(j * 64 + lane, n_group - 1)];
+      g[j] = *at_offset(group, min(j * 64 + lane, n_group - 1));
     }
     const float max0 = sub_max[min(lane, n_sub - 1)], max1 = sub_max[min(lane + 64, n_sub - 1)];
     const double sum0 = sub_sum[min(lane, n_sub - 1)], sum1 = sub_sum[min(lane + 64, n_sub - 1)];
@@ -531,7 +542,7 @@ __global__ __launch_bounds__(64 * kPickWaves) void beam_pick_kernel(BeamWork p) 
 #pragma unroll
       for (int s = 0; s < kAhead; ++s) {
         at[s] = (int)index_at(chosen[min(s0 + s, groups - 1)]) * kGroup + lane * 2;
-        c[s] = *reinterpret_cast<const Pair*>(x + min(at[s], V - 2));
+        c[s] = *reinterpret_cast<const Pair*>(at_offset(x, min(at[s], V - 2)));
       }
 #pragma unroll
       for (int s = 0; s < kAhead; ++s) {
@@ -571,17 +582,12 @@ __global__ __launch_bounds__(64 * kPickWaves) void beam_pick_kernel(BeamWork p) 
     });
     return list.n < k ? list.n : k;
   };
-#pragma unroll 1
-  for (int w = wave_id(); w < W; w += kPickWaves) {
-    const int n = choose(w);
-    if (lane == 0) s_count[w] = n;
-    wave_fence();  // (the lists are the next beam's)
-  }
-#pragma unroll 1
-  for (int w = wave_id(); w < W; w += kPickWaves) {
+  const int mine_n = choose();
+  if (lane == 0) s_count[w] = mine_n;
+  wave_fence();
+  if (lane < k) {
     const double by = divides(p.a) ? divisor(p.a, s_length[w]) : 1.0;
-    if (lane >= k) continue;
-    s_rank[w * k + lane] = lane < s_count[w] ? s_sum[w * k + lane] / by : -__builtin_huge_val();  // (none: after all that are)
+    s_rank[w * k + lane] = lane < mine_n ? s_sum[w * k + lane] / by : -__builtin_huge_val();  // (none: after all that are)
     s_before[w * k + lane] = 0;
   }
   __syncthreads();
@@ -595,24 +601,21 @@ __global__ __launch_bounds__(64 * kPickWaves) void beam_pick_kernel(BeamWork p) 
   int width = 1;
   while (width < k) width *= 2;
   const int i = lane & (width - 1), share = lane / width, shares = 64 / width, all = W * k;
-#pragma unroll 1
-  for (int w = wave_id(); w < W; w += kPickWaves) {
-    const int me = w * k + i, n = s_count[w];
-    const double mine = i < n ? s_rank[me] : 0;
-    int before = 0;
+  const int me = w * k + i;
+  const double mine = i < mine_n ? s_rank[me] : 0;
+  int before = 0;
 #pragma unroll 4
-    for (int e = share; e < all; e += shares) {
-      const double x = s_rank[e];
-      before += x > mine || (x == mine && e < me);
-    }
-    if (i < n) atomicAdd(&s_before[me], before);
-    wave_fence();
-    if (lane < n) {
-      const int to = s_before[w * k + lane];
-      if (to < k) put((int64_t)b * k + to, s_token[w * k + lane], w, s_sum[w * k + lane]);
-    }
+  for (int e = share; e < all; e += shares) {
+    const double x = s_rank[e];
+    before += x > mine || (x == mine && e < me);
   }
-  if (wave_id() == 0) {
+  if (i < mine_n) atomicAdd(&s_before[me], before);
+  wave_fence();
+  if (lane < mine_n) {
+    const int to = s_before[w * k + lane];
+    if (to < k) put((int64_t)b * k + to, s_token[w * k + lane], w, s_sum[w * k + lane]);
+  }
+  if (w == 0) {
     const int found = (int)wave_sum64(lane < W ? s_count[lane] : 0);
     if (lane >= found && lane < k) put((int64_t)b * k + lane, -1, -1, -__builtin_huge_val());
   }
@@ -643,10 +646,13 @@ hipError_t run(BeamWork p, hipStream_t stream) {
   const int64_t rows = p.a.B * p.a.W;
   beam_scan_kernel<T><<<(unsigned)(rows * p.n_seg), 64 * kScanWaves, 0, stream>>>(p);
   if (p.a.W <= kPickBeams && p.a.k <= kPickMost && p.a.V >= 2) {
-    beam_pick_kernel<T><<<(unsigned)p.a.B, 64 * std::min(p.a.W, kPickWaves), 0, stream>>>(p);
+    beam_pick_kernel<T><<<(unsigned)p.a.B, 64 * p.a.W, 0, stream>>>(p);
   } else {
     beam_row_kernel<T><<<(unsigned)rows, kRowThreads, 0, stream>>>(p);
-    beam_merge_kernel<<<(unsigned)p.a.B, 64, 0, stream>>>(p);
+    if (p.a.W <= 64)
+      beam_merge_kernel<1><<<(unsigned)p.a.B, 64, 0, stream>>>(p);
+    else
+      beam_merge_kernel<kBeamsMost / 64><<<(unsigned)p.a.B, 64, 0, stream>>>(p);
   }
   return hipGetLastError();
 }

@@ -387,6 +387,16 @@ def test_a_list_of_all_sorts():
     check_states(xs, p)
 
 
+def test_more_logits_than_32_bits_count():
+    x = torch.empty(1, 256, 2 ** 21, dtype=torch.bfloat16, device=DEV).expand(5, 256, 2 ** 21)   # (views of one GB)
+    x[0].normal_(generator=gen(90))
+    s = -torch.rand(5, 256, device=DEV, generator=gen(91))
+    want = swvr_amd.select_beams(x[:1], s[4:], 3)
+    y = torch.empty(5 * 256, 2 ** 21, dtype=torch.bfloat16, device=DEV).view(5, 256, 2 ** 21)     # 2.7e9 logits
+    y.copy_(x)
+    assert all(torch.equal(a[4:], b) for a, b in zip(swvr_amd.select_beams(y, s, 3), want))
+
+
 def test_offsets_past_32_bits():
     x = torch.empty(2, 3, 2 ** 30, dtype=torch.uint8, device=DEV)     # 6 GB
     for b in range(2):
@@ -422,7 +432,7 @@ def test_states_that_cannot_be_reordered_in_place():
     p = torch.zeros(2, 3, dtype=torch.int64, device=DEV)
     x = state((2, 3, 4), torch.float32)
     wide = state((2, 3, 4, 4, 4, 4, 4), torch.float32)[:, :, :3, :3, :3, :3, :3]
-    for bad in ([x, x], x[:, :1].expand(2, 3, 4), x[:1].expand(2, 3, 4), x[..., :1].expand(2, 3, 4), wide,
+    for bad in ([x, x], [x, p], x[:, :1].expand(2, 3, 4), x[:1].expand(2, 3, 4), x[..., :1].expand(2, 3, 4), wide,
                 state((20,), torch.float32).as_strided((2, 3, 4), (8, 2, 1)), state((3, 2, 2, 9), torch.float32)):
         with pytest.raises(ValueError):
             swvr_amd.reorder_beams(bad, p, inplace=True)
