@@ -246,7 +246,7 @@ def _(states, parents):
 def reorder_beams(states, parents, *, inplace=False):
     """The beams' states in the order of the beams that were kept: ``out[..., j, *] = state[..., parents[..., j], *]``.
 
-    states: a tensor, or a list or tuple of them (the caches of every layer, say: those of one shape and layout are one
+    states: a tensor, or a list or (named) tuple of them (the caches of every layer, say: those of one shape and layout are one
     launch), each ``[..., W, *]`` with the leading dimensions of ``parents`` ``[..., k]`` (integers) before the beams
     and anything after them, of any dtype; a part of a cache goes in as a view, ``cache[:, :, :, :length]``.  A parent
     outside 0 .. W - 1 (-1 of ``select_beams``, for a beam that there is none of) gives zeros.
@@ -254,7 +254,8 @@ def reorder_beams(states, parents, *, inplace=False):
     Gives new tensors (of the structure of ``states``), or with ``inplace`` the states themselves, reordered where they
     are: beams that keep their place are then neither read nor written.  In place k must be W, at most 64; leading
     dimensions have to be one in memory, the ones after the beams at most three after merging (one, where a beam has 4
-    GB), and no element may be part of a state twice, of two states or of the parents.  No gradient: where one would be recorded the call is refused.
+    GB), and no element may be part of a state twice, of two states or of the parents.  No gradient: where one would be
+    recorded the call is refused.
     """
     alone = isinstance(states, torch.Tensor)
     xs = [states] if alone else list(states)
@@ -293,4 +294,7 @@ def reorder_beams(states, parents, *, inplace=False):
             out = _reorder_op(xs, parents)
     if inplace:
         return states
-    return out[0] if alone else type(states)(out) if isinstance(states, (list, tuple)) else out
+    if alone:
+        return out[0]
+    kind = type(states)
+    return kind(*out) if hasattr(kind, "_fields") else kind(out) if isinstance(states, (list, tuple)) else out

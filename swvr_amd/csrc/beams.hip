@@ -14,7 +14,7 @@
 //   beam_row_kernel    per beam the lse, and its own k best: they lie in the k groups of the largest maxima (equal ones
 //                      by index), which alone are read again;
 //   beam_merge_kernel  per sequence the best of its beams' lists;
-// the last two in one, a workgroup per sequence (beam_pick_kernel), for up to 16 beams and 32 candidates.
+// the last two in one, a workgroup per sequence (beam_pick_kernel), for up to 256 candidates.
 #include <algorithm>
 
 #include "common.hpp"
@@ -38,6 +38,8 @@ struct BeamWork {
   double* sum;       // [rows][k]
   int* token;        // [rows][k]
   int* count;        // [rows]
+  u64* part_key;     // [B][parts][k], of a merge in two launches
+  uint16_t* part_from;
 };
 
 __device__ __forceinline__ double score_of(const BeamParams& a, int64_t row) {
@@ -181,7 +183,7 @@ __global__ __launch_bounds__(kRowThreads) void beam_row_kernel(BeamWork p) {
   __shared__ double s_sum[kRowThreads / 64];
   __shared__ float s_max[kRowThreads / 64];
   __shared__ u64 s_bound;
-  __shared__ int s_n;
+  __shared__ int s_n, s_more;
   const int64_t row = blockIdx.x;
   const int t = threadIdx.x, k = p.a.k;
   const double score = score_of(p.a, row);
@@ -222,60 +224,100 @@ __global__ __launch_bounds__(kRowThreads) void beam_row_kernel(BeamWork p) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
   if (lane_id() == 0) s_sum[wave_id()] = sum;
-  // The k first of n entries place(i), in order, to s_list; how many.  A bound that k of them reach (the k-th of the
-  // threads' best), the few that reach it, and of these the places; where they are too many for the list (many large
-  // ones with few threads) a round of maxima for each.
-  auto first = [&](int n, auto&& place) -> int {
-    // f(place) for this thread's entries, several of them read before the first is used
-    auto each = [&](auto&& f) {
-      constexpr int kAhead = 8;
+  // The k first of what n blocks of 8 hold, in order, to s_order; how many.  load(i, at, from): block i, its first one at
+  // index `at`, those before `from` another block's.  A bound that k of them reach (where `bound` is 0: the k-th of the
+  // threads' best), the few that reach it, and of these the places.
+  auto first = [&](int n, u64 bound, auto&& load) -> int {
+    // f(value, index) for this thread's, but for blocks whose largest is below `least`; several are read before the
+    // first is used
+    auto each = [&](float least, auto&& f) {
+      constexpr int kAhead = 4;
 #pragma unroll 1
       for (int i0 = t; i0 < n; i0 += kAhead * kRowThreads) {
-        u64 x[kAhead];
+        decltype(load(0, i0, i0)) x[kAhead];
+        int at[kAhead], from[kAhead];
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u) x[u] = i0 + u * kRowThreads < n ? place(i0 + u * kRowThreads) : 0;
+        for (int u = 0; u < kAhead; ++u) {
+          const int i = i0 + u * kRowThreads;
+          x[u] = load(i < n ? i : n - 1, at[u], from[u]);
+          if (i >= n) from[u] = at[u] + kLane;
+        }
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u) f(x[u]);
+        for (int u = 0; u < kAhead; ++u) {
+          float v[kLane], top = kNegInf;
+#pragma unroll
+          for (int e = 0; e < kLane; ++e) {
+            v[e] = at[u] + e >= from[u] ? (float)x[u][e] : kNegInf;
+            top = fmaxf(top, v[e]);  // (NaN: the other)
+          }
+          if (!(top >= least && top > kNegInf)) continue;
+#pragma unroll
+          for (int e = 0; e < kLane; ++e) f(v[e], at[u] + e);
+        }
       }
     };
-    u64 best = 0;
-    each([&](u64 x) { best = x > best ? x : best; });
-    __syncthreads();
-    s_best[t] = best;
-    if (t == 0) {
-      s_bound = 1;
-      s_n = 0;
+    if (bound == 0) {
+      float best = kNegInf;
+      each(kNegInf, [&](float x, int) { best = fmaxf(best, x); });
+      const u64 mine = place_of(key_of(best), t);
+      __syncthreads();
+      s_best[t] = mine;
+      if (t == 0) s_bound = 0;
+      __syncthreads();
+      if (mine && above(s_best, kRowThreads, mine) == k - 1) s_bound = (u64)key_at(mine) << 32;
+      __syncthreads();
+      bound = s_bound;
     }
-    __syncthreads();
-    if (best && above(s_best, kRowThreads, best) == k - 1) s_bound = best;
-    __syncthreads();
-    const u64 bound = s_bound;
-    each([&](u64 x) {
-      if (x < bound) return;
-      const int at = atomicAdd(&s_n, 1);
-      if (at < kListMost) s_list[at] = x;
-    });
-    __syncthreads();
-    int found = s_n;
+    auto collect = [&]() -> int {
+      __syncthreads();
+      if (t == 0) s_n = 0;
+      __syncthreads();
+      const float least = logit_of(key_at(bound));
+      each(least, [&](float x, int i) {
+        if (!(x >= least)) return;
+        const u64 y = place_of(key_of(x), i);
+        if (y == 0 || y < bound) return;
+        const int to = atomicAdd(&s_n, 1);
+        if (to < kListMost) s_list[to] = y;
+      });
+      __syncthreads();
+      return s_n;
+    };
+    int found = collect();
     if (found > kListMost) {
-      u64 last = ~0ull;
-      for (found = 0; found < k; ++found) {
-        best = 0;
-        each([&](u64 x) { best = x < last && x > best ? x : best; });
-        best = wave_max64(best);
+      // Too many reach it (equal ones, or the largest with few threads).  A higher bound, 8 bits at a time, by how many
+      // there are of each next byte: `need` of those with the bits so far are still to be had.
+      int* const count = reinterpret_cast<int*>(s_best);
+      int need = k;
+      bound = 0;
+#pragma unroll 1
+      for (int shift = 56; found > kListMost; shift -= 8) {
+        count[t] = 0;
         __syncthreads();
-        if (lane_id() == 0) s_best[wave_id()] = best;
+        each(kNegInf, [&](float x, int i) {
+          const u64 y = place_of(key_of(x), i);
+          if (y && (shift == 56 || (y ^ bound) >> (shift + 8) == 0)) atomicAdd(&count[y >> shift & 255], 1);
+        });
         __syncthreads();
-#pragma unroll
-        for (int i = 0; i < kRowThreads / 64; ++i) best = s_best[i] > best ? s_best[i] : best;
-        if (best == 0) break;
-        if (t == 0) s_list[found] = best;
-        last = best;
+        int more = 0;
+#pragma unroll 4
+        for (int i = t + 1; i < 256; ++i) more += count[i];
+        if (more < need && more + count[t] >= need) {  // (one thread's)
+          s_bound = bound | (u64)t << shift;
+          s_n = more;
+          s_more = count[t];
+        }
+        __syncthreads();
+        bound = s_bound;
+        need -= s_n;
+        found = k - need + s_more;  // how many reach it
+        __syncthreads();
       }
+      found = collect();
     }
-    __syncthreads();
     if (t < kPad) s_list[found + t] = 0;
     __syncthreads();
+#pragma unroll 1
     for (int i = t; i < found; i += kRowThreads) {
       const u64 x = s_list[i];
       const int r = above(s_list, found, x);
@@ -284,13 +326,20 @@ __global__ __launch_bounds__(kRowThreads) void beam_row_kernel(BeamWork p) {
     __syncthreads();
     return found < k ? found : k;
   };
-  const int groups = first(p.n_group, [&](int i) { return place_of(key_of(group[i]), i); });
+  const int groups = first(p.n_group / kLane, 0, [&](int i, int& at, int& from) {
+    at = from = i * kLane;
+    return whole_logits(group + at);
+  });
   if (t < groups) s_group[t] = (int)index_at(s_order[t]);
+  // k groups: each has one that reaches the last one's largest
+  const u64 reached = groups == k ? (u64)key_at(s_order[k - 1]) << 32 : 0;
   __syncthreads();
   const T* const x = static_cast<const T*>(p.a.logits) + row * p.a.ld;
-  const int n2 = first(groups * kGroup, [&](int i) -> u64 {
-    const int v = s_group[i / kGroup] * kGroup + i % kGroup;
-    return v < p.a.V ? place_of(key_of((float)x[v]), v) : 0;
+  const int V = (int)p.a.V;
+  const int n2 = first(groups * (kGroup / kLane), reached, [&](int i, int& at, int& from) {
+    from = s_group[i / (kGroup / kLane)] * kGroup + i % (kGroup / kLane) * kLane;
+    at = min(from, max(V - kLane, 0));  // (at the row's end the last 8)
+    return V < kLane ? load_logits(x, at, V) : whole_logits(x + at);
   });
   const double rest = log(s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3]);  // lse - m
   const double by = divides(p.a) ? divisor(p.a, length_of(p.a, row, 1)) : 1.0;
@@ -304,62 +353,68 @@ __global__ __launch_bounds__(kRowThreads) void beam_row_kernel(BeamWork p) {
   if (t == 0) p.count[row] = n2;
 }
 
-// One wave per sequence: a lane holds the first candidate left of its beam (of PER neighbouring ones); k times the best
-// of all is noted, and its beam's next comes up, from LDS as far as it holds them.  What was noted goes out at the end.
-template <int PER>
-__global__ __launch_bounds__(64) void beam_merge_kernel(BeamWork p) {
-  constexpr int kHeld = 4096;
-  __shared__ double s_rank[kHeld];
-  __shared__ int s_from[kBeamsMost];  // beam << 8 | place in its list
-  const int64_t b = blockIdx.x;
-  const int W = p.a.W, k = p.a.k, lane = threadIdx.x, held = min(k, kHeld / W);
-  for (int i = lane; i < W * held; i += 64) {
-    const int w = i / held, at = i % held;
-    if (at < p.count[b * W + w]) s_rank[i] = p.rank[(b * W + w) * k + at];
-  }
-  wave_fence();
-  auto key = [&](int w, int at) {  // larger for a larger rank; not 0
-    const double x = at < held ? s_rank[w * held + at] : p.rank[(b * W + w) * k + at];
-    const u64 y = (u64)__double_as_longlong(x + 0.0);
-    return y >> 63 ? ~y : y | (u64)1 << 63;
-  };
-  int at[PER], n[PER];
-  u64 head[PER];
-#pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int w = lane * PER + i;
-    at[i] = 0;
-    n[i] = w < W ? p.count[b * W + w] : 0;
-    head[i] = n[i] > 0 ? key(w, 0) : 0;
-  }
-  int found = 0;
-#pragma unroll 1
-  for (; found < k; ++found) {
-    u64 best = head[0];
-#pragma unroll
-    for (int i = 1; i < PER; ++i) best = head[i] > best ? head[i] : best;
-    const u64 top = wave_max64(best);
-    if (top == 0) break;
-    if (lane == __builtin_ctzll(__ballot(best == top))) {
-      bool open = true;  // the first of this lane's that has it
-#pragma unroll
-      for (int i = 0; i < PER; ++i)
-        if (open && head[i] == top) {
-          open = false;
-          const int w = lane * PER + i;
-          s_from[found] = w << 8 | at[i];
-          head[i] = ++at[i] < n[i] ? key(w, at[i]) : 0;
-        }
+// Lists are merged two by two in LDS: an entry's place in both is its own and the number in the other list that come
+// before it (of equal ones the lower beam's), found by halving.  A workgroup takes `per` of a sequence's beams; where
+// that leaves several lists, a second launch merges those.
+constexpr int kMergeHeld = 4096, kMergeThreads = 1024;
+__global__ __launch_bounds__(kMergeThreads) void beam_merge_kernel(BeamWork p, int per, bool second) {
+  __shared__ u64 s_key[2][kMergeHeld];        // larger for a larger rank; 0: none
+  __shared__ uint16_t s_from[2][kMergeHeld];  // beam << 8 | place in its list
+  const int W = p.a.W, k = p.a.k, t = threadIdx.x, threads = blockDim.x, parts = (W + per - 1) / per;
+  const int64_t b = second ? blockIdx.x : blockIdx.x / parts;
+  const int w0 = second ? 0 : (int)(blockIdx.x % parts) * per;
+  int lists = second ? parts : min(per, W - w0);
+  for (int e = t; e < lists * k; e += threads) {
+    const int w = w0 + e / k, i = e % k;
+    if (second) {
+      s_key[0][e] = p.part_key[b * parts * k + e];
+      s_from[0][e] = p.part_from[b * parts * k + e];
+    } else {
+      const u64 y = (u64)__double_as_longlong(p.rank[(b * W + w) * k + i] + 0.0);  // (-0 is 0)
+      s_key[0][e] = i >= p.count[b * W + w] ? 0 : y >> 63 ? ~y : y | (u64)1 << 63;
+      s_from[0][e] = (uint16_t)(w << 8 | i);
     }
   }
-  wave_fence();
-  for (int r = lane; r < k; r += 64) {
-    const int64_t to = b * k + r;
-    const int w = r < found ? s_from[r] >> 8 : -1;
-    const int64_t from = r < found ? (b * W + w) * k + (s_from[r] & 255) : 0;
-    const double score = r < found ? p.sum[from] : -__builtin_huge_val();
-    p.a.token[to] = r < found ? p.token[from] : -1;
-    p.a.parent[to] = w;
+  __syncthreads();
+  int in = 0, top = 1;
+  while (2 * top <= k) top *= 2;
+#pragma unroll 1
+  for (; lists > 1; lists = (lists + 1) / 2, in ^= 1) {
+#pragma unroll 1
+    for (int e = t; e < lists * k; e += threads) {
+      const int l = e / k;
+      const u64 x = s_key[in][e];
+      int to = e - l * k;
+      if ((l ^ 1) < lists) {
+        const u64* const other = s_key[in] + (l ^ 1) * k;
+        int n = 0;
+#pragma unroll 1
+        for (int step = top; step > 0; step >>= 1) {
+          if (n + step > k) continue;
+          const u64 y = other[n + step - 1];
+          n += y > x || (y == x && (l & 1)) ? step : 0;
+        }
+        to += n;
+      }
+      if (to < k) {
+        s_key[in ^ 1][(l >> 1) * k + to] = x;
+        s_from[in ^ 1][(l >> 1) * k + to] = s_from[in][e];
+      }
+    }
+    __syncthreads();
+  }
+  for (int r = t; r < k; r += threads) {
+    if (!second && parts > 1) {
+      p.part_key[(int64_t)blockIdx.x * k + r] = s_key[in][r];
+      p.part_from[(int64_t)blockIdx.x * k + r] = s_from[in][r];
+      continue;
+    }
+    const bool any = s_key[in][r] != 0;
+    const int w = s_from[in][r] >> 8;
+    const int64_t to = b * k + r, from = (b * W + w) * k + (s_from[in][r] & 255);
+    const double score = any ? p.sum[from] : -__builtin_huge_val();
+    p.a.token[to] = any ? p.token[from] : -1;
+    p.a.parent[to] = any ? w : -1;
     if (p.a.s64) static_cast<double*>(p.a.score)[to] = score;
     else static_cast<float*>(p.a.score)[to] = (float)score;
   }
@@ -369,7 +424,7 @@ __global__ __launch_bounds__(64) void beam_merge_kernel(BeamWork p) {
 // Bound by the latency of what follows upon each other: what the scan left, the few groups' logits, and one barrier
 // before the merge.  Loops stay loops, with as little as can be: unrolled to hold all maxima in registers this took 15 us
 // for 4 beams of 151936, most of it to fetch its own instructions.
-constexpr int kPickBeams = 16, kPickMost = 32, kPickList = 256;
+constexpr int kPickBeams = 16, kPickMost = 32, kPickAll = 256, kPickList = 256;
 
 // base + i as a scalar base and a 32-bit offset (not an address in two registers for each load in flight).
 template <class T>
@@ -457,9 +512,9 @@ __global__ __launch_bounds__(64 * kPickBeams) void beam_pick_kernel(BeamWork p) 
   __shared__ __attribute__((aligned(16))) u64 s_lists[kPickBeams][kPickList + kPad];
   __shared__ u64 s_chosen[kPickBeams][kPickMost];
   // candidate i of beam w at w k + i
-  __shared__ double s_rank[kPickBeams * kPickMost], s_sum[kPickBeams * kPickMost];
+  __shared__ double s_rank[kPickAll], s_sum[kPickAll];
   __shared__ int64_t s_length[kPickBeams];
-  __shared__ int s_token[kPickBeams * kPickMost], s_before[kPickBeams * kPickMost], s_count[kPickBeams];
+  __shared__ int s_token[kPickAll], s_before[kPickAll], s_count[kPickBeams];
   const int b = (int)blockIdx.x;
   const int lane = lane_id(), k = p.a.k, W = p.a.W;
   u64* const chosen = s_chosen[wave_id()];
@@ -623,12 +678,16 @@ __global__ __launch_bounds__(64 * kPickBeams) void beam_pick_kernel(BeamWork p) 
 
 int64_t up8(int64_t x) { return (x + 7) / 8 * 8; }
 
+int beams_a_part(int W, int k) { return std::min(W, kMergeHeld / k); }
+static_assert(kBeamsMost * kBeamsMost <= kMergeHeld / kBeamsMost * kMergeHeld, "what the parts leave is one workgroup's");
+
 struct BeamSizes {
   int n_sub, n_group;
-  int64_t group, sub_max, sub_sum, rank, sum, token, count;
-  int64_t all() const { return group + sub_max + sub_sum + rank + sum + token + count; }
+  int64_t group, sub_max, sub_sum, rank, sum, token, count, part_key, part_from;
+  int64_t all() const { return group + sub_max + sub_sum + rank + sum + token + count + part_key + part_from; }
 };
-BeamSizes beam_sizes(int64_t rows, int64_t V, int k) {
+BeamSizes beam_sizes(int64_t B, int W, int64_t V, int k) {
+  const int64_t rows = B * W;
   BeamSizes z;
   z.n_sub = (int)((V + kSub - 1) / kSub);
   z.n_group = z.n_sub * kSubGroups;
@@ -638,6 +697,10 @@ BeamSizes beam_sizes(int64_t rows, int64_t V, int k) {
   z.rank = z.sum = rows * k * 8;
   z.token = up8(rows * k * 4);
   z.count = up8(rows * 4);
+  const int per = beams_a_part(W, k);
+  const int64_t parts = per < W ? B * ((W + per - 1) / per) * k : 0;
+  z.part_key = parts * 8;
+  z.part_from = up8(parts * 2);
   return z;
 }
 
@@ -645,14 +708,17 @@ template <class T>
 hipError_t run(BeamWork p, hipStream_t stream) {
   const int64_t rows = p.a.B * p.a.W;
   beam_scan_kernel<T><<<(unsigned)(rows * p.n_seg), 64 * kScanWaves, 0, stream>>>(p);
-  if (p.a.W <= kPickBeams && p.a.k <= kPickMost && p.a.V >= 2) {
+  // In one launch up to 256 candidates of 16 beams, 32 each.  (Both launches, 151936 logits: 4 beams of 4 11.5 us, in two
+  // 18.1; 8 of 16 16.5, 20.9; 8 of 32 23.7, 22.7; 16 of 16 23.1, 22.4; 16 of 32 38.3, 24.4: a wave has a beam's list to
+  // itself, and each candidate looks at all others.)
+  if (p.a.W <= kPickBeams && p.a.k <= kPickMost && p.a.W * p.a.k <= kPickAll && p.a.V >= 2) {
     beam_pick_kernel<T><<<(unsigned)p.a.B, 64 * p.a.W, 0, stream>>>(p);
   } else {
     beam_row_kernel<T><<<(unsigned)rows, kRowThreads, 0, stream>>>(p);
-    if (p.a.W <= 64)
-      beam_merge_kernel<1><<<(unsigned)p.a.B, 64, 0, stream>>>(p);
-    else
-      beam_merge_kernel<kBeamsMost / 64><<<(unsigned)p.a.B, 64, 0, stream>>>(p);
+    const int per = beams_a_part(p.a.W, p.a.k), parts = (p.a.W + per - 1) / per;
+    auto threads = [&](int lists) { return (unsigned)std::min(kMergeThreads, (lists * p.a.k + 63) / 64 * 64); };
+    beam_merge_kernel<<<(unsigned)(p.a.B * parts), threads(per), 0, stream>>>(p, per, false);
+    if (parts > 1) beam_merge_kernel<<<(unsigned)p.a.B, threads(parts), 0, stream>>>(p, per, true);
   }
   return hipGetLastError();
 }
@@ -715,12 +781,11 @@ hipError_t reorder_run(const ReorderParams& p, hipStream_t stream) {
 
 }  // namespace
 
-size_t beams_workspace_bytes(int64_t B, int W, int64_t V, int k) { return (size_t)beam_sizes(B * W, V, k).all(); }
+size_t beams_workspace_bytes(int64_t B, int W, int64_t V, int k) { return (size_t)beam_sizes(B, W, V, k).all(); }
 
 hipError_t beams_launch(int dtype, const BeamParams& a, char* ws, hipStream_t stream) {
   if (a.B == 0) return hipSuccess;
-  const int64_t rows = a.B * a.W;
-  const BeamSizes z = beam_sizes(rows, a.V, a.k);
+  const BeamSizes z = beam_sizes(a.B, a.W, a.V, a.k);
   BeamWork p{};
   p.a = a;
   p.n_sub = z.n_sub;
@@ -733,6 +798,8 @@ hipError_t beams_launch(int dtype, const BeamParams& a, char* ws, hipStream_t st
   p.token = reinterpret_cast<int*>(ws += z.sum);
   p.count = reinterpret_cast<int*>(ws += z.token);
   p.sub_max = reinterpret_cast<float*>(ws += z.count);
+  p.part_key = reinterpret_cast<u64*>(ws += z.sub_max);
+  p.part_from = reinterpret_cast<uint16_t*>(ws += z.part_key);
   hipError_t e;
   timing_begin(kKindBeams, stream);
   switch (dtype) {

@@ -1,5 +1,6 @@
 """Host-side checks of the decoding operators that need no GPU: refused arguments, shapes under tracing, and the C ABI's
 own checks (nothing is launched)."""
+import collections
 import ctypes
 
 import pytest
@@ -124,6 +125,10 @@ def test_meta_tensors_give_shapes():
     c = torch.zeros(2, 5, 3, 7, 8, dtype=torch.int8, **META)
     assert swvr_amd.reorder_beams(c, parent).shape == (2, 5, 6, 7, 8)
     assert swvr_amd.reorder_beams([c], parent[..., :3], inplace=True)[0] is c
+    cache = collections.namedtuple("Cache", "k v")(c, c.float())
+    moved = swvr_amd.reorder_beams(cache, parent)
+    assert type(moved) is type(cache) and moved.k.shape == moved.v.shape == (2, 5, 6, 7, 8) and moved.v.dtype == torch.float32
+    assert swvr_amd.reorder_beams(cache, parent[..., :3], inplace=True) is cache
     w = int8.quantize_rows(torch.zeros(300, 100, **META))
     assert w.q.shape == (16, 2, 2048) and w.scale.shape == (300,) and w.shape == (300, 100)
     assert int8.dequantize(w).shape == (300, 100)

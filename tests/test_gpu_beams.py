@@ -92,6 +92,25 @@ def test_sizes(B, W, V, k, dtype):
     check(x, s, k)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("B,W,V,k", [(2, 17, 2, 5), (1, 20, 7, 3), (1, 17, 8, 64), (1, 33, 9, 33), (2, 2, 127, 33), (1, 17, 130, 1),
+                                     (1, 5, 3001, 250), (2, 64, 2050, 64), (1, 65, 700, 64), (1, 100, 515, 100), (1, 256, 300, 256),
+                                     (2, 255, 129, 17), (1, 2, 32000, 256), (1, 256, 64, 1)])
+def test_many_beams_and_candidates(B, W, V, k, dtype):
+    x, s = make(B, W, V, dtype, seed=7)
+    check(x, s, k)
+    s[:, 1::3] = -math.inf
+    check(x, s - 20 * torch.arange(W, device=DEV), k)     # (the first beams have most)
+
+
+def test_equal_ranks_of_many_beams():
+    x = torch.randn(1, 1, 300, device=DEV, generator=gen(8)).expand(1, 200, 300)
+    s = torch.full((1, 200), -1.5, device=DEV)
+    _, parent, _ = check(x, s, 256)
+    assert parent[0, :200].tolist() == list(range(200))
+    check(torch.zeros(1, 40, 9000, device=DEV), s[:, :40], 256)
+
+
 @pytest.mark.parametrize("V,k", [(262144, 5), (262145, 6), (300001, 256), (2 ** 21, 4)])
 def test_long_rows(V, k):
     x, s = make(1, 2, V, torch.float16)
@@ -132,7 +151,8 @@ def test_logits_in_order(k):
     # all alike but the first of every 64: the best logits lie with few threads, more than a list holds
     few = torch.where(torch.arange(100000, device=DEV) % 64 == 0, 0.0, 5.0)
     steep = torch.linspace(0, -200, 100000, device=DEV)
-    for x in (up, up.flip(0), few, 5 - few, steep):
+    far = torch.where(torch.arange(100000, device=DEV) % 2048 < 128, 9.0, 0.0)     # 49 groups of large equal ones
+    for x in (up, up.flip(0), few, 5 - few, steep, far):
         check(torch.stack([x, x])[None], torch.tensor([[-4.0, -4.5]], device=DEV), k)
 
 
