@@ -105,6 +105,9 @@ __device__ __forceinline__ Logits<T> load_logits(const T* x, int64_t i, int64_t 
   return c;
 }
 
+// Bound by the fp64 of the exponentials, 14 operations a logit: 512 rows of 151936 in bf16 56 us, where reading them takes
+// 32.  (A few rows are bound by the launch and one round trip, 5 us.)  A wave takes as many logits as it can have on the
+// way at once, and a row is spread over many.
 template <class T>
 __global__ __launch_bounds__(64 * kScanWaves) void beam_scan_kernel(BeamWork p) {
   const int64_t row = blockIdx.x / p.n_seg;
@@ -175,6 +178,9 @@ __device__ __forceinline__ double divisor(const BeamParams& a, int64_t length) {
 }
 __device__ __forceinline__ bool divides(const BeamParams& a) { return a.lengths && a.alpha != 0; }
 
+// A workgroup per beam.  Bound by what follows upon each other: 16 beams of 151936, 64 candidates 16.3 us (a logit at a
+// time and the bound from the threads' best in both rounds, 31), 256 beams and candidates 115 us, most of it the order
+// of a thousand group maxima.
 template <class T>
 __global__ __launch_bounds__(kRowThreads) void beam_row_kernel(BeamWork p) {
   __shared__ __attribute__((aligned(16))) u64 s_best[kRowThreads], s_list[kListMost + kPad];
@@ -355,7 +361,8 @@ __global__ __launch_bounds__(kRowThreads) void beam_row_kernel(BeamWork p) {
 
 // Lists are merged two by two in LDS: an entry's place in both is its own and the number in the other list that come
 // before it (of equal ones the lower beam's), found by halving.  A workgroup takes `per` of a sequence's beams; where
-// that leaves several lists, a second launch merges those.
+// that leaves several lists, a second launch merges those.  16 lists of 64 6.5 us, 256 of 256 28 us in two launches.  (A
+// wave that takes the best head k times: 25 and 130.)
 constexpr int kMergeHeld = 4096, kMergeThreads = 1024;
 __global__ __launch_bounds__(kMergeThreads) void beam_merge_kernel(BeamWork p, int per, bool second) {
   __shared__ u64 s_key[2][kMergeHeld];        // larger for a larger rank; 0: none
@@ -422,8 +429,8 @@ __global__ __launch_bounds__(kMergeThreads) void beam_merge_kernel(BeamWork p, i
 
 // ---- both in one launch: a workgroup per sequence, a wave per beam
 // Bound by the latency of what follows upon each other: what the scan left, the few groups' logits, and one barrier
-// before the merge.  Loops stay loops, with as little as can be: unrolled to hold all maxima in registers this took 15 us
-// for 4 beams of 151936, most of it to fetch its own instructions.
+// before the merge: 4 beams of 151936, 4 candidates 6.9 us, 64 sequences of 8 beams, 16 candidates 12.3.  Loops stay loops,
+// with as little as can be: unrolled throughout this took 15 us for the 4 beams, most of it to fetch its own instructions.
 constexpr int kPickBeams = 16, kPickMost = 32, kPickAll = 256, kPickList = 256;
 
 // base + i as a scalar base and a 32-bit offset (not an address in two registers for each load in flight).
@@ -725,7 +732,8 @@ hipError_t run(BeamWork p, hipStream_t stream) {
 
 // ---------------------------------------------------------------- states
 // A thread owns one column of V bytes of a state's beams: it reads the k parents' values before it writes any, so in
-// place no other thread's reads are in the way, and a beam that keeps its parent costs nothing.
+// place no other thread's reads are in the way, and a beam that keeps its parent costs nothing.  Bound by memory: 16 caches
+// of 16 x 8 beams, 8 heads of 1000 of 1280 x 128 in bf16, in place: 1140 us, 5.2 TB/s of what changes place.
 template <class Vec, int K>
 __global__ __launch_bounds__(256) void reorder_kernel(ReorderParams p, int64_t step0, int64_t b0, int j0) {
   const int64_t cols = p.run / (int64_t)sizeof(Vec);  // of a run

@@ -140,8 +140,9 @@ __device__ __forceinline__ uint4 quantize16(const Sixteen<Src>& x, float s, floa
 
 // TPR threads a row, a wave for many rows and a workgroup for few, each with NC pieces of 16 values in registers, so
 // that rows of up to 16 NC TPR values are read once (longer ones twice).  A piece goes out as one 16-byte chunk of the
-// image; the workgroup's rows are neighbours in it, 8 of them 128 bytes in a row.  (8 threads a row, whose chunks go out
-// together but who read their rows twice: 151936 x 2560 in bf16 415 us.)
+// image; the workgroup's rows are neighbours in it, 8 of them 128 bytes in a row.  Bound by reading x and writing a byte
+// a value: 151936 x 2560 in bf16 210 us, 5.6 TB/s.  (8 threads a row, whose chunks go out together without LDS but who
+// read their rows twice: 415 us.)
 constexpr int kManyRows = 8;
 template <class Src, int TPR, int NC>
 __global__ __launch_bounds__(TPR == 64 ? 64 * kManyRows : TPR) void int8_quantize_kernel(
@@ -217,7 +218,7 @@ __global__ __launch_bounds__(TPR == 64 ? 64 * kManyRows : TPR) void int8_quantiz
   }
 }
 
-// Rows of integers [R][ld] into an image, 8 threads a row.
+// Rows of integers [R][ld] into an image, 8 threads a row: 151936 x 2560 in 140 us, 5.5 TB/s of what is read and written.
 __global__ __launch_bounds__(256) void int8_pack_kernel(const int8_t* __restrict__ q, int64_t ld, int64_t R, int K, int S,
                                                         int vec, char* __restrict__ image) {
   const int64_t r = (int64_t)blockIdx.x * 32 + threadIdx.x / 8;
@@ -238,7 +239,8 @@ __global__ __launch_bounds__(256) void int8_pack_kernel(const int8_t* __restrict
 }
 
 // The values that an image stands for, in fp32 [R][K]: 32 rows x kUnpackK values through LDS, so that the image comes
-// in and rows go out in long pieces (16 bytes a lane; a chunk's 512 bytes padded to 528: no bank conflicts).
+// in and rows go out in long pieces (16 bytes a lane; a chunk's 512 bytes padded to 528: no bank conflicts).  151936 x
+// 2560 in 330 us, 5.9 TB/s.
 constexpr int kUnpackK = 256;
 __global__ __launch_bounds__(256) void int8_unpack_kernel(const char* __restrict__ image, const float* __restrict__ scale,
                                                           int64_t R, int K, int S, int pieces, float* __restrict__ out) {
@@ -287,7 +289,8 @@ __device__ __forceinline__ float bias_at(const Int8Params& p, int v) {
 __device__ __forceinline__ float wscale_at(const Int8Params& p, int v) { return v < p.V ? p.w_scale[v] : 0.f; }
 
 // Up to 32 NB tokens on few rows: a workgroup takes 32 G of W's rows, its four waves a quarter of the reduction each,
-// operands straight from memory; the quarters are added in LDS.
+// operands straight from memory; the quarters are added in LDS.  Bound by a round trip or two to memory: K = 4096, V =
+// 16000, one token 11.1 us with the quantisation.
 template <class Out, int NB, int G, int U>
 __global__ __launch_bounds__(256) void int8_few_kernel(Int8Params p) {
   constexpr int kRegs = G * NB * 16, kPitch = 65;
@@ -417,7 +420,9 @@ __device__ __forceinline__ void store_tile(const Int8Params& p, const i32x16_t (
   }
 }
 
-// Many tokens: BV x BM tiles of WV x WT waves, the readout's reduction loop (tile_reduce) on integer operands.
+// Many tokens: BV x BM tiles of WV x WT waves, the readout's reduction loop (tile_reduce) on integer operands.  Up to some
+// 300 tokens bound by reading W (48 tokens, K = 4096, V = 128256: 101 us, 5.2 TB/s), beyond by the matrix cores and the
+// epilogue: 8192 tokens 3420 us, 2520 TOP/s, of which the loop alone would take 3130.
 template <class Out, int BV, int BM, int WV, int WT, int NS>
 __global__ __launch_bounds__(64 * WV * WT) void int8_tile_kernel(Int8Params p) {
   constexpr int NT = 64 * WV * WT, FM = BV / WV / 32, FN = BM / WT / 32;
@@ -471,11 +476,12 @@ hipError_t quantize_typed(const Src* x, int64_t ld, int64_t R, int64_t K64, char
   const int K = (int)K64, S = (int)int8_slices(K);
   const int64_t rows = pad ? (R + kInt8Rows - 1) / kInt8Rows * kInt8Rows : R;
   const unsigned many = (unsigned)((rows + kManyRows - 1) / kManyRows);
-  // (a wave a row from 2048 rows on, 8 waves for each CU: 512 rows of 4096 in bf16 ...)
-  if (rows < 2048)
-    int8_quantize_kernel<Src, 256, 2><<<(unsigned)rows, 256, 0, stream>>>(x, ld, R, K, S, image, scale);
-  else if (K <= 1024)
+  // A wave a row where that is one piece for each lane or fills the card with 2048 rows.  (bf16: 1000 rows of 1000 4.2 us,
+  // with a workgroup a row 5.2; of 4096 500 rows 8.8 and 5.6, 2048 9.9 and 10.6, 8192 22 and 34.)
+  if (K <= 1024)
     int8_quantize_kernel<Src, 64, 1><<<many, 64 * kManyRows, 0, stream>>>(x, ld, R, K, S, image, scale);
+  else if (rows < 2048)
+    int8_quantize_kernel<Src, 256, 2><<<(unsigned)rows, 256, 0, stream>>>(x, ld, R, K, S, image, scale);
   else if (K <= 4096)
     int8_quantize_kernel<Src, 64, 4><<<many, 64 * kManyRows, 0, stream>>>(x, ld, R, K, S, image, scale);
   else
