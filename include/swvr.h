@@ -421,7 +421,8 @@ int swvr_int8_logits(int dtype, int out_dtype, int64_t N, int64_t K, int64_t V, 
  * counterpart.  scores [B,W] (fp64 with s64 = 1, else fp32) are the beams' sums so far.  Beam w's candidates are
  * its tokens v with sum = scores[b,w] + logit[v] - logsumexp(logits), or where finished[b,w] (one byte; NULL:
  * nowhere) is not 0 the one token end_id with sum = scores[b,w].  They are ranked by sum / length^length_penalty,
- * in fp64: length = lengths[b,w] (int64; NULL: 1 for all), plus 1 for a beam that is not finished, and at least 1.
+ * in fp64: length = lengths[b,w] (int64; NULL: nothing is divided), plus 1 for a beam that is not finished, and at
+ * least 1.
  * The k best go out in order (equal ones by beam, then logit, then token): token and parent (the beam) [B,k] int64,
  * score [B,k] the sum in the type of scores.  NaN and -inf logits are no candidates; a beam with a +inf logit, with
  * nothing else or with a score that is not finite has none.  Where fewer than k are left: token and parent -1,
