@@ -48,14 +48,10 @@ __device__ __forceinline__ double score_of(const BeamParams& a, int64_t row) {
 // A beam whose score is -inf, +inf or NaN has no candidates.
 __device__ __forceinline__ bool alive(double score) { return fabs(score) < __builtin_huge_val(); }
 
-// e^(x - m) in fp64: with t = (x - m) log2 e, n the whole number next to it, 2^n times 2^(t - n) by its Chebyshev
-// interpolant of degree 8 on [-1/2, 1/2], 1.1e-12 of itself off.  About 2^-1000 for what lies below, and for NaN.
-__device__ __forceinline__ double exp_rel(float x, double m) {
-  constexpr double kLog2e64 = 1.4426950408889634074;
-  constexpr double kRound = 6755399441055744.0;  // 1.5 2^52: sums with it are whole numbers, in the low bits
-  const double d = fmax((double)x - m, -693.0);
-  const double y = fma(d, kLog2e64, kRound);
-  const double f = fma(d, kLog2e64, kRound - y);
+// 2^(n + f) in fp64 by the Chebyshev interpolant of degree 8 on [-1/2, 1/2], 1.1e-12 of itself off; n from -1022 on
+// as kRound + n, whose low bits it is.
+constexpr double kLog2e64 = 1.4426950408889634074, kRound = 6755399441055744.0;  // 1.5 2^52: sums with it are whole numbers
+__device__ __forceinline__ double pow2(double f, double n) {
   double p = 1.3255224887502117e-06;
   p = fma(p, f, 1.531007940254368e-05);
   p = fma(p, f, 0.0001540345585240991);
@@ -66,7 +62,12 @@ __device__ __forceinline__ double exp_rel(float x, double m) {
   p = fma(p, f, 0.6931471805459335);
   p = fma(p, f, 1.0);
   // (on the high word alone: a 64-bit shift and addition are two instructions for one)
-  return __hiloint2double(__double2hiint(p) + (__double2loint(y) << 20), __double2loint(p));
+  return __hiloint2double(__double2hiint(p) + (__double2loint(n) << 20), __double2loint(p));
+}
+// e^(x - m), about 2^-1000 for what lies below, and for NaN.
+__device__ __forceinline__ double exp_rel(float x, double m) {
+  const double d = fmax((double)x - m, -693.0), y = fma(d, kLog2e64, kRound);
+  return pow2(fma(d, kLog2e64, kRound - y), y);
 }
 
 template <int CTRL>
@@ -87,6 +88,15 @@ __device__ __forceinline__ float max64(float x8) {
   return fmaxf(m, __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x8), 48)));
 }
 
+struct AddF64 {
+  __device__ __forceinline__ u64 operator()(u64 a, u64 b) const {
+    return (u64)__double_as_longlong(__longlong_as_double((long long)a) + __longlong_as_double((long long)b));
+  }
+};
+__device__ __forceinline__ double wave_sum_f64(double x) {
+  return __longlong_as_double((long long)last_lane64(wave_scan64((u64)__double_as_longlong(x), AddF64())));
+}
+
 // kLane consecutive logits from any element on (rows begin anywhere where V is odd), -inf past the row's end.
 template <class T>
 using Logits = typename Vec8<T>::type;
@@ -105,9 +115,9 @@ __device__ __forceinline__ Logits<T> load_logits(const T* x, int64_t i, int64_t 
   return c;
 }
 
-// Bound by the fp64 of the exponentials, 14 operations a logit: 512 rows of 151936 in bf16 56 us, where reading them takes
-// 32.  (A few rows are bound by the launch and one round trip, 5 us.)  A wave takes as many logits as it can have on the
-// way at once, and a row is spread over many.
+// Bound by the vector units, busy 80% of the time with 15 instructions a logit, 12 of them fp64's: 512 rows of 151936 in
+// bf16 54 us, where reading them takes 32.  (A few rows are bound by the launch and one round trip, 5 us.)  A wave takes
+// as many logits as it can have on the way at once, and a row is spread over many.
 template <class T>
 __global__ __launch_bounds__(64 * kScanWaves) void beam_scan_kernel(BeamWork p) {
   const int64_t row = blockIdx.x / p.n_seg;
@@ -125,14 +135,11 @@ __global__ __launch_bounds__(64 * kScanWaves) void beam_scan_kernel(BeamWork p) 
     for (int j = 0; j < kSteps; ++j) c[j] = load_logits(x, i0 + j * kStep, V);
   }
   float m = kNegInf, mine = kNegInf;  // mine: of the group of 16 lanes in step lane % 16
-  float l[kSteps][kLane];
 #pragma unroll
   for (int j = 0; j < kSteps; ++j) {
-#pragma unroll
-    for (int u = 0; u < kLane; ++u) l[j][u] = (float)c[j][u];
     float k = kNegInf;
 #pragma unroll
-    for (int u = 0; u < kLane; ++u) k = fmaxf(k, l[j][u]);  // (NaN: the other)
+    for (int u = 0; u < kLane; ++u) k = fmaxf(k, (float)c[j][u]);  // (NaN: the other)
     k = dpp_max<0x140>(max8(k));  // (row_mirror)
     mine = (lane_id() & 15) == j ? k : mine;
     m = fmaxf(m, k);
@@ -140,12 +147,26 @@ __global__ __launch_bounds__(64 * kScanWaves) void beam_scan_kernel(BeamWork p) 
   m = max64(m);
   const double by = m > kNegInf && m < kPosInf ? (double)m : 0.0;
   double sum = 0;
+  if (fabsf(m) < 0x1p22f) {
+    // Two operations less: powers of 2 relative to 2^M, M next to m log2 e, as xL - M - n in one fma is exact but for its
+    // last rounding (L's own error is taken off again with 2^(M - mL)); and m - 693 in fp32 is within 1.
+    const double M = rint(by * kLog2e64), base = kRound - M;
+    const float low = m - 693.f;
 #pragma unroll
-  for (int j = 0; j < kSteps; ++j)
+    for (int j = 0; j < kSteps; ++j)
 #pragma unroll
-    for (int u = 0; u < kLane; ++u) sum += exp_rel(l[j][u], by);
+      for (int u = 0; u < kLane; ++u) {
+        const double x = __builtin_amdgcn_fmed3f((float)c[j][u], low, m), y = fma(x, kLog2e64, base);  // (NaN: low)
+        sum += pow2(fma(x, kLog2e64, base - y), y);
+      }
+    sum *= pow2(fma(-by, kLog2e64, M), kRound);
+  } else {
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+    for (int j = 0; j < kSteps; ++j)
+#pragma unroll
+      for (int u = 0; u < kLane; ++u) sum += exp_rel((float)c[j][u], by);
+  }
+  sum = wave_sum_f64(sum);
   static_assert(kGroup == 16 * kLane, "a group is 16 lanes' logits of a step");
   if ((lane_id() & 15) < kSteps)
     p.group[row * p.n_group + sub * kSubGroups + (lane_id() & 15) * 4 + lane_id() / 16] = mine;
@@ -227,8 +248,7 @@ __global__ __launch_bounds__(kRowThreads) void beam_row_kernel(BeamWork p) {
     const float mi = p.sub_max[row * p.n_sub + i];
     if (mi > kNegInf) sum += p.sub_sum[row * p.n_sub + i] * exp((double)mi - (double)m);
   }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+  sum = wave_sum_f64(sum);
   if (lane_id() == 0) s_sum[wave_id()] = sum;
   // The k first of what n blocks of 8 hold, in order, to s_order; how many.  load(i, at, from): block i, its first one at
   // index `at`, those before `from` another block's.  A bound that k of them reach (where `bound` is 0: the k-th of the
@@ -439,12 +459,6 @@ __device__ __forceinline__ const T* at_offset(const T* base, int i) {
   return reinterpret_cast<const T*>(reinterpret_cast<const char*>(base) + (uint32_t)i * (uint32_t)sizeof(T));
 }
 
-struct AddF64 {
-  __device__ __forceinline__ u64 operator()(u64 a, u64 b) const {
-    return (u64)__double_as_longlong(__longlong_as_double((long long)a) + __longlong_as_double((long long)b));
-  }
-};
-
 // A list of a wave in LDS: the places of values that are at least `least` go to its end, but for -inf.  (Past kPickList
 // they are counted, not kept.)
 struct WaveList {
@@ -635,7 +649,7 @@ __global__ __launch_bounds__(64 * kPickBeams) void beam_pick_kernel(BeamWork p) 
       const double si = i == lane ? sum0 : i == lane + 64 ? sum1 : sub_sum[i];
       if (mi > kNegInf) sum += si * exp((double)mi - (double)m);
     }
-    sum = __longlong_as_double((long long)last_lane64(wave_scan64((u64)__double_as_longlong(sum), AddF64())));
+    sum = wave_sum_f64(sum);
     const double rest = log(sum);
     list.in_order(k, [&](u64 z, int r) {
       const double y = score + (((double)logit_of(key_at(z)) - (double)m) - rest);

@@ -176,6 +176,15 @@ def test_masks_infinities_and_nan():
         check(y, torch.zeros(1, 2, device=DEV), 5)
 
 
+@pytest.mark.parametrize("far", [-3e38, -4194304.0, -4194303.0, -70000.0, -100.0, 100.0, 70000.0, 4194000.0, 4194304.0, 1e7, 2e38])
+def test_logits_far_from_zero(far):
+    """Sums do not lose what a large maximum would swallow: differences alone count."""
+    x = torch.randn(1, 3, 5000, device=DEV, generator=gen(9)) * 5 + far
+    x[0, 1, 3000:] -= 600          # pieces that count for little
+    x[0, 2, 2500:4800] = torch.finfo(torch.float32).min
+    check(x, torch.tensor([[-3.0, -3.25, -2.0]], device=DEV), 8)
+
+
 @pytest.mark.parametrize("alpha", [0.0, 0.6, 1.0, 16.0])
 def test_finished_beams_and_lengths(alpha):
     x, s = make(6, 4, 3001, torch.bfloat16, seed=6)
