@@ -503,7 +503,10 @@ constexpr int64_t kFull = 240;
 // each CU, and with fewer rows the kernel without LDS, whose workgroups are smaller: (K = 4096, V = 16000, 1 token: 11.1
 // us, tiles 16.0; K = 2560, V = 151936, 48 tokens: 99 us, tiles 81.)  With more tokens the largest tile that fills the
 // card (200 tokens, K = 4096: 256 x 256 on V = 128256 142 us and 256 x 128 153; on V = 32000 52 and 37; 128 x 128 on V =
-// 16000 24, 256 x 128 28), and of 256 x 256 and 256 x 128 the one with the fewer padded tokens.
+// 16000 24, 256 x 128 28), and of 256 x 256 and 256 x 128 the one with the fewer padded tokens.  With K up to 512, in fp32
+// 1024, storing logits takes as long as forming them, and 256 x 128, two to a CU, does one beside the other: (500 tokens, V =
+// 50021 in bf16, K = 512 46 -> 40 us; 8192 on 50048 in fp32, K = 512 440 -> 405, K = 1024 595 -> 560; but 1000 on 32000,
+// K = 1024 62 -> 69, and K = 1536 74 -> 90.)
 template <class Out>
 hipError_t logits_typed(Int8Params p, hipStream_t stream) {
   // Logits past the caches where rows are whole lines (a wave writes 256 bytes of each): W and h stay in them.  (8192
@@ -512,13 +515,14 @@ hipError_t logits_typed(Int8Params p, hipStream_t stream) {
   p.lines = reinterpret_cast<uintptr_t>(p.out) % 128 == 0 && (int64_t)p.V * sizeof(Out) % 128 == 0;
   auto tiles = [&](int bv, int bm) { return (int64_t)((p.V + bv - 1) / bv) * ((p.N + bm - 1) / bm); };
   auto padded = [&](int bm) { return (int64_t)((p.N + bm - 1) / bm * bm); };
+  const bool stores = p.S * (int)kInt8K <= 256 * (int)sizeof(Out);
   if (p.N <= 32 && tiles(128, 32) < kFull)
     int8_few_kernel<Out, 1, 1, 4><<<(unsigned)((p.V + 31) / 32), 256, 0, stream>>>(p);
   else if (p.N > 32 && p.N <= 64 && tiles(64, 64) < kFull)
     int8_few_kernel<Out, 2, 1, 2><<<(unsigned)((p.V + 31) / 32), 256, 0, stream>>>(p);
   else if (p.N <= 64)
     tile_launch<Out, 128, 64, 2, 2, 4>(p, stream);
-  else if (p.N > 128 && tiles(256, 256) >= kFull && padded(256) <= 1.05 * padded(128))
+  else if (p.N > 128 && !stores && tiles(256, 256) >= kFull && padded(256) <= 1.05 * padded(128))
     tile_launch<Out, 256, 256, 2, 4, 3>(p, stream);
   else if (p.N > 128 && tiles(256, 128) >= kFull)
     tile_launch<Out, 256, 128, 4, 2, 3>(p, stream);

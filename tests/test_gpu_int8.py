@@ -161,6 +161,15 @@ def test_logits_of_every_tile(N, rows, V):
         check_logits(h, w, bias, dtype=dtype)
 
 
+@pytest.mark.parametrize("K", [520, 1090])
+@pytest.mark.parametrize("N,V", [(500, 31104), (250, 61441), (1100, 16127)])
+def test_logits_of_the_largest_tile(N, V, K):
+    h = torch.randn(N, K, device=DEV, generator=gen(N + 1)).to(torch.float16)
+    w = int8.quantize_rows(torch.randn(V, K, device=DEV, generator=gen(V + 1)).to(torch.bfloat16))
+    for dtype in (torch.float16, torch.float32):
+        check_logits(h, w, torch.randn(V, device=DEV, generator=gen(V + 2)), dtype=dtype)
+
+
 def test_more_values_than_32_bits_count():
     x = torch.randn(1000, 8192, device=DEV, generator=gen(40)).to(torch.bfloat16).repeat(300, 1)     # 2.5e9
     x[-1] *= 3
