@@ -176,17 +176,13 @@ def _reorder(states, parents, inplace):
     B = 1
     for n in ids.shape[:-1]:
         B *= n
-    groups, out, seen, last = {}, [], {parents.data_ptr()}, None
+    groups, out, kept, seen, last = {}, [], [], {parents.data_ptr()}, None
     for x in states:
-        if inplace:
-            if x.is_neg() or x.is_conj() or x._is_zerotensor():
+        if x.is_neg() or x.is_conj() or x._is_zerotensor():
+            if inplace:
                 raise ValueError("a lazily negated, conjugated or memoryless state cannot be reordered in place")
-            at = x.data_ptr()
-            if at in seen and x.numel():
-                raise ValueError("the same state twice, or the parents, cannot be reordered in place")
-            seen.add(at)
-        else:
-            x = _plain(x.resolve_conj() if x.is_conj() else x)
+            x = _plain(x.resolve_conj())
+            kept.append(x)
         layout = (x.shape, x.stride(), x.element_size())
         if layout != last:   # (the caches of all layers have one)
             last, (shape, strides, _) = layout, layout
@@ -204,17 +200,26 @@ def _reorder(states, parents, inplace):
                 src, dst = groups.setdefault(g, ([], []))
         if dense:
             x = x.contiguous()
-        y = x if inplace else torch.empty(new, dtype=x.dtype, device=x.device)
+            kept.append(x)
+        at = x.data_ptr()
+        if inplace:
+            if at in seen and g:
+                raise ValueError("the same state twice, or the parents, cannot be reordered in place")
+            seen.add(at)
+            y = x
+        else:
+            y = x.new_empty(new)
+            if g:
+                dst.append(y.data_ptr())
         out.append(y)
         if g:
-            src.append(x)
-            dst.append(y)
+            src.append(at)
     lib = _lib.load()
     for (run, n1, n2, steps, dense), (src, dst) in groups.items():
         n = len(src)
         beam = run * n1 * n2
-        at = (ctypes.c_void_p * n)(*(x.data_ptr() for x in src))
-        to = None if inplace else (ctypes.c_void_p * n)(*(x.data_ptr() for x in dst))
+        at = (ctypes.c_void_p * n)(*src)
+        to = None if inplace else (ctypes.c_void_p * n)(*dst)
         step = (ctypes.c_int64 * 4)(*steps)
         to_step = (ctypes.c_int64 * 4)(k * beam, beam, *dense)
         _lib.call(lib.swvr_reorder_beams, ids.device, n, at, to, B, W, k, ids.data_ptr(), ids.dtype == torch.int64, run, n1, n2,
