@@ -176,6 +176,27 @@ def test_masks_infinities_and_nan():
         check(y, torch.zeros(1, 2, device=DEV), 5)
 
 
+def test_masks_infinities_and_nan_of_many_candidates():
+    x, s = make(6, 20, 3000, torch.float32, seed=11)
+    x[0, :, 30:] = -math.inf                  # fewer candidates than are looked for
+    x[0, 3:] = -math.inf
+    x[1, 0], x[1, 1, ::2], x[1, 2, 77] = math.nan, math.nan, math.inf
+    x[2, :, 100:] = torch.finfo(torch.float32).min
+    x[3] = -math.inf
+    x[3, 19, 2999] = 0.0                      # one in all
+    s[4, 1:], s[5, ::2] = -math.inf, math.nan
+    out = check(x, s, 100)
+    assert (out[0][3] >= 0).sum() == 1 and (out[0][0] >= 0).sum() == 90
+    check(x[:, :2], s[:, :2], 40, finished=torch.arange(12, device=DEV).view(6, 2) % 3 == 0, end_id=7)
+
+
+@pytest.mark.parametrize("k", [3, 100])
+def test_equal_logits_of_the_longest_rows(k):
+    x = torch.randint(0, 2, (1, 2, 2 ** 21), device=DEV, generator=gen(12)).to(torch.bfloat16)
+    x[0, 1] = 0
+    check(x, torch.tensor([[-1.0, -2.0]], device=DEV), k)
+
+
 @pytest.mark.parametrize("far", [-3e38, -4194304.0, -4194303.0, -70000.0, -100.0, 100.0, 70000.0, 4194000.0, 4194304.0, 1e7, 2e38])
 def test_logits_far_from_zero(far):
     """Sums do not lose what a large maximum would swallow: differences alone count."""
