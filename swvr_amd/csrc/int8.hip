@@ -421,8 +421,9 @@ __device__ __forceinline__ void store_tile(const Int8Params& p, const i32x16_t (
 }
 
 // Many tokens: BV x BM tiles of WV x WT waves, the readout's reduction loop (tile_reduce) on integer operands.  Up to some
-// 300 tokens bound by reading W (48 tokens, K = 4096, V = 128256: 101 us, 5.2 TB/s), beyond by the matrix cores and the
-// epilogue: 8192 tokens 3420 us, 2520 TOP/s, of which the loop alone would take 3130.
+// 300 tokens bound by reading W (48 tokens, K = 4096, V = 128256: 101 us, 5.2 TB/s), beyond by the power that matrix cores
+// take: 8192 tokens 3430 to 3660 us, 2510 to 2350 TOP/s, at 1.4 GHz with the matrix cores busy in 75% of the cycles; the
+// loop alone would take 3130.
 template <class Out, int BV, int BM, int WV, int WT, int NS>
 __global__ __launch_bounds__(64 * WV * WT) void int8_tile_kernel(Int8Params p) {
   constexpr int NT = 64 * WV * WT, FM = BV / WV / 32, FN = BM / WT / 32;
