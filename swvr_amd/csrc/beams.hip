@@ -6,7 +6,7 @@
 // beam the ranks are in the order of the logits, so the arithmetic decides between beams alone; there candidates lie
 // close together (256 ranked ones of a step are some 1e-3 apart), so sums are formed in fp64: an exponential is off by
 // 1.1e-12 of itself and an lse by less, where fp32's 1e-7 would swap a pair in one of a few thousand steps.  What is
-// summed in which order depends on V alone: the same beams have the same sums wherever they stand.
+// summed in which order depends on V alone (row_sum): the same beams have the same sums wherever they stand.
 //
 // Launches:
 //   beam_scan_kernel   reads the logits once: per group of 128 its maximum, per sub-block of 2048 (a wave) its own and
@@ -96,6 +96,18 @@ struct AddF64 {
 __device__ __forceinline__ double wave_sum_f64(double x) {
   return __longlong_as_double((long long)last_lane64(wave_scan64((u64)__double_as_longlong(x), AddF64())));
 }
+
+// The sum of a row's exponentials relative to m from its sub-blocks' by(i) = e^(max_i - m) and sum(i): lane l's l, l + 64,
+// ... one after another, then over the wave.  The kernels that need it share this order, each wave with all of it.
+template <class By, class Sum>
+__device__ __forceinline__ double row_sum(int n_sub, By&& by, Sum&& sum) {
+  double x = 0;
+#pragma unroll 1
+  for (int i = lane_id(); i < n_sub; i += 64) x = fma(sum(i), by(i), x);
+  return wave_sum_f64(x);
+}
+// (0 for a sub-block without candidates)
+__device__ __forceinline__ double sub_weight(float mi, float m) { return mi > kNegInf ? exp((double)mi - (double)m) : 0.0; }
 
 // kLane consecutive logits from any element on (rows begin anywhere where V is odd), -inf past the row's end.
 template <class T>
@@ -207,7 +219,6 @@ __global__ __launch_bounds__(kRowThreads) void beam_row_kernel(BeamWork p) {
   __shared__ __attribute__((aligned(16))) u64 s_best[kRowThreads], s_list[kListMost + kPad];
   __shared__ u64 s_order[kBeamsMost];
   __shared__ int s_group[kBeamsMost];
-  __shared__ double s_sum[kRowThreads / 64];
   __shared__ float s_max[kRowThreads / 64];
   __shared__ u64 s_bound;
   __shared__ int s_n, s_more;
@@ -230,7 +241,7 @@ __global__ __launch_bounds__(kRowThreads) void beam_row_kernel(BeamWork p) {
     }
     return;
   }
-  // ---- lse, in an order of V alone
+  // ---- lse
   const float* const group = p.group + row * p.n_group;
   float m = kNegInf;
   for (int i = t; i < p.n_sub; i += kRowThreads) m = fmaxf(m, p.sub_max[row * p.n_sub + i]);
@@ -243,17 +254,22 @@ __global__ __launch_bounds__(kRowThreads) void beam_row_kernel(BeamWork p) {
     if (t == 0) p.count[row] = 0;
     return;
   }
-  double sum = 0;
+  // (the exponentials by all threads, added in `first`: the list's room is free until then)
+  static_assert(2 * (kBeamVocabMost / kSub) <= kListMost, "a weight and a sum for each sub-block");
   for (int i = t; i < p.n_sub; i += kRowThreads) {
-    const float mi = p.sub_max[row * p.n_sub + i];
-    if (mi > kNegInf) sum += p.sub_sum[row * p.n_sub + i] * exp((double)mi - (double)m);
+    s_list[2 * i] = (u64)__double_as_longlong(sub_weight(p.sub_max[row * p.n_sub + i], m));
+    s_list[2 * i + 1] = (u64)__double_as_longlong(p.sub_sum[row * p.n_sub + i]);
   }
-  sum = wave_sum_f64(sum);
-  if (lane_id() == 0) s_sum[wave_id()] = sum;
+  double rest = 0;  // lse - m
+  auto add_up = [&]() {
+    auto held = [&](int i) { return __longlong_as_double((long long)s_list[i]); };
+    rest = log(row_sum(p.n_sub, [&](int i) { return held(2 * i); }, [&](int i) { return held(2 * i + 1); }));
+  };
   // The k first of what n blocks of 8 hold, in order, to s_order; how many.  load(i, at, from): block i, its first one at
   // index `at`, those before `from` another block's.  A bound that k of them reach (where `bound` is 0: the k-th of the
-  // threads' best), the few that reach it, and of these the places.
-  auto first = [&](int n, u64 bound, auto&& load) -> int {
+  // threads' best), the few that reach it, and of these the places.  then(): once before the list's room is written, after a
+  // barrier (where `bound` is 0).
+  auto first = [&](int n, u64 bound, auto&& load, auto&& then) -> int {
     // f(value, index) for this thread's, but for blocks whose largest is below `least`; several are read before the
     // first is used
     auto each = [&](float least, auto&& f) {
@@ -289,6 +305,7 @@ __global__ __launch_bounds__(kRowThreads) void beam_row_kernel(BeamWork p) {
       __syncthreads();
       s_best[t] = mine;
       if (t == 0) s_bound = 0;
+      then();
       __syncthreads();
       if (mine && above(s_best, kRowThreads, mine) == k - 1) s_bound = (u64)key_at(mine) << 32;
       __syncthreads();
@@ -355,7 +372,7 @@ __global__ __launch_bounds__(kRowThreads) void beam_row_kernel(BeamWork p) {
   const int groups = first(p.n_group / kLane, 0, [&](int i, int& at, int& from) {
     at = from = i * kLane;
     return whole_logits(group + at);
-  });
+  }, add_up);
   if (t < groups) s_group[t] = (int)index_at(s_order[t]);
   // k groups: each has one that reaches the last one's largest
   const u64 reached = groups == k ? (u64)key_at(s_order[k - 1]) << 32 : 0;
@@ -366,8 +383,7 @@ __global__ __launch_bounds__(kRowThreads) void beam_row_kernel(BeamWork p) {
     from = s_group[i / (kGroup / kLane)] * kGroup + i % (kGroup / kLane) * kLane;
     at = min(from, max(V - kLane, 0));  // (at the row's end the last 8)
     return V < kLane ? load_logits(x, at, V) : whole_logits(x + at);
-  });
-  const double rest = log(s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3]);  // lse - m
+  }, [] {});
   const double by = divides(p.a) ? divisor(p.a, length_of(p.a, row, 1)) : 1.0;
   if (t < n2) {
     const u64 y = s_order[t];
@@ -641,16 +657,9 @@ __global__ __launch_bounds__(64 * kPickBeams) void beam_pick_kernel(BeamWork p) 
           }
         return y;
       });
-    // ---- lse - m, in an order of V alone
-    double sum = 0;
-#pragma unroll 1
-    for (int i = lane; i < n_sub; i += 64) {
-      const float mi = i == lane ? max0 : i == lane + 64 ? max1 : sub_max[i];
-      const double si = i == lane ? sum0 : i == lane + 64 ? sum1 : sub_sum[i];
-      if (mi > kNegInf) sum += si * exp((double)mi - (double)m);
-    }
-    sum = wave_sum_f64(sum);
-    const double rest = log(sum);
+    const double rest = log(row_sum(  // lse - m
+        n_sub, [&](int i) { return sub_weight(i == lane ? max0 : i == lane + 64 ? max1 : sub_max[i], m); },
+        [&](int i) { return i == lane ? sum0 : i == lane + 64 ? sum1 : sub_sum[i]; }));
     list.in_order(k, [&](u64 z, int r) {
       const double y = score + (((double)logit_of(key_at(z)) - (double)m) - rest);
       s_sum[w * k + r] = y;
