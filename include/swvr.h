@@ -405,8 +405,8 @@ int swvr_sample(int dtype, int64_t R, int64_t V, const void* logits, int64_t ld,
  *   swvr_int8_unpack     out [R,K] = scale q in fp32;
  *   swvr_int8_logits     out[n,v] = logit_scale sh[n] sw[v] sum_k qh[n,k] qw[v,k] + bias[v]
  *                        [N,V] in out_dtype, h [N,K] quantised so within the call (into the workspace),
- *                        the sum exact in 32-bit integers, the rest in fp32; bias [V] in bias_dtype or
- *                        NULL.  N up to 2^24. */
+ *                        the sum exact in 32-bit integers, the rest in fp32 (in fp64 where logit_scale sh sw
+ *                        leaves fp32); bias [V] in bias_dtype or NULL.  N up to 2^24. */
 size_t swvr_int8_size(int64_t R, int64_t K);
 int swvr_int8_quantize(int dtype, int64_t R, int64_t K, const void* x, int64_t ld, void* image, float* scale,
                        void* stream);

@@ -8,6 +8,8 @@
 // Rows are kept in the order in which the matrix cores take them (launch.hpp, kInt8Block): an operand of
 // v_mfma_i32_32x32x32_i8 is 16 consecutive bytes per lane, lane l's row l % 32 and values 16 (l / 32) on, which is
 // 1 KB in one piece for the wave, from memory as from LDS, free of bank conflicts without a swizzle.
+#include <type_traits>
+
 #include "common.hpp"
 #include "launch.hpp"
 
@@ -288,6 +290,21 @@ __device__ __forceinline__ float bias_at(const Int8Params& p, int v) {
 }
 __device__ __forceinline__ float wscale_at(const Int8Params& p, int v) { return v < p.V ? p.w_scale[v] : 0.f; }
 
+// logit_scale sh sw sum + bias.  The scales' product may leave fp32 where the logit does not (2^-106 sh of a token of zeros
+// times sw of a row of zeros; rows of 1e36 times a scale of 1e4, with a sum of 0): then in fp64, which holds all but the last
+// bits of it.  Whether that is so depends on the two scales alone.
+__device__ __forceinline__ bool holds(float x) {
+  x = fabsf(x);
+  return x >= 0x1p-126f && x < kPosInf;
+}
+__device__ __forceinline__ float near_logit(int sum, float csh, float sw, float bias) { return fmaf((float)sum, csh * sw, bias); }
+__device__ __forceinline__ float far_logit(int sum, float c, float sh, float sw, float bias) {
+  const float csh = c * sh;
+  if (holds(csh) && holds(csh * sw)) [[likely]]
+    return near_logit(sum, csh, sw, bias);
+  return (float)fma((double)c * (double)sh * (double)sw, (double)sum, (double)bias);
+}
+
 // Up to 32 NB tokens on few rows: a workgroup takes 32 G of W's rows, its four waves a quarter of the reduction each,
 // operands straight from memory; the quarters are added in LDS.  Bound by a round trip or two to memory: K = 4096, V =
 // 16000, one token 11.1 us with the quantisation.
@@ -354,7 +371,7 @@ __global__ __launch_bounds__(256) void int8_few_kernel(Int8Params p) {
   for (int n = threadIdx.x / (32 * G); n < p.N; n += 256 / (32 * G)) {
     const int at = ((g * NB + n / 32) * 16 + row / 8 * 4 + row % 4) * kPitch + (row / 4 % 2) * 32 + n % 32;
     const int sum = s_part[0][at] + s_part[1][at] + s_part[2][at] + s_part[3][at];
-    if (v < p.V) out[(int64_t)n * p.V + v] = (Out)fmaf((float)sum, p.scale * p.h_scale[n] * sw, bias);
+    if (v < p.V) out[(int64_t)n * p.V + v] = (Out)far_logit(sum, p.scale, p.h_scale[n], sw, bias);
   }
 }
 
@@ -366,7 +383,7 @@ struct __attribute__((packed, aligned(sizeof(Out)))) OutChunk {
 
 // A wave's 32 FM vocabulary rows (from v0) x 32 FN tokens (from n0), through `room` (ROOM bytes of LDS, this wave's): a
 // lane holds 4 rows of a token, and goes out with 16 bytes of a token's 256 (128 with fewer rows or less room).
-template <class Out, int FM, int FN, int ROOM>
+template <class Out, int FM, int FN, int ROOM, bool FAR>
 __device__ __forceinline__ void store_tile(const Int8Params& p, const i32x16_t (&acc)[FM][FN], char* room,
                                            const float* scale, const float* bias, int v0, int n0) {
   constexpr int E = (int)sizeof(Out), kFit = ROOM >= 32 * (256 + 16) ? 8 / E : 4 / E;
@@ -380,7 +397,7 @@ __device__ __forceinline__ void store_tile(const Int8Params& p, const i32x16_t (
 #pragma unroll
   for (int fn = 0; fn < FN; ++fn) {
     const int nb = n0 + fn * 32, n = nb + (lane & 31);
-    const float sh = n < p.N ? p.scale * p.h_scale[n] : 0.f;
+    const float sh = n < p.N ? p.h_scale[n] : 0.f, csh = p.scale * sh;
 #pragma unroll
     for (int f0 = 0; f0 < FM; f0 += FP) {
 #pragma unroll
@@ -393,7 +410,10 @@ __device__ __forceinline__ void store_tile(const Int8Params& p, const i32x16_t (
           const float sws[4] = {sw.x, sw.y, sw.z, sw.w}, bs[4] = {b.x, b.y, b.z, b.w};
           Four y;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) y.v[i] = (Out)fmaf((float)acc[f0 + f][fn][4 * g + i], sh * sws[i], bs[i]);
+          for (int i = 0; i < 4; ++i) {
+            const int sum = acc[f0 + f][fn][4 * g + i];
+            y.v[i] = (Out)(FAR ? far_logit(sum, p.scale, sh, sws[i], bs[i]) : near_logit(sum, csh, sws[i], bs[i]));
+          }
           *reinterpret_cast<Four*>(room + (lane & 31) * kPitch + c * E) = y;
         }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -420,6 +440,31 @@ __device__ __forceinline__ void store_tile(const Int8Params& p, const i32x16_t (
   }
 }
 
+// Whether a product of a wave's scales may leave fp32, which is where its logits take the long way.  None does with |sw| in
+// 2^-107 (what a row of zeros has) .. 2^60 and |c sh| in 2^-19 .. 2^60, or with 2^-16 .. and 2^-110 .. (a token of zeros).
+template <int FM, int FN>
+struct Scales {
+  float w[(FM + 1) / 2], h[(FN + 1) / 2];
+  __device__ __forceinline__ void load(const Int8Params& p, int v0, int n0) {
+#pragma unroll
+    for (int i = 0; i < (FM + 1) / 2; ++i) w[i] = p.w_scale[min(v0 + (i * 64 + lane_id()) % (32 * FM), p.V - 1)];
+#pragma unroll
+    for (int i = 0; i < (FN + 1) / 2; ++i) h[i] = p.h_scale[min(n0 + (i * 64 + lane_id()) % (32 * FN), p.N - 1)];
+  }
+  __device__ __forceinline__ bool far(float c) const {
+    bool small = false, any = false;
+#pragma unroll
+    for (int i = 0; i < (FM + 1) / 2; ++i) {
+      small |= fabsf(w[i]) < 0x1p-16f;
+      any |= !(fabsf(w[i]) >= 0x1p-107f && fabsf(w[i]) <= 0x1p60f);
+    }
+    const float least = __any(small) ? 0x1p-19f : 0x1p-110f;
+#pragma unroll
+    for (int i = 0; i < (FN + 1) / 2; ++i) any |= !(fabsf(c * h[i]) >= least && fabsf(c * h[i]) <= 0x1p60f);
+    return __any(any);
+  }
+};
+
 // Many tokens: BV x BM tiles of WV x WT waves, the readout's reduction loop (tile_reduce) on integer operands.  Up to some
 // 300 tokens bound by reading W (48 tokens, K = 4096, V = 128256: 101 us, 5.2 TB/s), beyond by the power that matrix cores
 // take: 8192 tokens 3430 to 3660 us, 2510 to 2350 TOP/s, at 1.4 GHz with the matrix cores busy in 75% of the cycles; the
@@ -435,10 +480,17 @@ __global__ __launch_bounds__(64 * WV * WT) void int8_tile_kernel(Int8Params p) {
   const int w = wave_id(), wv = w / WT, wt = w % WT;
   int vt, tb;
   grouped_tile(blockIdx.x, p.n_vt, p.n_tb, &vt, &tb);
+  const int v0 = vt * BV + wv * (BV / WV), n0 = tb * BM + wt * (BM / WT);  // the wave's
   for (int i = threadIdx.x; i < BV; i += NT) {
     s_scale[i] = wscale_at(p, vt * BV + i);
     s_bias[i] = bias_at(p, vt * BV + i);
   }
+  // Scales that are looked at in the epilogue: on the way from here in the large tiles, whose waves all store at once (2000
+  // tokens on V = 50021, K = 512 in bf16 86.3 us, loaded there 88.2), but loaded there in the small ones, which wait for
+  // the first operands (48 tokens on V = 16000, K = 4096 20.8 us, from here 21.7).
+  Scales<FM, FN> scales;
+  constexpr bool kEarly = NT > 256;
+  if constexpr (kEarly) scales.load(p, v0, n0);
   const uint32_t lds0 = lds_addr(smem);
   TA ta;
   ta.setup(p.w, vt * BV, p.S);
@@ -467,8 +519,15 @@ __global__ __launch_bounds__(64 * WV * WT) void int8_tile_kernel(Int8Params p) {
   tile_reduce<int8_t, 32, L>(acc, ta, th, smem, SB, ring, p.S, wv * (BV / WV), wt * (BM / WT), issue_next);  // (two steps a slice)
   stage_barrier();  // every wave has read its last operands: the ring holds the epilogue's rows
   constexpr int kRoom = NS * SB / (WV * WT);
-  store_tile<Out, FM, FN, kRoom>(p, acc, smem + w * kRoom, s_scale + wv * (BV / WV), s_bias + wv * (BV / WV),
-                          vt * BV + wv * (BV / WV), tb * BM + wt * (BM / WT));
+  if constexpr (!kEarly) scales.load(p, v0, n0);
+  auto store = [&](auto by) {
+    store_tile<Out, FM, FN, kRoom, decltype(by)::value>(p, acc, smem + w * kRoom, s_scale + wv * (BV / WV),
+                                                        s_bias + wv * (BV / WV), v0, n0);
+  };
+  if (scales.far(p.scale)) [[unlikely]]
+    store(std::true_type());
+  else
+    store(std::false_type());
 }
 
 template <class Src>

@@ -209,7 +209,8 @@ def head_logits(h, w, bias=None, *, logit_scale=1.0, dtype=None):
 
     h: ``[..., K]`` in bf16, fp16 or fp32 (up to 2^24 tokens), quantised per token as ``quantize_rows`` does; w:
     ``quantize_rows(W)`` or ``pack_rows(q, scale)`` of the [V, K] head; bias: ``[V]``.  The sum over K is exact, the
-    scales and the bias are applied in fp32, and the result is rounded once.  A token's logits do not depend on the
+    scales and the bias are applied in fp32 (in fp64 where the product of the scales leaves its range), and the result
+    is rounded once.  A token's logits do not depend on the
     others in the call.  A token or a row of W with an infinity or a NaN has NaN logits.  There is no gradient: where one
     would be recorded the call is refused.
     """
