@@ -194,8 +194,10 @@ def _checked(w):
 
 
 def dequantize(w):
-    """The values that ``w`` stands for, ``scale * q``, in fp32 [R, K]."""
+    """The values that ``w`` stands for, ``scale * q``, in fp32 [R, K].  No gradient: where the scales would record one the
+    call is refused."""
     q, scale, R, K = _checked(w)
+    _no_gradient("dequantize", scale)
     if eager(q, scale):
         return _unpack(q, scale, R, K)
     if q.device.type == "cpu":
@@ -227,7 +229,7 @@ def head_logits(h, w, bias=None, *, logit_scale=1.0, dtype=None):
     for name, x in (("w", q), ("bias", bias)):
         if x is not None and x.device != h.device:
             raise ValueError(f"{name} is on {x.device} but h on {h.device}")
-    _no_gradient("head_logits", h, bias)
+    _no_gradient("head_logits", h, scale, bias)
     if eager(h, q, scale, bias):
         return _logits(h, q, scale, bias, V, float(logit_scale), dtype)
     if h.device.type == "cpu":
