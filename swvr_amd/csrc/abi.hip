@@ -65,7 +65,7 @@ const char* kKindNames[kNumKinds] = {"fwd_tile_kernel",   "fwd_combine_kernel", 
                                      "mse_loss",          "quantize_e4m3",      "readout_f64",
                                      "probe_mfma",        "embedding",          "sort_ids",
                                      "distill",           "sample_tokens",      "int8_logits",
-                                     "select_beams",      "reorder_beams"};
+                                     "select_beams",      "reorder_beams",      "int8_rows"};
 
 bool is_dtype(int d) { return d == SWVR_BF16 || d == SWVR_F16 || d == SWVR_F32; }
 

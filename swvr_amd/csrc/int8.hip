@@ -600,13 +600,13 @@ hipError_t int8_quantize(int dtype, const void* x, int64_t ld, int64_t R, int64_
   if (R == 0) return hipSuccess;
   char* im = static_cast<char*>(image);
   hipError_t e;
-  timing_begin(kKindQuant, stream);
+  timing_begin(kKindInt8Rows, stream);
   switch (dtype) {
     case kBF16: e = quantize_typed(static_cast<const bf16_t*>(x), ld, R, K, im, scale, pad, stream); break;
     case kF16: e = quantize_typed(static_cast<const f16_t*>(x), ld, R, K, im, scale, pad, stream); break;
     default: e = quantize_typed(static_cast<const float*>(x), ld, R, K, im, scale, pad, stream); break;
   }
-  timing_end(kKindQuant, stream);
+  timing_end(kKindInt8Rows, stream);
   return e;
 }
 
@@ -614,20 +614,20 @@ hipError_t int8_pack(const void* q, int64_t ld, int64_t R, int64_t K, void* imag
   if (R == 0) return hipSuccess;
   const int vec = reinterpret_cast<uintptr_t>(q) % 16 == 0 && ld % 16 == 0;
   const int64_t rows = (R + kInt8Rows - 1) / kInt8Rows * kInt8Rows;
-  timing_begin(kKindQuant, stream);
+  timing_begin(kKindInt8Rows, stream);
   int8_pack_kernel<<<(unsigned)(rows / 32), 256, 0, stream>>>(static_cast<const int8_t*>(q), ld, R, (int)K,
                                                               (int)int8_slices(K), vec, static_cast<char*>(image));
-  timing_end(kKindQuant, stream);
+  timing_end(kKindInt8Rows, stream);
   return hipGetLastError();
 }
 
 hipError_t int8_unpack(const void* image, const float* scale, int64_t R, int64_t K, float* out, hipStream_t stream) {
   if (R == 0 || K == 0) return hipSuccess;
-  timing_begin(kKindQuant, stream);
+  timing_begin(kKindInt8Rows, stream);
   const int pieces = (int)((K + kUnpackK - 1) / kUnpackK);
   int8_unpack_kernel<<<(unsigned)((R + 31) / 32 * pieces), 256, 0, stream>>>(static_cast<const char*>(image), scale, R, (int)K,
                                                                              (int)int8_slices(K), pieces, out);
-  timing_end(kKindQuant, stream);
+  timing_end(kKindInt8Rows, stream);
   return hipGetLastError();
 }
 

@@ -28,6 +28,7 @@ enum KernelKind {
   kKindInt8,
   kKindBeams,
   kKindReorder,
+  kKindInt8Rows,
   kNumKinds
 };
 
