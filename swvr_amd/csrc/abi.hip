@@ -804,6 +804,9 @@ int swvr_int8_logits(int dtype, int out_dtype, int64_t N, int64_t K, int64_t V, 
   if (N == 0 || V == 0) return SWVR_OK;
   if (!h || !w_image || !w_scale || !out || !aligned16(w_image))
     return fail(SWVR_EINVAL, "h, the image (16-byte aligned), its scales and out must be non-null");
+  auto off = [](const void* x, int tag) { return reinterpret_cast<uintptr_t>(x) % (tag == SWVR_F32 ? 4 : 2) != 0; };
+  if (off(h, dtype) || off(out, out_dtype) || off(w_scale, SWVR_F32) || (bias && off(bias, bias_dtype)))
+    return fail(SWVR_EINVAL, "h, w_scale, bias and out must be aligned to their elements");
   const size_t need = swvr_int8_logits_workspace_size(N, K);
   if (workspace_bytes < need || !workspace || !aligned16(workspace))
     return fail(SWVR_EWORKSPACE, "int8 workspace of %zu bytes (16-byte aligned) needed, %zu given", need, workspace_bytes);
