@@ -143,8 +143,8 @@ __device__ __forceinline__ uint4 quantize16(const Sixteen<Src>& x, float s, floa
 // TPR threads a row, a wave for many rows and a workgroup for few, each with NC pieces of 16 values in registers, so
 // that rows of up to 16 NC TPR values are read once (longer ones twice).  A piece goes out as one 16-byte chunk of the
 // image; the workgroup's rows are neighbours in it, 8 of them 128 bytes in a row.  Bound by reading x and writing a byte
-// a value: 151936 x 2560 in bf16 210 us, 5.6 TB/s.  (8 threads a row, whose chunks go out together without LDS but who
-// read their rows twice: 415 us.)
+// a value: 151936 x 2560 in bf16 221 us, 5.3 TB/s, again and again; 240 after a dequantisation, whose stores fill the
+// caches.  (8 threads a row, whose chunks go out together without LDS but who read their rows twice: 415 us.)
 constexpr int kManyRows = 8;
 template <class Src, int TPR, int NC>
 __global__ __launch_bounds__(TPR == 64 ? 64 * kManyRows : TPR) void int8_quantize_kernel(
@@ -220,7 +220,8 @@ __global__ __launch_bounds__(TPR == 64 ? 64 * kManyRows : TPR) void int8_quantiz
   }
 }
 
-// Rows of integers [R][ld] into an image, 8 threads a row: 151936 x 2560 in 140 us, 5.5 TB/s of what is read and written.
+// Rows of integers [R][ld] into an image, 8 threads a row: 151936 x 2560 in 140 to 155 us, 5.6 to 5.0 TB/s of what is read and
+// written.
 __global__ __launch_bounds__(256) void int8_pack_kernel(const int8_t* __restrict__ q, int64_t ld, int64_t R, int K, int S,
                                                         int vec, char* __restrict__ image) {
   const int64_t r = (int64_t)blockIdx.x * 32 + threadIdx.x / 8;
@@ -242,7 +243,7 @@ __global__ __launch_bounds__(256) void int8_pack_kernel(const int8_t* __restrict
 
 // The values that an image stands for, in fp32 [R][K]: 32 rows x kUnpackK values through LDS, so that the image comes
 // in and rows go out in long pieces (16 bytes a lane; a chunk's 512 bytes padded to 528: no bank conflicts).  151936 x
-// 2560 in 330 us, 5.9 TB/s.
+// 2560 in 334 to 344 us, 5.8 to 5.7 TB/s.
 constexpr int kUnpackK = 256;
 __global__ __launch_bounds__(256) void int8_unpack_kernel(const char* __restrict__ image, const float* __restrict__ scale,
                                                           int64_t R, int K, int S, int pieces, float* __restrict__ out) {
@@ -467,8 +468,8 @@ struct Scales {
 
 // Many tokens: BV x BM tiles of WV x WT waves, the readout's reduction loop (tile_reduce) on integer operands.  Up to some
 // 300 tokens bound by reading W (48 tokens, K = 4096, V = 128256: 101 us, 5.2 TB/s), beyond by the power that matrix cores
-// take: 8192 tokens 3430 to 3660 us, 2510 to 2350 TOP/s, at 1.4 GHz with the matrix cores busy in 75% of the cycles; the
-// loop alone would take 3130.
+// take: 8192 tokens 3430 to 3660 us, 2510 to 2350 TOP/s, at 1.4 to 1.5 GHz with the matrix cores busy in 74% of the
+// cycles; the loop alone would take 3130.
 template <class Out, int BV, int BM, int WV, int WT, int NS>
 __global__ __launch_bounds__(64 * WV * WT) void int8_tile_kernel(Int8Params p) {
   constexpr int NT = 64 * WV * WT, FM = BV / WV / 32, FN = BM / WT / 32;
@@ -559,14 +560,18 @@ void tile_launch(Int8Params p, hipStream_t stream) {
 // Tiles that fill the card: about one for each of its 256 CUs.
 constexpr int64_t kFull = 240;
 
-// Up to 64 tokens reading W bounds a call, at 5.6 TB/s; tiles of 128 x 64 through LDS reach that wherever there is one for
-// each CU, and with fewer rows the kernel without LDS, whose workgroups are smaller: (K = 4096, V = 16000, 1 token: 11.1
-// us, tiles 16.0; K = 2560, V = 151936, 48 tokens: 99 us, tiles 81.)  With more tokens the largest tile that fills the
+// Up to 64 tokens reading W bounds a call, at up to 5.6 TB/s, which tiles of 128 x 64 through LDS reach; on few rows the
+// kernel without LDS, whose workgroups of 32 rows are more: (K = 4096, V = 16000, 1 token: 11.1 us, tiles 16.0; K = 2560, V =
+// 151936, 48 tokens: 99 us, tiles 81.)  The border: 32 tokens take tiles from 240 of them on (V = 30593), more tokens from
+// half as many (V = 15297), where both are alike (48 tokens, K = 4096, V = 15400 19.6 us without LDS and 20.2, 16000 19.6 and
+// 19.7, 20000 21.6 and 20.5, 28000 28.0 and 24.1; tiles of 64 x 64 18.2 on 16000, 22.1 on 20000, 24.1 on 28000).
+// With more tokens the largest tile that fills the
 // card (200 tokens, K = 4096: 256 x 256 on V = 128256 142 us and 256 x 128 153; on V = 32000 52 and 37; 128 x 128 on V =
 // 16000 24, 256 x 128 28), and of 256 x 256 and 256 x 128 the one with the fewer padded tokens.  With K up to 512, in fp32
-// 1024, storing logits takes as long as forming them, and 256 x 128, two to a CU, does one beside the other: (500 tokens, V =
-// 50021 in bf16, K = 512 46 -> 40 us; 8192 on 50048 in fp32, K = 512 440 -> 405, K = 1024 595 -> 560; but 1000 on 32000,
-// K = 1024 62 -> 69, and K = 1536 74 -> 90.)
+// 1024, storing logits takes as long as forming them, and 256 x 128, two to a CU, does one beside the other.  (256 x 256 and
+// 256 x 128: 500 tokens on V = 50021, K = 512 in bf16 33.4 and 32.5 us; 8192 on 50048, K = 512 in bf16 323 and 315, in fp32 402
+// and 382; 1000 on 32000, K = 1024 in fp32 55.5 and 49.9.  Past the border: 8192 on 50048, K = 1024 in bf16 468 and 465, K = 1536
+// 623 and 630, in fp32 701 and 707, but 1000 on 32000, K = 1024 in bf16 44.9 and 43.6, K = 1536 in fp32 69.5 and 64.5.)
 template <class Out>
 hipError_t logits_typed(Int8Params p, hipStream_t stream) {
   // Logits past the caches where rows are whole lines (a wave writes 256 bytes of each): W and h stay in them.  (8192
