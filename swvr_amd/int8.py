@@ -137,8 +137,10 @@ def _sizes(name, x):
 
 def _no_gradient(what, *tensors):
     no_tangents(*tensors)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise ValueError(f"{what} has no gradient: call it under torch.no_grad() or on detached tensors")
+    if torch.is_grad_enabled():
+        for t in tensors:  # (a loop, as in eager)
+            if t is not None and t.requires_grad:
+                raise ValueError(f"{what} has no gradient: call it under torch.no_grad() or on detached tensors")
 
 
 def quantize_rows(x):
